@@ -5,8 +5,10 @@
     import resnet20              # the reference's model file, unchanged
 
 Sub-modules: `adder` (adder2d, adder2d_function, adder), `adder_cuda` (the extension's entry
-points plus the fused forward/backward), `resnet` (ResNet-20/50 builders), `ddp` (bucketed
-gradient all-reduce for batch-sharded training), `build` (nvcc build of the C-ABI library).
+points plus the fused forward/backward), `resnet` (ResNet-20/50 builders), `batchnorm` and `layernorm` (norms with the residual
+add in their pass), `logprobs` (log probabilities, entropy, top classes, cross entropy), `optim` (AdamW, states in 32 or 8 bits),
+`train` (the training step), `ddp` (bucketed gradient all-reduce for batch-sharded training), `build` (nvcc build of the C-ABI
+library).
 """
 import sys as _sys
 

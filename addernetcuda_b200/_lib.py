@@ -6,8 +6,10 @@ import raises.  Nothing here computes on the CPU.
 from __future__ import annotations
 
 import ctypes
-from ctypes import c_char_p, c_float, c_int, c_longlong, c_size_t, c_uint, c_ulonglong, c_void_p, POINTER
+from ctypes import c_char_p, c_double, c_float, c_int, c_longlong, c_size_t, c_uint, c_ulonglong, c_void_p, POINTER
 from pathlib import Path
+
+import torch
 
 _PKG = Path(__file__).resolve().parent
 LIB_PATH = _PKG / "libadder_b200.so"
@@ -17,6 +19,8 @@ ADDER_OK = 0
 FLAG_FAST_CLAMP = 1
 FLAG_ACCUMULATE = 2
 FLAG_UNALIGNED = 4
+# element types of the operators that take more than fp32
+TYPE_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 # status codes of include/adder_b200.h
 (OK, ERR_NULL_POINTER, ERR_BAD_SHAPE, ERR_UNSUPPORTED, ERR_ALIGNMENT, ERR_WORKSPACE, ERR_CUDA, ERR_INTERNAL,
  ERR_TOO_LARGE, ERR_TIMEOUT) = range(10)
@@ -65,6 +69,15 @@ SIGNATURES = {
     "adder_b200_conv_backward_weight_workspace_bytes": (c_size_t, [c_int] * 13),
     "adder_b200_conv_backward_weight": (c_int, [c_void_p] * 4 + [c_float, c_void_p, c_size_t] + [c_int] * 13 + [c_void_p]),
     "adder_b200_forward_affine": (c_int, [c_void_p] * 5 + [c_int, c_void_p, *_GEOM, c_void_p]),
+    "adder_b200_layernorm_forward": (c_int, [c_void_p] * 8 + [c_longlong] * 4 + [c_int, c_int, c_float, c_void_p]),
+    "adder_b200_layernorm_backward_workspace_bytes": (c_size_t, [c_longlong, c_longlong]),
+    "adder_b200_layernorm_backward": (c_int, [c_void_p] * 10 + [c_size_t] + [c_longlong] * 3 + [c_int, c_int, c_void_p]),
+    "adder_b200_log_probs_forward": (c_int, [c_void_p, c_int, c_longlong, c_longlong, c_longlong, c_void_p, c_longlong, c_int] +
+                                     [c_void_p] * 6),
+    "adder_b200_log_probs_backward": (c_int, [c_void_p, c_int, c_longlong, c_longlong, c_longlong, c_void_p, c_longlong, c_int] +
+                                      [c_void_p] * 8),
+    "adder_b200_adamw_step": (c_int, [c_void_p, c_int, c_int, c_int, c_double, c_void_p] + [c_double] * 4 + [c_void_p, c_void_p]),
+    "adder_b200_adamw_state_values": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_longlong, c_void_p]),
     "adder_b200_device_status": (c_int, [POINTER(c_int), c_int]),
     "adder_b200_peer_area_bytes": (c_size_t, [c_longlong, c_int]),
     "adder_b200_ipc_export": (c_int, [c_void_p, c_void_p, POINTER(c_ulonglong)]),

@@ -1,8 +1,8 @@
 """The C++ host path of the eager layer calls (csrc/host.cpp), loaded on the first call with a CUDA tensor.
 
-`layer`, `conv`, `layer_with_stats`, `layer_affine`, `affine` and `column` return None for whatever they do not take - anything but
-contiguous fp32 CUDA tensors of a geometry the kernels are built for - and callers then go on in Python, which handles
-the rest or raises.  They always call the product library; inside a `_lib.tuning()` block they return None.
+`layer`, `conv`, `layer_with_stats`, `layer_affine`, `affine`, `column`, `layer_norm`, `log_probs` and `adamw` return None for whatever
+they do not take - the layers anything but contiguous fp32 CUDA tensors of a geometry the kernels are built for, the others anything but
+CUDA tensors of their types in rows or, `adamw`, contiguous - and callers then go on in Python, which handles the rest or raises.  They always call the product library; inside a `_lib.tuning()` block they return None.
 """
 from __future__ import annotations
 
@@ -20,8 +20,10 @@ _NAMES = ("adder_b200_status_string", "adder_b200_forward", "adder_b200_forward_
           "adder_b200_backward_input_workspace_bytes", "adder_b200_backward_input_with_workspace",
           "adder_b200_backward_weight_workspace_bytes", "adder_b200_backward_weight", "adder_b200_conv_forward",
           "adder_b200_conv_backward_input_workspace_bytes", "adder_b200_conv_backward_input_with_workspace",
-          "adder_b200_conv_backward_weight_workspace_bytes", "adder_b200_conv_backward_weight")
-_ENTRIES = ("layer", "conv", "layer_with_stats", "layer_affine", "affine", "column")
+          "adder_b200_conv_backward_weight_workspace_bytes", "adder_b200_conv_backward_weight",
+          "adder_b200_layernorm_forward", "adder_b200_layernorm_backward_workspace_bytes", "adder_b200_layernorm_backward",
+          "adder_b200_log_probs_forward", "adder_b200_log_probs_backward", "adder_b200_adamw_step")
+_ENTRIES = ("layer", "conv", "layer_with_stats", "layer_affine", "affine", "column", "layer_norm", "log_probs", "adamw")
 _mod = None
 
 
@@ -71,11 +73,12 @@ def sync() -> None:
 
 def _first_call(name):
     def call(tensor, *args):
-        if not (isinstance(tensor, torch.Tensor) and tensor.is_cuda):
+        first = tensor[0] if isinstance(tensor, (list, tuple)) and tensor else tensor
+        if not (isinstance(first, torch.Tensor) and first.is_cuda):
             return None
         load()
         return getattr(sys.modules[__name__], name)(tensor, *args)
     return call
 
 
-layer, conv, layer_with_stats, layer_affine, affine, column = (_first_call(n) for n in _ENTRIES)
+layer, conv, layer_with_stats, layer_affine, affine, column, layer_norm, log_probs, adamw = (_first_call(n) for n in _ENTRIES)

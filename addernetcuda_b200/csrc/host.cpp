@@ -2,8 +2,8 @@
 // (adder.py, adder_cuda.py, inference.py) does around a launch - checks, output allocation, the autograd node, the side stream
 // of the weight gradient.  A small layer's kernels take 10-20 us; the Python around its forward and backward took 150.
 //
-// Every entry point takes the common case only (contiguous fp32 CUDA tensors of a geometry the fused kernels are built for) and
-// returns None for anything else, errors included: the caller then goes through the Python layer, which handles or rejects it.
+// Every entry point takes the common case only (contiguous CUDA tensors, fp32 and of a geometry the fused kernels are built for where it
+// is a layer) and returns None for anything else, errors included: the caller then goes through the Python layer, which handles or rejects it.
 #include <torch/extension.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -38,6 +38,12 @@ struct Api {      // entry points of the loaded libadder_b200.so
     decltype(&adder_b200_conv_backward_input_with_workspace) conv_backward_input_with_workspace = nullptr;
     decltype(&adder_b200_conv_backward_weight_workspace_bytes) conv_backward_weight_workspace_bytes = nullptr;
     decltype(&adder_b200_conv_backward_weight) conv_backward_weight = nullptr;
+    decltype(&adder_b200_layernorm_forward) layernorm_forward = nullptr;
+    decltype(&adder_b200_layernorm_backward_workspace_bytes) layernorm_backward_workspace_bytes = nullptr;
+    decltype(&adder_b200_layernorm_backward) layernorm_backward = nullptr;
+    decltype(&adder_b200_log_probs_forward) log_probs_forward = nullptr;
+    decltype(&adder_b200_log_probs_backward) log_probs_backward = nullptr;
+    decltype(&adder_b200_adamw_step) adamw_step = nullptr;
 };
 // Written once, by the first bind to the product library, which is never unloaded: autograd nodes made by this path call through it
 // for as long as they live, from any thread.  `enabled` is what bind() switches, and only the Python entry points look at it.
@@ -69,13 +75,13 @@ struct Layer {      // geometry arguments of the C interface
 
 // What the kernels take.  A dual tensor of forward-mode differentiation is left to the Python layer, which refuses it: without a node,
 // its tangent would be dropped without a word.
-bool plain(const at::Tensor& t) {
+bool unwrapped(const at::Tensor& t) {
     static const c10::DispatchKeySet wrapped({c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::FuncTorchGradWrapper,
                                               c10::DispatchKey::Functionalize, c10::DispatchKey::Python,
                                               c10::DispatchKey::Conjugate, c10::DispatchKey::Negative});
-    return t.is_cuda() && t.scalar_type() == at::kFloat && t.layout() == at::kStrided && t.is_contiguous() && !t.key_set().has_any(wrapped) &&
-           !t._fw_grad(0).defined();
+    return t.is_cuda() && t.layout() == at::kStrided && !t.key_set().has_any(wrapped) && !t._fw_grad(0).defined();
 }
+bool plain(const at::Tensor& t) { return unwrapped(t) && t.scalar_type() == at::kFloat && t.is_contiguous(); }
 
 bool layer_of(const at::Tensor& x, const at::Tensor& w, int64_t stride, int64_t pad, Layer* L) {
     if (!plain(x) || !plain(w) || x.device() != w.device() || x.dim() != 4 || w.dim() != 4) return false;
@@ -347,6 +353,237 @@ struct AdderColumn : public torch::autograd::Function<AdderColumn> {
     }
 };
 
+// ------------------------------------------------------------------------------------------ layer norm, log probabilities, AdamW
+
+// ADDER_TYPE_* of a tensor, or -1
+int type_code(const at::Tensor& t) {
+    switch (t.scalar_type()) {
+        case at::kFloat: return ADDER_TYPE_F32;
+        case at::kBFloat16: return ADDER_TYPE_BF16;
+        case at::kHalf: return ADDER_TYPE_F16;
+        default: return -1;
+    }
+}
+
+// The last `inner` extents of t lie one after the other, and so do the rows that they make, *stride elements apart.
+bool rows_of(const at::Tensor& t, int64_t inner, int64_t d, int64_t* stride) {
+    if (t.is_contiguous()) {
+        *stride = d;
+        return true;
+    }
+    const auto sizes = t.sizes(), strides = t.strides();
+    int64_t want = 1, i = t.dim() - 1;
+    for (; i >= t.dim() - inner; --i) {
+        if (sizes[i] != 1 && strides[i] != want) return false;
+        want *= sizes[i];
+    }
+    bool first = true;
+    for (; i >= 0; --i) {
+        if (sizes[i] == 1) continue;
+        if (first) *stride = want = strides[i];
+        else if (strides[i] != want) return false;
+        first = false;
+        want *= sizes[i];
+    }
+    if (first) *stride = d;
+    return true;
+}
+
+struct Norm {      // a checked call
+    int64_t rows, d, x_stride, r_stride;
+    int type, weight_type;
+    double eps;
+};
+
+bool norm_of(const at::Tensor& x, const at::Tensor* r, const at::Tensor* w, const at::Tensor* b, at::IntArrayRef shape, double eps, Norm* n) {
+    n->type = type_code(x);
+    if (n->type < 0 || !unwrapped(x) || shape.empty() || x.dim() < (int64_t)shape.size() || !(eps >= 0.0)) return false;
+    if (x.sizes().slice(x.dim() - shape.size()) != shape) return false;
+    n->d = c10::multiply_integers(shape);
+    if (n->d == 0 || x.numel() == 0) return false;
+    n->rows = x.numel() / n->d;
+    n->r_stride = 0;
+    if (!rows_of(x, shape.size(), n->d, &n->x_stride)) return false;
+    if (r != nullptr && (!unwrapped(*r) || r->device() != x.device() || r->scalar_type() != x.scalar_type() || r->sizes() != x.sizes() ||
+                         !rows_of(*r, shape.size(), n->d, &n->r_stride)))
+        return false;
+    n->weight_type = n->type;
+    for (const at::Tensor* t : {w, b}) {
+        if (t == nullptr) continue;
+        if (!unwrapped(*t) || !t->is_contiguous() || t->device() != x.device() || t->sizes() != shape) return false;
+        n->weight_type = type_code(*t);
+        if (n->weight_type != n->type && n->weight_type != ADDER_TYPE_F32) return false;
+    }
+    if (w != nullptr && b != nullptr && w->scalar_type() != b->scalar_type()) return false;
+    n->eps = eps;
+    return true;
+}
+
+void* ptr(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+struct NormResult { at::Tensor y, h, mean, rstd; };
+
+NormResult norm_forward(const at::Tensor& x, const at::Tensor& r, const at::Tensor& w, const at::Tensor& b, const Norm& n, bool keep) {
+    const c10::cuda::CUDAGuard guard(x.device());
+    NormResult out;
+    out.y = empty_on(x, x.sizes(), x.scalar_type());
+    if (r.defined()) out.h = empty_on(x, x.sizes(), x.scalar_type());
+    if (keep) {
+        out.mean = empty_on(x, {n.rows});
+        out.rstd = empty_on(x, {n.rows});
+    }
+    check(api.layernorm_forward(ptr(x), ptr(r), ptr(w), ptr(b), ptr(out.y), ptr(out.h), static_cast<float*>(ptr(out.mean)),
+                                static_cast<float*>(ptr(out.rstd)), n.rows, n.d, n.x_stride, n.r_stride, n.type, n.weight_type, (float)n.eps,
+                                current_stream(x)), "adder_b200_layernorm_forward");
+    return out;
+}
+
+using Optional = std::optional<at::Tensor>;
+
+struct LayerNorm : public torch::autograd::Function<LayerNorm> {
+    static variable_list forward(AutogradContext* ctx, const Variable& x, const Optional& r, const Optional& w, const Optional& b, const Norm& n) {
+        const at::Tensor none;
+        auto out = norm_forward(x, r.value_or(none), w.value_or(none), b.value_or(none), n, true);
+        ctx->save_for_backward({r ? out.h : x, w.value_or(none), out.mean, out.rstd});
+        ctx->saved_data["sizes"] = std::vector<int64_t>{n.rows, n.d, n.type, n.weight_type, r.has_value(), b.has_value()};
+        if (b) ctx->saved_data["shape"] = b->sizes().vec();
+        ctx->set_materialize_grads(false);
+        return r ? variable_list{out.y, out.h} : variable_list{out.y};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const Variable none;
+        const auto sizes = ctx->saved_data["sizes"].toIntVector();
+        const int64_t rows = sizes[0], d = sizes[1];
+        const int type = (int)sizes[2], weight_type = (int)sizes[3];
+        const bool has_r = sizes[4], has_b = sizes[5];
+        at::Tensor dy = grads[0], dh = has_r ? grads[1] : none;
+        if (!dy.defined() && !dh.defined()) return {none, none, none, none, none};
+        const auto saved = ctx->get_saved_variables();
+        const Variable &h = saved[0], &w = saved[1], &mean = saved[2], &rstd = saved[3];
+        int64_t stride;
+        TORCH_CHECK(unwrapped(h) && type_code(h) == type && h.numel() == rows * d && plain(mean) && plain(rstd) && mean.numel() == rows &&
+                    rstd.numel() == rows && (!w.defined() || (unwrapped(w) && w.is_contiguous() && type_code(w) == weight_type && w.numel() == d)), SAVED);
+        const c10::cuda::CUDAGuard guard(h.device());
+        at::Tensor h2 = h;      // rows of consecutive elements
+        if (!rows_of(h, 1, d, &stride) || h.dim() == 0 || h.size(-1) != d) {
+            h2 = h.contiguous();
+            stride = d;
+        }
+        if (!dy.defined()) dy = at::zeros_like(h, at::MemoryFormat::Contiguous);
+        dy = dy.contiguous();
+        if (dh.defined()) dh = dh.contiguous();
+        for (const at::Tensor* g : {&dy, &dh})
+            TORCH_CHECK(!g->defined() || (g->scalar_type() == h.scalar_type() && g->device() == h.device() && g->sizes() == h.sizes()),
+                        "the gradient must have the type, device and shape of the output");
+        int edge = 0;
+        const bool need_x = ctx->needs_input_grad(edge++), need_r = has_r && ctx->needs_input_grad(edge++);
+        const bool need_w = w.defined() && ctx->needs_input_grad(edge++), need_b = has_b && ctx->needs_input_grad(edge++);
+        at::Tensor dx, dw, db, ws;
+        if (need_x || need_r) dx = empty_on(h, h.sizes(), h.scalar_type());
+        const at::ScalarType weight_scalar = weight_type == ADDER_TYPE_F32 ? at::kFloat : h.scalar_type();
+        if (need_w) dw = empty_on(h, w.sizes(), weight_scalar);
+        if (need_b) db = empty_on(h, ctx->saved_data["shape"].toIntVector(), weight_scalar);
+        const size_t bytes = need_w || need_b ? api.layernorm_backward_workspace_bytes(rows, d) : 0;
+        if (bytes > 0) ws = empty_on(h, {(int64_t)bytes}, at::kByte);
+        check(api.layernorm_backward(ptr(dy), ptr(dh), ptr(h2), ptr(w), mean.const_data_ptr<float>(), rstd.const_data_ptr<float>(), ptr(dx), ptr(dw),
+                                     ptr(db), ptr(ws), bytes, rows, d, stride, type, weight_type, current_stream(h)), "adder_b200_layernorm_backward");
+        return {need_x ? dx : none, need_r ? dx : none, dw, db, none};
+    }
+};
+
+struct LogProbs {      // a checked call
+    int64_t rows, classes, stride, ignore;
+    int type, top_k;
+    bool entropy;
+};
+
+bool log_probs_of(const at::Tensor& x, const at::Tensor* targets, int64_t top_k, LogProbs* n) {
+    n->type = type_code(x);
+    if (n->type < 0 || !unwrapped(x) || x.dim() < 1 || x.numel() == 0) return false;
+    n->classes = x.size(-1);
+    n->rows = x.numel() / n->classes;
+    if (top_k < 0 || top_k > 32 || top_k > n->classes || !rows_of(x, 1, n->classes, &n->stride)) return false;
+    n->top_k = (int)top_k;
+    return targets == nullptr || (unwrapped(*targets) && targets->scalar_type() == at::kLong && targets->is_contiguous() &&
+                                  targets->device() == x.device() && targets->sizes() == x.sizes().slice(0, x.dim() - 1));
+}
+
+struct LogProbsResult { at::Tensor log_prob, entropy, top, indices, stats; };
+
+LogProbsResult log_probs_forward(const at::Tensor& x, const at::Tensor& targets, const LogProbs& n, bool keep) {
+    const c10::cuda::CUDAGuard guard(x.device());
+    LogProbsResult out;
+    const auto lead = x.sizes().slice(0, x.dim() - 1);
+    if (targets.defined()) out.log_prob = empty_on(x, lead);
+    if (n.entropy) out.entropy = empty_on(x, lead);
+    if (n.top_k > 0) {
+        c10::SmallVector<int64_t, 5> sizes(lead.begin(), lead.end());
+        sizes.push_back(n.top_k);
+        out.top = empty_on(x, sizes);
+        out.indices = empty_on(x, sizes, at::kLong);
+    }
+    if (keep) out.stats = empty_on(x, {n.rows, 2});
+    check(api.log_probs_forward(ptr(x), n.type, n.rows, n.classes, n.stride, static_cast<const long long*>(ptr(targets)), n.ignore, n.top_k,
+                                static_cast<float*>(ptr(out.log_prob)), static_cast<float*>(ptr(out.entropy)), static_cast<float*>(ptr(out.stats)),
+                                static_cast<float*>(ptr(out.top)), static_cast<long long*>(ptr(out.indices)), current_stream(x)),
+          "adder_b200_log_probs_forward");
+    return out;
+}
+
+struct LogProbsNode : public torch::autograd::Function<LogProbsNode> {
+    // the outputs that there are, in the order of LogProbsResult
+    static variable_list forward(AutogradContext* ctx, const Variable& x, const Optional& targets, const LogProbs& n) {
+        const at::Tensor none;
+        auto out = log_probs_forward(x, targets.value_or(none), n, true);
+        ctx->save_for_backward({x, targets.value_or(none), out.stats, out.entropy, out.indices});
+        ctx->saved_data["args"] = std::vector<int64_t>{n.rows, n.classes, n.ignore, n.type, n.top_k, targets.has_value(), n.entropy};
+        ctx->set_materialize_grads(false);
+        if (out.indices.defined()) ctx->mark_non_differentiable({out.indices});
+        variable_list list;
+        for (const at::Tensor* t : {&out.log_prob, &out.entropy, &out.top, &out.indices})
+            if (t->defined()) list.push_back(*t);
+        return list;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const Variable none;
+        const auto a = ctx->saved_data["args"].toIntVector();
+        const int64_t rows = a[0], classes = a[1], ignore = a[2];
+        const int type = (int)a[3], top_k = (int)a[4];
+        size_t at = 0;
+        at::Tensor g_lp, g_ent, g_top;
+        if (a[5]) g_lp = grads[at++];
+        if (a[6]) g_ent = grads[at++];
+        if (top_k > 0) g_top = grads[at++];
+        if (!g_lp.defined() && !g_ent.defined() && !g_top.defined()) return {none, none, none};
+        const auto saved = ctx->get_saved_variables();
+        const Variable &x = saved[0], &targets = saved[1], &stats = saved[2], &entropy = saved[3], &indices = saved[4];
+        TORCH_CHECK(unwrapped(x) && type_code(x) == type && x.dim() >= 1 && x.size(-1) == classes && x.numel() == rows * classes && plain(stats) &&
+                    stats.numel() == 2 * rows && (!a[6] || (plain(entropy) && entropy.numel() == rows)), SAVED);
+        TORCH_CHECK((!a[5] || (unwrapped(targets) && targets.scalar_type() == at::kLong && targets.is_contiguous() && targets.numel() == rows)) &&
+                    (top_k == 0 || (unwrapped(indices) && indices.scalar_type() == at::kLong && indices.is_contiguous() &&
+                                    indices.numel() == rows * top_k)), SAVED);
+        const c10::cuda::CUDAGuard guard(x.device());
+        for (at::Tensor* g : {&g_lp, &g_ent, &g_top})
+            if (g->defined()) {
+                *g = g->contiguous();
+                TORCH_CHECK(g->scalar_type() == at::kFloat && g->device() == x.device() && g->numel() == (g == &g_top ? rows * top_k : rows),
+                            "the gradient must be a float32 tensor of the output's shape and device");
+            }
+        at::Tensor x2 = x;
+        int64_t stride;
+        if (!rows_of(x, 1, classes, &stride)) {
+            x2 = x.contiguous();
+            stride = classes;
+        }
+        at::Tensor dx = empty_on(x, x.sizes(), x.scalar_type());
+        check(api.log_probs_backward(ptr(x2), type, rows, classes, stride, static_cast<const long long*>(ptr(targets)), ignore, top_k,
+                                     static_cast<const long long*>(ptr(indices)), stats.const_data_ptr<float>(), static_cast<const float*>(ptr(entropy)),
+                                     static_cast<const float*>(ptr(g_lp)), static_cast<const float*>(ptr(g_ent)), static_cast<const float*>(ptr(g_top)),
+                                     ptr(dx), current_stream(x)), "adder_b200_log_probs_backward");
+        return {dx, none, none};
+    }
+};
+
 // ------------------------------------------------------------------------------------------ Python entry points
 
 const at::Tensor* tensor_arg(PyObject* o) { return THPVariable_CheckExact(o) ? &THPVariable_Unpack(o) : nullptr; }
@@ -491,6 +728,209 @@ PyObject* py_column(PyObject*, PyObject* const* args, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// A tensor that may be left out (None); false: something else.
+bool optional_tensor(PyObject* o, const at::Tensor** t) {
+    *t = o == Py_None ? nullptr : tensor_arg(o);
+    return o == Py_None || *t != nullptr;
+}
+bool double_arg(PyObject* o, double* v) {
+    if (PyFloat_CheckExact(o)) *v = PyFloat_AS_DOUBLE(o);
+    else if (PyLong_CheckExact(o)) *v = PyLong_AsDouble(o);
+    else return false;
+    if (PyErr_Occurred()) {
+        PyErr_Clear();
+        return false;
+    }
+    return true;
+}
+Optional optional(const at::Tensor* t) { return t != nullptr ? Optional(*t) : Optional(); }
+PyObject* wrap_or_none(at::Tensor t) {
+    if (!t.defined()) Py_RETURN_NONE;
+    return THPVariable_Wrap(std::move(t));
+}
+
+// layer_norm(x, residual or None, weight or None, bias or None, shape, eps) -> y, or (y, h) with a residual, or None
+PyObject* py_layer_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 6 || !available()) Py_RETURN_NONE;
+    const at::Tensor *x = tensor_arg(args[0]), *r, *w, *b;
+    double eps;
+    if (x == nullptr || !optional_tensor(args[1], &r) || !optional_tensor(args[2], &w) || !optional_tensor(args[3], &b) ||
+        !PyTuple_CheckExact(args[4]) || !double_arg(args[5], &eps))
+        Py_RETURN_NONE;
+    c10::SmallVector<int64_t, 5> shape(PyTuple_GET_SIZE(args[4]));
+    for (size_t i = 0; i < shape.size(); ++i)
+        if (!int_arg(PyTuple_GET_ITEM(args[4], i), &shape[i])) Py_RETURN_NONE;
+    Norm c;
+    if (!norm_of(*x, r, w, b, shape, eps, &c)) Py_RETURN_NONE;
+    at::Tensor y, h;
+    {
+        pybind11::gil_scoped_release no_gil;
+        bool node = false;
+        if (at::GradMode::is_enabled())
+            for (const at::Tensor* t : {x, r, w, b}) node = node || (t != nullptr && t->requires_grad());
+        if (node) {
+            auto out = LayerNorm::apply(*x, optional(r), optional(w), optional(b), c);
+            y = out[0];
+            if (r != nullptr) h = out[1];
+        } else {
+            const at::Tensor none;
+            auto out = norm_forward(*x, r != nullptr ? *r : none, w != nullptr ? *w : none, b != nullptr ? *b : none, c, false);
+            y = out.y; h = out.h;
+        }
+    }
+    if (r == nullptr) return THPVariable_Wrap(std::move(y));
+    return Py_BuildValue("(NN)", THPVariable_Wrap(std::move(y)), THPVariable_Wrap(std::move(h)));
+    END_HANDLE_TH_ERRORS
+}
+
+// log_probs(logits, targets or None, top_k, entropy, ignore_index) -> (log_prob, entropy, top_log_probs, top_indices), or None
+PyObject* py_log_probs(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 5 || !available()) Py_RETURN_NONE;
+    const at::Tensor *x = tensor_arg(args[0]), *targets;
+    int64_t top_k;
+    LogProbs c;
+    if (x == nullptr || !optional_tensor(args[1], &targets) || !int_arg(args[2], &top_k) || !PyBool_Check(args[3]) || !int_arg(args[4], &c.ignore) ||
+        !log_probs_of(*x, targets, top_k, &c))
+        Py_RETURN_NONE;
+    c.entropy = args[3] == Py_True;
+    if (targets == nullptr && top_k == 0 && !c.entropy) Py_RETURN_NONE;
+    at::Tensor out[4];
+    {
+        pybind11::gil_scoped_release no_gil;
+        if (at::GradMode::is_enabled() && x->requires_grad()) {
+            auto list = LogProbsNode::apply(*x, optional(targets), c);
+            size_t at = 0;
+            const bool there[4] = {targets != nullptr, c.entropy, top_k > 0, top_k > 0};
+            for (int i = 0; i < 4; ++i)
+                if (there[i]) out[i] = list[at++];
+        } else {
+            const at::Tensor none;
+            auto r = log_probs_forward(*x, targets != nullptr ? *targets : none, c, false);
+            out[0] = r.log_prob; out[1] = r.entropy; out[2] = r.top; out[3] = r.indices;
+        }
+    }
+    return Py_BuildValue("(NNNN)", wrap_or_none(std::move(out[0])), wrap_or_none(std::move(out[1])), wrap_or_none(std::move(out[2])),
+                         wrap_or_none(std::move(out[3])));
+    END_HANDLE_TH_ERRORS
+}
+
+// The addresses that one step writes to: no two may be equal.
+class Addresses {
+public:
+    explicit Addresses(size_t n) {
+        size_t size = 64;
+        while (size < 4 * n) size *= 2;
+        slots_.assign(size, 0);
+    }
+    bool add(const void* p) { return probe((uintptr_t)p, true); }
+    bool has(const void* p) { return !probe((uintptr_t)p, false); }
+
+private:
+    bool probe(uintptr_t p, bool insert) {      // false: it was there
+        for (size_t i = (p >> 4) * 0x9E3779B97F4A7C15ull >> 20;; ++i) {
+            uintptr_t& slot = slots_[i & (slots_.size() - 1)];
+            if (slot == p) return false;
+            if (slot == 0) {
+                if (insert) slot = p;
+                return true;
+            }
+        }
+    }
+    std::vector<uintptr_t> slots_;
+};
+
+// The items of a list or tuple of exact tensors
+bool tensor_list(PyObject* o, size_t n, std::vector<const at::Tensor*>* out) {
+    if (!PyList_CheckExact(o) && !PyTuple_CheckExact(o)) return false;
+    if ((size_t)PySequence_Fast_GET_SIZE(o) != n) return false;
+    PyObject** items = PySequence_Fast_ITEMS(o);
+    out->resize(n);
+    for (size_t i = 0; i < n; ++i) {
+        PyObject* t = items[i];
+        if (!THPVariable_CheckExact(t)) return false;
+        (*out)[i] = &THPVariable_Unpack(t);
+    }
+    return true;
+}
+
+// A number, or a float32 tensor of one element on the device
+bool scalar_arg(PyObject* o, const at::Device& dev, double* v, const float** device) {
+    *device = nullptr;
+    if (double_arg(o, v)) return true;
+    const at::Tensor* t = tensor_arg(o);
+    if (t == nullptr || !plain(*t) || t->numel() != 1 || t->device() != dev) return false;
+    *v = 0.0;
+    *device = t->const_data_ptr<float>();
+    return true;
+}
+
+// adamw(params, grads, exp_avgs, exp_avg_sqs, steps, lr, beta1, beta2, eps, weight_decay, scales or None, scales or None, grad_scale or None)
+// -> True, or None where nothing was done
+PyObject* py_adamw(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    if (nargs != 13 || !available() || (!PyList_CheckExact(args[0]) && !PyTuple_CheckExact(args[0]))) Py_RETURN_NONE;
+    const size_t n = PySequence_Fast_GET_SIZE(args[0]);
+    std::vector<const at::Tensor*> p, g, m, v, ms, vs, steps;
+    const bool eight = args[10] != Py_None;
+    if (n == 0 || !tensor_list(args[0], n, &p) || !tensor_list(args[1], n, &g) || !tensor_list(args[2], n, &m) || !tensor_list(args[3], n, &v)) Py_RETURN_NONE;
+    if (eight != (args[11] != Py_None) || (eight && (!tensor_list(args[10], n, &ms) || !tensor_list(args[11], n, &vs)))) Py_RETURN_NONE;
+    const at::Tensor* all_steps = tensor_arg(args[4]);
+    if (all_steps == nullptr && !tensor_list(args[4], n, &steps)) Py_RETURN_NONE;
+    const at::Device dev = p[0]->device();
+    const int type = type_code(*p[0]);
+    const at::ScalarType scalar = p[0]->scalar_type(), state = eight ? at::kByte : at::kFloat;
+    double lr, b1, b2, eps, wd;
+    const float *lr_device, *scale_device = nullptr;
+    if (type < 0 || !dev.is_cuda() || !scalar_arg(args[5], dev, &lr, &lr_device) || !double_arg(args[6], &b1) || !double_arg(args[7], &b2) ||
+        !double_arg(args[8], &eps) || !double_arg(args[9], &wd))
+        Py_RETURN_NONE;
+    if (args[12] != Py_None) {
+        double ignored;
+        if (tensor_arg(args[12]) == nullptr || !scalar_arg(args[12], dev, &ignored, &scale_device)) Py_RETURN_NONE;
+    }
+    const auto fits = [&](const at::Tensor& t, at::ScalarType type, const at::Tensor& like) {
+        return unwrapped(t) && t.scalar_type() == type && t.device() == dev && t.is_contiguous() && t.sizes() == like.sizes();
+    };
+    const auto counts = [&](const at::Tensor& t, at::ScalarType type, int64_t count) {
+        return unwrapped(t) && t.scalar_type() == type && t.device() == dev && t.is_contiguous() && t.numel() == count;
+    };
+    if (all_steps != nullptr && (!counts(*all_steps, at::kInt, 2 * (int64_t)n) || all_steps->dim() != 2 || all_steps->size(0) != (int64_t)n)) Py_RETURN_NONE;
+    Addresses written(6 * n);
+    std::vector<adder_b200_adamw_tensor> tensors(n);
+    for (size_t i = 0; i < n; ++i) {
+        const at::Tensor& q = *p[i];
+        if (!fits(q, scalar, q) || !fits(*g[i], scalar, q) || !fits(*m[i], state, q) || !fits(*v[i], state, q)) Py_RETURN_NONE;
+        if (all_steps == nullptr && !counts(*steps[i], at::kInt, 2)) Py_RETURN_NONE;
+        const int64_t count = (q.numel() + 255) / 256;
+        if (eight && (!counts(*ms[i], at::kFloat, count) || !counts(*vs[i], at::kFloat, count))) Py_RETURN_NONE;
+        adder_b200_adamw_tensor& t = tensors[i];
+        t.n = q.numel();
+        if (t.n == 0) continue;
+        t.param = q.data_ptr(); t.grad = g[i]->data_ptr(); t.exp_avg = m[i]->data_ptr(); t.exp_avg_sq = v[i]->data_ptr();
+        t.exp_avg_scale = eight ? ms[i]->data_ptr<float>() : nullptr;
+        t.exp_avg_sq_scale = eight ? vs[i]->data_ptr<float>() : nullptr;
+        t.step = all_steps != nullptr ? all_steps->data_ptr<int>() + 2 * i : steps[i]->data_ptr<int>();
+        if (!written.add(t.param) || !written.add(t.exp_avg) || !written.add(t.exp_avg_sq) || !written.add(t.step) ||
+            (eight && (!written.add(t.exp_avg_scale) || !written.add(t.exp_avg_sq_scale))))
+            Py_RETURN_NONE;
+    }
+    for (const auto& t : tensors)
+        if (t.n > 0 && written.has(t.grad)) Py_RETURN_NONE;
+    {
+        pybind11::gil_scoped_release no_gil;
+        const c10::cuda::CUDAGuard guard(dev);
+        check(api.adamw_step(tensors.data(), (int)n, type, eight ? 8 : 32, lr, lr_device, b1, b2, eps, wd, scale_device,
+                             c10::cuda::getCurrentCUDAStream(dev.index()).stream()), "adder_b200_adamw_step");
+        for (const auto* list : {&p, &m, &v})
+            for (const at::Tensor* t : *list)
+                if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+    }
+    Py_RETURN_TRUE;
+    END_HANDLE_TH_ERRORS
+}
+
 // bind({name: address}, adder module dict, adder_cuda module dict) switches the entry points on, bind(None, ...) off
 PyObject* py_bind(PyObject*, PyObject* const* args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
@@ -519,6 +959,12 @@ PyObject* py_bind(PyObject*, PyObject* const* args, Py_ssize_t n) {
         get("adder_b200_conv_backward_input_with_workspace", &a.conv_backward_input_with_workspace);
         get("adder_b200_conv_backward_weight_workspace_bytes", &a.conv_backward_weight_workspace_bytes);
         get("adder_b200_conv_backward_weight", &a.conv_backward_weight);
+        get("adder_b200_layernorm_forward", &a.layernorm_forward);
+        get("adder_b200_layernorm_backward_workspace_bytes", &a.layernorm_backward_workspace_bytes);
+        get("adder_b200_layernorm_backward", &a.layernorm_backward);
+        get("adder_b200_log_probs_forward", &a.log_probs_forward);
+        get("adder_b200_log_probs_backward", &a.log_probs_backward);
+        get("adder_b200_adamw_step", &a.adamw_step);
         api = a;
     }
     Py_INCREF(args[1]); Py_INCREF(args[2]);
@@ -532,6 +978,7 @@ PyObject* py_bind(PyObject*, PyObject* const* args, Py_ssize_t n) {
 #define ADDER_METHOD(name, fn) {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(fn)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {ADDER_METHOD("bind", py_bind), ADDER_METHOD("layer", py_layer), ADDER_METHOD("conv", py_conv), ADDER_METHOD("layer_with_stats", py_layer_with_stats),
                          ADDER_METHOD("layer_affine", py_layer_affine), ADDER_METHOD("affine", py_affine), ADDER_METHOD("column", py_column),
+                         ADDER_METHOD("layer_norm", py_layer_norm), ADDER_METHOD("log_probs", py_log_probs), ADDER_METHOD("adamw", py_adamw),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_adder_host", nullptr, -1, methods};
 

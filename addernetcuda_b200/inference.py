@@ -7,7 +7,8 @@ What the reference's test.py does around a trained network, without its dataset 
     map it is (running statistics are constants), applied together with the residual add and ReLU of the
     block in ONE kernel behind each adder layer (the adder output is not linear in the weights, so the
     affine map cannot move into them; it becomes the layer's epilogue instead);
-  * `accuracy` / `validate` are test.py:68-126: top-1 / top-5 over batches, no gradients.
+  * `accuracy` / `validate` are test.py:68-126: top-1 / top-5 over batches, no gradients; `evaluate` gives them with the mean loss and
+    entropy from one pass over the logits.
 """
 from __future__ import annotations
 
@@ -17,6 +18,7 @@ import torch
 import torch.nn as nn
 
 from . import _lib, _native, adder_cuda
+from .logprobs import token_log_probs
 
 
 def load_reference_checkpoint(model: nn.Module, state_dict: dict, strict: bool = True):
@@ -104,3 +106,25 @@ def validate(batches: Iterable[Tuple[torch.Tensor, torch.Tensor]], model: nn.Mod
             sums[i] += float(a) * labels.size(0)
         seen += labels.size(0)
     return tuple(s / max(seen, 1) for s in sums)
+
+
+@torch.no_grad()
+def evaluate(batches: Iterable[Tuple[torch.Tensor, torch.Tensor]], model: nn.Module, device=None, topk=(1, 5), ignore_index: int = -100):
+    """Top-k accuracies in percent, mean loss (-log p of the label) and mean entropy of `model`'s (CUDA) outputs over (inputs, labels)
+    batches: one pass over the logits [..., classes] of each batch, one host synchronisation in all.  Equal logits rank by index;
+    labels equal to `ignore_index` do not count."""
+    model.eval()
+    device = device if device is not None else next(model.parameters()).device
+    total = None
+    for inputs, labels in batches:
+        inputs, labels = inputs.to(device, non_blocking=True), labels.to(device, non_blocking=True)
+        out = model(inputs)
+        r = token_log_probs(out, labels, top_k=min(max(topk), out.shape[-1]), entropy=True, ignore_index=ignore_index)
+        counts = labels != ignore_index
+        hit = (r.top_indices == labels.unsqueeze(-1)) & counts.unsqueeze(-1)
+        sums = torch.stack([counts.sum().double(), -r.log_prob.double().sum(), torch.where(counts, r.entropy, 0.0).double().sum(),
+                            *(hit[..., :k].sum().double() for k in topk)])
+        total = sums if total is None else total + sums
+    values = total.tolist() if total is not None else [0.0] * (3 + len(topk))
+    n = max(values[0], 1.0)
+    return {"topk": tuple(100.0 * v / n for v in values[3:]), "loss": values[1] / n, "entropy": values[2] / n}

@@ -1,4 +1,4 @@
-"""Training-step harness: forward, loss, backward, (all-reduce,) SGD step — optionally captured in
+"""Training-step harness: forward, loss, backward, (all-reduce,) SGD or AdamW step — optionally captured in
 one CUDA graph so that the ~300 small kernels of a ResNet-20 step are launched with one call.
 
 It replaces, for benchmarking and parity, the per-batch body of the reference's training loop
@@ -15,7 +15,11 @@ import torch.nn as nn
 
 
 class TrainStep:
-    """One SGD training step on static device buffers.
+    """One training step on static device buffers.
+
+    `optimizer` is "sgd" (with `momentum`), "adamw" or "adamw8" (`optim.AdamW` with states in 32 or 8 bits), or a function of the
+    parameters that returns a torch.optim.Optimizer; `criterion` a module of (logits, labels), nn.CrossEntropyLoss where it is None
+    (`logprobs.TokenCrossEntropy` is this library's own).
 
     step(images, labels) copies the batch into the static buffers (from pinned host memory when the
     inputs are CPU tensors), runs the step (graph replay when `use_graph`), and returns the loss as
@@ -23,7 +27,8 @@ class TrainStep:
     """
 
     def __init__(self, model: nn.Module, batch_shape, num_classes: int, lr: float = 0.1, momentum: float = 0.9,
-                 weight_decay: float = 0.0, ddp=None, use_graph: bool = True, device="cuda:0"):
+                 weight_decay: float = 0.0, ddp=None, use_graph: bool = True, device="cuda:0", optimizer="sgd",
+                 criterion: Optional[nn.Module] = None):
         from . import strict_fp32
         strict_fp32()          # the benchmark configurations are fp32 end to end
         self.model = model
@@ -32,14 +37,25 @@ class TrainStep:
         self.images = torch.zeros(batch_shape, device=self.device)
         self.labels = torch.zeros(batch_shape[0], dtype=torch.long, device=self.device)
         self.num_classes = num_classes
-        self.opt = torch.optim.SGD(model.parameters(), lr=lr, momentum=momentum, weight_decay=weight_decay)
-        self.criterion = nn.CrossEntropyLoss()
+        self.opt = self._make_optimizer(optimizer, lr, momentum, weight_decay)
+        self.criterion = criterion if criterion is not None else nn.CrossEntropyLoss()
         self.loss = torch.zeros((), device=self.device)
         self.logits: Optional[torch.Tensor] = None
         self.use_graph = use_graph
         self.graph: Optional[torch.cuda.CUDAGraph] = None
         self.stream = torch.cuda.Stream(device=self.device)
         self._stage = None      # staging buffers, copy stream and events of prefetch()
+
+    def _make_optimizer(self, kind, lr, momentum, weight_decay):
+        params = self.model.parameters()
+        if callable(kind):
+            return kind(params)
+        if kind == "sgd":
+            return torch.optim.SGD(params, lr=lr, momentum=momentum, weight_decay=weight_decay)
+        if kind in ("adamw", "adamw8"):
+            from .optim import AdamW
+            return AdamW(params, lr=lr, weight_decay=weight_decay, state_bits=8 if kind == "adamw8" else 32)
+        raise ValueError(f'optimizer must be "sgd", "adamw", "adamw8" or a function of the parameters, got {kind!r}')
 
     def _body(self, update: bool = True) -> None:
         if self.ddp is not None:

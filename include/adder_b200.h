@@ -238,6 +238,87 @@ ADDER_API int adder_b200_forward_affine(const float* x, const float* w, const fl
                                         const float* residual, int relu, float* out, int n, int ci, int h, int wd,
                                         int co, int k, int stride, int pad, void* stream);
 
+/* ---- around the network: layer norm, log probabilities, the optimizer step --------------------------
+ * Operators of token models beside the batch norm, the loss and the SGD step of the reference's training loop
+ * (main.py:86-101); no reference counterpart.  Element types are ADDER_TYPE_*; everything is computed in fp32. */
+#define ADDER_TYPE_F32 0
+#define ADDER_TYPE_BF16 1
+#define ADDER_TYPE_F16 2
+
+/* Layer norm of `rows` rows of d elements of type dtype, with the sum of a residual stream before it:
+ *   h = x + residual, rounded to the type (h = x where residual is NULL);  y = (h - mean) / sqrt(var + eps) * weight + bias
+ * x and residual have x_stride and residual_stride elements from row to row; y and h (written where there is a residual) are
+ * contiguous.  weight and bias [d] are of weight_dtype, the same type or fp32, and may be NULL (1 and 0).  mean and rstd [rows], for the
+ * backward call, may be NULL together.  Any alignment that the types need; 16-byte aligned rows run faster. */
+ADDER_API int adder_b200_layernorm_forward(const void* x, const void* residual, const void* weight, const void* bias, void* y, void* h,
+                                           float* mean, float* rstd, long long rows, long long d, long long x_stride,
+                                           long long residual_stride, int dtype, int weight_dtype, float eps, void* stream);
+
+/* Gradients from dy (and dh, that of h itself, or NULL): dx [rows][d], which is the gradient of x and of the residual, and
+ * dweight, dbias [d], sums over the rows in an order that depends on the sizes alone.  Each of the three may be NULL.  dy, dh and dx are
+ * contiguous, h (x where there was no residual) has h_stride.  The workspace serves dweight and dbias. */
+ADDER_API size_t adder_b200_layernorm_backward_workspace_bytes(long long rows, long long d);
+ADDER_API int adder_b200_layernorm_backward(const void* dy, const void* dh, const void* h, const void* weight, const float* mean,
+                                            const float* rstd, void* dx, void* dweight, void* dbias, void* workspace,
+                                            size_t workspace_bytes, long long rows, long long d, long long h_stride, int dtype,
+                                            int weight_dtype, void* stream);
+
+/* Of each row of logits (rows x classes of type dtype, row_stride elements from row to row, consecutive within one; any alignment
+ * that the type needs), in fp32:
+ *   log_prob[row]  log softmax at targets[row]: 0 where the target is ignore_index, NaN where it is no class
+ *   entropy[row]   -sum p log p
+ *   top_log_probs, top_indices [row][top_k]  the top_k <= 32 largest, equal logits by index from the lowest
+ *   stats[row][2]  the row's maximum and the log of its sum of exponentials relative to it, for the backward call
+ * Outputs that are NULL are left out (targets may be NULL where log_prob is; the top ones go with top_k).  A row of nothing but
+ * -inf has log probabilities of -inf, entropy 0 and the first indices; one with a NaN or +inf gives NaN and indices of -1. */
+ADDER_API int adder_b200_log_probs_forward(const void* logits, int dtype, long long rows, long long classes, long long row_stride,
+                                           const long long* targets, long long ignore_index, int top_k, float* log_prob,
+                                           float* entropy, float* stats, float* top_log_probs, long long* top_indices, void* stream);
+
+/* grad_logits (contiguous, of the logits' type) <- the gradient of sum(grad_log_prob * log_prob + grad_entropy * entropy +
+ * grad_top * top_log_probs), from the forward's inputs, stats, entropy and top_indices.  Gradients that are NULL count as zeros.  Rows of
+ * nothing but -inf get zeros; rows with a NaN, or whose target is no class while grad_log_prob is given, NaN. */
+ADDER_API int adder_b200_log_probs_backward(const void* logits, int dtype, long long rows, long long classes, long long row_stride,
+                                            const long long* targets, long long ignore_index, int top_k, const long long* top_indices,
+                                            const float* stats, const float* entropy, const float* grad_log_prob,
+                                            const float* grad_entropy, const float* grad_top, void* grad_logits, void* stream);
+
+/* One tensor of an optimizer step: n elements, all pointers to device memory.
+ * param and grad have the step's element type; exp_avg and exp_avg_sq are fp32, or with 8-bit states one code a value with a scale for
+ * each 256 consecutive values (ceil(n / 256) of them; NULL with 32-bit states).  step points to two ints: the steps that this tensor
+ * has taken, which the call counts up, and a word that is 0 before and after it. */
+typedef struct {
+    void* param;
+    const void* grad;
+    void* exp_avg;
+    void* exp_avg_sq;
+    float* exp_avg_scale;
+    float* exp_avg_sq_scale;
+    int* step;
+    long long n;
+} adder_b200_adamw_tensor;
+
+/* One AdamW step over `count` tensors (a host array, read before the call returns), t = steps taken + 1:
+ *   g <- grad * grad_scale;  m <- beta1 m + (1 - beta1) g;  v <- beta2 v + (1 - beta2) g^2
+ *   p <- p (1 - lr weight_decay) - lr / (1 - beta1^t) * m / (sqrt(v / (1 - beta2^t)) + eps)
+ * lr_device and grad_scale, where not NULL, are one fp32 value each in device memory that is read when the kernel runs (lr then being
+ * ignored), so that a captured step follows a schedule.  state_bits is 32 or 8.
+ * 8-bit states: a block of 256 values is stored relative to its largest magnitude, which has the top code.  The code of a magnitude a is
+ * bits 19 and up of the fp32 number a * (1 / largest * top) * 2^-127, rounded to nearest even, and its block's scale is
+ * largest * (1 / top), every operation rounded to fp32: m has a sign and 3 exponent and 4 fraction bits (top = 248, codes 0-127, +128
+ * where negative), v 4 and 4 (top = 63488; code 1 at least where v > 0, so that no update is divided by a zero that was none).
+ * The update itself uses m and v as they were before they were stored.  Blocks whose largest value is below 2^-100 are stored as
+ * zeros; a block with a NaN or an infinity has no finite values any more.
+ * The buffers of different tensors must not overlap, nor the parameter, state and step buffers of one (a gradient may be shared).
+ * Any alignment that the element type needs will do. */
+ADDER_API int adder_b200_adamw_step(const adder_b200_adamw_tensor* tensors, int count, int dtype, int state_bits, double lr,
+                                    const float* lr_device, double beta1, double beta2, double eps, double weight_decay,
+                                    const float* grad_scale, void* stream);
+
+/* values[n] <- what 8-bit codes with their scales stand for (is_signed: those of m, else of v). */
+ADDER_API int adder_b200_adamw_state_values(const unsigned char* codes, const float* scales, int is_signed, float* values, long long n,
+                                            void* stream);
+
 /* Kernels that wait for the copy engine do so with a bounded number of polls; a wait that runs out sets a
  * flag on the device and the kernel returns early (its output is then garbage).  This reads the flag of the
  * current device into *status (0 = never happened) and, with reset != 0, clears it.  Synchronises with

@@ -1,0 +1,310 @@
+"""Layer norm (with the sum of a residual stream) against float64: outputs, statistics of what is stored, all gradients.
+
+Tolerances count roundings.  An output of type T is rounded once: half a step, u_T |value| with u = eps / 2.  Before that come fp32
+operations; sums are trees or up to D / 32 terms in sequence, whose rounding errors add up like a walk of sqrt(D / 32) steps, so
+K = 64 + 4 sqrt(D) roundings of 2^-24 relative to the largest terms that meet in the value are allowed (4: a factor for luck).
+"""
+import itertools
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+U = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+TINY = {torch.float32: 0.0, torch.bfloat16: 0.0, torch.float16: 2.0 ** -25}      # half a step of fp16's subnormal numbers
+
+
+def _inputs(rows, shape, dtype, wtype, residual, seed=0, mean=0.3):
+    torch.manual_seed(seed)
+    full = (rows, *shape)
+    x = (torch.randn(full) * 1.5 + mean).to(dtype).to(DEV)
+    r = torch.randn(full).to(dtype).to(DEV) if residual else None
+    w = (1 + 0.2 * torch.randn(shape)).to(wtype).to(DEV)
+    b = (0.2 * torch.randn(shape)).to(wtype).to(DEV)
+    dy, dh = torch.randn(full).to(dtype).to(DEV), torch.randn(full).to(dtype).to(DEV)
+    return x, r, w, b, dy, dh
+
+
+def _exact(x, r, w, b, dy, dh, eps):
+    """float64: y, h, dh_total, dw, db, and the scale that the roundings of each are relative to."""
+    rows = x.shape[0]
+    h = x if r is None else (x.double() + r.double()).to(x.dtype)
+    d = h.numel() // max(rows, 1)
+    hd = h.double().reshape(rows, d)
+    wd = w.double().reshape(d) if w is not None else torch.ones(d, dtype=torch.float64, device=x.device)
+    bd = b.double().reshape(d) if b is not None else torch.zeros(d, dtype=torch.float64, device=x.device)
+    mu = hd.mean(1, keepdim=True)
+    rs = 1 / ((hd - mu).square().mean(1, keepdim=True) + eps).sqrt()
+    xh = (hd - mu) * rs
+    y = xh * wd + bd
+    k = (64 + 4 * math.sqrt(d)) * 2.0 ** -24
+    e_xh = k * (hd.abs().amax(1, keepdim=True) * rs + xh.abs())          # error of a normalised value
+    out = {"h": h, "y": (y.reshape(x.shape), (e_xh * wd.abs() + k * bd.abs()).reshape(x.shape))}
+    if dy is not None:
+        dyd = dy.double().reshape(rows, d)
+        g = dyd * wd
+        m1, m2 = g.mean(1, keepdim=True), (g * xh).mean(1, keepdim=True)
+        dx = rs * (g - m1 - xh * m2)
+        big = rs * g.abs().amax(1, keepdim=True)
+        e_dx = k * big * (2 + xh.abs()) + big * e_xh * (1 + xh.abs())
+        if dh is not None:
+            dx = dx + dh.double().reshape(rows, d)
+            e_dx = e_dx + 2.0 ** -24 * dx.abs()
+        kr = (64 + 4 * math.sqrt(rows)) * 2.0 ** -24
+        dw, e_dw = (dyd * xh).sum(0), (dyd.abs() * (e_xh + kr * xh.abs())).sum(0)
+        db, e_db = dyd.sum(0), kr * dyd.abs().sum(0)
+        shape = x.shape[1:]
+        out |= {"dx": (dx.reshape(x.shape), e_dx.reshape(x.shape)), "dw": (dw.reshape(shape), e_dw.reshape(shape)),
+                "db": (db.reshape(shape), e_db.reshape(shape))}
+    return out
+
+
+def _near(name, got, want, err):
+    u, tiny = U[got.dtype], TINY[got.dtype]
+    off = (got.double() - want).abs()
+    limit = u * (want.abs() + err) + tiny + err
+    assert got.shape == want.shape, name
+    assert bool((off <= limit).all()), f"{name}: off by {float(off.max()):.3e}, {float((off / limit.clamp(min=1e-300)).max()):.2f} of what is allowed"
+
+
+def _run(x, r, w, b, dy, dh, eps=1e-5, shape=None):
+    from addernetcuda_b200.layernorm import layer_norm
+    leaves = [t.detach().requires_grad_() if t is not None else None for t in (x, r, w, b)]
+    out = layer_norm(leaves[0], shape or tuple(x.shape[1:]), leaves[2], leaves[3], eps, residual=leaves[1])
+    outs, gs = (list(out), [dy, dh]) if r is not None else ([out], [dy])
+    grads = torch.autograd.grad(outs, [t for t in leaves if t is not None], gs)
+    return outs, list(grads)
+
+
+WIDTHS = [1, 2, 3, 8, 31, 33, 64, 127, 128, 250, 256, 257, 511, 512, 520, 1001, 1024, 1032, 2047, 2048, 2056, 4095, 4096, 4104, 8192, 8193,
+          8200, 16384, 16392, 16385]
+
+
+@pytest.mark.parametrize("width", WIDTHS)
+@pytest.mark.parametrize("dtype,wtype", [(torch.float32, torch.float32), (torch.bfloat16, torch.bfloat16), (torch.bfloat16, torch.float32),
+                                         (torch.float16, torch.float16)], ids=str)
+def test_forward_and_gradients(width, dtype, wtype):
+    for rows, residual in ((5, False), (3, True)):
+        x, r, w, b, dy, dh = _inputs(rows, (width,), dtype, wtype, residual, seed=width + rows)
+        outs, grads = _run(x, r, w, b, dy, dh)
+        want = _exact(x, r, w, b, dy, dh if residual else None, 1e-5)
+        _near("y", outs[0], *want["y"])
+        if residual:
+            assert torch.equal(outs[1], want["h"])
+            assert torch.equal(grads[0], grads[1])
+        _near("dx", grads[0], *want["dx"])
+        _near("dw", grads[-2], *want["dw"])
+        _near("db", grads[-1], *want["db"])
+
+
+@pytest.mark.parametrize("rows", [1, 2, 7, 148, 297, 1023, 4099])
+@pytest.mark.parametrize("width", [24, 384, 1001, 2048])
+def test_sums_over_rows(rows, width):
+    x, r, w, b, dy, dh = _inputs(rows, (width,), torch.bfloat16, torch.float32, False, seed=rows)
+    _, grads = _run(x, r, w, b, dy, dh)
+    want = _exact(x, r, w, b, dy, None, 1e-5)
+    for name, g in zip(("dx", "dw", "db"), grads):
+        _near(name, g, *want[name])
+    again = _run(x, r, w, b, dy, dh)[1]
+    assert all(torch.equal(a, c) for a, c in zip(grads, again))      # one order of addition
+
+
+@pytest.mark.parametrize("width", [16400, 32768, 50176, 65544, 131071, 300000])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+def test_rows_longer_than_a_block_holds(width, dtype):
+    for rows, residual in ((3, True), (64, False)):
+        x, r, w, b, dy, dh = _inputs(rows, (width,), dtype, torch.float32, residual, seed=width)
+        outs, grads = _run(x, r, w, b, dy, dh)
+        want = _exact(x, r, w, b, dy, dh if residual else None, 1e-5)
+        _near("y", outs[0], *want["y"])
+        _near("dx", grads[0], *want["dx"])
+        _near("dw", grads[-2], *want["dw"])
+        _near("db", grads[-1], *want["db"])
+
+
+def test_images_normalised_as_a_whole_and_other_ranks():
+    from addernetcuda_b200.layernorm import FusedLayerNorm, layer_norm
+    x, _, w, b, dy, _ = _inputs(6, (16, 7, 5), torch.float32, torch.float32, False)
+    outs, grads = _run(x, None, w, b, dy, None)
+    want = _exact(x, None, w, b, dy, None, 1e-5)
+    _near("y", outs[0], *want["y"])
+    for name, g in zip(("dx", "dw", "db"), grads):
+        _near(name, g, *want[name])
+    m = FusedLayerNorm((16, 7, 5)).to(DEV)
+    with torch.no_grad():
+        m.weight.copy_(w); m.bias.copy_(b)
+    assert torch.equal(m(x), outs[0])
+    # memory in another order, and leading axes
+    assert torch.equal(m(x.to(memory_format=torch.channels_last)), outs[0])
+    lead = x.reshape(2, 3, 16, 7, 5)
+    assert torch.equal(layer_norm(lead, (16, 7, 5), w, b), outs[0].reshape(lead.shape))
+    flat = x.reshape(-1, 5)
+    assert layer_norm(flat, 5).shape == flat.shape and layer_norm(flat[0], 5).shape == (5,)
+    assert layer_norm(x[:0], (16, 7, 5), w, b).shape == (0, 16, 7, 5)
+
+
+@pytest.mark.parametrize("given", list(itertools.product([False, True], [False, True])), ids=str)
+def test_weight_and_bias_may_be_left_out(given):
+    for width in (40, 1001, 20000):
+        x, r, w, b, dy, dh = _inputs(4, (width,), torch.float32, torch.float32, True)
+        w, b = w if given[0] else None, b if given[1] else None
+        outs, grads = _run(x, r, w, b, dy, dh)
+        want = _exact(x, r, w, b, dy, dh, 1e-5)
+        _near("y", outs[0], *want["y"])
+        _near("dx", grads[0], *want["dx"])
+        for name, g in zip((["dw"] if given[0] else []) + (["db"] if given[1] else []), grads[2:]):
+            _near(name, g, *want[name])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+def test_views_strides_and_alignment(dtype):
+    """Rows apart from one another, a base that is not 16-byte aligned, an expanded row, a transposed matrix."""
+    from addernetcuda_b200.layernorm import layer_norm
+    for width in (64, 1000, 33000):
+        buf = torch.randn(5, width + 24, device=DEV).to(dtype)
+        w, b = torch.rand(width, device=DEV) + 0.5, torch.randn(width, device=DEV)
+        for x in (buf[:, :width], buf[:, 8:8 + width], buf[:, 1:1 + width], buf[::2, 3:3 + width], buf[:1, :width].expand(4, width),
+                  buf[:, :width].t().contiguous().t()):
+            dense = x.clone(memory_format=torch.contiguous_format)
+            xv, xd = x.detach().requires_grad_(), dense.requires_grad_()
+            y, yd = layer_norm(xv, width, w, b), layer_norm(xd, width, w, b)
+            want = _exact(dense.detach(), None, w, b, torch.ones_like(dense), None, 1e-5)
+            _near("y", y, *want["y"])
+            _near("y dense", yd, *want["y"])
+            g = torch.randn_like(dense)
+            a, c = torch.autograd.grad(y, xv, g)[0], torch.autograd.grad(yd, xd, g)[0]
+            want = _exact(dense.detach(), None, w, b, g, None, 1e-5)
+            _near("dx", a, *want["dx"])
+            _near("dx dense", c, *want["dx"])
+
+
+def test_only_the_gradients_that_are_needed():
+    from addernetcuda_b200.layernorm import layer_norm
+    x, r, w, b, dy, dh = _inputs(9, (136,), torch.float32, torch.float32, True)
+    want = _exact(x, r, w, b, dy, dh, 1e-5)
+    names = ("dx", "dx", "dw", "db")
+    for i in range(4):
+        leaves = [t.detach().requires_grad_(i == j) for j, t in enumerate((x, r, w, b))]
+        y, h = layer_norm(leaves[0], 136, leaves[2], leaves[3], residual=leaves[1])
+        g = torch.autograd.grad([y, h], leaves[i], [dy, dh]) if i < 2 else torch.autograd.grad(y, leaves[i], dy)
+        _near(names[i], g[0], *want[names[i]])
+    # only h is used: the norm's part is zero
+    xr = x.detach().requires_grad_()
+    _, h = layer_norm(xr, 136, w, b, residual=r)
+    assert torch.equal(torch.autograd.grad(h, xr, dh)[0], dh)
+    # only y
+    xr = x.detach().requires_grad_()
+    y, _ = layer_norm(xr, 136, w, b, residual=r)
+    _near("dx", torch.autograd.grad(y, xr, dy)[0], *_exact(x, r, w, b, dy, None, 1e-5)["dx"])
+
+
+def test_gradient_against_differences():
+    """Central differences of the float64 formula at the kernel's inputs: an independent check of the formulas above."""
+    from addernetcuda_b200.layernorm import layer_norm
+    torch.manual_seed(1)
+    x, w, b, dy = torch.randn(2, 12), torch.rand(12) + 0.5, torch.randn(12), torch.randn(2, 12)
+    xg = x.to(DEV).requires_grad_()
+    got = torch.autograd.grad(layer_norm(xg, 12, w.to(DEV), b.to(DEV)), xg, dy.to(DEV))[0].double().cpu()
+
+    def loss(v):
+        c = v - v.mean(1, keepdim=True)
+        return ((c / (c.square().mean(1, keepdim=True) + 1e-5).sqrt() * w.double() + b.double()) * dy.double()).sum()
+
+    e = 1e-5
+    for i in range(2):
+        for j in range(12):
+            v = x.double()
+            v[i, j] += e
+            up = loss(v)
+            v[i, j] -= 2 * e
+            assert abs(float(got[i, j]) - float((up - loss(v)) / (2 * e))) < 1e-5 * 10      # fp32 roundings of a dozen terms of size 3
+
+
+def test_constant_rows_large_means_and_non_finite_rows():
+    from addernetcuda_b200.layernorm import layer_norm
+    for width in (16, 1001, 2048, 20000):
+        w, b = torch.rand(width, device=DEV) + 0.5, torch.randn(width, device=DEV)
+        x = torch.full((3, width), 7.25, device=DEV)
+        assert torch.equal(layer_norm(x, width, w, b), b.expand(3, width))      # variance 0: 7.25 sums exactly at these widths
+        x, _, w, b, dy, _ = _inputs(3, (width,), torch.float32, torch.float32, False, mean=1000.0)
+        outs, grads = _run(x, None, w, b, dy, None)
+        want = _exact(x, None, w, b, dy, None, 1e-5)
+        _near("y", outs[0], *want["y"])
+        _near("dx", grads[0], *want["dx"])
+        x[1, width // 2] = float("nan")
+        x[2, 0] = float("inf")
+        y = layer_norm(x, width, w, b)
+        assert bool(y[0].isfinite().all()) and bool(y[1].isnan().all()) and bool(y[2].isnan().all())
+
+
+def test_refusals():
+    from addernetcuda_b200.layernorm import layer_norm
+    x = torch.randn(4, 8, device=DEV)
+    w = torch.ones(8, device=DEV)
+    with pytest.raises(ValueError, match="last axes"):
+        layer_norm(x, 9)
+    with pytest.raises(ValueError, match="last axes"):
+        layer_norm(x, (2, 4, 8))
+    with pytest.raises(ValueError, match="last axes"):
+        layer_norm(x[:, :0], 0)
+    with pytest.raises(ValueError, match="weight has shape"):
+        layer_norm(x, 8, w[:4])
+    with pytest.raises(TypeError, match="weight must be"):
+        layer_norm(x, 8, w.half())
+    with pytest.raises(TypeError, match="one type"):
+        layer_norm(x.bfloat16(), 8, w, w.bfloat16())
+    with pytest.raises(TypeError, match="float32, bfloat16 or float16"):
+        layer_norm(x.double(), 8)
+    with pytest.raises(ValueError, match="residual must have"):
+        layer_norm(x, 8, residual=x[:2])
+    with pytest.raises(ValueError, match="residual must have"):
+        layer_norm(x, 8, residual=x.half())
+    with pytest.raises(RuntimeError, match="CUDA"):
+        layer_norm(x, 8, w.cpu())
+    with pytest.raises(ValueError, match="eps"):
+        layer_norm(x, 8, eps=-1.0)
+    xr = x.requires_grad_()
+    g, = torch.autograd.grad(layer_norm(xr, 8).square().sum(), xr, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
+
+
+def test_without_the_host_path_the_results_are_the_same(monkeypatch):
+    from addernetcuda_b200 import _native
+    for width in (24, 1001, 2048, 20000):
+        for residual in (False, True):
+            args = _inputs(5, (width,), torch.bfloat16, torch.float32, residual)
+            outs, grads = _run(*args)
+            with monkeypatch.context() as m:
+                m.setattr(_native, "layer_norm", _native._absent)
+                outs2, grads2 = _run(*args)
+            assert all(torch.equal(a, c) for a, c in zip(outs + grads, outs2 + grads2))
+
+
+def test_streams_and_captured_replays():
+    from addernetcuda_b200.layernorm import layer_norm
+    x, r, w, b, dy, dh = _inputs(64, (512,), torch.bfloat16, torch.float32, True)
+    want = _run(x, r, w, b, dy, dh)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = _run(x, r, w, b, dy, dh)
+    side.synchronize()
+    assert all(torch.equal(a, c) for a, c in zip(want[0] + want[1], got[0] + got[1]))
+    xs, ws = x.clone(), w.clone()
+    graphs = []
+    for _ in range(2):      # two captured calls, replayed in either order
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = _run(xs, r, ws, b, dy, dh)
+        graphs.append((g, out))
+    for x2, order in ((x, (0, 1)), (x.flip(0).contiguous(), (1, 0))):
+        xs.copy_(x2)
+        for i in order:
+            graphs[i][0].replay()
+        torch.cuda.synchronize()
+        want = _run(x2, r, w, b, dy, dh)
+        for _, out in graphs:
+            assert all(torch.equal(a, c) for a, c in zip(want[0] + want[1], out[0] + out[1]))
