@@ -21,6 +21,7 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int LP_MAX_K = 32;
+constexpr int LP_TEAM = 256;            // threads of a CTA that has a row, or a part of one, to itself
 constexpr int LP_UNROLL = 4;            // vectors that a thread has in flight
 constexpr float LP_FLOOR = -200.f;      // 2^-200 is 0 in fp32: stands for exponents of -inf where 0 * -inf would be NaN
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
@@ -78,7 +79,7 @@ struct LpFwd {
     long long ignore;
     float* log_prob;      // may be null, as all of the following
     float* entropy;
-    float* stats;         // [rows][2]: M, ln s
+    float* stats;         // [rows][2]: M, s
     float* top_log_probs;
     long long* top_indices;
 };
@@ -126,9 +127,118 @@ template <int THREADS, class Shared> __device__ __forceinline__ uint64_t team_to
     return key;
 }
 
+template <class T> __device__ __forceinline__ uint32_t max_pair(uint32_t a, uint32_t b);
+template <> __device__ __forceinline__ uint32_t max_pair<__nv_bfloat16>(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+template <> __device__ __forceinline__ uint32_t max_pair<__half>(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+// The largest of a vector's values, NaN if one is: as a word of its type, so that 16-bit values are compared in pairs.
+template <class T> __device__ __forceinline__ uint32_t max_word(uint32_t a, uint32_t b) {
+    if constexpr (sizeof(T) == 4) return __float_as_uint(max_nan(__uint_as_float(a), __uint_as_float(b)));
+    else return max_pair<T>(a, b);
+}
+template <class T> __device__ __forceinline__ float word_max(uint32_t w) {
+    if constexpr (sizeof(T) == 4) {
+        return __uint_as_float(w);
+    } else {
+        const float2 p = unpack_pair<T>(w);
+        return max_nan(p.x, p.y);
+    }
+}
+
+// A thread's maximum m with s = sum 2^d and t = sum 2^d d over its values x, d = x log2(e) - ref.  ref is m log2(e) rounded (one fused
+// multiply-add a value); what it was rounded by is kept in `res` and comes off at the end.  Beyond |m| = 8192, where the rounding is no longer
+// small, d is (x - m) log2(e).
+template <bool ENTROPY> struct Running {
+    float m = -INFINITY, ref = 0.f, res = 0.f;
+    uint64_t s = 0, t = 0;      // pairs of fp32 sums
+
+    __device__ __forceinline__ bool small() const { return fabsf(m) < 8192.f; }
+    __device__ __forceinline__ void shift(float d) {
+        d = fmaxf(d, LP_FLOOR);
+        const float f = exp2_fast(d);
+        const uint64_t f2 = pack2(f, f);
+        if (ENTROPY) t = fma2(fma2(s, pack2(d, d), t), f2, 0);
+        s = fma2(s, f2, 0);
+    }
+    __device__ __forceinline__ void raise(float top) {
+        const float ref_new = top * LOG2E, res_new = fabsf(top) < 8192.f ? fmaf(top, LOG2E, -ref_new) : 0.f;
+        shift((m - top) * LOG2E + (res_new - res));
+        m = top; ref = ref_new; res = res_new;
+    }
+    // N values (N even), the largest of which is `top`
+    template <int N> __device__ __forceinline__ void take(const float (&f)[N], float top) {
+        if (top > m) raise(top);
+        if (m == -INFINITY && top == -INFINITY) return;      // nothing so far
+        if (small()) {
+            const uint64_t scale = pack2(LOG2E, LOG2E), minus = pack2(-ref, -ref);
+#pragma unroll
+            for (int i = 0; i < N; i += 2) add(fma2(pack2(f[i], f[i + 1]), scale, minus));
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; i += 2) add(pack2((f[i] - m) * LOG2E, (f[i + 1] - m) * LOG2E));
+        }
+    }
+    __device__ __forceinline__ void add(uint64_t pair) {
+        float d0, d1;
+        unpack2(pair, d0, d1);
+        if (ENTROPY) { d0 = max_nan(d0, LP_FLOOR); d1 = max_nan(d1, LP_FLOOR); }
+        const uint64_t e = pack2(exp2_fast(d0), exp2_fast(d1));
+        s = add2(s, e);
+        if (ENTROPY) t = fma2(e, pack2(d0, d1), t);
+    }
+    // Sums relative to m itself
+    __device__ __forceinline__ void finish(float* sum, float* dot) {
+        float a, b;
+        unpack2(s, a, b);
+        const float all = a + b;
+        unpack2(t, a, b);
+        const float f = exp2f(-res);
+        *sum = all * f;
+        *dot = ENTROPY ? ((a + b) - all * res) * f : 0.f;
+    }
+};
+
+// U vectors of a thread, THREADS apart from the v-th on: their values into the running sums, their maximum into `best`.
+template <class T, int THREADS, int U, bool ENTROPY, bool TOP>
+__device__ __forceinline__ void take_vectors(const uint4* vec, int v, Running<ENTROPY>& run, float& best, int& best_vec) {
+    constexpr int VE = Vec16<T>::N;
+    uint4 q[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) q[u] = __ldg(vec + v + u * THREADS);
+    uint32_t w[U], all;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        w[u] = max_word<T>(max_word<T>(q[u].x, q[u].y), max_word<T>(q[u].z, q[u].w));
+        all = u == 0 ? w[0] : max_word<T>(all, w[u]);
+    }
+    const float top = word_max<T>(all);
+    if (TOP && top > best) {
+        best = top;
+#pragma unroll
+        for (int u = U - 1; u >= 0; --u)
+            if (word_max<T>(w[u]) == top) best_vec = v + u * THREADS;
+    }
+    float f[U * VE];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        float g[VE];
+        Vec16<T>::unpack(q[u], g);
+#pragma unroll
+        for (int i = 0; i < VE; ++i) f[u * VE + i] = g[i];
+    }
+    run.take(f, top);
+}
+
 // grid: rows (times the cluster's size), or rows / 4 with a warp a row
 template <class T, int THREADS, bool CLUSTER, bool ENTROPY, bool TOP>
-__global__ void __launch_bounds__(THREADS == 32 ? 128 : THREADS) lp_forward_kernel(const LpFwd a) {
+__global__ void __launch_bounds__(THREADS == 32 ? 128 : THREADS, THREADS == 32 ? 8 : 1024 / THREADS) lp_forward_kernel(const LpFwd a) {
     constexpr int VE = Vec16<T>::N;
     constexpr int TEAMS = THREADS == 32 ? 4 : 1;
     constexpr int LIST = TOP ? THREADS * VE + 2 * VE : 1;
@@ -156,64 +266,18 @@ __global__ void __launch_bounds__(THREADS == 32 ? 128 : THREADS) lp_forward_kern
     const uint4* vec = reinterpret_cast<const uint4*>(x + head);
     const auto single_index = [&](int i) { return i < head ? i : i + nvec * VE; };
 
-    float m = -INFINITY, s = 0.f, tt = 0.f;
+    Running<ENTROPY> run;
     float best = -INFINITY;
     int best_vec = v0 + t;
-    const auto take = [&](float (&f)[VE * LP_UNROLL], int n, float top) {
-        if (top > m) {
-            const float d = fmaxf((m - top) * LOG2E, LP_FLOOR), scale = exp2_fast(d);
-            if (ENTROPY) tt = (tt + s * d) * scale;
-            s *= scale;
-            m = top;
-        }
-        if (m == -INFINITY && top == -INFINITY) return;      // nothing so far
-#pragma unroll
-        for (int i = 0; i < VE * LP_UNROLL; ++i) {
-            if (i >= n) break;
-            float d = (f[i] - m) * LOG2E;
-            if (ENTROPY) d = max_nan(d, LP_FLOOR);
-            const float e = exp2_fast(d);
-            s += e;
-            if (ENTROPY) tt = fmaf(e, d, tt);
-        }
-    };
-    for (int v = v0 + t; v < v1; v += THREADS * LP_UNROLL) {
-        float f[VE * LP_UNROLL];
-        uint4 q[LP_UNROLL];
-#pragma unroll
-        for (int u = 0; u < LP_UNROLL; ++u)
-            if (v + u * THREADS < v1) q[u] = __ldg(vec + v + u * THREADS);
-        float vm[LP_UNROLL], top = -INFINITY;
-        int there = 0;
-#pragma unroll
-        for (int u = 0; u < LP_UNROLL; ++u) {
-            vm[u] = -INFINITY;
-            if (v + u * THREADS < v1) {
-                float g[VE];
-                Vec16<T>::unpack(q[u], g);
-                vm[u] = g[0];
-#pragma unroll
-                for (int i = 0; i < VE; ++i) {
-                    f[u * VE + i] = g[i];
-                    if (i > 0) vm[u] = max_nan(vm[u], g[i]);
-                }
-                top = max_nan(top, vm[u]);
-                there = (u + 1) * VE;
-            }
-        }
-        if (TOP && top > best) {
-            best = top;
-#pragma unroll
-            for (int u = LP_UNROLL - 1; u >= 0; --u)
-                if (vm[u] == top) best_vec = v + u * THREADS;
-        }
-        take(f, there, top);
-    }
+    int v = v0 + t;
+    for (; v + (LP_UNROLL - 1) * THREADS < v1; v += THREADS * LP_UNROLL) take_vectors<T, THREADS, LP_UNROLL, ENTROPY, TOP>(vec, v, run, best, best_vec);
+    for (; v < v1; v += THREADS) take_vectors<T, THREADS, 1, ENTROPY, TOP>(vec, v, run, best, best_vec);
     if (t < singles) {
-        float f[VE * LP_UNROLL];
-        f[0] = to_float(x[single_index(t)]);
-        take(f, 1, f[0]);
+        const float f[2] = {to_float(x[single_index(t)]), -INFINITY};
+        run.take(f, f[0]);
     }
+    float m = run.m, s, tt;
+    run.finish(&s, &tt);
 
     // ---- the team's sums
 #pragma unroll
@@ -316,8 +380,8 @@ __global__ void __launch_bounds__(THREADS == 32 ? 128 : THREADS) lp_forward_kern
     const float ln_s = nothing ? 0.f : logf(s);
     if (t == 0) {
         if (a.stats != nullptr) {
-            a.stats[2 * row] = broken ? s : m;
-            a.stats[2 * row + 1] = ln_s;
+            a.stats[2 * row] = m;
+            a.stats[2 * row + 1] = s;
         }
         if (a.log_prob != nullptr) {
             const long long target = a.targets[row];
@@ -353,73 +417,114 @@ struct LpBwd {
     int segments;                 // parts of a row, each a CTA's (or warp's)
 };
 
+// The slope of a row's sum with respect to its logits, without what the selected classes add: -p (G + gH (log p + H)) with
+// p = 2^(x log2(e) - ref) scale, so that a value takes one fused multiply-add before its exponential.  What ref is rounded by is in
+// `scale` and `shift`; beyond |M| = 8192, where that is no longer small, M is subtracted first.
+template <bool ENTROPY> struct Slope {
+    float minus, ref, scale, g_ent, shift, sum;      // scale: -G / s, or -1 / s with an entropy
+    bool nothing;
+
+    __device__ __forceinline__ void set(float m, float s, float sum_, float g_ent_, float h) {
+        nothing = s == 0.f;
+        const bool small = fabsf(m) < 8192.f;
+        minus = small ? 0.f : m;
+        ref = small ? m * LOG2E : 0.f;
+        const float res = small ? fmaf(m, LOG2E, -ref) : 0.f;
+        sum = sum_; g_ent = g_ent_;
+        scale = -exp2f(-res) / s * (ENTROPY ? 1.f : sum);
+        shift = ENTROPY ? h - logf(s) - res * LN2 : 0.f;
+    }
+    // `far`: M is subtracted first
+    __device__ __forceinline__ uint64_t pair(float a, float b, bool far) const {
+        const uint64_t x = far ? add2(pack2(a, b), pack2(-minus, -minus)) : pack2(a, b);
+        float d0, d1;
+        unpack2(fma2(x, pack2(LOG2E, LOG2E), pack2(-ref, -ref)), d0, d1);
+        if (ENTROPY) { d0 = max_nan(d0, LP_FLOOR); d1 = max_nan(d1, LP_FLOOR); }
+        const uint64_t e = fma2(pack2(exp2_fast(d0), exp2_fast(d1)), pack2(scale, scale), 0);
+        if (!ENTROPY) return e;
+        // d log(2) + H - ln s is log p + H
+        const uint64_t lp = fma2(pack2(d0, d1), pack2(LN2, LN2), pack2(shift, shift));
+        return fma2(e, fma2(lp, pack2(g_ent, g_ent), pack2(sum, sum)), 0);
+    }
+    __device__ __forceinline__ float one(float v) const {
+        if (nothing) return 0.f;
+        float a, b;
+        unpack2(pair(v, v, minus != 0.f), a, b);
+        return a;
+    }
+};
+
+// Rows go from the last to the first: the forward call has just read them in the other order, and the last ones are still in L2.
 template <class T, int THREADS, bool ENTROPY>
 __global__ void __launch_bounds__(THREADS == 32 ? 128 : THREADS) lp_backward_kernel(const LpBwd a) {
     constexpr int VE = Vec16<T>::N;
     constexpr int TEAMS = THREADS == 32 ? 4 : 1;
     const int t = THREADS == 32 ? threadIdx.x & 31 : threadIdx.x;
     const long long unit = (long long)blockIdx.x * TEAMS + (THREADS == 32 ? threadIdx.x >> 5 : 0);
-    const long long row = unit / a.segments;
-    const int segment = (int)(unit - row * a.segments);
-    if (row >= a.rows) return;
+    const long long line = unit / a.segments;
+    const int segment = (int)(unit - line * a.segments);
+    if (line >= a.rows) return;
+    const long long row = a.rows - 1 - line;
     const T* x = static_cast<const T*>(a.x) + row * a.stride;
     T* dx = static_cast<T*>(a.dx) + row * (long long)a.classes;
 
-    const float m = a.stats[2 * row], ln_s = a.stats[2 * row + 1];
-    const long long target = a.targets != nullptr ? a.targets[row] : a.ignore;
-    const bool nothing = m == -INFINITY;
-    float g_target = 0.f, sum = 0.f;
-    if (a.g_log_prob != nullptr && target != a.ignore) g_target = target >= 0 && target < a.classes ? a.g_log_prob[row] : NAN;
-    sum = g_target;
-    if (a.g_top != nullptr)
-        for (int j = 0; j < a.k; ++j) sum += a.g_top[row * a.k + j];
-    const float g_ent = ENTROPY ? a.g_entropy[row] : 0.f, h = ENTROPY ? a.entropy[row] : 0.f;
-    const float log2_s = ln_s * LOG2E;
-    const auto slope = [&](float v) {      // without what the selected classes add
-        if (nothing) return 0.f;
-        const float d = v - m;
-        if (!ENTROPY) return -exp2_fast(fmaf(d, LOG2E, -log2_s)) * sum;
-        const float e = max_nan(fmaf(d, LOG2E, -log2_s), LP_FLOOR);
-        return -exp2_fast(e) * fmaf(g_ent, fmaf(e, LN2, h), sum);
-    };
-
     const int mis = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
     const bool same = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(dx)) & 15) == 0;
+    const int head = min(a.classes, mis == 0 ? 0 : VE - mis);
+    const int nvec = (a.classes - head) / VE;
+    const int v0 = (int)((long long)nvec * segment / a.segments), v1 = (int)((long long)nvec * (segment + 1) / a.segments);
+    const uint4* vec = reinterpret_cast<const uint4*>(x + head);
+    uint4 q[LP_UNROLL];      // in flight while the row's numbers arrive
+#pragma unroll
+    for (int u = 0; u < LP_UNROLL; ++u)
+        if (same && v0 + t + u * THREADS < v1) q[u] = __ldg(vec + v0 + t + u * THREADS);
+
+    const long long target = a.targets != nullptr ? a.targets[row] : a.ignore;
+    float g_target = 0.f;
+    if (a.g_log_prob != nullptr && target != a.ignore) g_target = target >= 0 && target < a.classes ? a.g_log_prob[row] : NAN;
+    float sum = g_target;
+    if (a.g_top != nullptr)
+        for (int j = 0; j < a.k; ++j) sum += a.g_top[row * a.k + j];
+    Slope<ENTROPY> slope;
+    slope.set(a.stats[2 * row], a.stats[2 * row + 1], sum, ENTROPY ? a.g_entropy[row] : 0.f, ENTROPY ? a.entropy[row] : 0.f);
+
     int begin, end;      // elements of this segment
     if (same) {
-        const int head = min(a.classes, mis == 0 ? 0 : VE - mis);
-        const int nvec = (a.classes - head) / VE;
-        const int v0 = (int)((long long)nvec * segment / a.segments), v1 = (int)((long long)nvec * (segment + 1) / a.segments);
-        const uint4* vec = reinterpret_cast<const uint4*>(x + head);
         uint4* out = reinterpret_cast<uint4*>(dx + head);
-        for (int v = v0 + t; v < v1; v += THREADS * LP_UNROLL) {
-            uint4 q[LP_UNROLL];
+        const auto put = [&](const uint4& in, int v, bool far) {
+            float f[VE];
+            Vec16<T>::unpack(in, f);
 #pragma unroll
-            for (int u = 0; u < LP_UNROLL; ++u)
-                if (v + u * THREADS < v1) q[u] = __ldg(vec + v + u * THREADS);
+            for (int i = 0; i < VE; i += 2) unpack2(slope.pair(f[i], f[i + 1], far), f[i], f[i + 1]);
+            __stcs(out + v, Vec16<T>::pack(f));
+        };
+        for (int v = v0 + t; v < v1; v += THREADS * LP_UNROLL) {
+            if (v != v0 + t) {
+#pragma unroll
+                for (int u = 0; u < LP_UNROLL; ++u)
+                    if (v + u * THREADS < v1) q[u] = __ldg(vec + v + u * THREADS);
+            }
 #pragma unroll
             for (int u = 0; u < LP_UNROLL; ++u)
                 if (v + u * THREADS < v1) {
-                    float f[VE];
-                    Vec16<T>::unpack(q[u], f);
-#pragma unroll
-                    for (int i = 0; i < VE; ++i) f[i] = slope(f[i]);
-                    out[v + u * THREADS] = Vec16<T>::pack(f);
+                    if (slope.nothing) out[v + u * THREADS] = make_uint4(0, 0, 0, 0);
+                    else if (slope.minus == 0.f) put(q[u], v + u * THREADS, false);
+                    else put(q[u], v + u * THREADS, true);
                 }
         }
         begin = segment == 0 ? 0 : head + v0 * VE;
         end = segment == a.segments - 1 ? a.classes : head + v1 * VE;
-        if (t < VE && segment == 0 && t < head) dx[t] = from_float<T>(slope(to_float(x[t])));
+        if (t < VE && segment == 0 && t < head) dx[t] = from_float<T>(slope.one(to_float(x[t])));
         const int tail = head + nvec * VE + t;
-        if (t < VE && segment == a.segments - 1 && tail < a.classes) dx[tail] = from_float<T>(slope(to_float(x[tail])));
+        if (t < VE && segment == a.segments - 1 && tail < a.classes) dx[tail] = from_float<T>(slope.one(to_float(x[tail])));
     } else {
         begin = (int)((long long)a.classes * segment / a.segments);
         end = (int)((long long)a.classes * (segment + 1) / a.segments);
-        for (int i = begin + t; i < end; i += THREADS) dx[i] = from_float<T>(slope(to_float(x[i])));
+        for (int i = begin + t; i < end; i += THREADS) dx[i] = from_float<T>(slope.one(to_float(x[i])));
     }
     // The selected classes, written again in whole: where two selections name one class, each writes the same sum.
     Team<THREADS>::sync();
-    if (nothing) return;
+    if (slope.nothing) return;
     const int selected = a.g_top != nullptr ? a.k : 0;
     for (int j = t; j <= selected; j += THREADS) {
         const long long i = j < selected ? a.top_indices[row * a.k + j] : (a.g_log_prob != nullptr && target != a.ignore ? target : -1);
@@ -427,7 +532,7 @@ __global__ void __launch_bounds__(THREADS == 32 ? 128 : THREADS) lp_backward_ker
         float g = i == target ? g_target : 0.f;
         for (int l = 0; l < selected; ++l)
             if (a.top_indices[row * a.k + l] == i) g += a.g_top[row * a.k + l];
-        dx[i] = from_float<T>(slope(to_float(x[i])) + g);
+        dx[i] = from_float<T>(slope.one(to_float(x[i])) + g);
     }
 }
 
@@ -486,8 +591,8 @@ int adder_b200_log_probs_forward(const void* logits, int dtype, long long rows, 
         // Few rows leave SMs idle: a row is then split over a cluster of up to 8 CTAs of at least 4096 elements.
         int parts = 1;
         while (parts < 8 && rows * parts * 2 <= sm_count() * 2 && classes >= 8192LL * parts) parts *= 2;
-        if (parts > 1) return choose_forward<T, 512, true>(a, parts, s);
-        return choose_forward<T, 512, false>(a, 1, s);
+        if (parts > 1) return choose_forward<T, LP_TEAM, true>(a, parts, s);
+        return choose_forward<T, LP_TEAM, false>(a, 1, s);
     });
 }
 

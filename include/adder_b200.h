@@ -268,7 +268,7 @@ ADDER_API int adder_b200_layernorm_backward(const void* dy, const void* dh, cons
  *   log_prob[row]  log softmax at targets[row]: 0 where the target is ignore_index, NaN where it is no class
  *   entropy[row]   -sum p log p
  *   top_log_probs, top_indices [row][top_k]  the top_k <= 32 largest, equal logits by index from the lowest
- *   stats[row][2]  the row's maximum and the log of its sum of exponentials relative to it, for the backward call
+ *   stats[row][2]  the row's maximum and its sum of exponentials relative to it, for the backward call
  * Outputs that are NULL are left out (targets may be NULL where log_prob is; the top ones go with top_k).  A row of nothing but
  * -inf has log probabilities of -inf, entropy 0 and the first indices; one with a NaN or +inf gives NaN and indices of -1. */
 ADDER_API int adder_b200_log_probs_forward(const void* logits, int dtype, long long rows, long long classes, long long row_stride,
