@@ -7,8 +7,8 @@
 //
 // The forward reads the logits once: every thread keeps a maximum of its own with the two sums relative to it, which are rescaled when
 // it rises, and the threads' triples are joined at the end.  The largest k need no second pass over the row either: the k-th largest of
-// the threads' maxima is a lower bound of the k-th largest value, so all candidates lie with the at most k threads (and those
-// that tie with them) whose maximum reaches it, and only their share of the row is read again.  The backward reads the logits and writes
+// the threads' maxima is a lower bound of the k-th largest value, so all candidates lie with the few threads
+// whose maximum reaches it, and only their share of the row is read again.  The backward reads the logits and writes
 // the gradient.  Both are bound by memory for large rows; few rows are split over a cluster of CTAs that join through shared memory.
 #include "kernels.h"
 #include "elements.cuh"
@@ -21,8 +21,9 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int LP_MAX_K = 32;
-constexpr int LP_TEAM = 256;            // threads of a CTA that has a row, or a part of one, to itself
-constexpr int LP_UNROLL = 4;            // vectors that a thread has in flight
+constexpr int LP_TEAM = 224;            // threads that stream one row; a CTA has one warp more, which finishes rows
+constexpr int LP_UNROLL = 4;            // backward: vectors that a thread has in flight
+constexpr int LP_GROUP = 4, LP_STAGES = 3;      // forward: vectors of a thread that are taken together, groups of them on their way or in use
 constexpr float LP_FLOOR = -200.f;      // 2^-200 is 0 in fp32: stands for exponents of -inf where 0 * -inf would be NaN
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
@@ -84,23 +85,37 @@ struct LpFwd {
     long long* top_indices;
 };
 
-// Threads that share a row: a warp, or a CTA (which may be one of a cluster).
-template <int THREADS> struct Team {
-    static __device__ __forceinline__ void sync() {
-        if constexpr (THREADS == 32) __syncwarp(); else __syncthreads();
-    }
+// Shared memory of the warp that finishes a row.
+template <class T, int STREAM, bool TOP> struct LpFinish {
+    static constexpr int VECTORS = STREAM == 32 ? 1 : 2;               // of a lane, that are looked at together
+    static constexpr int BATCH = VECTORS * 32 * Vec16<T>::N;           // values in them
+    static constexpr int LIST = TOP ? BATCH + 64 : 1;
+    uint64_t list[LIST];                   // candidates
+    int winners[TOP ? STREAM : 1];         // threads that hold some
+    int count;
+};
+// What the streaming threads hand over: each warp's sums, each thread's maximum and the vector that it is in.
+struct LpHand {
+    float m[LP_TEAM / 32], s[LP_TEAM / 32], t[LP_TEAM / 32];
+    float best[LP_TEAM];
+    int best_vec[LP_TEAM];
+};
+// What the CTAs of a cluster leave in the shared memory of the first.
+struct LpParts {
+    float m[8], s[8], t[8];
+    uint64_t top[8][32];
 };
 
-// What a team keeps in shared memory.
-template <int THREADS, int LIST> struct LpShared {
-    float m[THREADS / 32], s[THREADS / 32], t[THREADS / 32];
-    float row[3];                          // M, s, t of the team, then of the row
-    uint64_t sorted[THREADS / 32][32];     // sorted maxima of each warp
-    uint64_t top[32];                      // the best so far, sorted
-    uint64_t list[LIST];                   // candidates
-    int winners[THREADS];
-    int count, winner_count;
-};
+// Named barriers between the streaming warps and the finishing one; 0 is __syncthreads.
+enum { LP_EMPTY = 1, LP_FULL = 3 };      // two of each
+template <int ID> __device__ __forceinline__ void bar_sync(int buffer) {
+    if (buffer == 0) asm volatile("bar.sync %0, %1;" ::"n"(ID), "n"(LP_TEAM + 32) : "memory");
+    else asm volatile("bar.sync %0, %1;" ::"n"(ID + 1), "n"(LP_TEAM + 32) : "memory");
+}
+template <int ID> __device__ __forceinline__ void bar_arrive(int buffer) {
+    if (buffer == 0) asm volatile("bar.arrive %0, %1;" ::"n"(ID), "n"(LP_TEAM + 32) : "memory");
+    else asm volatile("bar.arrive %0, %1;" ::"n"(ID + 1), "n"(LP_TEAM + 32) : "memory");
+}
 
 // Joins (m, s, t) of two parts: sums relative to the larger maximum.  Equal maxima (both -inf among them) need no factor, and a sum that
 // is NaN stays one.
@@ -111,20 +126,6 @@ __device__ __forceinline__ void join(float& m, float& s, float& t, float m2, flo
     t = (t + s * d1) * f1 + (t2 + s2 * d2) * f2;
     s = s * f1 + s2 * f2;
     m = M;
-}
-
-// The 32 largest of one key a thread, sorted, in the lanes of the team's first warp (others: nothing of use).
-template <int THREADS, class Shared> __device__ __forceinline__ uint64_t team_top32(uint64_t key, int t, Shared& sh) {
-    const int lane = t & 31, warp = t >> 5;
-    key = sort_warp(key, lane);
-    if constexpr (THREADS > 32) {
-        for (int half = THREADS / 64; half > 0; half >>= 1) {
-            if (warp >= half && warp < 2 * half) sh.sorted[warp][lane] = key;
-            __syncthreads();
-            if (warp < half) key = merge_down(bigger(key, sh.sorted[warp + half][31 - lane]), lane, 32);
-        }
-    }
-    return key;
 }
 
 template <class T> __device__ __forceinline__ uint32_t max_pair(uint32_t a, uint32_t b);
@@ -158,6 +159,9 @@ template <class T> __device__ __forceinline__ float word_max(uint32_t w) {
 template <bool ENTROPY> struct Running {
     float m = -INFINITY, ref = 0.f, res = 0.f;
     uint64_t s = 0, t = 0;      // pairs of fp32 sums
+    // With an entropy values below this count as this: their exponential is 0 either way, and 0 * -inf would be NaN.  |m| / 64 covers
+    // its rounding to 16 bits.
+    __device__ __forceinline__ float floor_value() const { return m - 150.f - fabsf(m) * 0.015625f; }
 
     __device__ __forceinline__ bool small() const { return fabsf(m) < 8192.f; }
     __device__ __forceinline__ void shift(float d) {
@@ -172,26 +176,32 @@ template <bool ENTROPY> struct Running {
         shift((m - top) * LOG2E + (res_new - res));
         m = top; ref = ref_new; res = res_new;
     }
-    // N values (N even), the largest of which is `top`
-    template <int N> __device__ __forceinline__ void take(const float (&f)[N], float top) {
-        if (top > m) raise(top);
+    // N pairs of values, pair(i, floored) each, the largest of which is `top` and not above m
+    template <int N, class Pair> __device__ __forceinline__ void take(Pair&& pair, float top) {
         if (m == -INFINITY && top == -INFINITY) return;      // nothing so far
         if (small()) {
             const uint64_t scale = pack2(LOG2E, LOG2E), minus = pack2(-ref, -ref);
 #pragma unroll
-            for (int i = 0; i < N; i += 2) add(fma2(pack2(f[i], f[i + 1]), scale, minus));
+            for (int i = 0; i < N; ++i) {
+                const float2 f = pair(i, ENTROPY);
+                add(fma2(pack2(f.x, f.y), scale, minus));
+            }
         } else {
 #pragma unroll
-            for (int i = 0; i < N; i += 2) add(pack2((f[i] - m) * LOG2E, (f[i + 1] - m) * LOG2E));
+            for (int i = 0; i < N; ++i) {
+                const float2 f = pair(i, false);
+                float d0 = (f.x - m) * LOG2E, d1 = (f.y - m) * LOG2E;
+                if (ENTROPY) { d0 = max_nan(d0, LP_FLOOR); d1 = max_nan(d1, LP_FLOOR); }
+                add(pack2(d0, d1));
+            }
         }
     }
     __device__ __forceinline__ void add(uint64_t pair) {
         float d0, d1;
         unpack2(pair, d0, d1);
-        if (ENTROPY) { d0 = max_nan(d0, LP_FLOOR); d1 = max_nan(d1, LP_FLOOR); }
         const uint64_t e = pack2(exp2_fast(d0), exp2_fast(d1));
         s = add2(s, e);
-        if (ENTROPY) t = fma2(e, pack2(d0, d1), t);
+        if (ENTROPY) t = fma2(e, pair, t);
     }
     // Sums relative to m itself
     __device__ __forceinline__ void finish(float* sum, float* dot) {
@@ -205,13 +215,33 @@ template <bool ENTROPY> struct Running {
     }
 };
 
-// U vectors of a thread, THREADS apart from the v-th on: their values into the running sums, their maximum into `best`.
+// A row as a team sees it: aligned vectors v0 to v1 - 1 (shared out over the cluster), and up to VE - 1 single elements before and
+// behind all vectors, which are rank 0's.
+template <class T> struct LpRow {
+    static constexpr int VE = Vec16<T>::N;
+    const T* x;
+    const uint4* vec;
+    int head, nvec, singles, v0, v1;
+
+    __device__ __forceinline__ void set(const LpFwd& a, long long row, int rank, int parts) {
+        x = static_cast<const T*>(a.x) + row * a.stride;
+        const int mis = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
+        head = min(a.classes, mis == 0 ? 0 : VE - mis);
+        nvec = (a.classes - head) / VE;
+        singles = rank == 0 ? a.classes - nvec * VE : 0;
+        v0 = parts == 1 ? 0 : (int)((long long)nvec * rank / parts);
+        v1 = parts == 1 ? nvec : (int)((long long)nvec * (rank + 1) / parts);
+        vec = reinterpret_cast<const uint4*>(x + head);
+    }
+    // At least one, so that a row without vectors takes its turn.
+    __device__ __forceinline__ int groups(int threads) const { return max(1, (v1 - v0 + LP_GROUP * threads - 1) / (LP_GROUP * threads)); }
+    __device__ __forceinline__ int single(int i) const { return i < head ? i : i + nvec * VE; }
+};
+
+// A group's values into the running sums, its maximum into `best`.
 template <class T, int THREADS, int U, bool ENTROPY, bool TOP>
-__device__ __forceinline__ void take_vectors(const uint4* vec, int v, Running<ENTROPY>& run, float& best, int& best_vec) {
+__device__ __forceinline__ void take_group(const uint4 (&q)[U], int v, Running<ENTROPY>& run, float& best, int& best_vec) {
     constexpr int VE = Vec16<T>::N;
-    uint4 q[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) q[u] = __ldg(vec + v + u * THREADS);
     uint32_t w[U], all;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -225,179 +255,371 @@ __device__ __forceinline__ void take_vectors(const uint4* vec, int v, Running<EN
         for (int u = U - 1; u >= 0; --u)
             if (word_max<T>(w[u]) == top) best_vec = v + u * THREADS;
     }
-    float f[U * VE];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-        float g[VE];
-        Vec16<T>::unpack(q[u], g);
-#pragma unroll
-        for (int i = 0; i < VE; ++i) f[u * VE + i] = g[i];
-    }
-    run.take(f, top);
+    if (top > run.m) run.raise(top);
+    const float low = run.floor_value();
+    uint32_t low_word = __float_as_uint(low);
+    if constexpr (sizeof(T) == 2) low_word = pack_pair<T>(low, low);
+    run.template take<U * VE / 2>([&](int i, bool floored) {
+        const int u = i / (VE / 2), j = i % (VE / 2);
+        if constexpr (sizeof(T) == 4) {
+            float2 f = j == 0 ? make_float2(__uint_as_float(q[u].x), __uint_as_float(q[u].y)) : make_float2(__uint_as_float(q[u].z), __uint_as_float(q[u].w));
+            if (floored) { f.x = max_nan(f.x, low); f.y = max_nan(f.y, low); }
+            return f;
+        } else {
+            const uint32_t word = j == 0 ? q[u].x : j == 1 ? q[u].y : j == 2 ? q[u].z : q[u].w;
+            return unpack_pair<T>(floored ? max_pair<T>(word, low_word) : word);
+        }
+    }, top);
 }
 
-// grid: rows (times the cluster's size), or rows / 4 with a warp a row
+// Sums of a warp's lanes, in every lane.
+template <bool ENTROPY> __device__ __forceinline__ void join_lanes(float& m, float& s, float& t, int lanes) {
+    for (int off = lanes >> 1; off > 0; off >>= 1) {
+        const float m2 = __shfl_xor_sync(0xffffffffu, m, off), s2 = __shfl_xor_sync(0xffffffffu, s, off),
+                    t2 = ENTROPY ? __shfl_xor_sync(0xffffffffu, t, off) : 0.f;
+        join(m, s, t, m2, s2, t2);
+    }
+}
+
+__device__ __forceinline__ void copy16(uint32_t to, const uint4* from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(to), "l"(from) : "memory");
+}
+__device__ __forceinline__ uint4 read16(uint32_t from) {
+    uint4 q;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(q.x), "=r"(q.y), "=r"(q.z), "=r"(q.w) : "r"(from) : "memory");
+    return q;
+}
+
+// The vectors of a team's rows on their way through shared memory.  Every thread copies what it will read itself, so no thread waits
+// for another, and the copies of the next rows go on while a row is finished.
+template <class T, int THREADS> struct LpStream {
+    static constexpr int CTA = THREADS == 32 ? 128 : THREADS;      // threads that stream
+    static constexpr uint32_t SLOT = CTA * 16, STAGE = LP_GROUP * SLOT, RING = LP_STAGES * STAGE;      // bytes
+    uint32_t first, at;      // this thread's first slot, and the next to be filled
+    const uint4* src;        // of the next group
+    int left;                // vectors of the row from there on, in steps of one, of which every THREADS-th is this thread's
+    int groups;              // of the row
+    long long row, step;
+
+    __device__ __forceinline__ void set_row(const LpFwd& a, int t, int rank, int parts) {
+        LpRow<T> r;
+        r.set(a, row, rank, parts);
+        src = r.vec + r.v0 + t;
+        left = r.v1 - r.v0 - t;
+        groups = r.groups(THREADS);
+    }
+    __device__ __forceinline__ void issue(const LpFwd& a, int t, int rank, int parts) {
+        if (groups > 0) {
+            if (left > (LP_GROUP - 1) * THREADS) {
+#pragma unroll
+                for (int u = 0; u < LP_GROUP; ++u) copy16(at + u * SLOT, src + u * THREADS);
+            } else {
+#pragma unroll
+                for (int u = 0; u < LP_GROUP - 1; ++u)
+                    if (u * THREADS < left) copy16(at + u * SLOT, src + u * THREADS);
+            }
+            src += LP_GROUP * THREADS;
+            left -= LP_GROUP * THREADS;
+            if (--groups == 0) {
+                row += step;
+                if (row < a.rows) set_row(a, t, rank, parts);
+            }
+        }
+        cp_async_commit();
+        at = at == first + RING - STAGE ? first : at + STAGE;
+    }
+};
+
+// The k-th largest of the lanes' keys, 0 where fewer than k lanes have one.  Values first: one round takes all lanes of equal value.
+__device__ __forceinline__ uint64_t kth_largest(uint64_t key, int k) {
+    uint32_t value = (uint32_t)(key >> 32);
+    for (int found = 0;;) {
+        const uint32_t top = __reduce_max_sync(0xffffffffu, value);
+        if (top == 0) return 0;
+        const int n = __popc(__ballot_sync(0xffffffffu, value == top));
+        if (found + n < k) {
+            found += n;
+            if (value == top) value = 0;
+            continue;
+        }
+        uint32_t low = value == top ? (uint32_t)key : 0, last = 0;
+        for (; found < k; ++found) {
+            last = __reduce_max_sync(0xffffffffu, low);
+            if (low == last) low = 0;
+        }
+        return ((uint64_t)top << 32) | last;
+    }
+}
+
+// The rest of a row (or of its cluster rank's part), by one warp: joins the sums, adds the single elements, finds the k largest.
+// `high(i)`: an upper bound of the largest key of thread 32 i + lane, 0 where it has none.  `low`: lower bounds of the largest keys of
+// 32 disjoint parts of the row; the k-th largest of them bounds the k-th largest of all from below.
+template <class T, int STREAM, bool ENTROPY, bool TOP, class High>
+__device__ __forceinline__ void finish_part(const LpRow<T>& r, int k, float one, int lane, LpFinish<T, STREAM, TOP>& sh, uint64_t low, High&& high, float& m,
+                                            float& s, float& t, uint64_t& top) {
+    constexpr int VE = Vec16<T>::N;
+    if (r.singles > 0) {
+        Running<ENTROPY> run;
+        if (lane < r.singles) {
+            if (one > run.m) run.raise(one);
+            const float below = run.floor_value();
+            run.template take<1>([&](int, bool floored) { return floored ? make_float2(max_nan(one, below), below) : make_float2(one, -INFINITY); }, one);
+        }
+        float s2, t2;
+        run.finish(&s2, &t2);
+        join(m, s, t, run.m, s2, t2);
+    }
+    join_lanes<ENTROPY>(m, s, t, 32);
+    top = 0;
+    if constexpr (TOP) {
+        const uint64_t bound = kth_largest(low, k);
+        __syncwarp();
+        int winners = 0;
+#pragma unroll
+        for (int i = 0; i < STREAM / 32; ++i) {
+            const uint64_t h = high(i);
+            const bool in = h != 0 && h >= bound;
+            const unsigned who = __ballot_sync(0xffffffffu, in);
+            if (in) sh.winners[winners + __popc(who & ((1u << lane) - 1))] = 32 * i + lane;
+            winners += __popc(who);
+        }
+        if (lane == 0) sh.count = 0;
+        __syncwarp();
+        const auto offer = [&](float v, uint32_t index) {
+            const uint64_t key = key_of(v, index);
+            if (key >= bound) sh.list[atomicAdd(&sh.count, 1)] = key;
+        };
+        if (lane < r.singles) offer(one, (uint32_t)r.single(lane));
+        const int per = (r.v1 - r.v0 + STREAM - 1) / STREAM;      // vectors of a thread, the last perhaps not there
+        const int items = winners * per;
+        bool merged = false;
+        const auto merge = [&](int n) {
+            for (int at = 0; at < n; at += 32) {
+                const uint64_t batch = sort_warp(at + lane < n ? sh.list[at + lane] : 0, lane);
+                const uint64_t other = __shfl_sync(0xffffffffu, top, 31 - lane);
+                top = merged ? merge_down(bigger(batch, other), lane, 32) : batch;
+                merged = true;
+            }
+        };
+        using Finish = LpFinish<T, STREAM, TOP>;
+        for (int base = 0; base < items; base += Finish::VECTORS * 32) {
+            uint4 p[Finish::VECTORS];
+            int at[Finish::VECTORS];
+#pragma unroll
+            for (int u = 0; u < Finish::VECTORS; ++u) {
+                const int item = base + 32 * u + lane, w = item < items ? item / per : 0;
+                at[u] = item < items ? r.v0 + sh.winners[w] + (item - w * per) * STREAM : r.v1;
+                if (at[u] < r.v1) p[u] = __ldg(r.vec + at[u]);
+            }
+#pragma unroll
+            for (int u = 0; u < Finish::VECTORS; ++u) {
+                if (at[u] >= r.v1) continue;
+                const uint32_t largest = max_word<T>(max_word<T>(p[u].x, p[u].y), max_word<T>(p[u].z, p[u].w));
+                if (key_of(word_max<T>(largest), 0) < bound) continue;
+                float g[VE];
+                Vec16<T>::unpack(p[u], g);
+#pragma unroll
+                for (int i = 0; i < VE; ++i) offer(g[i], (uint32_t)(r.head + at[u] * VE + i));
+            }
+            __syncwarp();
+            const int n = sh.count;
+            if (n > Finish::LIST - Finish::BATCH) {      // no room for another batch
+                merge(n);
+                __syncwarp();
+                if (lane == 0) sh.count = 0;
+            }
+            __syncwarp();
+        }
+        __syncwarp();
+        const int n = sh.count;
+        if (merged || n > 32) {
+            merge(n);
+        } else {      // the usual case: each of a few candidates counts those above it
+            const uint64_t key = lane < n ? sh.list[lane] : 0;
+            int above = 0;
+            for (int i = 0; i < n; ++i) above += __shfl_sync(0xffffffffu, key, i) > key;
+            __syncwarp();
+            sh.list[lane] = 0;
+            __syncwarp();
+            if (lane < n) sh.list[above] = key;
+            __syncwarp();
+            top = sh.list[lane];
+        }
+        __syncwarp();
+    }
+}
+
+// The outputs of a row, by one warp whose lanes all have its sums.
+template <bool ENTROPY, bool TOP>
+__device__ __forceinline__ void write_row(const LpFwd& a, long long row, int lane, float m, float s, float t, uint64_t top, long long target, float at_target) {
+    const bool nothing = s == 0.f, broken = s != s;      // all -inf; a NaN or +inf among the logits
+    const float ln_s = nothing ? 0.f : logf(s);
+    if (lane == 0) {
+        if (a.stats != nullptr) *reinterpret_cast<float2*>(a.stats + 2 * row) = make_float2(m, s);
+        if (a.log_prob != nullptr) {
+            float lp = 0.f;
+            if (target != a.ignore) {
+                if (target < 0 || target >= a.classes || broken) lp = NAN;
+                else lp = nothing ? -INFINITY : (at_target - m) - ln_s;
+            }
+            a.log_prob[row] = lp;
+        }
+        if (ENTROPY) a.entropy[row] = broken ? NAN : nothing ? 0.f : LN2 * (log2f(s) - t / s);
+    }
+    if (TOP && lane < a.k) {
+        a.top_log_probs[row * a.k + lane] = broken ? NAN : nothing ? -INFINITY : (key_value(top) - m) - ln_s;
+        a.top_indices[row * a.k + lane] = broken ? -1 : (long long)key_index(top);
+    }
+}
+
+// THREADS threads stream every grid-th row (or, in a cluster, a part of one row).  A warp that has a row to itself finishes it, too; with
+// LP_TEAM threads another warp of the CTA does, while they are in the next row.
 template <class T, int THREADS, bool CLUSTER, bool ENTROPY, bool TOP>
-__global__ void __launch_bounds__(THREADS == 32 ? 128 : THREADS, THREADS == 32 ? 8 : 1024 / THREADS) lp_forward_kernel(const LpFwd a) {
+__global__ void __launch_bounds__(THREADS == 32 ? 128 : LP_TEAM + 32, THREADS == 32 ? 8 : 4) lp_forward_kernel(const LpFwd a) {
     constexpr int VE = Vec16<T>::N;
     constexpr int TEAMS = THREADS == 32 ? 4 : 1;
-    constexpr int LIST = TOP ? THREADS * VE + 2 * VE : 1;
-    __shared__ LpShared<THREADS, LIST> shared[TEAMS];
-    const int t = THREADS == 32 ? threadIdx.x & 31 : threadIdx.x;
-    const int team = THREADS == 32 ? threadIdx.x >> 5 : 0;
-    LpShared<THREADS, LIST>& sh = shared[team];
+    extern __shared__ uint4 ring[];         // [LP_STAGES][LP_GROUP][threads]
+    __shared__ LpFinish<T, THREADS, TOP> finishing[TEAMS];
+    __shared__ LpHand hand[THREADS == 32 ? 1 : 2];
+    __shared__ LpParts joined[1];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int t = THREADS == 32 ? lane : threadIdx.x;
     int rank = 0, parts = 1;
-    long long row;
+    long long row, step;
     if constexpr (CLUSTER) {
         rank = (int)cg::this_cluster().block_rank();
         parts = (int)cg::this_cluster().num_blocks();
         row = blockIdx.x / parts;
+        step = a.rows;      // a cluster has one row
+        asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");      // waited for before the first word crosses over
     } else {
-        row = (long long)blockIdx.x * TEAMS + team;
-        if (row >= a.rows) return;      // whole warps only, and warps of a CTA do not wait for one another
+        row = (long long)blockIdx.x * TEAMS + (THREADS == 32 ? warp : 0);
+        step = (long long)gridDim.x * TEAMS;
     }
-    const T* x = static_cast<const T*>(a.x) + row * a.stride;
-    // The row's aligned vectors, shared out over the cluster; up to VE - 1 single elements before and behind them are rank 0's.
-    const int mis = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
-    const int head = min(a.classes, mis == 0 ? 0 : VE - mis);
-    const int nvec = (a.classes - head) / VE;
-    const int singles = rank == 0 ? a.classes - nvec * VE : 0;
-    const int v0 = (int)((long long)nvec * rank / parts), v1 = (int)((long long)nvec * (rank + 1) / parts);
-    const uint4* vec = reinterpret_cast<const uint4*>(x + head);
-    const auto single_index = [&](int i) { return i < head ? i : i + nvec * VE; };
+    if (row >= a.rows) return;      // whole warps only, and warps of a CTA do not wait for one another
+    LpFinish<T, THREADS, TOP>& sh = finishing[THREADS == 32 ? warp : 0];
+    const auto low_key = [&](const LpRow<T>& r, int thread, float best, int best_vec) {
+        return r.v0 + thread < r.v1 ? key_of(best, (uint32_t)(r.head + best_vec * VE + VE - 1)) : 0;
+    };
+    const auto high_key = [&](const LpRow<T>& r, int thread, float best, int best_vec) {
+        return r.v0 + thread < r.v1 ? key_of(best, (uint32_t)(r.head + best_vec * VE)) : 0;
+    };
+    const bool finisher = warp == LP_TEAM / 32;
 
-    Running<ENTROPY> run;
-    float best = -INFINITY;
-    int best_vec = v0 + t;
-    int v = v0 + t;
-    for (; v + (LP_UNROLL - 1) * THREADS < v1; v += THREADS * LP_UNROLL) take_vectors<T, THREADS, LP_UNROLL, ENTROPY, TOP>(vec, v, run, best, best_vec);
-    for (; v < v1; v += THREADS) take_vectors<T, THREADS, 1, ENTROPY, TOP>(vec, v, run, best, best_vec);
-    if (t < singles) {
-        const float f[2] = {to_float(x[single_index(t)]), -INFINITY};
-        run.take(f, f[0]);
-    }
-    float m = run.m, s, tt;
-    run.finish(&s, &tt);
-
-    // ---- the team's sums
+    if constexpr (THREADS > 32) if (finisher) {
+        __syncwarp();
+        bar_arrive<LP_EMPTY>(0);
+        if (row + step < a.rows) bar_arrive<LP_EMPTY>(1);
+        int buffer = 0;
+        long long target_next = a.log_prob != nullptr ? a.targets[row] : 0;
+        for (; row < a.rows; row += step) {
+            LpRow<T> r;
+            r.set(a, row, rank, parts);
+            const long long target = target_next;
+            const float at_target = a.log_prob != nullptr && target >= 0 && target < a.classes ? to_float(r.x[target]) : 0.f;
+            if (a.log_prob != nullptr && row + step < a.rows) target_next = a.targets[row + step];
+            const float one = lane < r.singles ? to_float(r.x[r.single(lane)]) : -INFINITY;
+            __syncwarp();
+            bar_sync<LP_FULL>(buffer);
+            const LpHand& in = hand[buffer];
+            const bool some = lane < LP_TEAM / 32;
+            float m = some ? in.m[lane] : -INFINITY, s = some ? in.s[lane] : 0.f, tt = some ? in.t[lane] : 0.f;
+            uint64_t low = 0, top;
+            if (TOP) {
 #pragma unroll
-    for (int off = 16; off > 0; off >>= 1) {
-        const float m2 = __shfl_xor_sync(0xffffffffu, m, off), s2 = __shfl_xor_sync(0xffffffffu, s, off),
-                    t2 = ENTROPY ? __shfl_xor_sync(0xffffffffu, tt, off) : 0.f;
-        join(m, s, tt, m2, s2, t2);
-    }
-    if constexpr (THREADS > 32) {
-        if ((t & 31) == 0) { sh.m[t >> 5] = m; sh.s[t >> 5] = s; sh.t[t >> 5] = tt; }
-        __syncthreads();
-        if (t < 32) {
-            const bool in = t < THREADS / 32;
-            m = in ? sh.m[t] : -INFINITY; s = in ? sh.s[t] : 0.f; tt = in ? sh.t[t] : 0.f;
-#pragma unroll
-            for (int off = THREADS / 64; off > 0; off >>= 1) {
-                const float m2 = __shfl_xor_sync(0xffffffffu, m, off), s2 = __shfl_xor_sync(0xffffffffu, s, off),
-                            t2 = ENTROPY ? __shfl_xor_sync(0xffffffffu, tt, off) : 0.f;
-                join(m, s, tt, m2, s2, t2);
+                for (int i = 0; i < LP_TEAM / 32; ++i) low = bigger(low, low_key(r, 32 * i + lane, in.best[32 * i + lane], in.best_vec[32 * i + lane]));
             }
+            finish_part<T, LP_TEAM, ENTROPY, TOP>(r, a.k, one, lane, sh, low, [&](int i) {
+                return high_key(r, 32 * i + lane, in.best[32 * i + lane], in.best_vec[32 * i + lane]);
+            }, m, s, tt, top);
+            __syncwarp();
+            if (row + 2 * step < a.rows) bar_arrive<LP_EMPTY>(buffer);
+            buffer ^= 1;
+            if constexpr (CLUSTER) {      // every rank hands its part to rank 0
+                cg::cluster_group cluster = cg::this_cluster();
+                asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+                LpParts* to = cluster.map_shared_rank(&joined[0], 0);
+                if (lane == 0) { to->m[rank] = m; to->s[rank] = s; to->t[rank] = tt; }
+                if (TOP) to->top[rank][lane] = top;
+                cluster.sync();
+                if (rank != 0) return;
+                const bool there = lane < parts;
+                m = there ? joined[0].m[lane] : -INFINITY; s = there ? joined[0].s[lane] : 0.f; tt = there ? joined[0].t[lane] : 0.f;
+                join_lanes<ENTROPY>(m, s, tt, 32);
+                if (TOP)
+                    for (int i = 1; i < parts; ++i) top = merge_down(bigger(top, joined[0].top[i][31 - lane]), lane, 32);
+            }
+            write_row<ENTROPY, TOP>(a, row, lane, m, s, tt, top, target, at_target);
         }
+        return;
     }
-    if (t == 0) { sh.row[0] = m; sh.row[1] = s; sh.row[2] = tt; }
 
-    // ---- the team's k largest
-    if constexpr (TOP) {
-        const bool has = v0 + t < v1;
-        const uint32_t lowest = (uint32_t)(head + best_vec * VE);
-        // bounds of the thread's largest key, which is in best_vec
-        const uint64_t low = has ? key_of(best, lowest + VE - 1) : 0, high = has ? key_of(best, lowest) : 0;
-        const uint64_t maxima = team_top32<THREADS>(low, t, sh);
-        if (t < 32) sh.top[t] = maxima;
-        if (t == 0) { sh.winner_count = 0; sh.count = 0; }
-        Team<THREADS>::sync();
-        const uint64_t bound = sh.top[a.k - 1];
-        Team<THREADS>::sync();
-        if (t < 32) sh.top[t] = 0;
-        if (has && high >= bound) sh.winners[atomicAdd(&sh.winner_count, 1)] = t;
-        Team<THREADS>::sync();
-        const int per = (v1 - v0 + THREADS - 1) / THREADS;      // vectors of a thread, the last perhaps not there
-        const int items = sh.winner_count * per;
-        if (t < singles) {
-            const uint32_t i = (uint32_t)single_index(t);
-            const uint64_t key = key_of(to_float(x[i]), i);
-            if (key >= bound) sh.list[atomicAdd(&sh.count, 1)] = key;
-        }
-        for (int base = 0; base == 0 || base < items; base += THREADS) {
-            const int item = base + t;
-            if (item < items) {
-                const int v = v0 + sh.winners[item / per] + (item % per) * THREADS;
-                if (v < v1) {
-                    float g[VE];
-                    Vec16<T>::unpack(__ldg(vec + v), g);
+    using Stream = LpStream<T, THREADS>;
+    Stream stream;
+    stream.first = stream.at = smem_u32(ring) + threadIdx.x * 16;
+    stream.row = row; stream.step = step;
+    stream.set_row(a, t, rank, parts);
 #pragma unroll
-                    for (int i = 0; i < VE; ++i) {
-                        const uint64_t key = key_of(g[i], (uint32_t)(head + v * VE + i));
-                        if (key >= bound) sh.list[atomicAdd(&sh.count, 1)] = key;
-                    }
+    for (int i = 0; i < LP_STAGES - 1; ++i) stream.issue(a, t, rank, parts);
+    uint32_t from = stream.first;
+    int buffer = 0;
+    long long target_next = THREADS == 32 && a.log_prob != nullptr ? a.targets[row] : 0;
+    for (; row < a.rows; row += step) {
+        LpRow<T> r;
+        r.set(a, row, rank, parts);
+        // what is needed once the row is through
+        const long long target = target_next;
+        float at_target = 0.f, one = -INFINITY;
+        if constexpr (THREADS == 32) {
+            if (a.log_prob != nullptr && target >= 0 && target < a.classes) at_target = to_float(r.x[target]);
+            if (a.log_prob != nullptr && row + step < a.rows) target_next = a.targets[row + step];
+            if (lane < r.singles) one = to_float(r.x[r.single(lane)]);
+        }
+        Running<ENTROPY> run;
+        float best = -INFINITY;
+        int best_vec = r.v0 + t;
+        int v = r.v0 + t;
+        for (int g = r.groups(THREADS); g > 0; --g) {
+            stream.issue(a, t, rank, parts);
+            cp_async_wait<LP_STAGES - 1>();
+            if (v + (LP_GROUP - 1) * THREADS < r.v1) {
+                uint4 q[LP_GROUP];
+#pragma unroll
+                for (int u = 0; u < LP_GROUP; ++u) q[u] = read16(from + u * Stream::SLOT);
+                take_group<T, THREADS, LP_GROUP, ENTROPY, TOP>(q, v, run, best, best_vec);
+            } else {
+#pragma unroll 1
+                for (int u = 0; u < LP_GROUP - 1 && v + u * THREADS < r.v1; ++u) {
+                    const uint4 q[1] = {read16(from + u * Stream::SLOT)};
+                    take_group<T, THREADS, 1, ENTROPY, TOP>(q, v + u * THREADS, run, best, best_vec);
                 }
             }
-            Team<THREADS>::sync();
-            const int n = sh.count;
-            for (int at = 0; at < n; at += THREADS) {
-                const uint64_t batch = team_top32<THREADS>(at + t < n ? sh.list[at + t] : 0, t, sh);
-                if (t < 32) sh.top[t] = merge_down(bigger(batch, sh.top[31 - t]), t, 32);
-                Team<THREADS>::sync();
-            }
-            if (t == 0) sh.count = 0;
-            Team<THREADS>::sync();
+            from = from == stream.first + Stream::RING - Stream::STAGE ? stream.first : from + Stream::STAGE;
+            v += LP_GROUP * THREADS;
+        }
+        float m = run.m, s, tt;
+        run.finish(&s, &tt);
+        if constexpr (THREADS == 32) {
+            uint64_t top;
+            finish_part<T, 32, ENTROPY, TOP>(r, a.k, one, lane, sh, TOP ? low_key(r, t, best, best_vec) : 0,
+                                             [&](int) { return high_key(r, t, best, best_vec); }, m, s, tt, top);
+            write_row<ENTROPY, TOP>(a, row, lane, m, s, tt, top, target, at_target);
+        } else {
+            join_lanes<ENTROPY>(m, s, tt, 32);
+            __syncwarp();
+            bar_sync<LP_EMPTY>(buffer);
+            LpHand& out = hand[buffer];
+            if (lane == 0) { out.m[warp] = m; out.s[warp] = s; out.t[warp] = tt; }
+            if (TOP) { out.best[t] = best; out.best_vec[t] = best_vec; }
+            __syncwarp();
+            bar_arrive<LP_FULL>(buffer);
+            buffer ^= 1;
         }
     }
-
-    // ---- the row
     if constexpr (CLUSTER) {
-        cg::cluster_group cluster = cg::this_cluster();
-        cluster.sync();
-        if (rank == 0 && t < 32) {
-            for (int r = 1; r < parts; ++r) {
-                LpShared<THREADS, LIST>* other = cluster.map_shared_rank(&sh, r);
-                if (t == 0) {
-                    m = sh.row[0]; s = sh.row[1]; tt = sh.row[2];
-                    join(m, s, tt, other->row[0], other->row[1], other->row[2]);
-                    sh.row[0] = m; sh.row[1] = s; sh.row[2] = tt;
-                }
-                if (TOP) {
-                    const uint64_t key = merge_down(bigger(sh.top[t], other->top[31 - t]), t, 32);
-                    __syncwarp();
-                    sh.top[t] = key;
-                    __syncwarp();
-                }
-            }
-        }
-        cluster.sync();      // no CTA leaves while its shared memory is read
-        if (rank != 0) return;
-    }
-    if (t >= 32) return;
-    __syncwarp();
-    m = sh.row[0]; s = sh.row[1]; tt = sh.row[2];
-    const bool nothing = s == 0.f, broken = s != s;      // all -inf; a NaN or +inf among the logits
-    const float ln_s = nothing ? 0.f : logf(s);
-    if (t == 0) {
-        if (a.stats != nullptr) {
-            a.stats[2 * row] = m;
-            a.stats[2 * row + 1] = s;
-        }
-        if (a.log_prob != nullptr) {
-            const long long target = a.targets[row];
-            float lp = 0.f;
-            if (target != a.ignore) {
-                if (target < 0 || target >= a.classes || broken) lp = NAN;
-                else lp = nothing ? -INFINITY : (to_float(x[target]) - m) - ln_s;
-            }
-            a.log_prob[row] = lp;
-        }
-        if (ENTROPY) a.entropy[row] = broken ? NAN : nothing ? 0.f : LN2 * (log2f(s) - tt / s);
-    }
-    if (TOP && t < a.k) {
-        const uint64_t key = sh.top[t];
-        a.top_log_probs[row * a.k + t] = broken ? NAN : nothing ? -INFINITY : (key_value(key) - m) - ln_s;
-        a.top_indices[row * a.k + t] = broken ? -1 : (long long)key_index(key);
+        __syncwarp();
+        asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+        cg::this_cluster().sync();
     }
 }
 
@@ -523,7 +745,7 @@ __global__ void __launch_bounds__(THREADS == 32 ? 128 : THREADS) lp_backward_ker
         for (int i = begin + t; i < end; i += THREADS) dx[i] = from_float<T>(slope.one(to_float(x[i])));
     }
     // The selected classes, written again in whole: where two selections name one class, each writes the same sum.
-    Team<THREADS>::sync();
+    if constexpr (THREADS == 32) __syncwarp(); else __syncthreads();
     if (slope.nothing) return;
     const int selected = a.g_top != nullptr ? a.k : 0;
     for (int j = t; j <= selected; j += THREADS) {
@@ -538,10 +760,15 @@ __global__ void __launch_bounds__(THREADS == 32 ? 128 : THREADS) lp_backward_ker
 
 template <class T, int THREADS, bool CLUSTER, bool ENTROPY, bool TOP> int launch_forward(const LpFwd& a, int parts, cudaStream_t s) {
     const auto kernel = lp_forward_kernel<T, THREADS, CLUSTER, ENTROPY, TOP>;
+    constexpr int threads = THREADS == 32 ? 128 : LP_TEAM + 32;
+    const size_t ring = LpStream<T, THREADS>::RING;
+    const int st = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), ring);
+    if (st != ADDER_OK) return st;
     if constexpr (CLUSTER) {
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3((unsigned)(a.rows * parts));
-        cfg.blockDim = dim3(THREADS);
+        cfg.blockDim = dim3(threads);
+        cfg.dynamicSmemBytes = ring;
         cfg.stream = s;
         cudaLaunchAttribute attr[1];
         attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -555,8 +782,11 @@ template <class T, int THREADS, bool CLUSTER, bool ENTROPY, bool TOP> int launch
         count_launch();
         return ADDER_OK;
     } else {
-        const long long grid = THREADS == 32 ? (a.rows + 3) / 4 : a.rows;
-        kernel<<<(unsigned)grid, THREADS == 32 ? 128 : THREADS, 0, s>>>(a);
+        const long long rows = THREADS == 32 ? (a.rows + 3) / 4 : a.rows, most = (long long)sm_count() * (THREADS == 32 ? 8 : 4);
+        // A warp's rows take alike long, so all get as many; CTAs of whole rows spread theirs over all SMs (2048x128000 with entropy, 3.5 rows
+        // for each of 592 CTAs: 91 us, 101 with 512 CTAs of 4 rows; 16384x4000 by warps: 37 us, 33 with 1024 CTAs of 4 turns).
+        const long long turns = THREADS == 32 ? (rows + most - 1) / most : 1, grid = THREADS == 32 ? (rows + turns - 1) / turns : rows < most ? rows : most;
+        kernel<<<(unsigned)grid, threads, ring, s>>>(a);
         return launched();
     }
 }
@@ -582,12 +812,12 @@ int adder_b200_log_probs_forward(const void* logits, int dtype, long long rows, 
     if (dtype < ADDER_TYPE_F32 || dtype > ADDER_TYPE_F16) return ADDER_ERR_UNSUPPORTED;
     if (rows == 0) return ADDER_OK;
     if (!logits || (log_prob && !targets) || (top_k > 0 && (!top_log_probs || !top_indices))) return ADDER_ERR_NULL_POINTER;
-    if (!aligned_to(logits, dtype == ADDER_TYPE_F32 ? 4 : 2)) return ADDER_ERR_ALIGNMENT;
+    if (!aligned_to(logits, dtype == ADDER_TYPE_F32 ? 4 : 2) || !aligned_to(stats, 8)) return ADDER_ERR_ALIGNMENT;
     const LpFwd a{logits, rows, row_stride, (int)classes, top_k, targets, ignore_index, log_prob, entropy, stats, top_log_probs, top_indices};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     return with_type(dtype, [&](auto* type) {
         using T = std::remove_pointer_t<decltype(type)>;
-        if (classes <= 1024) return choose_forward<T, 32, false>(a, 1, s);
+        if (classes <= 1024 || (classes <= 8192 && rows >= 24LL * sm_count())) return choose_forward<T, 32, false>(a, 1, s);
         // Few rows leave SMs idle: a row is then split over a cluster of up to 8 CTAs of at least 4096 elements.
         int parts = 1;
         while (parts < 8 && rows * parts * 2 <= sm_count() * 2 && classes >= 8192LL * parts) parts *= 2;
