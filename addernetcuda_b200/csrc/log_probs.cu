@@ -21,9 +21,9 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int LP_MAX_K = 32;
-constexpr int LP_TEAM = 224;            // threads that stream one row; a CTA has one warp more, which finishes rows
+constexpr int LP_TEAM = 256;            // threads that stream one row; a CTA has one warp more, which finishes rows
 constexpr int LP_UNROLL = 4;            // backward: vectors that a thread has in flight
-constexpr int LP_GROUP = 4, LP_STAGES = 3;      // forward: vectors of a thread that are taken together, groups of them on their way or in use
+constexpr int LP_GROUP = 4, LP_STAGES = 2;      // forward: vectors of a thread that are taken together, groups of them on their way or in use
 constexpr float LP_FLOOR = -200.f;      // 2^-200 is 0 in fp32: stands for exponents of -inf where 0 * -inf would be NaN
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
@@ -87,18 +87,22 @@ struct LpFwd {
 
 // Shared memory of the warp that finishes a row.
 template <class T, int STREAM, bool TOP> struct LpFinish {
-    static constexpr int VECTORS = STREAM == 32 ? 1 : 2;               // of a lane, that are looked at together
+    static constexpr int VECTORS = STREAM == 32 ? 1 : 4;               // of a lane, that are looked at together
     static constexpr int BATCH = VECTORS * 32 * Vec16<T>::N;           // values in them
     static constexpr int LIST = TOP ? BATCH + 64 : 1;
     uint64_t list[LIST];                   // candidates
-    int winners[TOP ? STREAM : 1];         // threads that hold some
+    int first[TOP ? STREAM : 1];           // vectors where the share of a thread begins that may hold some
     int count;
 };
-// What the streaming threads hand over: each warp's sums, each thread's maximum and the vector that it is in.
+// A thread's largest value and the vector that it is in, and the largest of the groups of vectors that it is not in.
+struct Best {
+    float value, second;
+    int vec;
+};
+// What the streaming threads hand over.
 struct LpHand {
     float m[LP_TEAM / 32], s[LP_TEAM / 32], t[LP_TEAM / 32];
-    float best[LP_TEAM];
-    int best_vec[LP_TEAM];
+    Best best[LP_TEAM];
 };
 // What the CTAs of a cluster leave in the shared memory of the first.
 struct LpParts {
@@ -240,7 +244,7 @@ template <class T> struct LpRow {
 
 // A group's values into the running sums, its maximum into `best`.
 template <class T, int THREADS, int U, bool ENTROPY, bool TOP>
-__device__ __forceinline__ void take_group(const uint4 (&q)[U], int v, Running<ENTROPY>& run, float& best, int& best_vec) {
+__device__ __forceinline__ void take_group(const uint4 (&q)[U], int v, Running<ENTROPY>& run, Best& best) {
     constexpr int VE = Vec16<T>::N;
     uint32_t w[U], all;
 #pragma unroll
@@ -249,11 +253,12 @@ __device__ __forceinline__ void take_group(const uint4 (&q)[U], int v, Running<E
         all = u == 0 ? w[0] : max_word<T>(all, w[u]);
     }
     const float top = word_max<T>(all);
-    if (TOP && top > best) {
-        best = top;
+    if (TOP) best.second = fmaxf(best.second, fminf(best.value, top));
+    if (TOP && top > best.value) {
+        best.value = top;
 #pragma unroll
         for (int u = U - 1; u >= 0; --u)
-            if (word_max<T>(w[u]) == top) best_vec = v + u * THREADS;
+            if (word_max<T>(w[u]) == top) best.vec = v + u * THREADS;
     }
     if (top > run.m) run.raise(top);
     const float low = run.floor_value();
@@ -352,11 +357,12 @@ __device__ __forceinline__ uint64_t kth_largest(uint64_t key, int k) {
 }
 
 // The rest of a row (or of its cluster rank's part), by one warp: joins the sums, adds the single elements, finds the k largest.
-// `high(i)`: an upper bound of the largest key of thread 32 i + lane, 0 where it has none.  `low`: lower bounds of the largest keys of
-// 32 disjoint parts of the row; the k-th largest of them bounds the k-th largest of all from below.
-template <class T, int STREAM, bool ENTROPY, bool TOP, class High>
-__device__ __forceinline__ void finish_part(const LpRow<T>& r, int k, float one, int lane, LpFinish<T, STREAM, TOP>& sh, uint64_t low, High&& high, float& m,
-                                            float& s, float& t, uint64_t& top) {
+// `best(i)` is what thread 32 i + lane has found.  The best values of 32 disjoint parts of the row, one a lane, are sorted; the k-th
+// of them bounds the k-th largest of all from below, so all candidates lie with the threads that reach it: in the group of vectors that
+// holds their best, and elsewhere in their share only where their second group reaches it, too.  `fetch(v)` reads a vector again.
+template <class T, int STREAM, bool ENTROPY, bool TOP, class GetBest, class Fetch>
+__device__ __forceinline__ void finish_part(const LpRow<T>& r, int k, float one, int lane, LpFinish<T, STREAM, TOP>& sh, GetBest&& best, Fetch&& fetch,
+                                            float& m, float& s, float& t, uint64_t& top) {
     constexpr int VE = Vec16<T>::N;
     if (r.singles > 0) {
         Running<ENTROPY> run;
@@ -372,16 +378,29 @@ __device__ __forceinline__ void finish_part(const LpRow<T>& r, int k, float one,
     join_lanes<ENTROPY>(m, s, t, 32);
     top = 0;
     if constexpr (TOP) {
+        using Finish = LpFinish<T, STREAM, TOP>;
+        // a bound of the thread's largest key from below (above, with `up`): the best value is somewhere in its vector
+        const auto bound_of = [&](const Best& f, int thread, bool up) {
+            return r.v0 + thread < r.v1 ? key_of(f.value, (uint32_t)(r.head + f.vec * VE + (up ? 0 : VE - 1))) : 0;
+        };
+        uint64_t low = 0;
+#pragma unroll
+        for (int i = 0; i < STREAM / 32; ++i) low = bigger(low, bound_of(best(i), 32 * i + lane, false));
         const uint64_t bound = kth_largest(low, k);
         __syncwarp();
-        int winners = 0;
+        int one_group = 0, whole = 0;      // threads of which a group of vectors, or all, are looked at
 #pragma unroll
         for (int i = 0; i < STREAM / 32; ++i) {
-            const uint64_t h = high(i);
-            const bool in = h != 0 && h >= bound;
-            const unsigned who = __ballot_sync(0xffffffffu, in);
-            if (in) sh.winners[winners + __popc(who & ((1u << lane) - 1))] = 32 * i + lane;
-            winners += __popc(who);
+            const Best f = best(i);
+            const int thread = 32 * i + lane;
+            const uint64_t high = bound_of(f, thread, true);
+            const bool in = high != 0 && high >= bound, all = in && key_of(f.second, 0) >= bound;
+            const unsigned some = __ballot_sync(0xffffffffu, in && !all), every = __ballot_sync(0xffffffffu, all), before = (1u << lane) - 1;
+            const int group = (f.vec - r.v0 - thread) / (LP_GROUP * STREAM);
+            if (in && !all) sh.first[one_group + __popc(some & before)] = r.v0 + thread + group * LP_GROUP * STREAM;
+            if (all) sh.first[STREAM - 1 - whole - __popc(every & before)] = r.v0 + thread;
+            one_group += __popc(some);
+            whole += __popc(every);
         }
         if (lane == 0) sh.count = 0;
         __syncwarp();
@@ -390,8 +409,6 @@ __device__ __forceinline__ void finish_part(const LpRow<T>& r, int k, float one,
             if (key >= bound) sh.list[atomicAdd(&sh.count, 1)] = key;
         };
         if (lane < r.singles) offer(one, (uint32_t)r.single(lane));
-        const int per = (r.v1 - r.v0 + STREAM - 1) / STREAM;      // vectors of a thread, the last perhaps not there
-        const int items = winners * per;
         bool merged = false;
         const auto merge = [&](int n) {
             for (int at = 0; at < n; at += 32) {
@@ -401,15 +418,23 @@ __device__ __forceinline__ void finish_part(const LpRow<T>& r, int k, float one,
                 merged = true;
             }
         };
-        using Finish = LpFinish<T, STREAM, TOP>;
+        const int per = (r.v1 - r.v0 + STREAM - 1) / STREAM;      // vectors of a thread, the last perhaps not there
+        const int items = one_group * LP_GROUP + whole * per;
         for (int base = 0; base < items; base += Finish::VECTORS * 32) {
             uint4 p[Finish::VECTORS];
             int at[Finish::VECTORS];
 #pragma unroll
             for (int u = 0; u < Finish::VECTORS; ++u) {
-                const int item = base + 32 * u + lane, w = item < items ? item / per : 0;
-                at[u] = item < items ? r.v0 + sh.winners[w] + (item - w * per) * STREAM : r.v1;
-                if (at[u] < r.v1) p[u] = __ldg(r.vec + at[u]);
+                int item = base + 32 * u + lane;
+                at[u] = r.v1;
+                if (item < one_group * LP_GROUP) {
+                    at[u] = sh.first[item / LP_GROUP] + item % LP_GROUP * STREAM;
+                } else if (item < items) {
+                    item -= one_group * LP_GROUP;
+                    const int w = item / per;
+                    at[u] = sh.first[STREAM - 1 - w] + (item - w * per) * STREAM;
+                }
+                if (at[u] < r.v1) p[u] = fetch(at[u]);
             }
 #pragma unroll
             for (int u = 0; u < Finish::VECTORS; ++u) {
@@ -476,7 +501,6 @@ __device__ __forceinline__ void write_row(const LpFwd& a, long long row, int lan
 // LP_TEAM threads another warp of the CTA does, while they are in the next row.
 template <class T, int THREADS, bool CLUSTER, bool ENTROPY, bool TOP>
 __global__ void __launch_bounds__(THREADS == 32 ? 128 : LP_TEAM + 32, THREADS == 32 ? 8 : 4) lp_forward_kernel(const LpFwd a) {
-    constexpr int VE = Vec16<T>::N;
     constexpr int TEAMS = THREADS == 32 ? 4 : 1;
     extern __shared__ uint4 ring[];         // [LP_STAGES][LP_GROUP][threads]
     __shared__ LpFinish<T, THREADS, TOP> finishing[TEAMS];
@@ -498,12 +522,6 @@ __global__ void __launch_bounds__(THREADS == 32 ? 128 : LP_TEAM + 32, THREADS ==
     }
     if (row >= a.rows) return;      // whole warps only, and warps of a CTA do not wait for one another
     LpFinish<T, THREADS, TOP>& sh = finishing[THREADS == 32 ? warp : 0];
-    const auto low_key = [&](const LpRow<T>& r, int thread, float best, int best_vec) {
-        return r.v0 + thread < r.v1 ? key_of(best, (uint32_t)(r.head + best_vec * VE + VE - 1)) : 0;
-    };
-    const auto high_key = [&](const LpRow<T>& r, int thread, float best, int best_vec) {
-        return r.v0 + thread < r.v1 ? key_of(best, (uint32_t)(r.head + best_vec * VE)) : 0;
-    };
     const bool finisher = warp == LP_TEAM / 32;
 
     if constexpr (THREADS > 32) if (finisher) {
@@ -524,14 +542,11 @@ __global__ void __launch_bounds__(THREADS == 32 ? 128 : LP_TEAM + 32, THREADS ==
             const LpHand& in = hand[buffer];
             const bool some = lane < LP_TEAM / 32;
             float m = some ? in.m[lane] : -INFINITY, s = some ? in.s[lane] : 0.f, tt = some ? in.t[lane] : 0.f;
-            uint64_t low = 0, top;
-            if (TOP) {
-#pragma unroll
-                for (int i = 0; i < LP_TEAM / 32; ++i) low = bigger(low, low_key(r, 32 * i + lane, in.best[32 * i + lane], in.best_vec[32 * i + lane]));
-            }
-            finish_part<T, LP_TEAM, ENTROPY, TOP>(r, a.k, one, lane, sh, low, [&](int i) {
-                return high_key(r, 32 * i + lane, in.best[32 * i + lane], in.best_vec[32 * i + lane]);
-            }, m, s, tt, top);
+            uint64_t top;
+            // A short part of a row is in shared memory as a whole.
+            const bool here = CLUSTER && r.groups(THREADS) <= LP_STAGES;
+            finish_part<T, THREADS, ENTROPY, TOP>(r, a.k, one, lane, sh, [&](int i) { return in.best[32 * i + lane]; },
+                                                  [&](int v) { return here ? ring[v - r.v0] : __ldg(r.vec + v); }, m, s, tt, top);
             __syncwarp();
             if (row + 2 * step < a.rows) bar_arrive<LP_EMPTY>(buffer);
             buffer ^= 1;
@@ -576,9 +591,8 @@ __global__ void __launch_bounds__(THREADS == 32 ? 128 : LP_TEAM + 32, THREADS ==
             if (lane < r.singles) one = to_float(r.x[r.single(lane)]);
         }
         Running<ENTROPY> run;
-        float best = -INFINITY;
-        int best_vec = r.v0 + t;
         int v = r.v0 + t;
+        Best best{-INFINITY, -INFINITY, v};
         for (int g = r.groups(THREADS); g > 0; --g) {
             stream.issue(a, t, rank, parts);
             cp_async_wait<LP_STAGES - 1>();
@@ -586,12 +600,12 @@ __global__ void __launch_bounds__(THREADS == 32 ? 128 : LP_TEAM + 32, THREADS ==
                 uint4 q[LP_GROUP];
 #pragma unroll
                 for (int u = 0; u < LP_GROUP; ++u) q[u] = read16(from + u * Stream::SLOT);
-                take_group<T, THREADS, LP_GROUP, ENTROPY, TOP>(q, v, run, best, best_vec);
+                take_group<T, THREADS, LP_GROUP, ENTROPY, TOP>(q, v, run, best);
             } else {
 #pragma unroll 1
                 for (int u = 0; u < LP_GROUP - 1 && v + u * THREADS < r.v1; ++u) {
                     const uint4 q[1] = {read16(from + u * Stream::SLOT)};
-                    take_group<T, THREADS, 1, ENTROPY, TOP>(q, v + u * THREADS, run, best, best_vec);
+                    take_group<T, THREADS, 1, ENTROPY, TOP>(q, v + u * THREADS, run, best);
                 }
             }
             from = from == stream.first + Stream::RING - Stream::STAGE ? stream.first : from + Stream::STAGE;
@@ -601,8 +615,7 @@ __global__ void __launch_bounds__(THREADS == 32 ? 128 : LP_TEAM + 32, THREADS ==
         run.finish(&s, &tt);
         if constexpr (THREADS == 32) {
             uint64_t top;
-            finish_part<T, 32, ENTROPY, TOP>(r, a.k, one, lane, sh, TOP ? low_key(r, t, best, best_vec) : 0,
-                                             [&](int) { return high_key(r, t, best, best_vec); }, m, s, tt, top);
+            finish_part<T, 32, ENTROPY, TOP>(r, a.k, one, lane, sh, [&](int) { return best; }, [&](int v) { return __ldg(r.vec + v); }, m, s, tt, top);
             write_row<ENTROPY, TOP>(a, row, lane, m, s, tt, top, target, at_target);
         } else {
             join_lanes<ENTROPY>(m, s, tt, 32);
@@ -610,7 +623,7 @@ __global__ void __launch_bounds__(THREADS == 32 ? 128 : LP_TEAM + 32, THREADS ==
             bar_sync<LP_EMPTY>(buffer);
             LpHand& out = hand[buffer];
             if (lane == 0) { out.m[warp] = m; out.s[warp] = s; out.t[warp] = tt; }
-            if (TOP) { out.best[t] = best; out.best_vec[t] = best_vec; }
+            if (TOP) out.best[t] = best;
             __syncwarp();
             bar_arrive<LP_FULL>(buffer);
             buffer ^= 1;
@@ -820,7 +833,7 @@ int adder_b200_log_probs_forward(const void* logits, int dtype, long long rows, 
         if (classes <= 1024 || (classes <= 8192 && rows >= 24LL * sm_count())) return choose_forward<T, 32, false>(a, 1, s);
         // Few rows leave SMs idle: a row is then split over a cluster of up to 8 CTAs of at least 4096 elements.
         int parts = 1;
-        while (parts < 8 && rows * parts * 2 <= sm_count() * 2 && classes >= 8192LL * parts) parts *= 2;
+        while (parts < 8 && rows * parts * 2 <= sm_count() * 4 && classes >= 8192LL * parts) parts *= 2;
         if (parts > 1) return choose_forward<T, LP_TEAM, true>(a, parts, s);
         return choose_forward<T, LP_TEAM, false>(a, 1, s);
     });
