@@ -5,12 +5,16 @@
 //   dw = sum over rows of dy xh, db = sum over rows of dy
 //
 // Bound by memory: x (and the residual) read, y (and h) written; h and dy (and dh) read, dx written.  A row is held in the registers of
-// the threads that share it, so it is read once; its variance is taken about its mean, in a second pass over the registers.
+// the threads that share it, so it is read once; a thread keeps its columns from row to row, and with them the weights and, in the
+// backward pass, its sums of dw and db, which are added up over the CTAs by a second kernel, always in the same order.
 #include "kernels.h"
 #include "elements.cuh"
 #include <cooperative_groups.h>
 #include <algorithm>
 #include <cmath>
+#include <map>
+#include <mutex>
+#include <tuple>
 #include <initializer_list>
 #include <type_traits>
 
@@ -64,137 +68,427 @@ template <class T, int N> __device__ __forceinline__ void store_some(T* p, const
     else *reinterpret_cast<uint4*>(p) = Vec16<T>::pack(f);
 }
 
-// Sum over the G threads of a team; `part` is that team's own shared memory and is free again after the next barrier.
+// Sum over the threads of a CTA; `part` is free again after the next barrier.
 template <int G> __device__ __forceinline__ float team_sum(float v, float* part, int t) {
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
-    if constexpr (G > 32) {
-        if ((t & 31) == 0) part[t >> 5] = v;
-        __syncthreads();
-        v = part[0];
+    if ((t & 31) == 0) part[t >> 5] = v;
+    __syncthreads();
+    v = part[0];
 #pragma unroll
-        for (int i = 1; i < G / 32; ++i) v += part[i];
-    }
+    for (int i = 1; i < G / 32; ++i) v += part[i];
     return v;
 }
 
-template <int G> constexpr int LN_TEAMS = G >= 128 ? 1 : 128 / G;      // teams of a CTA
+// Vectors of a row that belong to a CTA of a cluster (all, without one): first and end.
+template <bool CLUSTER> __device__ __forceinline__ int2 share_of(int nvec) {
+    if constexpr (!CLUSTER) return make_int2(0, nvec);
+    const long long rank = cg::this_cluster().block_rank(), parts = cg::this_cluster().num_blocks();
+    return make_int2((int)(nvec * rank / parts), (int)(nvec * (rank + 1) / parts));
+}
 
-// A team of G threads a row, VEC consecutive elements at a time, NV times.
-template <class T, class W, int G, int VEC, int NV>
-__global__ void __launch_bounds__(G * LN_TEAMS<G>) ln_forward_kernel(const LnFwd a) {
-    __shared__ float part[2][G / 32];
-    const int t = threadIdx.x % G;
-    const long long row = (long long)blockIdx.x * LN_TEAMS<G> + threadIdx.x / G;
-    if (row >= a.rows) return;      // whole warps: a team of more is a CTA
-    const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
-    float f[NV][VEC];
-    float sum = 0.f;
+template <int TEAMS, int G> __device__ __forceinline__ void team_barrier(int team) {
+    if constexpr (G == 32) __syncwarp();
+    else if constexpr (TEAMS == 1) __syncthreads();
+    else asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "n"(G) : "memory");
+}
+
+// Shapes of the kernels that hold rows in registers: a team of G threads a row (times the cluster's size), NV vectors of VEC consecutive
+// elements a thread, a thread's next STAGES - 1 rows on their way through shared memory.  A thread copies what it reads itself, so only the
+// sums of a row need a barrier.  STAGES = 0: elements are loaded when they are needed, one at a time.
+template <class T_, class W_, int G_, int VEC_, int NV_, int STAGES_, bool CLUSTER_> struct LnShape {
+    using T = T_;
+    using W = W_;
+    static constexpr int G = G_, VEC = VEC_, NV = NV_, STAGES = STAGES_;
+    static constexpr bool CLUSTER = CLUSTER_;
+    static constexpr int THREADS = G > 256 ? G : 256, TEAMS = THREADS / G, WARPS = G / 32;
+    static constexpr int LINE = THREADS * 16;      // bytes of one vector of each thread
+    static size_t ring(int arrays) { return (size_t)STAGES * arrays * NV * LINE; }
+};
+
+// A thread's values of a row are held as pairs of fp32, which one instruction adds or multiplies: P pairs of each vector, or, element by
+// element, of two elements.
+template <class S> struct LnPairs {
+    static constexpr int P = S::NV * S::VEC / 2;
+    uint64_t p[P];
+};
+// Whether the pair's vector (element by element: its first element) is in the row.
+template <class S> __device__ __forceinline__ bool ln_in(int pair, int v, int v1) { return v + (2 * pair / S::VEC) * S::G < v1; }
+
+// Copies of one array's part of a row into a thread's slots, and out of them; zeros where there is no element.
+template <class S> __device__ __forceinline__ void ln_issue(uint32_t slot, const typename S::T* row, int v, int v1) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int c = (i * G + t) * VEC;
-        if (c < a.d) {
-            load_some<T, VEC>(x + c, f[i]);
-        } else {
+    for (int i = 0; i < S::NV; ++i)
+        if (v + i * S::G < v1)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(slot + i * S::LINE), "l"(row + (size_t)(v + i * S::G) * S::VEC) : "memory");
+}
+template <class S> __device__ __forceinline__ void ln_fetch(LnPairs<S>& f, uint32_t slot, const typename S::T* row, int v, int v1) {
+    using T = typename S::T;
+    if constexpr (S::STAGES > 0) {
+        uint4 q[S::NV];
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) f[i][j] = 0.f;
+        for (int i = 0; i < S::NV; ++i) {
+            q[i] = make_uint4(0, 0, 0, 0);
+            if (v + i * S::G < v1)
+                asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(q[i].x), "=r"(q[i].y), "=r"(q[i].z), "=r"(q[i].w) : "r"(slot + i * S::LINE) : "memory");
         }
-    }
-    if (a.residual != nullptr) {
-        const T* r = static_cast<const T*>(a.residual) + row * a.r_stride;
-        T* h = static_cast<T*>(a.h) + row * (long long)a.d;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int c = (i * G + t) * VEC;
-            if (c < a.d) {
-                float g[VEC];
-                load_some<T, VEC>(r + c, g);
+        for (int i = 0; i < S::NV; ++i) {
+            float e[S::VEC];
+            Vec16<T>::unpack(q[i], e);
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) f[i][j] = to_float(from_float<T>(f[i][j] + g[j]));      // the norm is taken of what is stored
-                store_some<T, VEC>(h + c, f[i]);
-            }
+            for (int j = 0; j < S::VEC; j += 2) f.p[(i * S::VEC + j) / 2] = pack2(e[j], e[j + 1]);
         }
-    }
+    } else {
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) sum += f[i][j];
-    const float mean = team_sum<G>(sum, part[0], t) / a.d;
-    float sq = 0.f;
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-        if ((i * G + t) * VEC < a.d) {
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) sq += (f[i][j] - mean) * (f[i][j] - mean);
-        }
-    const float rs = 1.f / sqrtf(team_sum<G>(sq, part[1], t) / a.d + a.eps);
-    if (t == 0 && a.mean != nullptr) { a.mean[row] = mean; a.rstd[row] = rs; }
-    T* y = static_cast<T*>(a.y) + row * (long long)a.d;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int c = (i * G + t) * VEC;
-        if (c < a.d) {
-            float w[VEC], b[VEC];
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) { w[j] = 1.f; b[j] = 0.f; }
-            if (a.w != nullptr) load_some<W, VEC>(static_cast<const W*>(a.w) + c, w);
-            if (a.b != nullptr) load_some<W, VEC>(static_cast<const W*>(a.b) + c, b);
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) f[i][j] = fmaf((f[i][j] - mean) * rs, w[j], b[j]);
-            store_some<T, VEC>(y + c, f[i]);
+        for (int i = 0; i < S::NV; i += 2) {
+            const float lo = v + i * S::G < v1 ? to_float(row[v + i * S::G]) : 0.f;
+            const float hi = v + (i + 1) * S::G < v1 ? to_float(row[v + (i + 1) * S::G]) : 0.f;
+            f.p[i / 2] = pack2(lo, hi);
         }
     }
 }
+template <class S> __device__ __forceinline__ void ln_store(typename S::T* row, const LnPairs<S>& f, int v, int v1) {
+    using T = typename S::T;
+    if constexpr (S::VEC > 1) {
+#pragma unroll
+        for (int i = 0; i < S::NV; ++i)
+            if (v + i * S::G < v1) {
+                float e[S::VEC];
+#pragma unroll
+                for (int j = 0; j < S::VEC; j += 2) unpack2(f.p[(i * S::VEC + j) / 2], e[j], e[j + 1]);
+                *reinterpret_cast<uint4*>(row + (size_t)(v + i * S::G) * S::VEC) = Vec16<T>::pack(e);
+            }
+    } else {
+#pragma unroll
+        for (int i = 0; i < S::NV; i += 2) {
+            float lo, hi;
+            unpack2(f.p[i / 2], lo, hi);
+            if (v + i * S::G < v1) row[v + i * S::G] = from_float<T>(lo);
+            if (v + (i + 1) * S::G < v1) row[v + (i + 1) * S::G] = from_float<T>(hi);
+        }
+    }
+}
+template <class S> __device__ __forceinline__ void ln_weights(LnPairs<S>& f, const void* w, float missing, int v, int v1) {
+    float e[S::NV][S::VEC];
+#pragma unroll
+    for (int i = 0; i < S::NV; ++i) {
+#pragma unroll
+        for (int j = 0; j < S::VEC; ++j) e[i][j] = missing;
+        if (w != nullptr && v + i * S::G < v1) load_some<typename S::W, S::VEC>(static_cast<const typename S::W*>(w) + (size_t)(v + i * S::G) * S::VEC, e[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < LnPairs<S>::P; ++i) f.p[i] = pack2((&e[0][0])[2 * i], (&e[0][0])[2 * i + 1]);
+}
 
-template <class T, class W, int G, int VEC, int NV>
-__global__ void __launch_bounds__(G * LN_TEAMS<G>) ln_dx_kernel(const LnBwd a) {
-    __shared__ float part[2][G / 32];
-    const int t = threadIdx.x % G;
-    const long long row = (long long)blockIdx.x * LN_TEAMS<G> + threadIdx.x / G;
-    if (row >= a.rows) return;
-    const T* h = static_cast<const T*>(a.h) + row * a.h_stride;
-    const T* dy = static_cast<const T*>(a.dy) + row * (long long)a.d;
-    const float mean = a.mean[row], rs = a.rstd[row];
-    float g[NV][VEC], xh[NV][VEC];
-    float s1 = 0.f, s2 = 0.f;
+// Which rows a team takes, and the ring of the rows on their way.
+template <class S> struct LnWalk {
+    long long row, ahead, step;      // the next to be read, the next to be copied
+    uint32_t ring, fill, read;       // bytes
+    int arrays;
+
+    __device__ __forceinline__ void start(void* smem, int arrays_) {
+        const long long parts = S::CLUSTER ? (long long)cg::this_cluster().num_blocks() : 1;
+        row = ahead = blockIdx.x / parts * S::TEAMS + threadIdx.x / S::G;
+        step = gridDim.x / parts * S::TEAMS;
+        ring = fill = read = smem_u32(smem) + threadIdx.x * 16;
+        arrays = arrays_;
+    }
+    __device__ __forceinline__ uint32_t advance(uint32_t at) const {
+        const uint32_t stage = (uint32_t)arrays * S::NV * S::LINE, last = S::STAGES > 1 ? S::STAGES - 1 : 0;
+        return at == ring + last * stage ? ring : at + stage;
+    }
+    static __device__ __forceinline__ uint32_t slot(uint32_t at, int array) { return at + array * S::NV * S::LINE; }
+};
+
+// Exchange of a row's sums between the warps of a team, and between the CTAs of a cluster.
+template <class S> struct LnSums {
+    float2 part[2][S::TEAMS][S::WARPS];
+    float2 ranks[2][8];
+    float2 count[S::WARPS];      // elements of a row that each warp holds, and one over that (0 where it holds none)
+    float2 rank_count[8];        // and each CTA of the cluster
+};
+
+__device__ __forceinline__ float2 count_of(int n) { return make_float2((float)n, n > 0 ? 1.f / (float)n : 0.f); }
+template <class S> __device__ __forceinline__ void ln_count(LnSums<S>& sh, int v0, int v1, int nvec) {
+    if (threadIdx.x < S::WARPS) {
+        int n = 0;
+        for (int i = 0; i < S::NV; ++i) n += max(0, min(32, v1 - (v0 + i * S::G + 32 * (int)threadIdx.x)));
+        sh.count[threadIdx.x] = count_of(n * S::VEC);
+    }
+    if constexpr (S::CLUSTER) {
+        const long long parts = cg::this_cluster().num_blocks(), i = threadIdx.x;
+        if (i < parts) sh.rank_count[i] = count_of((int)(nvec * (i + 1) / parts - nvec * i / parts) * S::VEC);
+        cg::this_cluster().sync();      // the others are there to be written to
+    } else {
+        __syncthreads();
+    }
+}
+
+template <int LANES> __device__ __forceinline__ float lanes_sum(float v) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int c = (i * G + t) * VEC;
-        if (c < a.d) {
-            float w[VEC];
+    for (int off = LANES / 2; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+    return v;
+}
+// A pair (a, b) of every warp of the team, in lane i % WARPS of every warp that of warp i.  `turn` alternates, so that one barrier a row is
+// enough: who writes a row's pairs has seen the barrier after all had read those of the row before the last.
+template <class S> __device__ __forceinline__ float2 ln_exchange(float a, float b, LnSums<S>& sh, int team, int t, int turn) {
+    if ((t & 31) == 0) sh.part[turn][team][t >> 5] = make_float2(a, b);
+    team_barrier<S::TEAMS, S::G>(team);
+    return sh.part[turn][team][t % S::WARPS];
+}
+// The same over the CTAs of a cluster, in lane i % 8; zeros beyond its size.
+template <class S> __device__ __forceinline__ float2 ln_exchange_ranks(float a, float b, LnSums<S>& sh, int t, int turn) {
+    cg::cluster_group cluster = cg::this_cluster();
+    const int parts = (int)cluster.num_blocks();
+    if (t < parts) cluster.map_shared_rank(&sh.ranks[turn][0], t)[cluster.block_rank()] = make_float2(a, b);
+    cluster.sync();
+    return t % 8 < parts ? sh.ranks[turn][t % 8] : make_float2(0.f, 0.f);
+}
+
+// Two sums at once, over all threads that share the row.
+template <class S> __device__ __forceinline__ float2 ln_sum2(float a, float b, LnSums<S>& sh, int team, int t, int turn) {
+    a = lanes_sum<32>(a);
+    b = lanes_sum<32>(b);
+    if constexpr (S::WARPS > 1) {
+        const float2 p = ln_exchange<S>(a, b, sh, team, t, turn);
+        a = lanes_sum<S::WARPS>(p.x);
+        b = lanes_sum<S::WARPS>(p.y);
+    }
+    if constexpr (S::CLUSTER) {
+        const float2 p = ln_exchange_ranks<S>(a, b, sh, t, turn);
+        a = lanes_sum<8>(p.x);
+        b = lanes_sum<8>(p.y);
+    }
+    return make_float2(a, b);
+}
+
+// Mean and sum of squared differences from it: each warp has both of its own elements, and what the warps' means differ from the whole one
+// by comes on top, so one barrier does and nothing cancels.
+template <class S> __device__ __forceinline__ float2 ln_moments(const LnPairs<S>& f, int v, int v1, float inv_d, LnSums<S>& sh, int team, int t, int turn) {
+    uint64_t sum2 = 0;
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) w[j] = 1.f;
-            load_some<T, VEC>(h + c, xh[i]);
-            load_some<T, VEC>(dy + c, g[i]);
-            if (a.w != nullptr) load_some<W, VEC>(static_cast<const W*>(a.w) + c, w);
+    for (int i = 0; i < LnPairs<S>::P; ++i) sum2 = add2(sum2, f.p[i]);      // zeros where there is no element
+    float lo, hi;
+    unpack2(sum2, lo, hi);
+    const float sum = lanes_sum<32>(lo + hi);
+    constexpr bool one = S::WARPS == 1 && !S::CLUSTER;
+    const float mine = sum * (one ? inv_d : sh.count[t >> 5].y);
+    const uint64_t minus = pack2(-mine, -mine);
+    uint64_t sq2 = 0;
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                g[i][j] *= w[j];
-                xh[i][j] = (xh[i][j] - mean) * rs;
-                s1 += g[i][j];
-                s2 = fmaf(g[i][j], xh[i][j], s2);
+    for (int i = 0; i < LnPairs<S>::P; ++i) {
+        if constexpr (S::VEC > 1) {
+            if (ln_in<S>(i, v, v1)) {
+                const uint64_t e = add2(f.p[i], minus);
+                sq2 = fma2(e, e, sq2);
             }
+        } else {
+            float a, b;
+            unpack2(add2(f.p[i], minus), a, b);
+            const uint64_t e = pack2(v + 2 * i * S::G < v1 ? a : 0.f, v + (2 * i + 1) * S::G < v1 ? b : 0.f);
+            sq2 = fma2(e, e, sq2);
         }
     }
-    s1 = team_sum<G>(s1, part[0], t) / a.d;
-    s2 = team_sum<G>(s2, part[1], t) / a.d;
-    T* dx = static_cast<T*>(a.dx) + row * (long long)a.d;
+    unpack2(sq2, lo, hi);
+    float sq = lanes_sum<32>(lo + hi), mean = mine;
+    if constexpr (!one) {
+        float2 p = ln_exchange<S>(sum, sq, sh, team, t, turn), n = sh.count[t % S::WARPS];
+        float all = lanes_sum<S::WARPS>(p.x), held = 0.f;
+        if constexpr (S::CLUSTER) held = sh.rank_count[cg::this_cluster().block_rank()].y;
+        mean = all * (S::CLUSTER ? held : inv_d);
+        float e = p.x * n.y - mean;
+        sq = lanes_sum<S::WARPS>(fmaf(n.x * e, e, p.y));
+        if constexpr (S::CLUSTER) {
+            p = ln_exchange_ranks<S>(all, sq, sh, t, turn);
+            n = t % 8 < (int)cg::this_cluster().num_blocks() ? sh.rank_count[t % 8] : make_float2(0.f, 0.f);
+            mean = lanes_sum<8>(p.x) * inv_d;
+            e = p.x * n.y - mean;
+            sq = lanes_sum<8>(fmaf(n.x * e, e, p.y));
+        }
+    }
+    return make_float2(mean, sq);
+}
+
+// 1 / sqrt(x), the approximate one and a step of Newton's method.
+__device__ __forceinline__ float inverse_root(float x) {
+    const float r = rsqrtf(x);
+    return r * fmaf(-0.5f * x * r, r, 1.5f);
+}
+
+template <class S> __global__ void __launch_bounds__(S::THREADS, S::THREADS > 256 ? 1 : 3) ln_forward_kernel(const LnFwd a) {
+    extern __shared__ uint4 smem[];
+    __shared__ LnSums<S> sh;
+    using T = typename S::T;
+    constexpr int P = LnPairs<S>::P;
+    const int t = threadIdx.x % S::G, team = threadIdx.x / S::G;
+    const int2 share = share_of<S::CLUSTER>(a.d / S::VEC);
+    const int v = share.x + t, v1 = share.y;
+    const float inv_d = 1.f / a.d;
+    LnWalk<S> walk;
+    walk.start(smem, a.residual != nullptr ? 2 : 1);
+    const auto issue = [&] {
+        if (walk.ahead < a.rows) {
+            ln_issue<S>(walk.slot(walk.fill, 0), static_cast<const T*>(a.x) + walk.ahead * a.x_stride, v, v1);
+            if (a.residual != nullptr) ln_issue<S>(walk.slot(walk.fill, 1), static_cast<const T*>(a.residual) + walk.ahead * a.r_stride, v, v1);
+            walk.ahead += walk.step;
+        }
+        cp_async_commit();
+        walk.fill = walk.advance(walk.fill);
+    };
+    if constexpr (S::STAGES > 0)
+        for (int i = 0; i < S::STAGES - 1; ++i) issue();
+    ln_count<S>(sh, share.x, share.y, a.d / S::VEC);
+    LnPairs<S> w, b;
+    ln_weights<S>(w, a.w, 1.f, v, v1);
+    ln_weights<S>(b, a.b, 0.f, v, v1);
+    int turn = 0;
+    for (; walk.row < a.rows; walk.row += walk.step) {
+        if constexpr (S::STAGES > 0) {
+            issue();
+            cp_async_wait<(S::STAGES > 0 ? S::STAGES - 1 : 0)>();
+        }
+        const long long row = walk.row;
+        LnPairs<S> f;
+        ln_fetch<S>(f, walk.slot(walk.read, 0), static_cast<const T*>(a.x) + row * a.x_stride, v, v1);
+        if (a.residual != nullptr) {
+            LnPairs<S> r;
+            ln_fetch<S>(r, walk.slot(walk.read, 1), static_cast<const T*>(a.residual) + row * a.r_stride, v, v1);
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int c = (i * G + t) * VEC;
-        if (c < a.d) {
-            float o[VEC];
+            for (int i = 0; i < P; ++i) {
+                f.p[i] = add2(f.p[i], r.p[i]);
+                if constexpr (sizeof(T) == 2) {      // the norm is taken of what is stored
+                    float lo, hi;
+                    unpack2(f.p[i], lo, hi);
+                    const float2 held = unpack_pair<T>(pack_pair<T>(lo, hi));
+                    f.p[i] = pack2(held.x, held.y);
+                }
+            }
+            ln_store<S>(static_cast<T*>(a.h) + row * a.d, f, v, v1);
+        }
+        if constexpr (S::STAGES > 0) walk.read = walk.advance(walk.read);
+        const float2 mom = ln_moments<S>(f, v, v1, inv_d, sh, team, t, turn);
+        turn ^= 1;
+        const float rs = inverse_root(mom.y * inv_d + a.eps);
+        if (a.mean != nullptr && t == 0 && share.x == 0) { a.mean[row] = mom.x; a.rstd[row] = rs; }
+        const uint64_t minus = pack2(-mom.x, -mom.x), scale = pack2(rs, rs);
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) o[j] = rs * (g[i][j] - s1 - xh[i][j] * s2);
+        for (int i = 0; i < P; ++i) f.p[i] = fma2(fma2(add2(f.p[i], minus), scale, 0), w.p[i], b.p[i]);
+        ln_store<S>(static_cast<T*>(a.y) + row * a.d, f, v, v1);
+    }
+    if constexpr (S::CLUSTER) cg::this_cluster().sync();      // no CTA leaves while its shared memory is written
+}
+
+// dx of every row; with SUMS this thread's columns of dw and db, added up over its rows and then over the CTA's teams into
+// part[CTA or cluster][2][d].
+template <class S, bool SUMS> __global__ void __launch_bounds__(S::THREADS, S::THREADS > 256 ? 1 : 2) ln_backward_kernel(const LnBwd a, float* part) {
+    extern __shared__ uint4 smem[];
+    __shared__ LnSums<S> sh;
+    using T = typename S::T;
+    const int t = threadIdx.x % S::G, team = threadIdx.x / S::G;
+    const int2 share = share_of<S::CLUSTER>(a.d / S::VEC);
+    const int v = share.x + t, v1 = share.y;
+    if constexpr (S::CLUSTER) cg::this_cluster().sync();      // the others are there to be written to
+    LnWalk<S> walk;
+    walk.start(smem, a.dh != nullptr ? 3 : 2);
+    const auto issue = [&] {
+        if (walk.ahead < a.rows) {
+            ln_issue<S>(walk.slot(walk.fill, 0), static_cast<const T*>(a.h) + walk.ahead * a.h_stride, v, v1);
+            ln_issue<S>(walk.slot(walk.fill, 1), static_cast<const T*>(a.dy) + walk.ahead * a.d, v, v1);
+            if (a.dh != nullptr) ln_issue<S>(walk.slot(walk.fill, 2), static_cast<const T*>(a.dh) + walk.ahead * a.d, v, v1);
+            walk.ahead += walk.step;
+        }
+        cp_async_commit();
+        walk.fill = walk.advance(walk.fill);
+    };
+    if constexpr (S::STAGES > 0)
+        for (int i = 0; i < S::STAGES - 1; ++i) issue();
+    constexpr int P = LnPairs<S>::P;
+    const float inv_d = 1.f / a.d;
+    LnPairs<S> w, dw, db;
+    ln_weights<S>(w, a.w, 1.f, v, v1);
+#pragma unroll
+    for (int i = 0; i < P; ++i) dw.p[i] = db.p[i] = 0;
+    float mean = 0.f, rs = 0.f;
+    if (walk.row < a.rows) { mean = a.mean[walk.row]; rs = a.rstd[walk.row]; }
+    int turn = 0;
+    for (; walk.row < a.rows; walk.row += walk.step) {
+        if constexpr (S::STAGES > 0) {
+            issue();
+            cp_async_wait<(S::STAGES > 0 ? S::STAGES - 1 : 0)>();
+        }
+        const long long row = walk.row, next = row + walk.step;
+        float mean_next = 0.f, rs_next = 0.f;
+        if (next < a.rows) { mean_next = a.mean[next]; rs_next = a.rstd[next]; }
+        LnPairs<S> xh, g;
+        ln_fetch<S>(xh, walk.slot(walk.read, 0), static_cast<const T*>(a.h) + row * a.h_stride, v, v1);
+        ln_fetch<S>(g, walk.slot(walk.read, 1), static_cast<const T*>(a.dy) + row * a.d, v, v1);
+        uint64_t s1 = 0, s2 = 0;
+        const uint64_t minus = pack2(-mean, -mean), scale = pack2(rs, rs);
+#pragma unroll
+        for (int i = 0; i < P; ++i) {      // dy is 0 where there is no element
+            xh.p[i] = fma2(add2(xh.p[i], minus), scale, 0);
+            if (SUMS) {
+                dw.p[i] = fma2(g.p[i], xh.p[i], dw.p[i]);
+                db.p[i] = add2(db.p[i], g.p[i]);
+            }
+            g.p[i] = fma2(g.p[i], w.p[i], 0);
+            s1 = add2(s1, g.p[i]);
+            s2 = fma2(g.p[i], xh.p[i], s2);
+        }
+        if (a.dx != nullptr) {
+            float a1, b1, a2, b2;
+            unpack2(s1, a1, b1);
+            unpack2(s2, a2, b2);
+            const float2 m = ln_sum2<S>(a1 + b1, a2 + b2, sh, team, t, turn);
+            turn ^= 1;
+            const float c1 = -m.x * inv_d, c2 = -m.y * inv_d;
+            const uint64_t shift = pack2(c1, c1), slope = pack2(c2, c2);
+#pragma unroll
+            for (int i = 0; i < P; ++i) g.p[i] = fma2(fma2(xh.p[i], slope, add2(g.p[i], shift)), scale, 0);
             if (a.dh != nullptr) {
-                float e[VEC];
-                load_some<T, VEC>(static_cast<const T*>(a.dh) + row * (long long)a.d + c, e);
+                LnPairs<S> e;
+                ln_fetch<S>(e, walk.slot(walk.read, 2), static_cast<const T*>(a.dh) + row * a.d, v, v1);
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) o[j] += e[j];
+                for (int i = 0; i < P; ++i) g.p[i] = add2(g.p[i], e.p[i]);
             }
-            store_some<T, VEC>(dx + c, o);
+            ln_store<S>(static_cast<T*>(a.dx) + row * a.d, g, v, v1);
+        }
+        if constexpr (S::STAGES > 0) walk.read = walk.advance(walk.read);
+        mean = mean_next; rs = rs_next;
+    }
+    if constexpr (SUMS) {
+        const int parts = S::CLUSTER ? (int)cg::this_cluster().num_blocks() : 1;
+        float* out = part + (size_t)(blockIdx.x / parts) * 2 * a.d;
+        // one team writes its sums to the workspace, several add them up in their order, in shared memory
+        float* to = out;
+        if constexpr (S::TEAMS > 1) {
+            cp_async_wait<0>();
+            __syncthreads();
+            to = reinterpret_cast<float*>(smem) + team * 2 * a.d;
+        }
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            float lo, hi;
+            const int c = S::VEC > 1 ? (v + 2 * i / S::VEC * S::G) * S::VEC + 2 * i % S::VEC : v + 2 * i * S::G, c2 = S::VEC > 1 ? c + 1 : c + S::G;
+            const bool in = ln_in<S>(i, v, v1), in2 = S::VEC > 1 ? in : c2 < v1;
+            unpack2(dw.p[i], lo, hi);
+            if (in) to[c] = lo;
+            if (in2) to[c2] = hi;
+            unpack2(db.p[i], lo, hi);
+            if (in) to[a.d + c] = lo;
+            if (in2) to[a.d + c2] = hi;
+        }
+        if constexpr (S::TEAMS > 1) {
+            __syncthreads();
+            for (int c = threadIdx.x; c < 2 * a.d; c += S::THREADS) {
+                float sum = 0.f;
+                for (int i = 0; i < S::TEAMS; ++i) sum += reinterpret_cast<float*>(smem)[i * 2 * a.d + c];
+                out[c] = sum;
+            }
         }
     }
+    if constexpr (S::CLUSTER) cg::this_cluster().sync();
 }
 
 // ------------------------------------------------------------------------------------------ rows too long for registers
@@ -291,16 +585,23 @@ template <class T> __global__ void __launch_bounds__(LN_COLS * LN_LANES) ln_colu
     }
 }
 
-template <class W> __global__ void __launch_bounds__(256) ln_columns_finish_kernel(const float* part, int splits, int d, W* dw, W* db) {
-    const int c = blockIdx.x * 256 + threadIdx.x;
-    if (c >= d) return;
-    float w = 0.f, b = 0.f;
-    for (int s = 0; s < splits; ++s) {
-        w += part[((long long)s * 2) * d + c];
-        b += part[((long long)s * 2 + 1) * d + c];
+// Sums of the columns of part[parts][2][d]: a CTA has 32 columns, 32 lanes of every 32nd part each.
+template <class W> __global__ void __launch_bounds__(1024) ln_columns_finish_kernel(const float* part, int parts, int d, W* dw, W* db) {
+    __shared__ float sums[32][33];
+    const int c = blockIdx.x * 32 + threadIdx.x % 32, line = threadIdx.x / 32;
+    float s = 0.f;
+    if (c < 2 * d)
+        for (int p = line; p < parts; p += 32) s += part[(size_t)p * 2 * d + c];
+    sums[line][threadIdx.x % 32] = s;
+    __syncthreads();
+    s = sums[threadIdx.x % 32][line];      // lanes of a warp: the lines of one column
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
+    const int column = blockIdx.x * 32 + line;
+    if (threadIdx.x % 32 == 0 && column < 2 * d) {
+        if (column < d) { if (dw != nullptr) dw[column] = from_float<W>(s); }
+        else if (db != nullptr) db[column - d] = from_float<W>(s);
     }
-    if (dw != nullptr) dw[c] = from_float<W>(w);
-    if (db != nullptr) db[c] = from_float<W>(b);
 }
 
 // ------------------------------------------------------------------------------------------ host
@@ -312,17 +613,21 @@ int ln_splits(long long rows, int d) {
     return (int)std::max(1LL, std::min(splits, 1024LL));
 }
 
-template <class Args, class Kernel> int launch_long(const Args& a, Kernel kernel, cudaStream_t s) {
+int ln_most_parts(long long rows) { return (int)std::min(rows, 4LL * sm_count()); }
+
+// Launches `kernel` in clusters of `parts` CTAs (1: none).
+template <class Kernel, class... Args> int launch_clusters(Kernel kernel, unsigned grid, unsigned threads, size_t smem, int parts, cudaStream_t s, const Args&... args) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(a.rows * 8));
-    cfg.blockDim = dim3(LN_LONG);
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = 8; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    attr[0].val.clusterDim.x = parts; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    if (cudaLaunchKernelEx(&cfg, kernel, a) != cudaSuccess) {
+    cfg.numAttrs = parts > 1 ? 1 : 0;
+    if (cudaLaunchKernelEx(&cfg, kernel, args...) != cudaSuccess) {
         (void)cudaGetLastError();
         return ADDER_ERR_CUDA;
     }
@@ -330,20 +635,71 @@ template <class Args, class Kernel> int launch_long(const Args& a, Kernel kernel
     return ADDER_OK;
 }
 
-// A launch of the kernel whose registers hold a row of d elements, by f(G, VEC, NV) as integral constants; false: none does.
-template <int N> using Int = std::integral_constant<int, N>;
-template <int VE, class F> bool by_width(int d, bool vectors, F&& f) {
+// CTAs of a kernel that fit on an SM, remembered for each kernel and device.
+int resident(const void* kernel, int threads, size_t smem) {
+    static std::mutex mu;
+    static std::map<std::tuple<const void*, int, size_t>, int> known;
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return 1;
+    std::lock_guard<std::mutex> lock(mu);
+    auto it = known.find({kernel, dev, smem});
+    if (it == known.end()) {
+        int n = 0;
+        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, smem) != cudaSuccess) (void)cudaGetLastError();
+        it = known.emplace(std::make_tuple(kernel, dev, smem), std::max(n, 1)).first;
+    }
+    return it->second;
+}
+
+// CTAs (clusters of `parts`) that share `rows`: as many as are resident, and no more than there are rows for.
+template <class S> long long ln_groups(const void* kernel, size_t smem, long long rows, int parts) {
+    const long long most = std::min(4LL, (long long)resident(kernel, S::THREADS, smem)) * sm_count() / parts;
+    return std::max(1LL, std::min(most, (rows + S::TEAMS - 1) / S::TEAMS));
+}
+
+template <class S> int launch_forward(const LnFwd& a, int parts, cudaStream_t s) {
+    const auto kernel = ln_forward_kernel<S>;
+    const size_t smem = S::ring(a.residual != nullptr ? 2 : 1);
+    const int st = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), smem);
+    if (st != ADDER_OK) return st;
+    const long long groups = ln_groups<S>(reinterpret_cast<const void*>(kernel), smem, a.rows, parts);
+    return launch_clusters(kernel, (unsigned)(groups * parts), S::THREADS, smem, parts, s, a);
+}
+
+// *groups: parts of the workspace that are written
+template <class S, bool SUMS> int launch_backward(const LnBwd& a, float* part, int parts, int* groups, cudaStream_t s) {
+    const auto kernel = ln_backward_kernel<S, SUMS>;
+    const size_t teams = SUMS && S::TEAMS > 1 ? (size_t)S::TEAMS * 2 * a.d * sizeof(float) : 0;
+    const size_t smem = std::max(S::ring(a.dh != nullptr ? 3 : 2), teams);
+    const int st = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), smem);
+    if (st != ADDER_OK) return st;
+    *groups = (int)ln_groups<S>(reinterpret_cast<const void*>(kernel), smem, a.rows, parts);
+    return launch_clusters(kernel, (unsigned)(*groups * parts), S::THREADS, smem, parts, s, a, part);
+}
+
+// f(shape, cluster size) for the shape whose registers hold a row of d elements; false: none does.  A thread has up to 16 elements; rows of
+// more than 8192 are shared by a cluster.
+template <class T, class W, class F> bool with_shape(int d, bool vectors, F&& f) {
+    constexpr int VE = Vec16<T>::N, NV = 16 / VE, STAGES = NV == 2 ? 3 : 2;      // as much shared memory as two CTAs an SM leave
     if (vectors) {
-        if (d <= 32 * VE) f(Int<32>(), Int<VE>(), Int<1>());
-        else if (d <= 128 * VE) f(Int<32>(), Int<VE>(), Int<4>());
-        else if (d <= 512 * VE) f(Int<128>(), Int<VE>(), Int<4>());
-        else if (d <= 2048 * VE) f(Int<512>(), Int<VE>(), Int<4>());
-        else return false;
+        if (d <= 32 * VE) f(LnShape<T, W, 32, VE, 1, 3, false>(), 1);
+        else if (d <= 512) f(LnShape<T, W, 32, VE, NV, STAGES, false>(), 1);
+        else if (d <= 1024) f(LnShape<T, W, 64, VE, NV, STAGES, false>(), 1);
+        else if (d <= 2048) f(LnShape<T, W, 128, VE, NV, STAGES, false>(), 1);
+        else if (d <= 4096) f(LnShape<T, W, 256, VE, NV, STAGES, false>(), 1);
+        else if (d <= 8192) f(LnShape<T, W, 512, VE, NV, 2, false>(), 1);
+        else if (d <= 8 * 8192) {
+            const int nvec = d / VE;      // the largest share has to fit
+            int parts = 2;
+            while ((nvec + parts - 1) / parts > 512 * NV) parts *= 2;
+            f(LnShape<T, W, 512, VE, NV, 2, true>(), parts);
+        } else return false;
     } else {
-        if (d <= 128) f(Int<32>(), Int<1>(), Int<4>());
-        else if (d <= 512) f(Int<32>(), Int<1>(), Int<16>());
-        else if (d <= 2048) f(Int<128>(), Int<1>(), Int<16>());
-        else if (d <= 8192) f(Int<512>(), Int<1>(), Int<16>());
+        if (d <= 128) f(LnShape<T, W, 32, 1, 4, 0, false>(), 1);
+        else if (d <= 512) f(LnShape<T, W, 32, 1, 16, 0, false>(), 1);
+        else if (d <= 2048) f(LnShape<T, W, 128, 1, 16, 0, false>(), 1);
+        else if (d <= 8192) f(LnShape<T, W, 512, 1, 16, 0, false>(), 1);
+        else if (d <= 8 * 8192) f(LnShape<T, W, 512, 1, 16, 0, true>(), d <= 2 * 8192 ? 2 : d <= 4 * 8192 ? 4 : 8);
         else return false;
     }
     return true;
@@ -392,18 +748,16 @@ int adder_b200_layernorm_forward(const void* x, const void* residual, const void
                              all_aligned({x, residual, weight, bias, y, h}, 16);
         return with_weight_type<T>(weight_dtype, [&](auto* wt) {
             using W = std::remove_pointer_t<decltype(wt)>;
-            const bool held = by_width<VE>((int)d, vectors, [&](auto g, auto vec, auto nv) {
-                constexpr int G = g, teams = LN_TEAMS<G>;
-                ln_forward_kernel<T, W, G, vec, nv><<<(unsigned)((rows + teams - 1) / teams), G * teams, 0, s>>>(a);
-            });
-            return held ? launched() : launch_long(a, ln_forward_long_kernel<T, W>, s);
+            int status = ADDER_OK;
+            const bool held = with_shape<T, W>((int)d, vectors, [&](auto shape, int parts) { status = launch_forward<decltype(shape)>(a, parts, s); });
+            return held ? status : launch_clusters(ln_forward_long_kernel<T, W>, (unsigned)(rows * 8), LN_LONG, 0, 8, s, a);
         });
     });
 }
 
 size_t adder_b200_layernorm_backward_workspace_bytes(long long rows, long long d) {
     if (rows <= 0 || d <= 0 || d > 2147483647LL - 65536) return 0;
-    return (size_t)ln_splits(rows, (int)d) * 2 * d * sizeof(float);
+    return (size_t)std::max(ln_splits(rows, (int)d), ln_most_parts(rows)) * 2 * d * sizeof(float);
 }
 
 int adder_b200_layernorm_backward(const void* dy, const void* dh, const void* h, const void* weight, const float* mean, const float* rstd,
@@ -423,9 +777,10 @@ int adder_b200_layernorm_backward(const void* dy, const void* dh, const void* h,
     if (!dy || !h || !mean || !rstd) return ADDER_ERR_NULL_POINTER;
     if (h_stride < 0) return ADDER_ERR_BAD_SHAPE;
     const unsigned size = dtype == ADDER_TYPE_F32 ? 4 : 2;
-    if (!all_aligned({dy, dh, h, dx}, size) || !all_aligned({weight, dweight, dbias}, (unsigned)wsize) || !all_aligned({mean, rstd, workspace}, 4))
+    if (!all_aligned({dy, dh, h, dx}, size) || !all_aligned({weight, dweight, dbias}, (unsigned)wsize) || !all_aligned({mean, rstd}, 4) || !aligned_to(workspace, 16))
         return ADDER_ERR_ALIGNMENT;
     const bool sums = dweight != nullptr || dbias != nullptr;
+    if (!sums && dx == nullptr) return ADDER_OK;
     if (sums && (workspace == nullptr || workspace_bytes < adder_b200_layernorm_backward_workspace_bytes(rows, d))) return ADDER_ERR_WORKSPACE;
     const LnBwd a{dy, dh, h, weight, mean, rstd, dx, rows, h_stride, (int)d};
     return with_type(dtype, [&](auto* type) {
@@ -434,20 +789,24 @@ int adder_b200_layernorm_backward(const void* dy, const void* dh, const void* h,
         const bool vectors = d % VE == 0 && h_stride % VE == 0 && all_aligned({dy, dh, h, weight, dx}, 16);
         return with_weight_type<T>(weight_dtype, [&](auto* wt) {
             using W = std::remove_pointer_t<decltype(wt)>;
-            int status = ADDER_OK;
-            if (dx != nullptr) {
-                const bool held = by_width<VE>((int)d, vectors, [&](auto g, auto vec, auto nv) {
-                    constexpr int G = g, teams = LN_TEAMS<G>;
-                    ln_dx_kernel<T, W, G, vec, nv><<<(unsigned)((rows + teams - 1) / teams), G * teams, 0, s>>>(a);
-                });
-                status = held ? launched() : launch_long(a, ln_dx_long_kernel<T, W>, s);
+            int status = ADDER_OK, groups = 0;
+            float* part = static_cast<float*>(workspace);
+            const bool held = with_shape<T, W>((int)d, vectors, [&](auto shape, int parts) {
+                using S = decltype(shape);
+                status = sums ? launch_backward<S, true>(a, part, parts, &groups, s) : launch_backward<S, false>(a, part, parts, &groups, s);
+            });
+            if (!held) {
+                if (dx != nullptr) status = launch_clusters(ln_dx_long_kernel<T, W>, (unsigned)(rows * 8), LN_LONG, 0, 8, s, a);
+                if (status != ADDER_OK) return status;
+                groups = ln_splits(rows, (int)d);
+                if (sums) {
+                    ln_columns_kernel<T><<<dim3((unsigned)((d + LN_COLS - 1) / LN_COLS), groups), LN_COLS * LN_LANES, 0, s>>>(a, part);
+                    status = launched();
+                }
             }
             if (status != ADDER_OK || !sums) return status;
-            const int splits = ln_splits(rows, (int)d);
-            float* part = static_cast<float*>(workspace);
-            ln_columns_kernel<T><<<dim3((unsigned)((d + LN_COLS - 1) / LN_COLS), splits), LN_COLS * LN_LANES, 0, s>>>(a, part);
-            ln_columns_finish_kernel<W><<<(unsigned)((d + 255) / 256), 256, 0, s>>>(part, splits, (int)d, static_cast<W*>(dweight), static_cast<W*>(dbias));
-            return launched(2);
+            ln_columns_finish_kernel<W><<<(unsigned)((2 * d + 31) / 32), 1024, 0, s>>>(part, groups, (int)d, static_cast<W*>(dweight), static_cast<W*>(dbias));
+            return launched();
         });
     });
 }
