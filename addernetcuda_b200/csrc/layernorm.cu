@@ -52,6 +52,12 @@ struct LnBwd {
 template <class T, int N> __device__ __forceinline__ void load_some(const T* p, float (&f)[N]) {
     if constexpr (N == 1) {
         f[0] = to_float(*p);
+    } else if constexpr (N == 2 && sizeof(T) == 2) {
+        const float2 v = unpack_pair<T>(__ldg(reinterpret_cast<const unsigned*>(p)));
+        f[0] = v.x; f[1] = v.y;
+    } else if constexpr (N == 2) {
+        const float2 v = __ldg(reinterpret_cast<const float2*>(p));
+        f[0] = v.x; f[1] = v.y;
     } else {
         constexpr int V = Vec16<T>::N;
 #pragma unroll
@@ -65,6 +71,7 @@ template <class T, int N> __device__ __forceinline__ void load_some(const T* p, 
 }
 template <class T, int N> __device__ __forceinline__ void store_some(T* p, const float (&f)[N]) {
     if constexpr (N == 1) *p = from_float<T>(f[0]);
+    else if constexpr (N == 2) *reinterpret_cast<unsigned*>(p) = pack_pair<T>(f[0], f[1]);
     else *reinterpret_cast<uint4*>(p) = Vec16<T>::pack(f);
 }
 
@@ -94,14 +101,15 @@ template <int TEAMS, int G> __device__ __forceinline__ void team_barrier(int tea
 }
 
 // Shapes of the kernels that hold rows in registers: a team of G threads a row (times the cluster's size), NV vectors of VEC consecutive
-// elements a thread, a thread's next STAGES - 1 rows on their way through shared memory.  A thread copies what it reads itself, so only the
-// sums of a row need a barrier.  STAGES = 0: elements are loaded when they are needed, one at a time.
-template <class T_, class W_, int G_, int VEC_, int NV_, int STAGES_, bool CLUSTER_> struct LnShape {
+// elements a thread.  STAGES > 0: CTAs that stay, a thread's next STAGES - 1 rows on their way through shared memory; a thread copies what it
+// reads itself, so only the sums of a row need a barrier.  STAGES = 0: a row a team, and many CTAs an SM (or, with 512 threads, CTAs that
+// stay, without the copies).
+template <class T_, class W_, int G_, int VEC_, int NV_, int STAGES_, bool CLUSTER_, int THREADS_ = 256> struct LnShape {
     using T = T_;
     using W = W_;
     static constexpr int G = G_, VEC = VEC_, NV = NV_, STAGES = STAGES_;
     static constexpr bool CLUSTER = CLUSTER_;
-    static constexpr int THREADS = G > 256 ? G : 256, TEAMS = THREADS / G, WARPS = G / 32;
+    static constexpr int THREADS = G > THREADS_ ? G : THREADS_, TEAMS = THREADS / G, WARPS = G / 32;
     static constexpr int LINE = THREADS * 16;      // bytes of one vector of each thread
     static size_t ring(int arrays) { return (size_t)STAGES * arrays * NV * LINE; }
 };
@@ -140,34 +148,33 @@ template <class S> __device__ __forceinline__ void ln_fetch(LnPairs<S>& f, uint3
             for (int j = 0; j < S::VEC; j += 2) f.p[(i * S::VEC + j) / 2] = pack2(e[j], e[j + 1]);
         }
     } else {
+        float e[S::NV][S::VEC];
 #pragma unroll
-        for (int i = 0; i < S::NV; i += 2) {
-            const float lo = v + i * S::G < v1 ? to_float(row[v + i * S::G]) : 0.f;
-            const float hi = v + (i + 1) * S::G < v1 ? to_float(row[v + (i + 1) * S::G]) : 0.f;
-            f.p[i / 2] = pack2(lo, hi);
+        for (int i = 0; i < S::NV; ++i) {
+#pragma unroll
+            for (int j = 0; j < S::VEC; ++j) e[i][j] = 0.f;
+            if (v + i * S::G < v1) {
+                const T* p = row + (size_t)(v + i * S::G) * S::VEC;
+                if constexpr (S::VEC > 2) {      // read once: the first-level cache is the weights'
+                    uint4 q;
+                    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(q.x), "=r"(q.y), "=r"(q.z), "=r"(q.w) : "l"(p));
+                    Vec16<T>::unpack(q, e[i]);
+                } else {
+                    load_some<T, S::VEC>(p, e[i]);
+                }
+            }
         }
+#pragma unroll
+        for (int i = 0; i < LnPairs<S>::P; ++i) f.p[i] = pack2((&e[0][0])[2 * i], (&e[0][0])[2 * i + 1]);
     }
 }
 template <class S> __device__ __forceinline__ void ln_store(typename S::T* row, const LnPairs<S>& f, int v, int v1) {
-    using T = typename S::T;
-    if constexpr (S::VEC > 1) {
+    float e[S::NV][S::VEC];
 #pragma unroll
-        for (int i = 0; i < S::NV; ++i)
-            if (v + i * S::G < v1) {
-                float e[S::VEC];
+    for (int i = 0; i < LnPairs<S>::P; ++i) unpack2(f.p[i], (&e[0][0])[2 * i], (&e[0][0])[2 * i + 1]);
 #pragma unroll
-                for (int j = 0; j < S::VEC; j += 2) unpack2(f.p[(i * S::VEC + j) / 2], e[j], e[j + 1]);
-                *reinterpret_cast<uint4*>(row + (size_t)(v + i * S::G) * S::VEC) = Vec16<T>::pack(e);
-            }
-    } else {
-#pragma unroll
-        for (int i = 0; i < S::NV; i += 2) {
-            float lo, hi;
-            unpack2(f.p[i / 2], lo, hi);
-            if (v + i * S::G < v1) row[v + i * S::G] = from_float<T>(lo);
-            if (v + (i + 1) * S::G < v1) row[v + (i + 1) * S::G] = from_float<T>(hi);
-        }
-    }
+    for (int i = 0; i < S::NV; ++i)
+        if (v + i * S::G < v1) store_some<typename S::T, S::VEC>(row + (size_t)(v + i * S::G) * S::VEC, e[i]);
 }
 template <class S> __device__ __forceinline__ void ln_weights(LnPairs<S>& f, const void* w, float missing, int v, int v1) {
     float e[S::NV][S::VEC];
@@ -188,14 +195,13 @@ template <class S> struct LnWalk {
     int arrays;
 
     __device__ __forceinline__ void start(void* smem, int arrays_) {
-        const long long parts = S::CLUSTER ? (long long)cg::this_cluster().num_blocks() : 1;
-        row = ahead = blockIdx.x / parts * S::TEAMS + threadIdx.x / S::G;
-        step = gridDim.x / parts * S::TEAMS;
+        row = ahead = (long long)blockIdx.x * S::TEAMS + threadIdx.x / S::G;
+        step = (long long)gridDim.x * S::TEAMS;
         ring = fill = read = smem_u32(smem) + threadIdx.x * 16;
         arrays = arrays_;
     }
     __device__ __forceinline__ uint32_t advance(uint32_t at) const {
-        const uint32_t stage = (uint32_t)arrays * S::NV * S::LINE, last = S::STAGES > 1 ? S::STAGES - 1 : 0;
+        const uint32_t stage = (uint32_t)arrays * S::NV * S::LINE, last = S::STAGES > 0 ? S::STAGES - 1 : 0;
         return at == ring + last * stage ? ring : at + stage;
     }
     static __device__ __forceinline__ uint32_t slot(uint32_t at, int array) { return at + array * S::NV * S::LINE; }
@@ -219,10 +225,15 @@ template <class S> __device__ __forceinline__ void ln_count(LnSums<S>& sh, int v
     if constexpr (S::CLUSTER) {
         const long long parts = cg::this_cluster().num_blocks(), i = threadIdx.x;
         if (i < parts) sh.rank_count[i] = count_of((int)(nvec * (i + 1) / parts - nvec * i / parts) * S::VEC);
-        cg::this_cluster().sync();      // the others are there to be written to
-    } else {
-        __syncthreads();
     }
+    __syncthreads();
+}
+// The CTAs of a cluster tell one another that they have begun, and wait for that before the first word crosses over.
+template <bool CLUSTER> __device__ __forceinline__ void cluster_arrive() {
+    if constexpr (CLUSTER) asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");
+}
+template <bool CLUSTER> __device__ __forceinline__ void cluster_wait() {
+    if constexpr (CLUSTER) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
 }
 
 template <int LANES> __device__ __forceinline__ float lanes_sum(float v) {
@@ -237,7 +248,8 @@ template <class S> __device__ __forceinline__ float2 ln_exchange(float a, float 
     team_barrier<S::TEAMS, S::G>(team);
     return sh.part[turn][team][t % S::WARPS];
 }
-// The same over the CTAs of a cluster, in lane i % 8; zeros beyond its size.
+// The same over the CTAs of a cluster, in lane i % 8; zeros beyond its size.  Once in a kernel: what is written to a CTA is there when it
+// passes the barrier, after which it may leave.
 template <class S> __device__ __forceinline__ float2 ln_exchange_ranks(float a, float b, LnSums<S>& sh, int t, int turn) {
     cg::cluster_group cluster = cg::this_cluster();
     const int parts = (int)cluster.num_blocks();
@@ -316,14 +328,27 @@ __device__ __forceinline__ float inverse_root(float x) {
     return r * fmaf(-0.5f * x * r, r, 1.5f);
 }
 
+// h = x + residual, rounded to what is stored: the norm is taken of that.
+template <class S> __device__ __forceinline__ void ln_add(LnPairs<S>& f, const LnPairs<S>& r) {
+    using T = typename S::T;
+#pragma unroll
+    for (int i = 0; i < LnPairs<S>::P; ++i) {
+        f.p[i] = add2(f.p[i], r.p[i]);
+        if constexpr (sizeof(T) == 2) {
+            float lo, hi;
+            unpack2(f.p[i], lo, hi);
+            const float2 held = unpack_pair<T>(pack_pair<T>(lo, hi));
+            f.p[i] = pack2(held.x, held.y);
+        }
+    }
+}
+
 template <class S> __global__ void __launch_bounds__(S::THREADS, S::THREADS > 256 ? 1 : 3) ln_forward_kernel(const LnFwd a) {
     extern __shared__ uint4 smem[];
     __shared__ LnSums<S> sh;
     using T = typename S::T;
-    constexpr int P = LnPairs<S>::P;
     const int t = threadIdx.x % S::G, team = threadIdx.x / S::G;
-    const int2 share = share_of<S::CLUSTER>(a.d / S::VEC);
-    const int v = share.x + t, v1 = share.y;
+    const int v = t, v1 = a.d / S::VEC;
     const float inv_d = 1.f / a.d;
     LnWalk<S> walk;
     walk.start(smem, a.residual != nullptr ? 2 : 1);
@@ -336,59 +361,128 @@ template <class S> __global__ void __launch_bounds__(S::THREADS, S::THREADS > 25
         cp_async_commit();
         walk.fill = walk.advance(walk.fill);
     };
-    if constexpr (S::STAGES > 0)
-        for (int i = 0; i < S::STAGES - 1; ++i) issue();
-    ln_count<S>(sh, share.x, share.y, a.d / S::VEC);
+    for (int i = 0; i < S::STAGES - 1; ++i) issue();
+    ln_count<S>(sh, 0, v1, v1);
     LnPairs<S> w, b;
     ln_weights<S>(w, a.w, 1.f, v, v1);
     ln_weights<S>(b, a.b, 0.f, v, v1);
     int turn = 0;
     for (; walk.row < a.rows; walk.row += walk.step) {
-        if constexpr (S::STAGES > 0) {
-            issue();
-            cp_async_wait<(S::STAGES > 0 ? S::STAGES - 1 : 0)>();
-        }
+        issue();
+        cp_async_wait<S::STAGES - 1>();
         const long long row = walk.row;
         LnPairs<S> f;
-        ln_fetch<S>(f, walk.slot(walk.read, 0), static_cast<const T*>(a.x) + row * a.x_stride, v, v1);
+        ln_fetch<S>(f, walk.slot(walk.read, 0), nullptr, v, v1);
         if (a.residual != nullptr) {
             LnPairs<S> r;
-            ln_fetch<S>(r, walk.slot(walk.read, 1), static_cast<const T*>(a.residual) + row * a.r_stride, v, v1);
-#pragma unroll
-            for (int i = 0; i < P; ++i) {
-                f.p[i] = add2(f.p[i], r.p[i]);
-                if constexpr (sizeof(T) == 2) {      // the norm is taken of what is stored
-                    float lo, hi;
-                    unpack2(f.p[i], lo, hi);
-                    const float2 held = unpack_pair<T>(pack_pair<T>(lo, hi));
-                    f.p[i] = pack2(held.x, held.y);
-                }
-            }
+            ln_fetch<S>(r, walk.slot(walk.read, 1), nullptr, v, v1);
+            ln_add<S>(f, r);
             ln_store<S>(static_cast<T*>(a.h) + row * a.d, f, v, v1);
         }
-        if constexpr (S::STAGES > 0) walk.read = walk.advance(walk.read);
+        walk.read = walk.advance(walk.read);
         const float2 mom = ln_moments<S>(f, v, v1, inv_d, sh, team, t, turn);
         turn ^= 1;
         const float rs = inverse_root(mom.y * inv_d + a.eps);
-        if (a.mean != nullptr && t == 0 && share.x == 0) { a.mean[row] = mom.x; a.rstd[row] = rs; }
+        if (a.mean != nullptr && t == 0) { a.mean[row] = mom.x; a.rstd[row] = rs; }
         const uint64_t minus = pack2(-mom.x, -mom.x), scale = pack2(rs, rs);
 #pragma unroll
-        for (int i = 0; i < P; ++i) f.p[i] = fma2(fma2(add2(f.p[i], minus), scale, 0), w.p[i], b.p[i]);
+        for (int i = 0; i < LnPairs<S>::P; ++i) f.p[i] = fma2(fma2(add2(f.p[i], minus), scale, 0), w.p[i], b.p[i]);
         ln_store<S>(static_cast<T*>(a.y) + row * a.d, f, v, v1);
     }
-    if constexpr (S::CLUSTER) cg::this_cluster().sync();      // no CTA leaves while its shared memory is written
 }
 
-// dx of every row; with SUMS this thread's columns of dw and db, added up over its rows and then over the CTA's teams into
-// part[CTA or cluster][2][d].
-template <class S, bool SUMS> __global__ void __launch_bounds__(S::THREADS, S::THREADS > 256 ? 1 : 2) ln_backward_kernel(const LnBwd a, float* part) {
-    extern __shared__ uint4 smem[];
+template <class S> __global__ void __launch_bounds__(S::THREADS, S::NV * S::VEC <= 16 ? 4 : S::VEC > 2 ? 3 : 2) ln_forward_row_kernel(const LnFwd a) {
     __shared__ LnSums<S> sh;
+    cluster_arrive<S::CLUSTER>();
     using T = typename S::T;
     const int t = threadIdx.x % S::G, team = threadIdx.x / S::G;
     const int2 share = share_of<S::CLUSTER>(a.d / S::VEC);
     const int v = share.x + t, v1 = share.y;
-    if constexpr (S::CLUSTER) cg::this_cluster().sync();      // the others are there to be written to
+    const float inv_d = 1.f / a.d;
+    const long long parts = S::CLUSTER ? (long long)cg::this_cluster().num_blocks() : 1;
+    const long long row = blockIdx.x / parts * S::TEAMS + team;
+    LnPairs<S> f;
+    if (row < a.rows) {
+        ln_fetch<S>(f, 0, static_cast<const T*>(a.x) + row * a.x_stride, v, v1);
+        if (a.residual != nullptr) {
+            LnPairs<S> r;
+            ln_fetch<S>(r, 0, static_cast<const T*>(a.residual) + row * a.r_stride, v, v1);
+            ln_add<S>(f, r);
+            ln_store<S>(static_cast<T*>(a.h) + row * a.d, f, v, v1);
+        }
+    }
+    ln_count<S>(sh, share.x, share.y, a.d / S::VEC);
+    cluster_wait<S::CLUSTER>();
+    if (row < a.rows) {      // the same for all of a team, and for a cluster
+        const float2 mom = ln_moments<S>(f, v, v1, inv_d, sh, team, t, 0);
+        const float rs = inverse_root(mom.y * inv_d + a.eps);
+        if (a.mean != nullptr && t == 0 && share.x == 0) { a.mean[row] = mom.x; a.rstd[row] = rs; }
+        const uint64_t minus = pack2(-mom.x, -mom.x), scale = pack2(rs, rs);
+        LnPairs<S> w;
+        ln_weights<S>(w, a.w, 1.f, v, v1);
+#pragma unroll
+        for (int i = 0; i < LnPairs<S>::P; ++i) f.p[i] = fma2(fma2(add2(f.p[i], minus), scale, 0), w.p[i], 0);
+        ln_weights<S>(w, a.b, 0.f, v, v1);
+#pragma unroll
+        for (int i = 0; i < LnPairs<S>::P; ++i) f.p[i] = add2(f.p[i], w.p[i]);
+        ln_store<S>(static_cast<T*>(a.y) + row * a.d, f, v, v1);
+    }
+}
+
+template <class S> __global__ void __launch_bounds__(S::THREADS, S::NV * S::VEC > 16 ? 2 : 3) ln_dx_row_kernel(const LnBwd a) {
+    __shared__ LnSums<S> sh;
+    cluster_arrive<S::CLUSTER>();
+    using T = typename S::T;
+    const int t = threadIdx.x % S::G, team = threadIdx.x / S::G;
+    const int2 share = share_of<S::CLUSTER>(a.d / S::VEC);
+    const int v = share.x + t, v1 = share.y;
+    const float inv_d = 1.f / a.d;
+    const long long parts = S::CLUSTER ? (long long)cg::this_cluster().num_blocks() : 1;
+    const long long row = blockIdx.x / parts * S::TEAMS + team;
+    LnPairs<S> xh, g, w;
+    float mean = 0.f, rs = 0.f;
+    if (row < a.rows) {
+        mean = a.mean[row]; rs = a.rstd[row];
+        ln_fetch<S>(xh, 0, static_cast<const T*>(a.h) + row * a.h_stride, v, v1);
+        ln_fetch<S>(g, 0, static_cast<const T*>(a.dy) + row * a.d, v, v1);
+    }
+    cluster_wait<S::CLUSTER>();
+    if (row < a.rows) {
+        ln_weights<S>(w, a.w, 1.f, v, v1);
+        uint64_t s1 = 0, s2 = 0;
+        const uint64_t minus = pack2(-mean, -mean), scale = pack2(rs, rs);
+#pragma unroll
+        for (int i = 0; i < LnPairs<S>::P; ++i) {      // dy is 0 where there is no element
+            xh.p[i] = fma2(add2(xh.p[i], minus), scale, 0);
+            g.p[i] = fma2(g.p[i], w.p[i], 0);
+            s1 = add2(s1, g.p[i]);
+            s2 = fma2(g.p[i], xh.p[i], s2);
+        }
+        float a1, b1, a2, b2;
+        unpack2(s1, a1, b1);
+        unpack2(s2, a2, b2);
+        const float2 m = ln_sum2<S>(a1 + b1, a2 + b2, sh, team, t, 0);
+        const float c1 = -m.x * inv_d, c2 = -m.y * inv_d;
+        const uint64_t shift = pack2(c1, c1), slope = pack2(c2, c2);
+#pragma unroll
+        for (int i = 0; i < LnPairs<S>::P; ++i) g.p[i] = fma2(fma2(xh.p[i], slope, add2(g.p[i], shift)), scale, 0);
+        if (a.dh != nullptr) {
+            ln_fetch<S>(w, 0, static_cast<const T*>(a.dh) + row * a.d, v, v1);
+#pragma unroll
+            for (int i = 0; i < LnPairs<S>::P; ++i) g.p[i] = add2(g.p[i], w.p[i]);
+        }
+        ln_store<S>(static_cast<T*>(a.dx) + row * a.d, g, v, v1);
+    }
+}
+
+// dx of every row; with SUMS this thread's columns of dw and db, added up over its rows and then over the CTA's teams into
+// part[CTA or cluster][2][d].
+template <class S, bool SUMS> __global__ void __launch_bounds__(S::THREADS, 1) ln_backward_kernel(const LnBwd a, float* part) {
+    extern __shared__ uint4 smem[];
+    __shared__ LnSums<S> sh;
+    using T = typename S::T;
+    const int t = threadIdx.x % S::G, team = threadIdx.x / S::G;
+    const int v = t, v1 = a.d / S::VEC;
     LnWalk<S> walk;
     walk.start(smem, a.dh != nullptr ? 3 : 2);
     const auto issue = [&] {
@@ -458,8 +552,7 @@ template <class S, bool SUMS> __global__ void __launch_bounds__(S::THREADS, S::T
         mean = mean_next; rs = rs_next;
     }
     if constexpr (SUMS) {
-        const int parts = S::CLUSTER ? (int)cg::this_cluster().num_blocks() : 1;
-        float* out = part + (size_t)(blockIdx.x / parts) * 2 * a.d;
+        float* out = part + (size_t)blockIdx.x * 2 * a.d;
         // one team writes its sums to the workspace, several add them up in their order, in shared memory
         float* to = out;
         if constexpr (S::TEAMS > 1) {
@@ -488,7 +581,6 @@ template <class S, bool SUMS> __global__ void __launch_bounds__(S::THREADS, S::T
             }
         }
     }
-    if constexpr (S::CLUSTER) cg::this_cluster().sync();
 }
 
 // ------------------------------------------------------------------------------------------ rows too long for registers
@@ -562,57 +654,73 @@ template <class T, class W> __global__ void __launch_bounds__(LN_LONG) ln_dx_lon
 
 // ------------------------------------------------------------------------------------------ gradients of weight and bias
 
-constexpr int LN_COLS = 32, LN_LANES = 8;      // a CTA's columns, and the rows that it reads at once
+constexpr int LN_COLS = 32, LN_LINES = 8;      // a CTA's columns (of VEC elements), and the rows that it reads at once
 
 // grid (column tiles, splits): part[split][2][d]
-template <class T> __global__ void __launch_bounds__(LN_COLS * LN_LANES) ln_columns_kernel(const LnBwd a, float* part) {
-    __shared__ float sw[LN_LANES][LN_COLS], sb[LN_LANES][LN_COLS];
+template <class T, int VEC> __global__ void __launch_bounds__(LN_COLS * LN_LINES) ln_columns_kernel(const LnBwd a, float* part) {
+    __shared__ float sums[2][LN_LINES][LN_COLS * VEC + 1];
     const int lane = threadIdx.x % LN_COLS, line = threadIdx.x / LN_COLS;
-    const int c = blockIdx.x * LN_COLS + lane;
-    float dw = 0.f, db = 0.f;
-    if (c < a.d)
-        for (long long row = (long long)blockIdx.y * LN_LANES + line; row < a.rows; row += (long long)gridDim.y * LN_LANES) {
-            const float g = to_float(static_cast<const T*>(a.dy)[row * a.d + c]);
-            dw = fmaf(g, (to_float(static_cast<const T*>(a.h)[row * a.h_stride + c]) - a.mean[row]) * a.rstd[row], dw);
-            db += g;
+    const int c = (blockIdx.x * LN_COLS + lane) * VEC;
+    float dw[VEC], db[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) dw[j] = db[j] = 0.f;
+    if (c < a.d) {
+#pragma unroll 4
+        for (long long row = (long long)blockIdx.y * LN_LINES + line; row < a.rows; row += (long long)gridDim.y * LN_LINES) {
+            float g[VEC], h[VEC];
+            load_some<T, VEC>(static_cast<const T*>(a.dy) + row * a.d + c, g);
+            load_some<T, VEC>(static_cast<const T*>(a.h) + row * a.h_stride + c, h);
+            const float mean = a.mean[row], rs = a.rstd[row];
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                dw[j] = fmaf(g[j], (h[j] - mean) * rs, dw[j]);
+                db[j] += g[j];
+            }
         }
-    sw[line][lane] = dw; sb[line][lane] = db;
+    }
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) { sums[0][line][lane * VEC + j] = dw[j]; sums[1][line][lane * VEC + j] = db[j]; }
     __syncthreads();
-    if (line < 2 && c < a.d) {
+    for (int i = threadIdx.x; i < 2 * LN_COLS * VEC; i += LN_COLS * LN_LINES) {
+        const int which = i / (LN_COLS * VEC), k = i % (LN_COLS * VEC), column = blockIdx.x * LN_COLS * VEC + k;
+        if (column >= a.d) continue;
         float s = 0.f;
-        for (int i = 0; i < LN_LANES; ++i) s += line == 0 ? sw[i][lane] : sb[i][lane];
-        part[((long long)blockIdx.y * 2 + line) * a.d + c] = s;
+        for (int l = 0; l < LN_LINES; ++l) s += sums[which][l][k];
+        part[((size_t)blockIdx.y * 2 + which) * a.d + column] = s;
     }
 }
 
-// Sums of the columns of part[parts][2][d]: a CTA has 32 columns, 32 lanes of every 32nd part each.
-template <class W> __global__ void __launch_bounds__(1024) ln_columns_finish_kernel(const float* part, int parts, int d, W* dw, W* db) {
-    __shared__ float sums[32][33];
-    const int c = blockIdx.x * 32 + threadIdx.x % 32, line = threadIdx.x / 32;
+// Sums of the columns of part[parts][2][d]: LINES threads a column, each with every LINES-th part.
+template <class W, int LINES> __global__ void __launch_bounds__(256) ln_columns_finish_kernel(const float* part, int parts, int d, W* dw, W* db) {
+    constexpr int COLS = 256 / LINES;
+    __shared__ float sums[LINES][COLS];
+    const int c = blockIdx.x * COLS + threadIdx.x % COLS, line = threadIdx.x / COLS;
     float s = 0.f;
-    if (c < 2 * d)
-        for (int p = line; p < parts; p += 32) s += part[(size_t)p * 2 * d + c];
-    sums[line][threadIdx.x % 32] = s;
-    __syncthreads();
-    s = sums[threadIdx.x % 32][line];      // lanes of a warp: the lines of one column
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
-    const int column = blockIdx.x * 32 + line;
-    if (threadIdx.x % 32 == 0 && column < 2 * d) {
-        if (column < d) { if (dw != nullptr) dw[column] = from_float<W>(s); }
-        else if (db != nullptr) db[column - d] = from_float<W>(s);
+    if (c < 2 * d) {
+        const float* p = part + (size_t)line * 2 * d + c;
+#pragma unroll 8
+        for (int i = line; i < parts; i += LINES, p += (size_t)LINES * 2 * d) s += *p;
     }
+    if constexpr (LINES > 1) {
+        sums[line][threadIdx.x % COLS] = s;
+        __syncthreads();
+        if (line > 0) return;
+#pragma unroll
+        for (int i = 1; i < LINES; ++i) s += sums[i][threadIdx.x];
+    }
+    if (c < d) { if (dw != nullptr) dw[c] = from_float<W>(s); }
+    else if (c < 2 * d && db != nullptr) db[c - d] = from_float<W>(s);
 }
 
 // ------------------------------------------------------------------------------------------ host
 
-int ln_splits(long long rows, int d) {
-    const long long tiles = (d + LN_COLS - 1) / LN_COLS;
-    long long splits = (8LL * sm_count() + tiles - 1) / tiles;
-    splits = std::min(splits, (rows + LN_LANES - 1) / LN_LANES);
-    return (int)std::max(1LL, std::min(splits, 1024LL));
+// Splits of the rows of the column sums: some 6 CTAs an SM, at least 4 rows a line of a CTA.
+int ln_splits(long long rows, int d, int vec) {
+    const long long tiles = (d + LN_COLS * vec - 1) / (LN_COLS * vec);
+    long long splits = (6LL * sm_count() + tiles - 1) / tiles;
+    splits = std::min(splits, (rows + 4 * LN_LINES - 1) / (4 * LN_LINES));
+    return (int)std::max(1LL, std::min(splits, 512LL));
 }
-
 int ln_most_parts(long long rows) { return (int)std::min(rows, 4LL * sm_count()); }
 
 // Launches `kernel` in clusters of `parts` CTAs (1: none).
@@ -651,58 +759,101 @@ int resident(const void* kernel, int threads, size_t smem) {
     return it->second;
 }
 
-// CTAs (clusters of `parts`) that share `rows`: as many as are resident, and no more than there are rows for.
-template <class S> long long ln_groups(const void* kernel, size_t smem, long long rows, int parts) {
-    const long long most = std::min(4LL, (long long)resident(kernel, S::THREADS, smem)) * sm_count() / parts;
-    return std::max(1LL, std::min(most, (rows + S::TEAMS - 1) / S::TEAMS));
+// CTAs that share `rows`: as many as are resident, and no more than there are rows for.
+template <class S> int ln_ctas(const void* kernel, size_t smem, long long rows) {
+    const long long most = std::min(4LL, (long long)resident(kernel, S::THREADS, smem)) * sm_count();
+    return (int)std::max(1LL, std::min(most, (rows + S::TEAMS - 1) / S::TEAMS));
 }
 
 template <class S> int launch_forward(const LnFwd& a, int parts, cudaStream_t s) {
-    const auto kernel = ln_forward_kernel<S>;
-    const size_t smem = S::ring(a.residual != nullptr ? 2 : 1);
-    const int st = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), smem);
-    if (st != ADDER_OK) return st;
-    const long long groups = ln_groups<S>(reinterpret_cast<const void*>(kernel), smem, a.rows, parts);
-    return launch_clusters(kernel, (unsigned)(groups * parts), S::THREADS, smem, parts, s, a);
+    if constexpr (S::STAGES == 0) {
+        return launch_clusters(ln_forward_row_kernel<S>, (unsigned)((a.rows + S::TEAMS - 1) / S::TEAMS * parts), S::THREADS, 0, parts, s, a);
+    } else {
+        const auto kernel = ln_forward_kernel<S>;
+        const size_t smem = S::ring(a.residual != nullptr ? 2 : 1);
+        const int st = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), smem);
+        if (st != ADDER_OK) return st;
+        return launch_clusters(kernel, (unsigned)ln_ctas<S>(reinterpret_cast<const void*>(kernel), smem, a.rows), S::THREADS, smem, 1, s, a);
+    }
 }
 
-// *groups: parts of the workspace that are written
-template <class S, bool SUMS> int launch_backward(const LnBwd& a, float* part, int parts, int* groups, cudaStream_t s) {
+// dx, and with `sums` parts of dw and db: *groups of them are written.
+template <class S, bool SUMS> int launch_stay_backward(const LnBwd& a, float* part, int* groups, cudaStream_t s) {
     const auto kernel = ln_backward_kernel<S, SUMS>;
     const size_t teams = SUMS && S::TEAMS > 1 ? (size_t)S::TEAMS * 2 * a.d * sizeof(float) : 0;
     const size_t smem = std::max(S::ring(a.dh != nullptr ? 3 : 2), teams);
     const int st = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), smem);
     if (st != ADDER_OK) return st;
-    *groups = (int)ln_groups<S>(reinterpret_cast<const void*>(kernel), smem, a.rows, parts);
-    return launch_clusters(kernel, (unsigned)(*groups * parts), S::THREADS, smem, parts, s, a, part);
+    *groups = ln_ctas<S>(reinterpret_cast<const void*>(kernel), smem, a.rows);
+    return launch_clusters(kernel, (unsigned)*groups, S::THREADS, smem, 1, s, a, part);
+}
+template <class T, int VEC> int launch_columns(const LnBwd& a, float* part, int* groups, cudaStream_t s) {
+    *groups = ln_splits(a.rows, a.d, VEC);
+    ln_columns_kernel<T, VEC><<<dim3((unsigned)((a.d + LN_COLS * VEC - 1) / (LN_COLS * VEC)), *groups), LN_COLS * LN_LINES, 0, s>>>(a, part);
+    return launched();
+}
+template <class S> int launch_backward(const LnBwd& a, float* part, bool sums, int parts, int* groups, cudaStream_t s) {
+    if constexpr (S::STAGES > 0 || S::THREADS == 512) {
+        return sums ? launch_stay_backward<S, true>(a, part, groups, s) : launch_stay_backward<S, false>(a, part, groups, s);
+    } else {
+        if (a.dx != nullptr) {
+            const int st = launch_clusters(ln_dx_row_kernel<S>, (unsigned)((a.rows + S::TEAMS - 1) / S::TEAMS * parts), S::THREADS, 0, parts, s, a);
+            if (st != ADDER_OK) return st;
+        }
+        return sums ? launch_columns<typename S::T, S::VEC>(a, part, groups, s) : ADDER_OK;
+    }
 }
 
-// f(shape, cluster size) for the shape whose registers hold a row of d elements; false: none does.  A thread has up to 16 elements; rows of
-// more than 8192 are shared by a cluster.
-template <class T, class W, class F> bool with_shape(int d, bool vectors, F&& f) {
-    constexpr int VE = Vec16<T>::N, NV = 16 / VE, STAGES = NV == 2 ? 3 : 2;      // as much shared memory as two CTAs an SM leave
-    if (vectors) {
-        if (d <= 32 * VE) f(LnShape<T, W, 32, VE, 1, 3, false>(), 1);
-        else if (d <= 512) f(LnShape<T, W, 32, VE, NV, STAGES, false>(), 1);
-        else if (d <= 1024) f(LnShape<T, W, 64, VE, NV, STAGES, false>(), 1);
-        else if (d <= 2048) f(LnShape<T, W, 128, VE, NV, STAGES, false>(), 1);
-        else if (d <= 4096) f(LnShape<T, W, 256, VE, NV, STAGES, false>(), 1);
-        else if (d <= 8192) f(LnShape<T, W, 512, VE, NV, 2, false>(), 1);
-        else if (d <= 8 * 8192) {
-            const int nvec = d / VE;      // the largest share has to fit
-            int parts = 2;
-            while ((nvec + parts - 1) / parts > 512 * NV) parts *= 2;
-            f(LnShape<T, W, 512, VE, NV, 2, true>(), parts);
-        } else return false;
+// f(shape, cluster size) for the shape whose registers hold a row of d elements, in vectors of vec; false: none does.  Whole 16-byte
+// vectors go through the ring up to 8192 elements, 16 a thread.  Other rows, and longer ones, which a cluster shares, are held up to 32 a thread
+// by CTAs of one row; the backward pass (THREADS = 512) stays where it can, for the sums over the rows.
+template <class T, class W, int THREADS, class F> bool with_shape(int d, int vec, F&& f) {
+    constexpr int VE = Vec16<T>::N, NV = 16 / VE, STAGES = NV == 2 ? 3 : 2;      // as much shared memory as two CTAs of 256 threads leave
+    const auto by_row = [&](auto v) {
+        constexpr int V = decltype(v)::value;
+        if constexpr (THREADS == 512) {
+            if (d <= 128) return f(LnShape<T, W, 32, V, 4 / V, 0, false, 512>(), 1);
+            if (d <= 512) return f(LnShape<T, W, 32, V, 16 / V, 0, false, 512>(), 1);
+            if (d <= 2048) return f(LnShape<T, W, 128, V, 16 / V, 0, false, 512>(), 1);
+            if (d <= 8192) return f(LnShape<T, W, 512, V, 16 / V, 0, false, 512>(), 1);
+        }
+        if (d <= 128) f(LnShape<T, W, 32, V, 4 / V, 0, false>(), 1);
+        else if (d <= 512) f(LnShape<T, W, 32, V, 16 / V, 0, false>(), 1);
+        else if (d <= 2048) f(LnShape<T, W, 128, V, 16 / V, 0, false>(), 1);
+        else if (d <= 4096) f(LnShape<T, W, 128, V, 32 / V, 0, false>(), 1);
+        else if (d <= 8192) f(LnShape<T, W, 256, V, 32 / V, 0, false>(), 1);
+        else f(LnShape<T, W, 256, V, 32 / V, 0, true>(), (d / V + 256 * (32 / V) - 1) / (256 * (32 / V)));
+    };
+    if (d > 8 * 8192) return false;
+    if (vec == VE) {
+        if (d <= 32 * VE) f(LnShape<T, W, 32, VE, 1, 3, false, THREADS>(), 1);
+        else if (d <= 512) f(LnShape<T, W, 32, VE, NV, STAGES, false, THREADS>(), 1);
+        else if (d <= 1024) f(LnShape<T, W, 64, VE, NV, STAGES, false, THREADS>(), 1);
+        else if (d <= 2048) f(LnShape<T, W, 128, VE, NV, STAGES, false, THREADS>(), 1);
+        else if (d <= 4096) f(LnShape<T, W, 256, VE, NV, STAGES, false, THREADS>(), 1);
+        else if (d <= 8192) f(LnShape<T, W, 512, VE, NV, 2, false, THREADS>(), 1);
+        else f(LnShape<T, W, 256, VE, 32 / VE, 0, true>(), (d / VE + 256 * (32 / VE) - 1) / (256 * (32 / VE)));
+    } else if (vec == 2) {
+        if constexpr (sizeof(T) == 2) by_row(std::integral_constant<int, 2>());
     } else {
-        if (d <= 128) f(LnShape<T, W, 32, 1, 4, 0, false>(), 1);
-        else if (d <= 512) f(LnShape<T, W, 32, 1, 16, 0, false>(), 1);
-        else if (d <= 2048) f(LnShape<T, W, 128, 1, 16, 0, false>(), 1);
-        else if (d <= 8192) f(LnShape<T, W, 512, 1, 16, 0, false>(), 1);
-        else if (d <= 8 * 8192) f(LnShape<T, W, 512, 1, 16, 0, true>(), d <= 2 * 8192 ? 2 : d <= 4 * 8192 ? 4 : 8);
-        else return false;
+        by_row(std::integral_constant<int, 1>());
     }
     return true;
+}
+// The largest vector that the rows of all tensors allow: 16 bytes, two 16-bit elements, one element.
+template <class T> int ln_vector(int d, std::initializer_list<long long> strides, std::initializer_list<const void*> tensors,
+                                 std::initializer_list<const void*> weights, unsigned wsize) {
+    const auto fits = [&](int vec) {
+        if (d % vec != 0) return false;
+        for (long long s : strides)
+            if (s % vec != 0) return false;
+        for (const void* p : tensors)
+            if (!aligned_to(p, vec * sizeof(T))) return false;
+        for (const void* p : weights)
+            if (!aligned_to(p, std::min(16u, vec * wsize))) return false;
+        return true;
+    };
+    return fits(Vec16<T>::N) ? Vec16<T>::N : sizeof(T) == 2 && fits(2) ? 2 : 1;
 }
 template <class T, class F> int with_weight_type(int wtype, F&& f) {
     if (wtype == ADDER_TYPE_F32) return f(static_cast<float*>(nullptr));
@@ -743,13 +894,11 @@ int adder_b200_layernorm_forward(const void* x, const void* residual, const void
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     return with_type(dtype, [&](auto* type) {
         using T = std::remove_pointer_t<decltype(type)>;
-        constexpr int VE = Vec16<T>::N;
-        const bool vectors = d % VE == 0 && x_stride % VE == 0 && (!residual || residual_stride % VE == 0) &&
-                             all_aligned({x, residual, weight, bias, y, h}, 16);
+        const int vec = ln_vector<T>((int)d, {x_stride, residual ? residual_stride : 0}, {x, residual, y, h}, {weight, bias}, wsize);
         return with_weight_type<T>(weight_dtype, [&](auto* wt) {
             using W = std::remove_pointer_t<decltype(wt)>;
             int status = ADDER_OK;
-            const bool held = with_shape<T, W>((int)d, vectors, [&](auto shape, int parts) { status = launch_forward<decltype(shape)>(a, parts, s); });
+            const bool held = with_shape<T, W, 256>((int)d, vec, [&](auto shape, int parts) { status = launch_forward<decltype(shape)>(a, parts, s); });
             return held ? status : launch_clusters(ln_forward_long_kernel<T, W>, (unsigned)(rows * 8), LN_LONG, 0, 8, s, a);
         });
     });
@@ -757,7 +906,7 @@ int adder_b200_layernorm_forward(const void* x, const void* residual, const void
 
 size_t adder_b200_layernorm_backward_workspace_bytes(long long rows, long long d) {
     if (rows <= 0 || d <= 0 || d > 2147483647LL - 65536) return 0;
-    return (size_t)std::max(ln_splits(rows, (int)d), ln_most_parts(rows)) * 2 * d * sizeof(float);
+    return (size_t)std::max(ln_splits(rows, (int)d, 8), ln_most_parts(rows)) * 2 * d * sizeof(float);
 }
 
 int adder_b200_layernorm_backward(const void* dy, const void* dh, const void* h, const void* weight, const float* mean, const float* rstd,
@@ -785,27 +934,22 @@ int adder_b200_layernorm_backward(const void* dy, const void* dh, const void* h,
     const LnBwd a{dy, dh, h, weight, mean, rstd, dx, rows, h_stride, (int)d};
     return with_type(dtype, [&](auto* type) {
         using T = std::remove_pointer_t<decltype(type)>;
-        constexpr int VE = Vec16<T>::N;
-        const bool vectors = d % VE == 0 && h_stride % VE == 0 && all_aligned({dy, dh, h, weight, dx}, 16);
+        const int vec = ln_vector<T>((int)d, {h_stride}, {dy, dh, h, dx}, {weight}, (unsigned)wsize);
         return with_weight_type<T>(weight_dtype, [&](auto* wt) {
             using W = std::remove_pointer_t<decltype(wt)>;
             int status = ADDER_OK, groups = 0;
             float* part = static_cast<float*>(workspace);
-            const bool held = with_shape<T, W>((int)d, vectors, [&](auto shape, int parts) {
-                using S = decltype(shape);
-                status = sums ? launch_backward<S, true>(a, part, parts, &groups, s) : launch_backward<S, false>(a, part, parts, &groups, s);
+            const bool held = with_shape<T, W, 512>((int)d, vec, [&](auto shape, int parts) {
+                status = launch_backward<decltype(shape)>(a, part, sums, parts, &groups, s);
             });
             if (!held) {
                 if (dx != nullptr) status = launch_clusters(ln_dx_long_kernel<T, W>, (unsigned)(rows * 8), LN_LONG, 0, 8, s, a);
-                if (status != ADDER_OK) return status;
-                groups = ln_splits(rows, (int)d);
-                if (sums) {
-                    ln_columns_kernel<T><<<dim3((unsigned)((d + LN_COLS - 1) / LN_COLS), groups), LN_COLS * LN_LANES, 0, s>>>(a, part);
-                    status = launched();
-                }
+                if (status == ADDER_OK && sums) status = vec == Vec16<T>::N ? launch_columns<T, Vec16<T>::N>(a, part, &groups, s) : launch_columns<T, 1>(a, part, &groups, s);
             }
             if (status != ADDER_OK || !sums) return status;
-            ln_columns_finish_kernel<W><<<(unsigned)((2 * d + 31) / 32), 1024, 0, s>>>(part, groups, (int)d, static_cast<W*>(dweight), static_cast<W*>(dbias));
+            // up to 16 parts one after another, more by 16 threads
+            if (groups <= 16) ln_columns_finish_kernel<W, 1><<<(unsigned)((2 * d + 255) / 256), 256, 0, s>>>(part, groups, (int)d, static_cast<W*>(dweight), static_cast<W*>(dbias));
+            else ln_columns_finish_kernel<W, 16><<<(unsigned)((2 * d + 15) / 16), 256, 0, s>>>(part, groups, (int)d, static_cast<W*>(dweight), static_cast<W*>(dbias));
             return launched();
         });
     });
