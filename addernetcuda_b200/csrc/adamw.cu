@@ -13,16 +13,16 @@ namespace adder {
 namespace {
 
 constexpr int AW_THREADS = 256;
-constexpr int AW_CHUNK = AW_THREADS * 8;      // elements of one tensor that a CTA updates: 8 to a thread, one scale block to a warp
+constexpr int AW_TILE = AW_THREADS * 8;       // elements that a CTA takes at once: 8 to a thread, one scale block to a warp
 constexpr int AW_BLOCK = 256;                 // values that share a scale
 
 using Tensor = adder_b200_adamw_tensor;
 
-// 48 tensors fit in the 4 KB of parameters that every launch takes at full speed, 480 in the 32 KB that it takes at most.
+// 48 tensors fit in 4 KB of launch parameters, 480 in the 32 KB that there may be.
 template <int CAP> struct Table {
     Tensor t[CAP];
     int first[CAP + 1];      // first chunk of each tensor
-    int count;
+    int count, tiles;        // tiles of a chunk
 };
 
 struct Hyper {
@@ -31,25 +31,49 @@ struct Hyper {
     const float* grad_scale;
 };
 
-// Eight consecutive elements of a tensor, `valid` of them in it.
-template <class T> __device__ __forceinline__ void load8(const T* p, int valid, float (&f)[8]) {
-    constexpr int N = Vec16<T>::N;
-    if (valid == 8 && aligned_to(p, 16)) {
+// Eight consecutive elements of a tensor as they lie in memory, `valid` of them in it (zeros in place of the others).
+template <class T> struct Raw8 {
+    static constexpr int Q = sizeof(T) / 2;      // 16-byte words
+    uint4 q[Q];
+    __device__ __forceinline__ void load(const T* p, int valid) {
+        if (valid == 8 && aligned_to(p, 16)) {
 #pragma unroll
-        for (int i = 0; i < 8 / N; ++i) {
-            float v[N];
-            Vec16<T>::unpack(reinterpret_cast<const uint4*>(p)[i], v);
+            for (int i = 0; i < Q; ++i) q[i] = reinterpret_cast<const uint4*>(p)[i];
+        } else {
+            uint32_t w[4 * Q];
 #pragma unroll
-            for (int j = 0; j < N; ++j) f[i * N + j] = v[j];
+            for (int i = 0; i < 4 * Q; ++i) w[i] = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (i < valid) {
+                    if constexpr (sizeof(T) == 4) w[i] = __float_as_uint(p[i]);
+                    else w[i / 2] |= (uint32_t)reinterpret_cast<const unsigned short*>(p)[i] << (16 * (i & 1));
+                }
+#pragma unroll
+            for (int i = 0; i < Q; ++i) q[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
         }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = i < valid ? to_float(p[i]) : 0.f;
     }
-}
-template <class T> __device__ __forceinline__ void store8(T* p, int valid, const float (&f)[8]) {
-    constexpr int N = Vec16<T>::N;
+    // as four pairs of fp32
+    __device__ __forceinline__ void pairs(uint64_t (&f)[4]) const {
+        if constexpr (sizeof(T) == 4) {
+            f[0] = pack2(__uint_as_float(q[0].x), __uint_as_float(q[0].y)); f[1] = pack2(__uint_as_float(q[0].z), __uint_as_float(q[0].w));
+            f[2] = pack2(__uint_as_float(q[Q - 1].x), __uint_as_float(q[Q - 1].y)); f[3] = pack2(__uint_as_float(q[Q - 1].z), __uint_as_float(q[Q - 1].w));
+        } else {
+            const uint32_t w[4] = {q[0].x, q[0].y, q[0].z, q[0].w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float2 v = unpack_pair<T>(w[i]);
+                f[i] = pack2(v.x, v.y);
+            }
+        }
+    }
+};
+template <class T> __device__ __forceinline__ void store8(T* p, int valid, const uint64_t (&pairs)[4]) {
+    float f[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) unpack2(pairs[i], f[2 * i], f[2 * i + 1]);
     if (valid == 8 && aligned_to(p, 16)) {
+        constexpr int N = Vec16<T>::N;
 #pragma unroll
         for (int i = 0; i < 8 / N; ++i) {
             float v[N];
@@ -83,49 +107,99 @@ __device__ __forceinline__ void store_codes(unsigned char* p, int valid, uint2 c
 }
 
 constexpr float TOP_M = 248.f, TOP_V = 63488.f, SMALLEST = 0x1p-100f;
+__device__ __forceinline__ uint64_t twice(float v) { return pack2(v, v); }
 
-// The magnitude of a code is the fp32 number with the code at bit 19 (a subnormal one where the exponent field is 0), times 2^127.
-template <bool SIGNED> __device__ __forceinline__ float decode(uint32_t code, float scale) {
-    const float mag = __fmul_rn(__uint_as_float((SIGNED ? code & 127u : code) << 19), 0x1p127f);
-    return __fmul_rn(SIGNED && code >= 128u ? -mag : mag, scale);
+// The magnitude of a code is the fp32 number with the code at bit 19 (a subnormal one where the exponent field is 0), times 2^127; a sign at bit
+// 7 of the code goes to bit 31.  Eight codes, as pairs.
+template <bool SIGNED> __device__ __forceinline__ float code_bits(uint32_t word, int i) {
+    constexpr uint32_t mask = (SIGNED ? 127u : 255u) << 19;
+    const uint32_t mag = (i < 3 ? word << (19 - 8 * i) : word >> 5) & mask;
+    if (!SIGNED) return __uint_as_float(mag);
+    return __uint_as_float(mag | ((word << (24 - 8 * i)) & 0x80000000u));
 }
-template <bool SIGNED> __device__ __forceinline__ uint32_t encode(float x, float inv) {
-    const uint32_t bits = __float_as_uint(__fmul_rn(__fmul_rn(fabsf(x), inv), 0x1p-127f));
-    uint32_t code = min((bits + 0x3ffffu + ((bits >> 19) & 1u)) >> 19, SIGNED ? 127u : 255u);
-    if (SIGNED) return x < 0.f ? code | 128u : code;
-    return x > 0.f && inv > 0.f ? max(code, 1u) : code;
-}
-
-// Stores the warp's block of 256 values, eight to a lane.  Each operation rounds to fp32 by itself (no fused multiply-add), so that the
-// codes are defined bit by bit.
-template <bool SIGNED> __device__ __forceinline__ void store_block(unsigned char* codes, float* scale, int valid, const float (&x)[8]) {
-    uint32_t top = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);      // NaN above infinity above the rest
-    float largest = __uint_as_float(__reduce_max_sync(0xffffffffu, top));
-    if (largest < SMALLEST) largest = 0.f;
-    const float limit = SIGNED ? TOP_M : TOP_V;
-    const float inv = largest > 0.f ? __fmul_rn(__frcp_rn(largest), limit) : 0.f;
-    uint2 c = make_uint2(0, 0);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) c.x |= encode<SIGNED>(x[i], inv) << (8 * i);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) c.y |= encode<SIGNED>(x[i + 4], inv) << (8 * i);
-    store_codes(codes, valid, c);
-    if ((threadIdx.x & 31) == 0) *scale = __fmul_rn(largest, 1.f / limit);
-}
-template <bool SIGNED> __device__ __forceinline__ void load_block(const unsigned char* codes, const float* scale, int valid, float (&x)[8]) {
-    const uint2 c = load_codes(codes, valid);
-    const float sc = *scale;
+template <bool SIGNED> __device__ __forceinline__ void decode(uint2 c, float scale, uint64_t (&x)[4]) {
+    const uint64_t up = twice(0x1p127f), sc = twice(scale);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        x[i] = decode<SIGNED>((c.x >> (8 * i)) & 255u, sc);
-        x[i + 4] = decode<SIGNED>((c.y >> (8 * i)) & 255u, sc);
+        const uint32_t word = i < 2 ? c.x : c.y;
+        x[i] = mul2(mul2(pack2(code_bits<SIGNED>(word, 2 * (i & 1)), code_bits<SIGNED>(word, 2 * (i & 1) + 1)), up), sc);
     }
 }
 
+// Code of a value that has been scaled to the code's range and by 2^-127: rounded to nearest even at bit 19, and moved to the top byte (a
+// sign, that of the value plus 0, to its top bit: a negative value keeps it where it rounds to 0, -0 has none).
+template <bool SIGNED> __device__ __forceinline__ uint32_t round_to_code(float scaled, float x) {
+    const uint32_t bits = __float_as_uint(scaled);
+    uint32_t r = bits + 0x3ffffu + ((bits >> 19) & 1u);
+    if (SIGNED) return ((r << 5) & 0x7fffffffu) | (__float_as_uint(x) & 0x80000000u);
+    if (x > 0.f) r = max(r, 1u << 19);
+    return r << 5;
+}
+__device__ __forceinline__ uint32_t top_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    return __byte_perm(__byte_perm(a, b, 0x0073), __byte_perm(c, d, 0x0073), 0x5410);
+}
+
+// Stores the warp's block of 256 values, eight to a lane.  Each operation rounds to fp32 by itself, so that the codes are defined bit by
+// bit.
+template <bool SIGNED> __device__ __forceinline__ void store_block(unsigned char* codes, float* scale, int valid, const uint64_t (&x)[4]) {
+    float f[8], top = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) unpack2(x[i], f[2 * i], f[2 * i + 1]);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) asm("max.NaN.f32 %0, %0, %1;" : "+f"(top) : "f"(fabsf(f[i])));
+    float largest = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));      // NaN above infinity above the rest
+    if (largest < SMALLEST) largest = 0.f;
+    const float limit = SIGNED ? TOP_M : TOP_V;
+    const float inv = largest > 0.f ? __fmul_rn(__frcp_rn(largest), limit) : 0.f;
+    uint32_t r[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        float a, b;
+        if (SIGNED) unpack2(add2(x[i], 0), f[2 * i], f[2 * i + 1]);
+        unpack2(mul2(mul2(x[i], twice(inv)), twice(0x1p-127f)), a, b);
+        r[2 * i] = round_to_code<SIGNED>(a, f[2 * i]);
+        r[2 * i + 1] = round_to_code<SIGNED>(b, f[2 * i + 1]);
+    }
+    uint2 c = make_uint2(top_bytes(r[0], r[1], r[2], r[3]), top_bytes(r[4], r[5], r[6], r[7]));
+    if (largest == 0.f) c = SIGNED ? make_uint2(c.x & 0x80808080u, c.y & 0x80808080u) : make_uint2(0, 0);
+    store_codes(codes, valid, c);
+    if ((threadIdx.x & 31) == 0) *scale = __fmul_rn(largest, 1.f / limit);
+}
+
+__device__ __forceinline__ float root_of(float x) {
+    float r;
+    asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+// What a thread reads of a tile.
+template <class T, int BITS> struct Tile {
+    Raw8<T> p, g;
+    Raw8<float> m, v;
+    __device__ __forceinline__ void load(const Tensor& t, long long at, int valid) {
+        p.load(static_cast<const T*>(t.param) + at, valid);
+        g.load(static_cast<const T*>(t.grad) + at, valid);
+        m.load(static_cast<const float*>(t.exp_avg) + at, valid);
+        v.load(static_cast<const float*>(t.exp_avg_sq) + at, valid);
+    }
+};
+template <class T> struct Tile<T, 8> {
+    Raw8<T> p, g;
+    uint2 m, v;
+    float sm, sv;
+    __device__ __forceinline__ void load(const Tensor& t, long long at, int valid) {
+        p.load(static_cast<const T*>(t.param) + at, valid);
+        g.load(static_cast<const T*>(t.grad) + at, valid);
+        m = load_codes(static_cast<const unsigned char*>(t.exp_avg) + at, valid);
+        v = load_codes(static_cast<const unsigned char*>(t.exp_avg_sq) + at, valid);
+        sm = t.exp_avg_scale[at / AW_BLOCK];
+        sv = t.exp_avg_sq_scale[at / AW_BLOCK];
+    }
+};
+__device__ __forceinline__ int valid_at(long long n, long long at) { return n - at >= 8 ? 8 : n > at ? (int)(n - at) : 0; }
+
 template <class T, int BITS, int CAP>
-__global__ void __launch_bounds__(AW_THREADS) adamw_kernel(const __grid_constant__ Table<CAP> table, const __grid_constant__ Hyper h) {
+__global__ void __launch_bounds__(AW_THREADS, BITS == 8 ? 4 : 3) adamw_kernel(const __grid_constant__ Table<CAP> table, const __grid_constant__ Hyper h) {
     const int chunk = blockIdx.x;
     int lo = 0, hi = table.count;
     while (hi - lo > 1) {
@@ -133,6 +207,11 @@ __global__ void __launch_bounds__(AW_THREADS) adamw_kernel(const __grid_constant
         if (table.first[mid] <= chunk) lo = mid; else hi = mid;
     }
     const Tensor& t = table.t[lo];
+    const long long start = (long long)(chunk - table.first[lo]) * table.tiles * AW_TILE, end = min(t.n, start + (long long)table.tiles * AW_TILE);
+    long long at = start + threadIdx.x * 8;
+    const auto has = [&](long long a) { return (a & ~(long long)(AW_BLOCK - 1)) < end; };      // the warp's block begins in the chunk
+    Tile<T, BITS> tile;
+    if (has(at)) tile.load(t, at, valid_at(t.n, at));
     const int step = t.step[0] + 1;
     // 1 - b^t through expm1, which keeps its digits where b^t is near 1
     const float lr = h.lr_device != nullptr ? *h.lr_device : h.lr;
@@ -141,36 +220,47 @@ __global__ void __launch_bounds__(AW_THREADS) adamw_kernel(const __grid_constant
     const float keep = 1.f - lr * h.wd;
     const float gs = h.grad_scale != nullptr ? *h.grad_scale : 1.f;
 
-    const long long at = (long long)(chunk - table.first[lo]) * AW_CHUNK + threadIdx.x * 8;
-    const long long left = t.n - at;
-    const int valid = left >= 8 ? 8 : left > 0 ? (int)left : 0;
-    const long long block = at / AW_BLOCK;
-    if (block * AW_BLOCK < t.n) {      // the same for all lanes of a warp
-        float p[8], g[8], m[8], v[8];
-        load8(static_cast<const T*>(t.param) + at, valid, p);
-        load8(static_cast<const T*>(t.grad) + at, valid, g);
+    while (has(at)) {
+        const int valid = valid_at(t.n, at);
+        Tile<T, BITS> next;
+        if (has(at + AW_TILE)) next.load(t, at + AW_TILE, valid_at(t.n, at + AW_TILE));
+        uint64_t p[4], g[4], m[4], v[4];
+        tile.p.pairs(p);
+        tile.g.pairs(g);
         if constexpr (BITS == 32) {
-            load8(static_cast<const float*>(t.exp_avg) + at, valid, m);
-            load8(static_cast<const float*>(t.exp_avg_sq) + at, valid, v);
+            tile.m.pairs(m);
+            tile.v.pairs(v);
         } else {
-            load_block<true>(static_cast<const unsigned char*>(t.exp_avg) + at, t.exp_avg_scale + block, valid, m);
-            load_block<false>(static_cast<const unsigned char*>(t.exp_avg_sq) + at, t.exp_avg_sq_scale + block, valid, v);
+            decode<true>(tile.m, tile.sm, m);
+            decode<false>(tile.v, tile.sv, v);
         }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float gi = __fmul_rn(g[i], gs);
-            m[i] = __fadd_rn(__fmul_rn(m[i], h.b1), __fmul_rn(gi, h.c1));
-            v[i] = __fadd_rn(__fmul_rn(v[i], h.b2), __fmul_rn(__fmul_rn(gi, gi), h.c2));
-            p[i] = p[i] * keep - size * __fdividef(m[i], fmaf(__fsqrt_rn(v[i]), root, h.eps));
+        for (int i = 0; i < 4; ++i) {
+            // Products and sums are scalar here, each rounded by itself: a mul.rn.f32x2 and the add behind it come out as one fused
+            // multiply-add, whose sum rounds once, and codes would differ from their definition.
+            float g0, g1, m0, m1, v0, v1;
+            unpack2(mul2(g[i], twice(gs)), g0, g1);
+            unpack2(m[i], m0, m1);
+            unpack2(v[i], v0, v1);
+            m0 = __fadd_rn(__fmul_rn(m0, h.b1), __fmul_rn(g0, h.c1));
+            m1 = __fadd_rn(__fmul_rn(m1, h.b1), __fmul_rn(g1, h.c1));
+            v0 = __fadd_rn(__fmul_rn(v0, h.b2), __fmul_rn(__fmul_rn(g0, g0), h.c2));
+            v1 = __fadd_rn(__fmul_rn(v1, h.b2), __fmul_rn(__fmul_rn(g1, g1), h.c2));
+            m[i] = pack2(m0, m1);
+            v[i] = pack2(v0, v1);
+            const float u0 = __fdividef(m0, fmaf(root_of(v0), root, h.eps)), u1 = __fdividef(m1, fmaf(root_of(v1), root, h.eps));
+            p[i] = fma2(pack2(u0, u1), twice(-size), mul2(p[i], twice(keep)));
         }
         store8(static_cast<T*>(t.param) + at, valid, p);
         if constexpr (BITS == 32) {
             store8(static_cast<float*>(t.exp_avg) + at, valid, m);
             store8(static_cast<float*>(t.exp_avg_sq) + at, valid, v);
         } else {
-            store_block<true>(static_cast<unsigned char*>(t.exp_avg) + at, t.exp_avg_scale + block, valid, m);
-            store_block<false>(static_cast<unsigned char*>(t.exp_avg_sq) + at, t.exp_avg_sq_scale + block, valid, v);
+            store_block<true>(static_cast<unsigned char*>(t.exp_avg) + at, t.exp_avg_scale + at / AW_BLOCK, valid, m);
+            store_block<false>(static_cast<unsigned char*>(t.exp_avg_sq) + at, t.exp_avg_sq_scale + at / AW_BLOCK, valid, v);
         }
+        tile = next;
+        at += AW_TILE;
     }
     // Every thread of every chunk has read the step count when the last chunk arrives: that one counts it up.
     __syncthreads();
@@ -185,29 +275,39 @@ __global__ void __launch_bounds__(AW_THREADS) adamw_kernel(const __grid_constant
 
 template <bool SIGNED>
 __global__ void __launch_bounds__(AW_THREADS) adamw_values_kernel(const unsigned char* codes, const float* scales, float* values, long long n) {
-    const long long at = ((long long)blockIdx.x * AW_THREADS + threadIdx.x) * 8;
-    if (at >= n) return;
-    const int valid = n - at >= 8 ? 8 : (int)(n - at);
-    float x[8];
-    load_block<SIGNED>(codes + at, scales + at / AW_BLOCK, valid, x);
-    store8(values + at, valid, x);
-}
-
-template <class T, int CAP> int launch_table(const Table<CAP>& table, const Hyper& h, int bits, int chunks, cudaStream_t s) {
-    if (bits == 32) adamw_kernel<T, 32, CAP><<<chunks, AW_THREADS, 0, s>>>(table, h);
-    else adamw_kernel<T, 8, CAP><<<chunks, AW_THREADS, 0, s>>>(table, h);
-    return launched();
+    constexpr int TILES = 4;
+    const long long first = (long long)blockIdx.x * TILES * AW_TILE + threadIdx.x * 8;
+    uint2 c[TILES];
+    float sc[TILES];
+#pragma unroll
+    for (int i = 0; i < TILES; ++i) {
+        const long long at = first + i * AW_TILE;
+        if (at < n) {
+            c[i] = load_codes(codes + at, valid_at(n, at));
+            sc[i] = scales[at / AW_BLOCK];
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < TILES; ++i) {
+        const long long at = first + i * AW_TILE;
+        if (at >= n) break;
+        uint64_t x[4];
+        decode<SIGNED>(c[i], sc[i], x);
+        store8(values + at, valid_at(n, at), x);
+    }
 }
 
 // Launches over as many tensors from `tensors` on as a table takes; *next is the first that is left.
-template <class T, int CAP> int launch_some(const Tensor* tensors, int count, int* next, const Hyper& h, int bits, cudaStream_t s) {
+template <class T, int CAP> int launch_some(const Tensor* tensors, int count, int* next, const Hyper& h, int bits, int tiles, cudaStream_t s) {
     Table<CAP> table;
     table.count = 0;
+    table.tiles = tiles;
+    const long long elements = (long long)tiles * AW_TILE;
     long long chunks = 0;
     int i = *next;
     for (; i < count && table.count < CAP; ++i) {
         if (tensors[i].n == 0) continue;
-        const long long more = (tensors[i].n + AW_CHUNK - 1) / AW_CHUNK;
+        const long long more = (tensors[i].n + elements - 1) / elements;
         if (chunks + more > 2147483647LL) break;
         table.first[table.count] = (int)chunks;
         table.t[table.count++] = tensors[i];
@@ -216,7 +316,9 @@ template <class T, int CAP> int launch_some(const Tensor* tensors, int count, in
     *next = i;
     if (table.count == 0) return ADDER_OK;
     table.first[table.count] = (int)chunks;
-    return launch_table<T, CAP>(table, h, bits, (int)chunks, s);
+    if (bits == 32) adamw_kernel<T, 32, CAP><<<(unsigned)chunks, AW_THREADS, 0, s>>>(table, h);
+    else adamw_kernel<T, 8, CAP><<<(unsigned)chunks, AW_THREADS, 0, s>>>(table, h);
+    return launched();
 }
 
 }  // namespace
@@ -235,11 +337,13 @@ int adder_b200_adamw_step(const adder_b200_adamw_tensor* tensors, int count, int
     if (count == 0) return ADDER_OK;
     if (tensors == nullptr) return ADDER_ERR_NULL_POINTER;
     const unsigned size = dtype == ADDER_TYPE_F32 ? 4 : 2;
+    long long elements = 0;
     for (int i = 0; i < count; ++i) {
         const adder_b200_adamw_tensor& t = tensors[i];
         if (t.n < 0) return ADDER_ERR_BAD_SHAPE;
         if (t.n == 0) continue;
-        if (t.n > (2147483647LL - 1) * AW_CHUNK) return ADDER_ERR_UNSUPPORTED;
+        if (t.n > 2147483647LL * AW_TILE) return ADDER_ERR_UNSUPPORTED;
+        elements += t.n;
         if (!t.param || !t.grad || !t.exp_avg || !t.exp_avg_sq || !t.step) return ADDER_ERR_NULL_POINTER;
         if (state_bits == 8 && (!t.exp_avg_scale || !t.exp_avg_sq_scale)) return ADDER_ERR_NULL_POINTER;
         if (!aligned_to(t.param, size) || !aligned_to(t.grad, size) || !aligned_to(t.step, 4)) return ADDER_ERR_ALIGNMENT;
@@ -252,12 +356,18 @@ int adder_b200_adamw_step(const adder_b200_adamw_tensor* tensors, int count, int
     h.eps = (float)eps; h.wd = (float)weight_decay;
     h.ln_b1 = (float)std::log(beta1); h.ln_b2 = (float)std::log(beta2);      // -inf for 0: 1 - 0^t = 1
     h.lr_device = lr_device; h.grad_scale = grad_scale;
+    // Small models get a CTA for every tile, so that all SMs take part; large ones up to 8 tiles a CTA, which fetches one while it computes
+    // another.
+    int tiles = 1;
+    while (tiles < 8 && elements >= 8LL * sm_count() * tiles * AW_TILE) tiles *= 2;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     return with_type(dtype, [&](auto* type) {
         using T = std::remove_pointer_t<decltype(type)>;
         for (int next = 0; next < count;) {
-            const int st = count - next <= 48 ? launch_some<T, 48>(tensors, count, &next, h, state_bits, s)
-                                              : launch_some<T, 480>(tensors, count, &next, h, state_bits, s);
+            const int left = count - next;
+            const int st = left <= 48 ? launch_some<T, 48>(tensors, count, &next, h, state_bits, tiles, s)
+                           : left <= 176 ? launch_some<T, 176>(tensors, count, &next, h, state_bits, tiles, s)
+                                         : launch_some<T, 480>(tensors, count, &next, h, state_bits, tiles, s);
             if (st != ADDER_OK) return st;
         }
         return (int)ADDER_OK;
@@ -269,7 +379,7 @@ int adder_b200_adamw_state_values(const unsigned char* codes, const float* scale
     if (n == 0) return ADDER_OK;
     if (!codes || !scales || !values) return ADDER_ERR_NULL_POINTER;
     if (!aligned_to(scales, 4) || !aligned_to(values, 4)) return ADDER_ERR_ALIGNMENT;
-    const long long grid = (n + AW_CHUNK - 1) / AW_CHUNK;
+    const long long grid = (n + 4 * AW_TILE - 1) / (4 * AW_TILE);
     if (grid > 2147483647LL) return ADDER_ERR_UNSUPPORTED;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (is_signed) adamw_values_kernel<true><<<(unsigned)grid, AW_THREADS, 0, s>>>(codes, scales, values, n);

@@ -153,16 +153,7 @@ template <class S> __device__ __forceinline__ void ln_fetch(LnPairs<S>& f, uint3
         for (int i = 0; i < S::NV; ++i) {
 #pragma unroll
             for (int j = 0; j < S::VEC; ++j) e[i][j] = 0.f;
-            if (v + i * S::G < v1) {
-                const T* p = row + (size_t)(v + i * S::G) * S::VEC;
-                if constexpr (S::VEC > 2) {      // read once: the first-level cache is the weights'
-                    uint4 q;
-                    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(q.x), "=r"(q.y), "=r"(q.z), "=r"(q.w) : "l"(p));
-                    Vec16<T>::unpack(q, e[i]);
-                } else {
-                    load_some<T, S::VEC>(p, e[i]);
-                }
-            }
+            if (v + i * S::G < v1) load_some<T, S::VEC>(row + (size_t)(v + i * S::G) * S::VEC, e[i]);
         }
 #pragma unroll
         for (int i = 0; i < LnPairs<S>::P; ++i) f.p[i] = pack2((&e[0][0])[2 * i], (&e[0][0])[2 * i + 1]);
@@ -386,7 +377,7 @@ template <class S> __global__ void __launch_bounds__(S::THREADS, S::THREADS > 25
         if (a.mean != nullptr && t == 0) { a.mean[row] = mom.x; a.rstd[row] = rs; }
         const uint64_t minus = pack2(-mom.x, -mom.x), scale = pack2(rs, rs);
 #pragma unroll
-        for (int i = 0; i < LnPairs<S>::P; ++i) f.p[i] = fma2(fma2(add2(f.p[i], minus), scale, 0), w.p[i], b.p[i]);
+        for (int i = 0; i < LnPairs<S>::P; ++i) f.p[i] = fma2(mul2(add2(f.p[i], minus), scale), w.p[i], b.p[i]);
         ln_store<S>(static_cast<T*>(a.y) + row * a.d, f, v, v1);
     }
 }
@@ -421,7 +412,7 @@ template <class S> __global__ void __launch_bounds__(S::THREADS, S::NV * S::VEC 
         LnPairs<S> w;
         ln_weights<S>(w, a.w, 1.f, v, v1);
 #pragma unroll
-        for (int i = 0; i < LnPairs<S>::P; ++i) f.p[i] = fma2(fma2(add2(f.p[i], minus), scale, 0), w.p[i], 0);
+        for (int i = 0; i < LnPairs<S>::P; ++i) f.p[i] = mul2(mul2(add2(f.p[i], minus), scale), w.p[i]);
         ln_weights<S>(w, a.b, 0.f, v, v1);
 #pragma unroll
         for (int i = 0; i < LnPairs<S>::P; ++i) f.p[i] = add2(f.p[i], w.p[i]);
@@ -453,8 +444,8 @@ template <class S> __global__ void __launch_bounds__(S::THREADS, S::NV * S::VEC 
         const uint64_t minus = pack2(-mean, -mean), scale = pack2(rs, rs);
 #pragma unroll
         for (int i = 0; i < LnPairs<S>::P; ++i) {      // dy is 0 where there is no element
-            xh.p[i] = fma2(add2(xh.p[i], minus), scale, 0);
-            g.p[i] = fma2(g.p[i], w.p[i], 0);
+            xh.p[i] = mul2(add2(xh.p[i], minus), scale);
+            g.p[i] = mul2(g.p[i], w.p[i]);
             s1 = add2(s1, g.p[i]);
             s2 = fma2(g.p[i], xh.p[i], s2);
         }
@@ -465,7 +456,7 @@ template <class S> __global__ void __launch_bounds__(S::THREADS, S::NV * S::VEC 
         const float c1 = -m.x * inv_d, c2 = -m.y * inv_d;
         const uint64_t shift = pack2(c1, c1), slope = pack2(c2, c2);
 #pragma unroll
-        for (int i = 0; i < LnPairs<S>::P; ++i) g.p[i] = fma2(fma2(xh.p[i], slope, add2(g.p[i], shift)), scale, 0);
+        for (int i = 0; i < LnPairs<S>::P; ++i) g.p[i] = mul2(fma2(xh.p[i], slope, add2(g.p[i], shift)), scale);
         if (a.dh != nullptr) {
             ln_fetch<S>(w, 0, static_cast<const T*>(a.dh) + row * a.d, v, v1);
 #pragma unroll
@@ -521,12 +512,12 @@ template <class S, bool SUMS> __global__ void __launch_bounds__(S::THREADS, 1) l
         const uint64_t minus = pack2(-mean, -mean), scale = pack2(rs, rs);
 #pragma unroll
         for (int i = 0; i < P; ++i) {      // dy is 0 where there is no element
-            xh.p[i] = fma2(add2(xh.p[i], minus), scale, 0);
+            xh.p[i] = mul2(add2(xh.p[i], minus), scale);
             if (SUMS) {
                 dw.p[i] = fma2(g.p[i], xh.p[i], dw.p[i]);
                 db.p[i] = add2(db.p[i], g.p[i]);
             }
-            g.p[i] = fma2(g.p[i], w.p[i], 0);
+            g.p[i] = mul2(g.p[i], w.p[i]);
             s1 = add2(s1, g.p[i]);
             s2 = fma2(g.p[i], xh.p[i], s2);
         }
@@ -539,7 +530,7 @@ template <class S, bool SUMS> __global__ void __launch_bounds__(S::THREADS, 1) l
             const float c1 = -m.x * inv_d, c2 = -m.y * inv_d;
             const uint64_t shift = pack2(c1, c1), slope = pack2(c2, c2);
 #pragma unroll
-            for (int i = 0; i < P; ++i) g.p[i] = fma2(fma2(xh.p[i], slope, add2(g.p[i], shift)), scale, 0);
+            for (int i = 0; i < P; ++i) g.p[i] = mul2(fma2(xh.p[i], slope, add2(g.p[i], shift)), scale);
             if (a.dh != nullptr) {
                 LnPairs<S> e;
                 ln_fetch<S>(e, walk.slot(walk.read, 2), static_cast<const T*>(a.dh) + row * a.d, v, v1);

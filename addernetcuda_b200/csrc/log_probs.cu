@@ -172,8 +172,8 @@ template <bool ENTROPY> struct Running {
         d = fmaxf(d, LP_FLOOR);
         const float f = exp2_fast(d);
         const uint64_t f2 = pack2(f, f);
-        if (ENTROPY) t = fma2(fma2(s, pack2(d, d), t), f2, 0);
-        s = fma2(s, f2, 0);
+        if (ENTROPY) t = mul2(fma2(s, pack2(d, d), t), f2);
+        s = mul2(s, f2);
     }
     __device__ __forceinline__ void raise(float top) {
         const float ref_new = top * LOG2E, res_new = fabsf(top) < 8192.f ? fmaf(top, LOG2E, -ref_new) : 0.f;
@@ -675,11 +675,11 @@ template <bool ENTROPY> struct Slope {
         float d0, d1;
         unpack2(fma2(x, pack2(LOG2E, LOG2E), pack2(-ref, -ref)), d0, d1);
         if (ENTROPY) { d0 = max_nan(d0, LP_FLOOR); d1 = max_nan(d1, LP_FLOOR); }
-        const uint64_t e = fma2(pack2(exp2_fast(d0), exp2_fast(d1)), pack2(scale, scale), 0);
+        const uint64_t e = mul2(pack2(exp2_fast(d0), exp2_fast(d1)), pack2(scale, scale));
         if (!ENTROPY) return e;
         // d log(2) + H - ln s is log p + H
         const uint64_t lp = fma2(pack2(d0, d1), pack2(LN2, LN2), pack2(shift, shift));
-        return fma2(e, fma2(lp, pack2(g_ent, g_ent), pack2(sum, sum)), 0);
+        return mul2(e, fma2(lp, pack2(g_ent, g_ent), pack2(sum, sum)));
     }
     __device__ __forceinline__ float one(float v) const {
         if (nothing) return 0.f;
