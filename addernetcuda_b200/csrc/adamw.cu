@@ -35,23 +35,24 @@ struct Hyper {
 template <class T> struct Raw8 {
     static constexpr int Q = sizeof(T) / 2;      // 16-byte words
     uint4 q[Q];
+    // all eight, from shared memory
+    __device__ __forceinline__ void read(uint32_t at) {
+#pragma unroll
+        for (int i = 0; i < Q; ++i)
+            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(q[i].x), "=r"(q[i].y), "=r"(q[i].z), "=r"(q[i].w) : "r"(at + 16 * i) : "memory");
+    }
     __device__ __forceinline__ void load(const T* p, int valid) {
-        if (valid == 8 && aligned_to(p, 16)) {
+        uint32_t w[4 * Q];
 #pragma unroll
-            for (int i = 0; i < Q; ++i) q[i] = reinterpret_cast<const uint4*>(p)[i];
-        } else {
-            uint32_t w[4 * Q];
+        for (int i = 0; i < 4 * Q; ++i) w[i] = 0;
 #pragma unroll
-            for (int i = 0; i < 4 * Q; ++i) w[i] = 0;
+        for (int i = 0; i < 8; ++i)
+            if (i < valid) {
+                if constexpr (sizeof(T) == 4) w[i] = __float_as_uint(p[i]);
+                else w[i / 2] |= (uint32_t)reinterpret_cast<const unsigned short*>(p)[i] << (16 * (i & 1));
+            }
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (i < valid) {
-                    if constexpr (sizeof(T) == 4) w[i] = __float_as_uint(p[i]);
-                    else w[i / 2] |= (uint32_t)reinterpret_cast<const unsigned short*>(p)[i] << (16 * (i & 1));
-                }
-#pragma unroll
-            for (int i = 0; i < Q; ++i) q[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
-        }
+        for (int i = 0; i < Q; ++i) q[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
     }
     // as four pairs of fp32
     __device__ __forceinline__ void pairs(uint64_t (&f)[4]) const {
@@ -68,35 +69,31 @@ template <class T> struct Raw8 {
         }
     }
 };
-template <class T> __device__ __forceinline__ void store8(T* p, int valid, const uint64_t (&pairs)[4]) {
+template <bool WHOLE, class T> __device__ __forceinline__ void store8(T* p, int valid, const uint64_t (&pairs)[4]) {
     float f[8];
 #pragma unroll
     for (int i = 0; i < 4; ++i) unpack2(pairs[i], f[2 * i], f[2 * i + 1]);
-    if (valid == 8 && aligned_to(p, 16)) {
-        constexpr int N = Vec16<T>::N;
-#pragma unroll
-        for (int i = 0; i < 8 / N; ++i) {
-            float v[N];
-#pragma unroll
-            for (int j = 0; j < N; ++j) v[j] = f[i * N + j];
-            reinterpret_cast<uint4*>(p)[i] = Vec16<T>::pack(v);
-        }
-    } else {
+    if constexpr (!WHOLE) {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
             if (i < valid) p[i] = from_float<T>(f[i]);
+    } else if constexpr (sizeof(T) == 4) {
+        asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                     ::"l"(p), "f"(f[0]), "f"(f[1]), "f"(f[2]), "f"(f[3]), "f"(f[4]), "f"(f[5]), "f"(f[6]), "f"(f[7]) : "memory");
+    } else {
+        *reinterpret_cast<uint4*>(p) = Vec16<T>::pack(f);
     }
 }
-__device__ __forceinline__ uint2 load_codes(const unsigned char* p, int valid) {
-    if (valid == 8 && aligned_to(p, 8)) return *reinterpret_cast<const uint2*>(p);
+template <bool WHOLE> __device__ __forceinline__ uint2 load_codes(const unsigned char* p, int valid) {
+    if constexpr (WHOLE) return *reinterpret_cast<const uint2*>(p);
     uint32_t w[2] = {0, 0};
 #pragma unroll
     for (int i = 0; i < 8; ++i)
         if (i < valid) w[i >> 2] |= (uint32_t)p[i] << (8 * (i & 3));
     return make_uint2(w[0], w[1]);
 }
-__device__ __forceinline__ void store_codes(unsigned char* p, int valid, uint2 c) {
-    if (valid == 8 && aligned_to(p, 8)) {
+template <bool WHOLE> __device__ __forceinline__ void store_codes(unsigned char* p, int valid, uint2 c) {
+    if constexpr (WHOLE) {
         *reinterpret_cast<uint2*>(p) = c;
         return;
     }
@@ -110,12 +107,12 @@ constexpr float TOP_M = 248.f, TOP_V = 63488.f, SMALLEST = 0x1p-100f;
 __device__ __forceinline__ uint64_t twice(float v) { return pack2(v, v); }
 
 // The magnitude of a code is the fp32 number with the code at bit 19 (a subnormal one where the exponent field is 0), times 2^127; a sign at bit
-// 7 of the code goes to bit 31.  Eight codes, as pairs.
+// 7 of the code goes to bit 31.  Eight codes, as pairs.  What bounds the 8-bit step beside memory is the integer pipe, half as wide as the
+// one that multiplies: shifts are products here.
 template <bool SIGNED> __device__ __forceinline__ float code_bits(uint32_t word, int i) {
-    constexpr uint32_t mask = (SIGNED ? 127u : 255u) << 19;
-    const uint32_t mag = (i < 3 ? word << (19 - 8 * i) : word >> 5) & mask;
-    if (!SIGNED) return __uint_as_float(mag);
-    return __uint_as_float(mag | ((word << (24 - 8 * i)) & 0x80000000u));
+    const uint32_t at19 = __byte_perm(word, 0, 0x4044 | (i << 8)) * 8u;
+    if (!SIGNED) return __uint_as_float(at19);
+    return __uint_as_float((at19 & (1u << 26)) * 31u + at19);      // 2^26 becomes 2^31
 }
 template <bool SIGNED> __device__ __forceinline__ void decode(uint2 c, float scale, uint64_t (&x)[4]) {
     const uint64_t up = twice(0x1p127f), sc = twice(scale);
@@ -126,14 +123,10 @@ template <bool SIGNED> __device__ __forceinline__ void decode(uint2 c, float sca
     }
 }
 
-// Code of a value that has been scaled to the code's range and by 2^-127: rounded to nearest even at bit 19, and moved to the top byte (a
-// sign, that of the value plus 0, to its top bit: a negative value keeps it where it rounds to 0, -0 has none).
-template <bool SIGNED> __device__ __forceinline__ uint32_t round_to_code(float scaled, float x) {
+// Code of a magnitude that has been scaled to the code's range and by 2^-127: rounded to nearest even at bit 19, moved to the top byte.
+__device__ __forceinline__ uint32_t round_to_code(float scaled) {
     const uint32_t bits = __float_as_uint(scaled);
-    uint32_t r = bits + 0x3ffffu + ((bits >> 19) & 1u);
-    if (SIGNED) return ((r << 5) & 0x7fffffffu) | (__float_as_uint(x) & 0x80000000u);
-    if (x > 0.f) r = max(r, 1u << 19);
-    return r << 5;
+    return (bits + 0x3ffffu + ((bits >> 19) & 1u)) * 32u;
 }
 __device__ __forceinline__ uint32_t top_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     return __byte_perm(__byte_perm(a, b, 0x0073), __byte_perm(c, d, 0x0073), 0x5410);
@@ -141,7 +134,7 @@ __device__ __forceinline__ uint32_t top_bytes(uint32_t a, uint32_t b, uint32_t c
 
 // Stores the warp's block of 256 values, eight to a lane.  Each operation rounds to fp32 by itself, so that the codes are defined bit by
 // bit.
-template <bool SIGNED> __device__ __forceinline__ void store_block(unsigned char* codes, float* scale, int valid, const uint64_t (&x)[4]) {
+template <bool SIGNED, bool WHOLE> __device__ __forceinline__ void store_block(unsigned char* codes, float* scale, int valid, const uint64_t (&x)[4]) {
     float f[8], top = 0.f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) unpack2(x[i], f[2 * i], f[2 * i + 1]);
@@ -155,51 +148,177 @@ template <bool SIGNED> __device__ __forceinline__ void store_block(unsigned char
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         float a, b;
-        if (SIGNED) unpack2(add2(x[i], 0), f[2 * i], f[2 * i + 1]);
         unpack2(mul2(mul2(x[i], twice(inv)), twice(0x1p-127f)), a, b);
-        r[2 * i] = round_to_code<SIGNED>(a, f[2 * i]);
-        r[2 * i + 1] = round_to_code<SIGNED>(b, f[2 * i + 1]);
+        r[2 * i] = round_to_code(a);
+        r[2 * i + 1] = round_to_code(b);
     }
-    uint2 c = make_uint2(top_bytes(r[0], r[1], r[2], r[3]), top_bytes(r[4], r[5], r[6], r[7]));
-    if (largest == 0.f) c = SIGNED ? make_uint2(c.x & 0x80808080u, c.y & 0x80808080u) : make_uint2(0, 0);
-    store_codes(codes, valid, c);
+    uint32_t c[2] = {top_bytes(r[0], r[1], r[2], r[3]), top_bytes(r[4], r[5], r[6], r[7])};
+    if (largest == 0.f) c[0] = c[1] = 0;
+    if constexpr (SIGNED) {      // a negative value keeps its sign where it rounds to 0; -0, which is none, loses it in the sum with 0
+#pragma unroll
+        for (int i = 0; i < 4; ++i) unpack2(add2(x[i], 0), f[2 * i], f[2 * i + 1]);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint32_t signs = top_bytes(__float_as_uint(f[4 * i]), __float_as_uint(f[4 * i + 1]), __float_as_uint(f[4 * i + 2]), __float_as_uint(f[4 * i + 3]));
+            c[i] = (c[i] & 0x7f7f7f7fu) | (signs & 0x80808080u);
+        }
+    } else if (largest > 0.f) {      // a value above 0 has code 1 at least
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            if ((c[i] - 0x01010101u) & ~c[i] & 0x80808080u) {      // a byte of 0 among the four
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (((c[i] >> (8 * j)) & 255u) == 0 && f[4 * i + j] > 0.f) c[i] |= 1u << (8 * j);
+            }
+    }
+    store_codes<WHOLE>(codes, valid, make_uint2(c[0], c[1]));
     if ((threadIdx.x & 31) == 0) *scale = __fmul_rn(largest, 1.f / limit);
 }
 
+// Approximate to 2^-23 or so, like the reciprocal below, and 0 below 2^-126: nothing beside eps.
+__device__ __forceinline__ float reciprocal_of(float x) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
 __device__ __forceinline__ float root_of(float x) {
     float r;
-    asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+    asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
 
-// What a thread reads of a tile.
+// A thread's places in the tensors, and what it reads there.
+template <class T, int BITS> struct Place {
+    T* p;
+    const T* g;
+    float *m, *v;
+    __device__ __forceinline__ Place(const Tensor& t, long long at)
+        : p(static_cast<T*>(t.param) + at), g(static_cast<const T*>(t.grad) + at), m(static_cast<float*>(t.exp_avg) + at), v(static_cast<float*>(t.exp_avg_sq) + at) {}
+    __device__ __forceinline__ void advance() { p += AW_TILE; g += AW_TILE; m += AW_TILE; v += AW_TILE; }
+    __device__ __forceinline__ bool whole() const { return aligned_to(p, 8 * sizeof(T)) && aligned_to(g, 16) && aligned_to(m, 32) && aligned_to(v, 32); }
+};
+template <class T> struct Place<T, 8> {
+    T* p;
+    const T* g;
+    unsigned char *m, *v;
+    float *sm, *sv;
+    __device__ __forceinline__ Place(const Tensor& t, long long at)
+        : p(static_cast<T*>(t.param) + at), g(static_cast<const T*>(t.grad) + at), m(static_cast<unsigned char*>(t.exp_avg) + at),
+          v(static_cast<unsigned char*>(t.exp_avg_sq) + at), sm(t.exp_avg_scale + at / AW_BLOCK), sv(t.exp_avg_sq_scale + at / AW_BLOCK) {}
+    __device__ __forceinline__ void advance() {
+        p += AW_TILE; g += AW_TILE; m += AW_TILE; v += AW_TILE;
+        sm += AW_TILE / AW_BLOCK; sv += AW_TILE / AW_BLOCK;
+    }
+    __device__ __forceinline__ bool whole() const { return aligned_to(p, 8 * sizeof(T)) && aligned_to(g, 16) && aligned_to(m, 8) && aligned_to(v, 8); }
+};
+// A warp's 256 elements of each tensor on their way through shared memory, STAGES tiles deep.  Lanes copy consecutive 16-byte words, so what
+// a lane reads may be another's copy: the warp waits for its copies together.  Offsets in a stage, in bytes.
+template <class T, int BITS> struct Ring {
+    static constexpr int E = AW_BLOCK * sizeof(T), F = BITS == 32 ? AW_BLOCK * 4 : AW_BLOCK;
+    static constexpr int P = 0, G = E, M = 2 * E, V = 2 * E + F, S = 2 * E + 2 * F, STAGE = S + (BITS == 8 ? 16 : 0);
+    static constexpr int STAGES = BITS == 8 ? 4 : sizeof(T) == 2 ? 3 : 2;
+    static constexpr int WARP = STAGES * STAGE, BYTES = AW_THREADS / 32 * WARP;
+
+    template <int N> static __device__ __forceinline__ void copy(uint32_t to, const void* from, int lane) {      // N bytes
+        const char* p = static_cast<const char*>(from);
+        if constexpr (N >= 512) {
+#pragma unroll
+            for (int i = 0; i < N / 512; ++i)
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(to + 512 * i + 16 * lane), "l"(p + 512 * i + 16 * lane) : "memory");
+        } else {
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 8;\n" ::"r"(to + 8 * lane), "l"(p + 8 * lane) : "memory");
+        }
+    }
+    // `at` is of the warp's first element
+    static __device__ __forceinline__ void fill(uint32_t stage, const Place<T, BITS>& at, int tile, int lane) {
+        const int o = tile * AW_TILE;
+        copy<E>(stage + P, at.p + o, lane);
+        copy<E>(stage + G, at.g + o, lane);
+        copy<F>(stage + M, at.m + o, lane);
+        copy<F>(stage + V, at.v + o, lane);
+        if constexpr (BITS == 8) {
+            const int b = tile * (AW_TILE / AW_BLOCK);
+            if (lane < 2) asm volatile("cp.async.ca.shared.global [%0], [%1], 4;\n" ::"r"(stage + S + 4 * lane), "l"((lane == 0 ? at.sm : at.sv) + b) : "memory");
+        }
+    }
+};
+
 template <class T, int BITS> struct Tile {
     Raw8<T> p, g;
     Raw8<float> m, v;
-    __device__ __forceinline__ void load(const Tensor& t, long long at, int valid) {
-        p.load(static_cast<const T*>(t.param) + at, valid);
-        g.load(static_cast<const T*>(t.grad) + at, valid);
-        m.load(static_cast<const float*>(t.exp_avg) + at, valid);
-        v.load(static_cast<const float*>(t.exp_avg_sq) + at, valid);
+    __device__ __forceinline__ void load(const Place<T, BITS>& at, int valid) {
+        p.load(at.p, valid); g.load(at.g, valid); m.load(at.m, valid); v.load(at.v, valid);
+    }
+    __device__ __forceinline__ void read(uint32_t stage, int lane) {
+        using R = Ring<T, BITS>;
+        p.read(stage + R::P + lane * 8 * sizeof(T)); g.read(stage + R::G + lane * 8 * sizeof(T));
+        m.read(stage + R::M + lane * 32); v.read(stage + R::V + lane * 32);
     }
 };
 template <class T> struct Tile<T, 8> {
     Raw8<T> p, g;
     uint2 m, v;
     float sm, sv;
-    __device__ __forceinline__ void load(const Tensor& t, long long at, int valid) {
-        p.load(static_cast<const T*>(t.param) + at, valid);
-        g.load(static_cast<const T*>(t.grad) + at, valid);
-        m = load_codes(static_cast<const unsigned char*>(t.exp_avg) + at, valid);
-        v = load_codes(static_cast<const unsigned char*>(t.exp_avg_sq) + at, valid);
-        sm = t.exp_avg_scale[at / AW_BLOCK];
-        sv = t.exp_avg_sq_scale[at / AW_BLOCK];
+    __device__ __forceinline__ void load(const Place<T, 8>& at, int valid) {
+        p.load(at.p, valid); g.load(at.g, valid);
+        m = load_codes<false>(at.m, valid);
+        v = load_codes<false>(at.v, valid);
+        sm = *at.sm; sv = *at.sv;
+    }
+    __device__ __forceinline__ void read(uint32_t stage, int lane) {
+        using R = Ring<T, 8>;
+        p.read(stage + R::P + lane * 8 * sizeof(T)); g.read(stage + R::G + lane * 8 * sizeof(T));
+        asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(m.x), "=r"(m.y) : "r"(stage + R::M + lane * 8) : "memory");
+        asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(stage + R::V + lane * 8) : "memory");
+        asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(sm), "=f"(sv) : "r"(stage + R::S) : "memory");
     }
 };
 __device__ __forceinline__ int valid_at(long long n, long long at) { return n - at >= 8 ? 8 : n > at ? (int)(n - at) : 0; }
 
+// The numbers of a step: size = lr / (1 - b1^t), root = 1 / sqrt(1 - b2^t), keep = 1 - lr wd.
+struct StepNumbers { float size, root, keep, scale; };
+
+template <class T, int BITS, bool WHOLE>
+__device__ __forceinline__ void update(const Place<T, BITS>& at, const Tile<T, BITS>& tile, int valid, const Hyper& h, const StepNumbers& n) {
+    uint64_t p[4], g[4], m[4], v[4];
+    tile.p.pairs(p);
+    tile.g.pairs(g);
+    if constexpr (BITS == 32) {
+        tile.m.pairs(m);
+        tile.v.pairs(v);
+    } else {
+        decode<true>(tile.m, tile.sm, m);
+        decode<false>(tile.v, tile.sv, v);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        // Products and sums are scalar here, each rounded by itself: a mul.rn.f32x2 and the add behind it come out as one fused
+        // multiply-add, whose sum rounds once, and codes would differ from their definition.
+        float g0, g1, m0, m1, v0, v1, d0, d1;
+        unpack2(mul2(g[i], twice(n.scale)), g0, g1);
+        unpack2(m[i], m0, m1);
+        unpack2(v[i], v0, v1);
+        m0 = __fadd_rn(__fmul_rn(m0, h.b1), __fmul_rn(g0, h.c1));
+        m1 = __fadd_rn(__fmul_rn(m1, h.b1), __fmul_rn(g1, h.c1));
+        v0 = __fadd_rn(__fmul_rn(v0, h.b2), __fmul_rn(__fmul_rn(g0, g0), h.c2));
+        v1 = __fadd_rn(__fmul_rn(v1, h.b2), __fmul_rn(__fmul_rn(g1, g1), h.c2));
+        m[i] = pack2(m0, m1);
+        v[i] = pack2(v0, v1);
+        unpack2(fma2(pack2(root_of(v0), root_of(v1)), twice(n.root), twice(h.eps)), d0, d1);
+        p[i] = fma2(mul2(m[i], pack2(reciprocal_of(d0), reciprocal_of(d1))), twice(-n.size), mul2(p[i], twice(n.keep)));
+    }
+    store8<WHOLE>(at.p, valid, p);
+    if constexpr (BITS == 32) {
+        store8<WHOLE>(at.m, valid, m);
+        store8<WHOLE>(at.v, valid, v);
+    } else {
+        store_block<true, WHOLE>(at.m, at.sm, valid, m);
+        store_block<false, WHOLE>(at.v, at.sv, valid, v);
+    }
+}
+
 template <class T, int BITS, int CAP>
-__global__ void __launch_bounds__(AW_THREADS, BITS == 8 ? 4 : 3) adamw_kernel(const __grid_constant__ Table<CAP> table, const __grid_constant__ Hyper h) {
+__global__ void __launch_bounds__(AW_THREADS, 4) adamw_kernel(const __grid_constant__ Table<CAP> table, const __grid_constant__ Hyper h) {
     const int chunk = blockIdx.x;
     int lo = 0, hi = table.count;
     while (hi - lo > 1) {
@@ -208,59 +327,41 @@ __global__ void __launch_bounds__(AW_THREADS, BITS == 8 ? 4 : 3) adamw_kernel(co
     }
     const Tensor& t = table.t[lo];
     const long long start = (long long)(chunk - table.first[lo]) * table.tiles * AW_TILE, end = min(t.n, start + (long long)table.tiles * AW_TILE);
-    long long at = start + threadIdx.x * 8;
-    const auto has = [&](long long a) { return (a & ~(long long)(AW_BLOCK - 1)) < end; };      // the warp's block begins in the chunk
-    Tile<T, BITS> tile;
-    if (has(at)) tile.load(t, at, valid_at(t.n, at));
+    using R = Ring<T, BITS>;
+    extern __shared__ uint4 smem[];
+    const int lane = threadIdx.x & 31;
+    const uint32_t ring = smem_u32(smem) + (threadIdx.x >> 5) * R::WARP;
+    Place<T, BITS> at(t, start + threadIdx.x * 8);
+    Place<T, BITS> warp(t, start + (threadIdx.x & ~31) * 8);      // of the warp's first element
+    const int whole = warp.whole() ? (int)((end - start) / AW_TILE) : 0;      // tiles that are copied in words; the same for all threads
+#pragma unroll
+    for (int i = 0; i < R::STAGES - 1; ++i) {
+        if (i < whole) R::fill(ring + i * R::STAGE, warp, i, lane);
+        cp_async_commit();
+    }
     const int step = t.step[0] + 1;
     // 1 - b^t through expm1, which keeps its digits where b^t is near 1
     const float lr = h.lr_device != nullptr ? *h.lr_device : h.lr;
-    const float size = lr / -expm1f((float)step * h.ln_b1);
-    const float root = rsqrtf(-expm1f((float)step * h.ln_b2));
-    const float keep = 1.f - lr * h.wd;
-    const float gs = h.grad_scale != nullptr ? *h.grad_scale : 1.f;
+    const StepNumbers n{lr / -expm1f((float)step * h.ln_b1), rsqrtf(-expm1f((float)step * h.ln_b2)), 1.f - lr * h.wd,
+                        h.grad_scale != nullptr ? *h.grad_scale : 1.f};
 
-    while (has(at)) {
-        const int valid = valid_at(t.n, at);
-        Tile<T, BITS> next;
-        if (has(at + AW_TILE)) next.load(t, at + AW_TILE, valid_at(t.n, at + AW_TILE));
-        uint64_t p[4], g[4], m[4], v[4];
-        tile.p.pairs(p);
-        tile.g.pairs(g);
-        if constexpr (BITS == 32) {
-            tile.m.pairs(m);
-            tile.v.pairs(v);
-        } else {
-            decode<true>(tile.m, tile.sm, m);
-            decode<false>(tile.v, tile.sv, v);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            // Products and sums are scalar here, each rounded by itself: a mul.rn.f32x2 and the add behind it come out as one fused
-            // multiply-add, whose sum rounds once, and codes would differ from their definition.
-            float g0, g1, m0, m1, v0, v1;
-            unpack2(mul2(g[i], twice(gs)), g0, g1);
-            unpack2(m[i], m0, m1);
-            unpack2(v[i], v0, v1);
-            m0 = __fadd_rn(__fmul_rn(m0, h.b1), __fmul_rn(g0, h.c1));
-            m1 = __fadd_rn(__fmul_rn(m1, h.b1), __fmul_rn(g1, h.c1));
-            v0 = __fadd_rn(__fmul_rn(v0, h.b2), __fmul_rn(__fmul_rn(g0, g0), h.c2));
-            v1 = __fadd_rn(__fmul_rn(v1, h.b2), __fmul_rn(__fmul_rn(g1, g1), h.c2));
-            m[i] = pack2(m0, m1);
-            v[i] = pack2(v0, v1);
-            const float u0 = __fdividef(m0, fmaf(root_of(v0), root, h.eps)), u1 = __fdividef(m1, fmaf(root_of(v1), root, h.eps));
-            p[i] = fma2(pack2(u0, u1), twice(-size), mul2(p[i], twice(keep)));
-        }
-        store8(static_cast<T*>(t.param) + at, valid, p);
-        if constexpr (BITS == 32) {
-            store8(static_cast<float*>(t.exp_avg) + at, valid, m);
-            store8(static_cast<float*>(t.exp_avg_sq) + at, valid, v);
-        } else {
-            store_block<true>(static_cast<unsigned char*>(t.exp_avg) + at, t.exp_avg_scale + at / AW_BLOCK, valid, m);
-            store_block<false>(static_cast<unsigned char*>(t.exp_avg_sq) + at, t.exp_avg_sq_scale + at / AW_BLOCK, valid, v);
-        }
-        tile = next;
-        at += AW_TILE;
+    Tile<T, BITS> tile;
+    for (int i = 0; i < whole; ++i) {
+        __syncwarp();      // all lanes have read the stage that is filled now
+        if (i + R::STAGES - 1 < whole) R::fill(ring + (i + R::STAGES - 1) % R::STAGES * R::STAGE, warp, R::STAGES - 1, lane);
+        cp_async_commit();
+        cp_async_wait<R::STAGES - 1>();
+        __syncwarp();      // and all have waited for their copies
+        tile.read(ring + i % R::STAGES * R::STAGE, lane);
+        update<T, BITS, true>(at, tile, 8, h, n);
+        at.advance();
+        warp.advance();
+    }
+    for (long long e = start + (long long)whole * AW_TILE + threadIdx.x * 8; (e & ~(long long)(AW_BLOCK - 1)) < end; e += AW_TILE) {      // whole warps
+        const int valid = valid_at(t.n, e);
+        tile.load(at, valid);
+        update<T, BITS, false>(at, tile, valid, h, n);
+        at.advance();
     }
     // Every thread of every chunk has read the step count when the last chunk arrives: that one counts it up.
     __syncthreads();
@@ -277,24 +378,35 @@ template <bool SIGNED>
 __global__ void __launch_bounds__(AW_THREADS) adamw_values_kernel(const unsigned char* codes, const float* scales, float* values, long long n) {
     constexpr int TILES = 4;
     const long long first = (long long)blockIdx.x * TILES * AW_TILE + threadIdx.x * 8;
+    const bool whole = aligned_to(codes, 8) && aligned_to(values, 32);
     uint2 c[TILES];
     float sc[TILES];
 #pragma unroll
     for (int i = 0; i < TILES; ++i) {
         const long long at = first + i * AW_TILE;
-        if (at < n) {
-            c[i] = load_codes(codes + at, valid_at(n, at));
-            sc[i] = scales[at / AW_BLOCK];
-        }
+        if (at >= n) continue;
+        const int valid = valid_at(n, at);
+        c[i] = whole && valid == 8 ? load_codes<true>(codes + at, 8) : load_codes<false>(codes + at, valid);
+        sc[i] = scales[at / AW_BLOCK];
     }
 #pragma unroll
     for (int i = 0; i < TILES; ++i) {
         const long long at = first + i * AW_TILE;
         if (at >= n) break;
+        const int valid = valid_at(n, at);
         uint64_t x[4];
         decode<SIGNED>(c[i], sc[i], x);
-        store8(values + at, valid_at(n, at), x);
+        if (whole && valid == 8) store8<true>(values + at, 8, x);
+        else store8<false>(values + at, valid, x);
     }
+}
+
+template <class T, int BITS, int CAP> int launch_kernel(const Table<CAP>& table, const Hyper& h, unsigned chunks, cudaStream_t s) {
+    const auto kernel = adamw_kernel<T, BITS, CAP>;
+    const int st = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), Ring<T, BITS>::BYTES);
+    if (st != ADDER_OK) return st;
+    kernel<<<chunks, AW_THREADS, Ring<T, BITS>::BYTES, s>>>(table, h);
+    return launched();
 }
 
 // Launches over as many tensors from `tensors` on as a table takes; *next is the first that is left.
@@ -316,9 +428,7 @@ template <class T, int CAP> int launch_some(const Tensor* tensors, int count, in
     *next = i;
     if (table.count == 0) return ADDER_OK;
     table.first[table.count] = (int)chunks;
-    if (bits == 32) adamw_kernel<T, 32, CAP><<<(unsigned)chunks, AW_THREADS, 0, s>>>(table, h);
-    else adamw_kernel<T, 8, CAP><<<(unsigned)chunks, AW_THREADS, 0, s>>>(table, h);
-    return launched();
+    return bits == 32 ? launch_kernel<T, 32, CAP>(table, h, (unsigned)chunks, s) : launch_kernel<T, 8, CAP>(table, h, (unsigned)chunks, s);
 }
 
 }  // namespace
