@@ -292,16 +292,18 @@ __device__ __forceinline__ void update(const Place<T, BITS>& at, const Tile<T, B
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        // Products and sums are scalar here, each rounded by itself: a mul.rn.f32x2 and the add behind it come out as one fused
+        // Sums are scalar here, and each operation rounds by itself: a mul.rn.f32x2 and an add.rn.f32x2 behind it come out as one fused
         // multiply-add, whose sum rounds once, and codes would differ from their definition.
-        float g0, g1, m0, m1, v0, v1, d0, d1;
-        unpack2(mul2(g[i], twice(n.scale)), g0, g1);
-        unpack2(m[i], m0, m1);
-        unpack2(v[i], v0, v1);
-        m0 = __fadd_rn(__fmul_rn(m0, h.b1), __fmul_rn(g0, h.c1));
-        m1 = __fadd_rn(__fmul_rn(m1, h.b1), __fmul_rn(g1, h.c1));
-        v0 = __fadd_rn(__fmul_rn(v0, h.b2), __fmul_rn(__fmul_rn(g0, g0), h.c2));
-        v1 = __fadd_rn(__fmul_rn(v1, h.b2), __fmul_rn(__fmul_rn(g1, g1), h.c2));
+        float m0, m1, v0, v1, a0, a1, d0, d1;
+        g[i] = mul2(g[i], twice(n.scale));
+        unpack2(mul2(m[i], twice(h.b1)), m0, m1);
+        unpack2(mul2(g[i], twice(h.c1)), a0, a1);
+        m0 = __fadd_rn(m0, a0);
+        m1 = __fadd_rn(m1, a1);
+        unpack2(mul2(v[i], twice(h.b2)), v0, v1);
+        unpack2(mul2(mul2(g[i], g[i]), twice(h.c2)), a0, a1);
+        v0 = __fadd_rn(v0, a0);
+        v1 = __fadd_rn(v1, a1);
         m[i] = pack2(m0, m1);
         v[i] = pack2(v0, v1);
         unpack2(fma2(pack2(root_of(v0), root_of(v1)), twice(n.root), twice(h.eps)), d0, d1);
