@@ -6,6 +6,7 @@
 // is a layer) and returns None for anything else, errors included: the caller then goes through the Python layer, which handles or rejects it.
 #include <torch/extension.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/forward_grad.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <ATen/cuda/CUDAContext.h>
@@ -821,7 +822,7 @@ class Addresses {
 public:
     explicit Addresses(size_t n) {
         size_t size = 64;
-        while (size < 4 * n) size *= 2;
+        while (size < 2 * n) size *= 2;
         slots_.assign(size, 0);
     }
     bool add(const void* p) { return probe((uintptr_t)p, true); }
@@ -829,7 +830,7 @@ public:
 
 private:
     bool probe(uintptr_t p, bool insert) {      // false: it was there
-        for (size_t i = (p >> 4) * 0x9E3779B97F4A7C15ull >> 20;; ++i) {
+        for (size_t i = (p >> 3) * 0x9E3779B97F4A7C15ull >> 32;; ++i) {
             uintptr_t& slot = slots_[i & (slots_.size() - 1)];
             if (slot == p) return false;
             if (slot == 0) {
@@ -872,7 +873,9 @@ PyObject* py_adamw(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     HANDLE_TH_ERRORS
     if (nargs != 13 || !available() || (!PyList_CheckExact(args[0]) && !PyTuple_CheckExact(args[0]))) Py_RETURN_NONE;
     const size_t n = PySequence_Fast_GET_SIZE(args[0]);
-    std::vector<const at::Tensor*> p, g, m, v, ms, vs, steps;
+    // kept from call to call for their memory alone
+    static thread_local std::vector<const at::Tensor*> p, g, m, v, ms, vs, steps;
+    static thread_local std::vector<adder_b200_adamw_tensor> tensors;
     const bool eight = args[10] != Py_None;
     if (n == 0 || !tensor_list(args[0], n, &p) || !tensor_list(args[1], n, &g) || !tensor_list(args[2], n, &m) || !tensor_list(args[3], n, &v)) Py_RETURN_NONE;
     if (eight != (args[11] != Py_None) || (eight && (!tensor_list(args[10], n, &ms) || !tensor_list(args[11], n, &vs)))) Py_RETURN_NONE;
@@ -890,15 +893,22 @@ PyObject* py_adamw(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
         double ignored;
         if (tensor_arg(args[12]) == nullptr || !scalar_arg(args[12], dev, &ignored, &scale_device)) Py_RETURN_NONE;
     }
-    const auto fits = [&](const at::Tensor& t, at::ScalarType type, const at::Tensor& like) {
-        return unwrapped(t) && t.scalar_type() == type && t.device() == dev && t.is_contiguous() && t.sizes() == like.sizes();
+    // Tensors of one kind have one set of dispatch keys, so what the first parameter is is asked once; and without a level of forward-mode
+    // differentiation no tensor has a tangent (asking each view for its own took as long as all the rest).
+    if (!unwrapped(*p[0])) Py_RETURN_NONE;
+    const c10::DispatchKeySet keys = p[0]->key_set();
+    const bool no_tangents = torch::autograd::ForwardADLevel::try_get_by_idx(0) == nullptr;
+    const auto ordinary = [&](const at::Tensor& t, at::ScalarType type) {
+        if (!t.defined()) return false;
+        const c10::TensorImpl* impl = t.unsafeGetTensorImpl();
+        return impl->key_set() == keys && (no_tangents || !t._fw_grad(0).defined()) && impl->dtype() == c10::scalarTypeToTypeMeta(type) &&
+               impl->device() == dev && impl->is_contiguous();
     };
-    const auto counts = [&](const at::Tensor& t, at::ScalarType type, int64_t count) {
-        return unwrapped(t) && t.scalar_type() == type && t.device() == dev && t.is_contiguous() && t.numel() == count;
-    };
+    const auto fits = [&](const at::Tensor& t, at::ScalarType type, const at::Tensor& like) { return ordinary(t, type) && t.sizes() == like.sizes(); };
+    const auto counts = [&](const at::Tensor& t, at::ScalarType type, int64_t count) { return ordinary(t, type) && t.numel() == count; };
     if (all_steps != nullptr && (!counts(*all_steps, at::kInt, 2 * (int64_t)n) || all_steps->dim() != 2 || all_steps->size(0) != (int64_t)n)) Py_RETURN_NONE;
     Addresses written(6 * n);
-    std::vector<adder_b200_adamw_tensor> tensors(n);
+    tensors.resize(n);
     for (size_t i = 0; i < n; ++i) {
         const at::Tensor& q = *p[i];
         if (!fits(q, scalar, q) || !fits(*g[i], scalar, q) || !fits(*m[i], state, q) || !fits(*v[i], state, q)) Py_RETURN_NONE;
