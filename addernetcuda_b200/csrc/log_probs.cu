@@ -88,10 +88,13 @@ struct LpFwd {
 // Shared memory of the warp that finishes a row.
 template <class T, int STREAM, bool TOP> struct LpFinish {
     static constexpr int VECTORS = STREAM == 32 ? 1 : 4;               // of a lane, that are looked at together
-    static constexpr int BATCH = VECTORS * 32 * Vec16<T>::N;           // values in them
-    static constexpr int LIST = TOP ? BATCH + 64 : 1;
-    uint64_t list[LIST];                   // candidates
+    static constexpr int LIST = 96, HOT = VECTORS * 32;
+    uint64_t list[TOP ? LIST : 1];         // candidates
+    uint64_t sorted[TOP ? 32 : 1];
+    uint4 hot[TOP ? HOT : 1];              // vectors that hold some
+    int hot_at[TOP ? HOT : 1];
     int first[TOP ? STREAM : 1];           // vectors where the share of a thread begins that may hold some
+    uint64_t bound;
     int count;
 };
 // A thread's largest value and the vector that it is in, and the largest of the groups of vectors that it is not in.
@@ -356,14 +359,8 @@ __device__ __forceinline__ uint64_t kth_largest(uint64_t key, int k) {
     }
 }
 
-// The rest of a row (or of its cluster rank's part), by one warp: joins the sums, adds the single elements, finds the k largest.
-// `best(i)` is what thread 32 i + lane has found.  The best values of 32 disjoint parts of the row, one a lane, are sorted; the k-th
-// of them bounds the k-th largest of all from below, so all candidates lie with the threads that reach it: in the group of vectors that
-// holds their best, and elsewhere in their share only where their second group reaches it, too.  `fetch(v)` reads a vector again.
-template <class T, int STREAM, bool ENTROPY, bool TOP, class GetBest, class Fetch>
-__device__ __forceinline__ void finish_part(const LpRow<T>& r, int k, float one, int lane, LpFinish<T, STREAM, TOP>& sh, GetBest&& best, Fetch&& fetch,
-                                            float& m, float& s, float& t, uint64_t& top) {
-    constexpr int VE = Vec16<T>::N;
+// The sums of a row (or of its cluster rank's part) in every lane of one warp, the single elements with them.
+template <class T, bool ENTROPY> __device__ __forceinline__ void finish_sums(const LpRow<T>& r, float one, int lane, float& m, float& s, float& t) {
     if (r.singles > 0) {
         Running<ENTROPY> run;
         if (lane < r.singles) {
@@ -376,102 +373,148 @@ __device__ __forceinline__ void finish_part(const LpRow<T>& r, int k, float one,
         join(m, s, t, run.m, s2, t2);
     }
     join_lanes<ENTROPY>(m, s, t, 32);
-    top = 0;
-    if constexpr (TOP) {
-        using Finish = LpFinish<T, STREAM, TOP>;
-        // a bound of the thread's largest key from below (above, with `up`): the best value is somewhere in its vector
-        const auto bound_of = [&](const Best& f, int thread, bool up) {
-            return r.v0 + thread < r.v1 ? key_of(f.value, (uint32_t)(r.head + f.vec * VE + (up ? 0 : VE - 1))) : 0;
-        };
-        uint64_t low = 0;
+}
+
+// A bound of a thread's largest key from below (above, with `up`): its best value is somewhere in its vector.
+template <class T> __device__ __forceinline__ uint64_t bound_of(const LpRow<T>& r, const Best& f, int thread, bool up) {
+    return r.v0 + thread < r.v1 ? key_of(f.value, (uint32_t)(r.head + f.vec * Vec16<T>::N + (up ? 0 : Vec16<T>::N - 1))) : 0;
+}
+
+// A key that at least k elements reach, by one warp: the k-th largest best of 32 disjoint sets of threads, one a lane, or, for more than 8, of
+// 64 (by sorting, and with some 1.3 k candidates where 32 sets give up to 4 k).  best(i): of thread 32 i + lane.
+template <class T, int STREAM, class GetBest> __device__ __forceinline__ uint64_t find_bound(const LpRow<T>& r, int k, int lane, GetBest&& best) {
+    constexpr int N = STREAM / 32;
+    uint64_t low[2] = {0, 0};
 #pragma unroll
-        for (int i = 0; i < STREAM / 32; ++i) low = bigger(low, bound_of(best(i), 32 * i + lane, false));
-        const uint64_t bound = kth_largest(low, k);
+    for (int i = 0; i < N; ++i) low[i < (N + 1) / 2 ? 0 : 1] = bigger(low[i < (N + 1) / 2 ? 0 : 1], bound_of(r, best(i), 32 * i + lane, false));
+    if (N == 1) return kth_largest(low[0], k);
+    if (k <= 8) return kth_largest(bigger(low[0], low[1]), k);
+    const uint64_t a = sort_warp(low[0], lane), b = sort_warp(low[1], lane);
+    return __shfl_sync(0xffffffffu, merge_down(bigger(a, __shfl_sync(0xffffffffu, b, 31 - lane)), lane, 32), k - 1);
+}
+
+// Candidates of one warp, which keeps their number n in every lane.
+template <class Finish> struct Candidates {
+    Finish& sh;
+    int lane, n = 0;
+    bool merged = false;
+    uint64_t top = 0;      // where there were many: the 32 largest of those taken off the list, sorted
+
+    __device__ __forceinline__ void offer(bool in, uint64_t key) {
+        const unsigned who = __ballot_sync(0xffffffffu, in);
+        if (who == 0) return;
+        if (in) sh.list[n + __popc(who & ((1u << lane) - 1))] = key;
+        n += __popc(who);
+        if (n > Finish::LIST - 32) merge();
+    }
+    __device__ __forceinline__ void merge() {
         __syncwarp();
-        int one_group = 0, whole = 0;      // threads of which a group of vectors, or all, are looked at
-#pragma unroll
-        for (int i = 0; i < STREAM / 32; ++i) {
-            const Best f = best(i);
-            const int thread = 32 * i + lane;
-            const uint64_t high = bound_of(f, thread, true);
-            const bool in = high != 0 && high >= bound, all = in && key_of(f.second, 0) >= bound;
-            const unsigned some = __ballot_sync(0xffffffffu, in && !all), every = __ballot_sync(0xffffffffu, all), before = (1u << lane) - 1;
-            const int group = (f.vec - r.v0 - thread) / (LP_GROUP * STREAM);
-            if (in && !all) sh.first[one_group + __popc(some & before)] = r.v0 + thread + group * LP_GROUP * STREAM;
-            if (all) sh.first[STREAM - 1 - whole - __popc(every & before)] = r.v0 + thread;
-            one_group += __popc(some);
-            whole += __popc(every);
+        for (int at = 0; at < n; at += 32) {
+            const uint64_t batch = sort_warp(at + lane < n ? sh.list[at + lane] : 0, lane);
+            const uint64_t other = __shfl_sync(0xffffffffu, top, 31 - lane);
+            top = merged ? merge_down(bigger(batch, other), lane, 32) : batch;
+            merged = true;
         }
-        if (lane == 0) sh.count = 0;
+        n = 0;
         __syncwarp();
-        const auto offer = [&](float v, uint32_t index) {
-            const uint64_t key = key_of(v, index);
-            if (key >= bound) sh.list[atomicAdd(&sh.count, 1)] = key;
-        };
-        if (lane < r.singles) offer(one, (uint32_t)r.single(lane));
-        bool merged = false;
-        const auto merge = [&](int n) {
-            for (int at = 0; at < n; at += 32) {
-                const uint64_t batch = sort_warp(at + lane < n ? sh.list[at + lane] : 0, lane);
-                const uint64_t other = __shfl_sync(0xffffffffu, top, 31 - lane);
-                top = merged ? merge_down(bigger(batch, other), lane, 32) : batch;
-                merged = true;
-            }
-        };
-        const int per = (r.v1 - r.v0 + STREAM - 1) / STREAM;      // vectors of a thread, the last perhaps not there
-        const int items = one_group * LP_GROUP + whole * per;
-        for (int base = 0; base < items; base += Finish::VECTORS * 32) {
-            uint4 p[Finish::VECTORS];
-            int at[Finish::VECTORS];
-#pragma unroll
-            for (int u = 0; u < Finish::VECTORS; ++u) {
-                int item = base + 32 * u + lane;
-                at[u] = r.v1;
-                if (item < one_group * LP_GROUP) {
-                    at[u] = sh.first[item / LP_GROUP] + item % LP_GROUP * STREAM;
-                } else if (item < items) {
-                    item -= one_group * LP_GROUP;
-                    const int w = item / per;
-                    at[u] = sh.first[STREAM - 1 - w] + (item - w * per) * STREAM;
-                }
-                if (at[u] < r.v1) p[u] = fetch(at[u]);
-            }
-#pragma unroll
-            for (int u = 0; u < Finish::VECTORS; ++u) {
-                if (at[u] >= r.v1) continue;
-                const uint32_t largest = max_word<T>(max_word<T>(p[u].x, p[u].y), max_word<T>(p[u].z, p[u].w));
-                if (key_of(word_max<T>(largest), 0) < bound) continue;
-                float g[VE];
-                Vec16<T>::unpack(p[u], g);
-#pragma unroll
-                for (int i = 0; i < VE; ++i) offer(g[i], (uint32_t)(r.head + at[u] * VE + i));
-            }
-            __syncwarp();
-            const int n = sh.count;
-            if (n > Finish::LIST - Finish::BATCH) {      // no room for another batch
-                merge(n);
-                __syncwarp();
-                if (lane == 0) sh.count = 0;
-            }
-            __syncwarp();
+    }
+    // The largest, sorted, one a lane.  Up to 64 candidates each count those above them.
+    __device__ __forceinline__ uint64_t finish() {
+        if (merged) {
+            merge();
+            return top;
         }
         __syncwarp();
-        const int n = sh.count;
-        if (merged || n > 32) {
-            merge(n);
-        } else {      // the usual case: each of a few candidates counts those above it
-            const uint64_t key = lane < n ? sh.list[lane] : 0;
-            int above = 0;
-            for (int i = 0; i < n; ++i) above += __shfl_sync(0xffffffffu, key, i) > key;
-            __syncwarp();
-            sh.list[lane] = 0;
-            __syncwarp();
-            if (lane < n) sh.list[above] = key;
-            __syncwarp();
-            top = sh.list[lane];
+        sh.sorted[lane] = 0;
+        const uint64_t key0 = lane < n ? sh.list[lane] : 0, key1 = lane + 32 < n ? sh.list[lane + 32] : 0;
+        int above0 = 0, above1 = 0;
+        if (n <= 32) {
+            for (int i = 0; i < n; ++i) above0 += sh.list[i] > key0;
+        } else {
+            for (int i = 0; i < n; ++i) {
+                const uint64_t other = sh.list[i];
+                above0 += other > key0;
+                above1 += other > key1;
+            }
+        }
+        __syncwarp();
+        if (lane < n && above0 < 32) sh.sorted[above0] = key0;
+        if (lane + 32 < n && above1 < 32) sh.sorted[above1] = key1;
+        __syncwarp();
+        return sh.sorted[lane];
+    }
+};
+
+// The k largest of a row, sorted, one a lane of one warp (at least k of the 32).  All candidates lie with the threads whose best reaches the bound:
+// in the group of vectors that holds it, and elsewhere in their share only where their second group reaches it, too.  `fetch(v)` reads a
+// vector again.
+template <class T, int STREAM, class GetBest, class Fetch>
+__device__ __forceinline__ uint64_t find_top(const LpRow<T>& r, uint64_t bound, float one, int lane, LpFinish<T, STREAM, true>& sh, GetBest&& best, Fetch&& fetch) {
+    using Finish = LpFinish<T, STREAM, true>;
+    constexpr int VE = Vec16<T>::N;
+    Candidates<Finish> found{sh, lane};
+    int one_group = 0, whole = 0;      // threads of which a group of vectors, or all, are looked at
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < STREAM / 32; ++i) {
+        const Best f = best(i);
+        const int thread = 32 * i + lane;
+        const uint64_t high = bound_of(r, f, thread, true);
+        const bool in = high != 0 && high >= bound, all = in && key_of(f.second, 0) >= bound;
+        const unsigned some = __ballot_sync(0xffffffffu, in && !all), every = __ballot_sync(0xffffffffu, all), before = (1u << lane) - 1;
+        const int group = (f.vec - r.v0 - thread) / (LP_GROUP * STREAM);
+        if (in && !all) sh.first[one_group + __popc(some & before)] = r.v0 + thread + group * LP_GROUP * STREAM;
+        if (all) sh.first[STREAM - 1 - whole - __popc(every & before)] = r.v0 + thread;
+        one_group += __popc(some);
+        whole += __popc(every);
+    }
+    __syncwarp();
+    if (r.singles > 0) {
+        const uint64_t key = lane < r.singles ? key_of(one, (uint32_t)r.single(lane)) : 0;
+        found.offer(key != 0 && key >= bound, key);
+    }
+    const int per = (r.v1 - r.v0 + STREAM - 1) / STREAM;      // vectors of a thread, the last perhaps not there
+    const int items = one_group * LP_GROUP + whole * per;
+    for (int base = 0; base < items; base += Finish::HOT) {
+        uint4 p[Finish::VECTORS];
+        int at[Finish::VECTORS];
+#pragma unroll
+        for (int u = 0; u < Finish::VECTORS; ++u) {
+            int item = base + 32 * u + lane;
+            at[u] = r.v1;
+            if (item < one_group * LP_GROUP) {
+                at[u] = sh.first[item / LP_GROUP] + item % LP_GROUP * STREAM;
+            } else if (item < items) {
+                item -= one_group * LP_GROUP;
+                const int w = item / per;
+                at[u] = sh.first[STREAM - 1 - w] + (item - w * per) * STREAM;
+            }
+            if (at[u] < r.v1) p[u] = fetch(at[u]);
+        }
+        int hot = 0;      // vectors that hold a candidate; the elements of those are then looked at one a lane
+#pragma unroll
+        for (int u = 0; u < Finish::VECTORS; ++u) {
+            bool in = false;
+            if (at[u] < r.v1)
+                in = key_of(word_max<T>(max_word<T>(max_word<T>(p[u].x, p[u].y), max_word<T>(p[u].z, p[u].w))), 0) >= bound;
+            const unsigned who = __ballot_sync(0xffffffffu, in);
+            if (in) {
+                const int slot = hot + __popc(who & ((1u << lane) - 1));
+                sh.hot[slot] = p[u];
+                sh.hot_at[slot] = r.head + at[u] * VE;
+            }
+            hot += __popc(who);
+        }
+        __syncwarp();
+        for (int e = 0; e < hot * VE; e += 32) {
+            const int i = (e + lane) / VE, j = (e + lane) % VE;
+            uint64_t key = 0;
+            if (i < hot) key = key_of(to_float(reinterpret_cast<const T*>(&sh.hot[i])[j]), (uint32_t)(sh.hot_at[i] + j));
+            found.offer(key != 0 && key >= bound, key);
         }
         __syncwarp();
     }
+    return found.finish();
 }
 
 // The outputs of a row, by one warp whose lanes all have its sums.
@@ -526,8 +569,10 @@ __global__ void __launch_bounds__(THREADS == 32 ? 128 : LP_TEAM + 32, THREADS ==
 
     if constexpr (THREADS > 32) if (finisher) {
         __syncwarp();
-        bar_arrive<LP_EMPTY>(0);
-        if (row + step < a.rows) bar_arrive<LP_EMPTY>(1);
+        if (!CLUSTER) {      // where there is one row, nobody waits for these
+            bar_arrive<LP_EMPTY>(0);
+            if (row + step < a.rows) bar_arrive<LP_EMPTY>(1);
+        }
         int buffer = 0;
         long long target_next = a.log_prob != nullptr ? a.targets[row] : 0;
         for (; row < a.rows; row += step) {
@@ -542,11 +587,31 @@ __global__ void __launch_bounds__(THREADS == 32 ? 128 : LP_TEAM + 32, THREADS ==
             const LpHand& in = hand[buffer];
             const bool some = lane < LP_TEAM / 32;
             float m = some ? in.m[lane] : -INFINITY, s = some ? in.s[lane] : 0.f, tt = some ? in.t[lane] : 0.f;
-            uint64_t top;
-            // A short part of a row is in shared memory as a whole.
-            const bool here = CLUSTER && r.groups(THREADS) <= LP_STAGES;
-            finish_part<T, THREADS, ENTROPY, TOP>(r, a.k, one, lane, sh, [&](int i) { return in.best[32 * i + lane]; },
-                                                  [&](int v) { return here ? ring[v - r.v0] : __ldg(r.vec + v); }, m, s, tt, top);
+            finish_sums<T, ENTROPY>(r, one, lane, m, s, tt);
+            uint64_t top = 0;
+            if constexpr (TOP) {
+                const auto best = [&](int i) { return in.best[32 * i + lane]; };
+                const auto fetch = [&](int v) { return __ldg(r.vec + v); };
+                const uint64_t bound = find_bound<T, THREADS>(r, a.k, lane, best);
+                if constexpr (CLUSTER) {      // few rows: the streaming threads have nothing else to do than to look through their own vectors
+                    if (lane == 0) { sh.bound = bound; sh.count = 0; }
+                    __syncwarp();
+                    bar_sync<LP_EMPTY>(0);
+                    bar_sync<LP_EMPTY>(1);
+                    Candidates<LpFinish<T, THREADS, TOP>> found{sh, lane, sh.count};
+                    if (found.n <= LpFinish<T, THREADS, TOP>::LIST - 32) {
+                        if (r.singles > 0) {
+                            const uint64_t key = lane < r.singles ? key_of(one, (uint32_t)r.single(lane)) : 0;
+                            found.offer(key != 0 && key >= bound, key);
+                        }
+                        top = found.finish();
+                    } else {
+                        top = find_top<T, THREADS>(r, bound, one, lane, sh, best, fetch);
+                    }
+                } else {
+                    top = find_top<T, THREADS>(r, bound, one, lane, sh, best, fetch);
+                }
+            }
             __syncwarp();
             if (row + 2 * step < a.rows) bar_arrive<LP_EMPTY>(buffer);
             buffer ^= 1;
@@ -561,8 +626,17 @@ __global__ void __launch_bounds__(THREADS == 32 ? 128 : LP_TEAM + 32, THREADS ==
                 const bool there = lane < parts;
                 m = there ? joined[0].m[lane] : -INFINITY; s = there ? joined[0].s[lane] : 0.f; tt = there ? joined[0].t[lane] : 0.f;
                 join_lanes<ENTROPY>(m, s, tt, 32);
-                if (TOP)
-                    for (int i = 1; i < parts; ++i) top = merge_down(bigger(top, joined[0].top[i][31 - lane]), lane, 32);
+                if constexpr (TOP) {      // by halves: the merges of a round do not depend on one another
+                    uint64_t part[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) part[i] = i < parts ? joined[0].top[i][lane] : 0;
+#pragma unroll
+                    for (int half = 4; half > 0; half >>= 1)
+#pragma unroll
+                        for (int i = 0; i < half; ++i)
+                            part[i] = merge_down(bigger(part[i], __shfl_sync(0xffffffffu, part[i + half], 31 - lane)), lane, 32);
+                    top = part[0];
+                }
             }
             write_row<ENTROPY, TOP>(a, row, lane, m, s, tt, top, target, at_target);
         }
@@ -614,19 +688,48 @@ __global__ void __launch_bounds__(THREADS == 32 ? 128 : LP_TEAM + 32, THREADS ==
         float m = run.m, s, tt;
         run.finish(&s, &tt);
         if constexpr (THREADS == 32) {
-            uint64_t top;
-            finish_part<T, 32, ENTROPY, TOP>(r, a.k, one, lane, sh, [&](int) { return best; }, [&](int v) { return __ldg(r.vec + v); }, m, s, tt, top);
+            uint64_t top = 0;
+            finish_sums<T, ENTROPY>(r, one, lane, m, s, tt);
+            if constexpr (TOP) {
+                const auto mine = [&](int) { return best; };
+                top = find_top<T, 32>(r, find_bound<T, 32>(r, a.k, lane, mine), one, lane, sh, mine, [&](int v) { return __ldg(r.vec + v); });
+            }
             write_row<ENTROPY, TOP>(a, row, lane, m, s, tt, top, target, at_target);
         } else {
             join_lanes<ENTROPY>(m, s, tt, 32);
             __syncwarp();
-            bar_sync<LP_EMPTY>(buffer);
+            if (!CLUSTER) bar_sync<LP_EMPTY>(buffer);
             LpHand& out = hand[buffer];
             if (lane == 0) { out.m[warp] = m; out.s[warp] = s; out.t[warp] = tt; }
             if (TOP) out.best[t] = best;
             __syncwarp();
             bar_arrive<LP_FULL>(buffer);
             buffer ^= 1;
+            if constexpr (CLUSTER && TOP) {      // candidates of this thread, as long as the list has room for all
+                bar_sync<LP_EMPTY>(0);
+                const uint64_t bound = sh.bound, high = bound_of(r, best, t, true);
+                if (high != 0 && high >= bound) {
+                    const bool all = key_of(best.second, 0) >= bound;
+                    const int begin = all ? r.v0 + t : r.v0 + t + (best.vec - r.v0 - t) / (LP_GROUP * THREADS) * LP_GROUP * THREADS;
+                    const int end = all ? r.v1 : min(r.v1, begin + LP_GROUP * THREADS);
+                    const bool here = r.groups(THREADS) <= LP_STAGES;      // a short part is still in shared memory as a whole
+                    for (int v = begin; v < end; v += THREADS) {
+                        const uint4 p = here ? ring[v - r.v0] : __ldg(r.vec + v);
+                        if (key_of(word_max<T>(max_word<T>(max_word<T>(p.x, p.y), max_word<T>(p.z, p.w))), 0) < bound) continue;
+                        float g[Vec16<T>::N];
+                        Vec16<T>::unpack(p, g);
+#pragma unroll
+                        for (int i = 0; i < Vec16<T>::N; ++i) {
+                            const uint64_t key = key_of(g[i], (uint32_t)(r.head + v * Vec16<T>::N + i));
+                            if (key < bound) continue;
+                            const int slot = atomicAdd(&sh.count, 1);
+                            if (slot < LpFinish<T, THREADS, TOP>::LIST) sh.list[slot] = key;
+                        }
+                    }
+                }
+                __syncwarp();
+                bar_arrive<LP_EMPTY>(1);
+            }
         }
     }
     if constexpr (CLUSTER) {
