@@ -91,16 +91,15 @@ __device__ __forceinline__ uint64_t sub2(uint64_t a, uint64_t b) {
     asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
 __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
     uint64_t r;
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
     return r;
 }
+
+// A product, as a fused multiply-add of 0: mul.rn.f32x2 takes two instructions (the gradient of 4096x32000 fp32 logits with an entropy
+// 188 us, 171 this way).  A product of -0 becomes 0.
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) { return fma2(a, b, 0ull); }
 
 // What a forward kernel does with an output before it stores it: nothing (scale == nullptr), or the evaluation-mode batch norm
 // behind the layer, relu?(y * scale[c] + shift[c] + residual).  The same operations in the same order as a pass of their own

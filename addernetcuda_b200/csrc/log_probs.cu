@@ -772,12 +772,14 @@ template <bool ENTROPY> struct Slope {
         scale = -exp2f(-res) / s * (ENTROPY ? 1.f : sum);
         shift = ENTROPY ? h - logf(s) - res * LN2 : 0.f;
     }
-    // `far`: M is subtracted first
-    __device__ __forceinline__ uint64_t pair(float a, float b, bool far) const {
+    // Values below this count as this with an entropy: their exponential is 0 either way (as in Running).
+    __device__ __forceinline__ float floor_value(float m) const { return m - 150.f - fabsf(m) * 0.015625f; }
+    // `far`: M is subtracted first.  `floored`: the values have been held to floor_value.
+    __device__ __forceinline__ uint64_t pair(float a, float b, bool far, bool floored) const {
         const uint64_t x = far ? add2(pack2(a, b), pack2(-minus, -minus)) : pack2(a, b);
         float d0, d1;
         unpack2(fma2(x, pack2(LOG2E, LOG2E), pack2(-ref, -ref)), d0, d1);
-        if (ENTROPY) { d0 = max_nan(d0, LP_FLOOR); d1 = max_nan(d1, LP_FLOOR); }
+        if (ENTROPY && !floored) { d0 = max_nan(d0, LP_FLOOR); d1 = max_nan(d1, LP_FLOOR); }
         const uint64_t e = mul2(pack2(exp2_fast(d0), exp2_fast(d1)), pack2(scale, scale));
         if (!ENTROPY) return e;
         // d log(2) + H - ln s is log p + H
@@ -787,7 +789,7 @@ template <bool ENTROPY> struct Slope {
     __device__ __forceinline__ float one(float v) const {
         if (nothing) return 0.f;
         float a, b;
-        unpack2(pair(v, v, minus != 0.f), a, b);
+        unpack2(pair(v, v, minus != 0.f, false), a, b);
         return a;
     }
 };
@@ -824,16 +826,26 @@ __global__ void __launch_bounds__(THREADS == 32 ? 128 : THREADS) lp_backward_ker
     if (a.g_top != nullptr)
         for (int j = 0; j < a.k; ++j) sum += a.g_top[row * a.k + j];
     Slope<ENTROPY> slope;
+    const float low = slope.floor_value(a.stats[2 * row]);
     slope.set(a.stats[2 * row], a.stats[2 * row + 1], sum, ENTROPY ? a.g_entropy[row] : 0.f, ENTROPY ? a.entropy[row] : 0.f);
 
     int begin, end;      // elements of this segment
     if (same) {
         uint4* out = reinterpret_cast<uint4*>(dx + head);
-        const auto put = [&](const uint4& in, int v, bool far) {
+        uint32_t low_word = 0;
+        if constexpr (sizeof(T) == 2) low_word = pack_pair<T>(low, low);
+        const auto put = [&](uint4 in, int v, bool far) {
+            constexpr bool words = ENTROPY && sizeof(T) == 2;      // two values at once
+            if constexpr (words) {
+                if (!far) {
+                    in.x = max_pair<T>(in.x, low_word); in.y = max_pair<T>(in.y, low_word);
+                    in.z = max_pair<T>(in.z, low_word); in.w = max_pair<T>(in.w, low_word);
+                }
+            }
             float f[VE];
             Vec16<T>::unpack(in, f);
 #pragma unroll
-            for (int i = 0; i < VE; i += 2) unpack2(slope.pair(f[i], f[i + 1], far), f[i], f[i + 1]);
+            for (int i = 0; i < VE; i += 2) unpack2(slope.pair(f[i], f[i + 1], far, words && !far), f[i], f[i + 1]);
             __stcs(out + v, Vec16<T>::pack(f));
         };
         for (int v = v0 + t; v < v1; v += THREADS * LP_UNROLL) {
@@ -907,6 +919,10 @@ template <class T, int THREADS, bool CLUSTER, bool ENTROPY, bool TOP> int launch
     }
 }
 
+// A warp a row: short rows, and longer ones where there are enough to fill the SMs (16384 x 4000 bf16: forward 33 us, by CTAs 94; backward see
+// below).
+bool warp_rows(long long rows, long long classes) { return classes <= 1024 || (classes <= 8192 && rows >= 24LL * sm_count()); }
+
 template <class T, int THREADS, bool CLUSTER> int choose_forward(const LpFwd& a, int parts, cudaStream_t s) {
     if (a.entropy != nullptr)
         return a.k > 0 ? launch_forward<T, THREADS, CLUSTER, true, true>(a, parts, s) : launch_forward<T, THREADS, CLUSTER, true, false>(a, parts, s);
@@ -933,7 +949,7 @@ int adder_b200_log_probs_forward(const void* logits, int dtype, long long rows, 
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     return with_type(dtype, [&](auto* type) {
         using T = std::remove_pointer_t<decltype(type)>;
-        if (classes <= 1024 || (classes <= 8192 && rows >= 24LL * sm_count())) return choose_forward<T, 32, false>(a, 1, s);
+        if (warp_rows(rows, classes)) return choose_forward<T, 32, false>(a, 1, s);
         // Few rows leave SMs idle: a row is then split over a cluster of up to 8 CTAs of at least 4096 elements.
         int parts = 1;
         while (parts < 8 && rows * parts * 2 <= sm_count() * 4 && classes >= 8192LL * parts) parts *= 2;
@@ -956,7 +972,7 @@ int adder_b200_log_probs_backward(const void* logits, int dtype, long long rows,
     const unsigned size = dtype == ADDER_TYPE_F32 ? 4 : 2;
     if (!aligned_to(logits, size) || !aligned_to(grad_logits, size)) return ADDER_ERR_ALIGNMENT;
     const long long tile = 256LL * LP_UNROLL * (16 / size);      // elements that a CTA takes at once
-    const bool warps = classes <= 1024;
+    const bool warps = warp_rows(rows, classes);
     const long long segments = warps ? 1 : (classes + tile - 1) / tile;
     const long long grid = warps ? (rows + 3) / 4 : rows * segments;
     if (grid > 2147483647LL) return ADDER_ERR_UNSUPPORTED;
