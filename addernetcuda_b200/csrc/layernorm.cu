@@ -110,8 +110,8 @@ template <class T_, class W_, int G_, int VEC_, int NV_, int STAGES_, bool CLUST
     static constexpr int G = G_, VEC = VEC_, NV = NV_, STAGES = STAGES_;
     static constexpr bool CLUSTER = CLUSTER_;
     static constexpr int THREADS = G > THREADS_ ? G : THREADS_, TEAMS = THREADS / G, WARPS = G / 32;
-    static constexpr int LINE = THREADS * 16;      // bytes of one vector of each thread
-    static size_t ring(int arrays) { return (size_t)STAGES * arrays * NV * LINE; }
+    static __host__ __device__ constexpr int line() { return THREADS * 16; }      // bytes of one vector of each thread
+    static size_t ring(int arrays) { return (size_t)STAGES * arrays * NV * line(); }
 };
 
 // A thread's values of a row are held as pairs of fp32, which one instruction adds or multiplies: P pairs of each vector, or, element by
@@ -128,7 +128,7 @@ template <class S> __device__ __forceinline__ void ln_issue(uint32_t slot, const
 #pragma unroll
     for (int i = 0; i < S::NV; ++i)
         if (v + i * S::G < v1)
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(slot + i * S::LINE), "l"(row + (size_t)(v + i * S::G) * S::VEC) : "memory");
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(slot + i * S::line()), "l"(row + (size_t)(v + i * S::G) * S::VEC) : "memory");
 }
 template <class S> __device__ __forceinline__ void ln_fetch(LnPairs<S>& f, uint32_t slot, const typename S::T* row, int v, int v1) {
     using T = typename S::T;
@@ -138,7 +138,7 @@ template <class S> __device__ __forceinline__ void ln_fetch(LnPairs<S>& f, uint3
         for (int i = 0; i < S::NV; ++i) {
             q[i] = make_uint4(0, 0, 0, 0);
             if (v + i * S::G < v1)
-                asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(q[i].x), "=r"(q[i].y), "=r"(q[i].z), "=r"(q[i].w) : "r"(slot + i * S::LINE) : "memory");
+                asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(q[i].x), "=r"(q[i].y), "=r"(q[i].z), "=r"(q[i].w) : "r"(slot + i * S::line()) : "memory");
         }
 #pragma unroll
         for (int i = 0; i < S::NV; ++i) {
@@ -192,10 +192,10 @@ template <class S> struct LnWalk {
         arrays = arrays_;
     }
     __device__ __forceinline__ uint32_t advance(uint32_t at) const {
-        const uint32_t stage = (uint32_t)arrays * S::NV * S::LINE, last = S::STAGES > 0 ? S::STAGES - 1 : 0;
+        const uint32_t stage = (uint32_t)arrays * S::NV * S::line(), last = S::STAGES > 0 ? S::STAGES - 1 : 0;
         return at == ring + last * stage ? ring : at + stage;
     }
-    static __device__ __forceinline__ uint32_t slot(uint32_t at, int array) { return at + array * S::NV * S::LINE; }
+    static __device__ __forceinline__ uint32_t slot(uint32_t at, int array) { return at + array * S::NV * S::line(); }
 };
 
 // Exchange of a row's sums between the warps of a team, and between the CTAs of a cluster.
@@ -574,6 +574,180 @@ template <class S, bool SUMS> __global__ void __launch_bounds__(S::THREADS, 1) l
     }
 }
 
+// ------------------------------------------------------------------------------------------ long rows, held in shared memory
+
+// One CTA an SM, which has a row and the next one in shared memory: with enough rows for all SMs nothing is exchanged between CTAs.  A
+// thread copies the vectors that it reads itself.
+constexpr int LN_WIDE = 1024;
+
+template <class T> __device__ __forceinline__ void wide_copy(uint4* to, const T* row, int nvec) {
+    const uint32_t base = smem_u32(to);
+    for (int v = threadIdx.x; v < nvec; v += LN_WIDE)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(base + 16 * v), "l"(row + (size_t)v * Vec16<T>::N) : "memory");
+}
+// Sums over the CTA; `part` alternates between two arrays.
+__device__ __forceinline__ float2 wide_sum2(float a, float b, float2* part) {
+    a = lanes_sum<32>(a);
+    b = lanes_sum<32>(b);
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = make_float2(a, b);
+    __syncthreads();
+    const float2 p = part[threadIdx.x & 31];
+    return make_float2(lanes_sum<32>(p.x), lanes_sum<32>(p.y));
+}
+template <class T> __device__ __forceinline__ void vector_pairs(const uint4& q, uint64_t (&f)[Vec16<T>::N / 2]) {
+    float e[Vec16<T>::N];
+    Vec16<T>::unpack(q, e);
+#pragma unroll
+    for (int i = 0; i < Vec16<T>::N / 2; ++i) f[i] = pack2(e[2 * i], e[2 * i + 1]);
+}
+template <class T> __device__ __forceinline__ uint4 pairs_vector(const uint64_t (&f)[Vec16<T>::N / 2]) {
+    float e[Vec16<T>::N];
+#pragma unroll
+    for (int i = 0; i < Vec16<T>::N / 2; ++i) unpack2(f[i], e[2 * i], e[2 * i + 1]);
+    return Vec16<T>::pack(e);
+}
+template <class W, int N> __device__ __forceinline__ void weight_pairs(const void* w, float missing, int v, uint64_t (&f)[N / 2]) {
+    float e[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) e[i] = missing;
+    if (w != nullptr) load_some<W, N>(static_cast<const W*>(w) + (size_t)v * N, e);
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) f[i] = pack2(e[2 * i], e[2 * i + 1]);
+}
+
+template <class T, class W> __global__ void __launch_bounds__(LN_WIDE) ln_forward_wide_kernel(const LnFwd a) {
+    extern __shared__ uint4 smem[];
+    __shared__ float2 part[2][LN_WIDE / 32];
+    constexpr int N = Vec16<T>::N, P = N / 2;
+    const int nvec = a.d / N, arrays = a.residual != nullptr ? 2 : 1;
+    const float inv_d = 1.f / a.d;
+    const auto issue = [&](long long row, uint4* to) {
+        if (row < a.rows) {
+            wide_copy<T>(to, static_cast<const T*>(a.x) + row * a.x_stride, nvec);
+            if (arrays == 2) wide_copy<T>(to + nvec, static_cast<const T*>(a.residual) + row * a.r_stride, nvec);
+        }
+        cp_async_commit();
+    };
+    long long row = blockIdx.x;
+    issue(row, smem);
+    for (int turn = 0; row < a.rows; row += gridDim.x, turn ^= 1) {
+        uint4* held = smem + turn * arrays * nvec;
+        issue(row + gridDim.x, smem + (turn ^ 1) * arrays * nvec);
+        cp_async_wait<1>();
+        uint64_t sum = 0;
+        for (int v = threadIdx.x; v < nvec; v += LN_WIDE) {
+            uint64_t f[P];
+            vector_pairs<T>(held[v], f);
+            if (arrays == 2) {
+                uint64_t r[P];
+                vector_pairs<T>(held[nvec + v], r);
+#pragma unroll
+                for (int i = 0; i < P; ++i) f[i] = add2(f[i], r[i]);
+                const uint4 h = pairs_vector<T>(f);      // rounded: the norm is taken of what is stored
+                held[v] = h;
+                reinterpret_cast<uint4*>(static_cast<T*>(a.h) + row * a.d)[v] = h;
+                vector_pairs<T>(h, f);
+            }
+#pragma unroll
+            for (int i = 0; i < P; ++i) sum = add2(sum, f[i]);
+        }
+        float lo, hi;
+        unpack2(sum, lo, hi);
+        const float mean = wide_sum2(lo + hi, 0.f, part[0]).x * inv_d;
+        const uint64_t minus = pack2(-mean, -mean);
+        uint64_t sq = 0;
+        for (int v = threadIdx.x; v < nvec; v += LN_WIDE) {
+            uint64_t f[P];
+            vector_pairs<T>(held[v], f);
+#pragma unroll
+            for (int i = 0; i < P; ++i) {
+                const uint64_t e = add2(f[i], minus);
+                sq = fma2(e, e, sq);
+            }
+        }
+        unpack2(sq, lo, hi);
+        const float rs = inverse_root(wide_sum2(lo + hi, 0.f, part[1]).x * inv_d + a.eps);
+        if (a.mean != nullptr && threadIdx.x == 0) { a.mean[row] = mean; a.rstd[row] = rs; }
+        const uint64_t scale = pack2(rs, rs);
+#pragma unroll 2
+        for (int v = threadIdx.x; v < nvec; v += LN_WIDE) {
+            uint64_t f[P], w[P], b[P];
+            weight_pairs<W, N>(a.w, 1.f, v, w);
+            weight_pairs<W, N>(a.b, 0.f, v, b);
+            vector_pairs<T>(held[v], f);
+#pragma unroll
+            for (int i = 0; i < P; ++i) f[i] = fma2(mul2(add2(f[i], minus), scale), w[i], b[i]);
+            reinterpret_cast<uint4*>(static_cast<T*>(a.y) + row * a.d)[v] = pairs_vector<T>(f);
+        }
+    }
+}
+
+template <class T, class W> __global__ void __launch_bounds__(LN_WIDE) ln_dx_wide_kernel(const LnBwd a) {
+    extern __shared__ uint4 smem[];
+    __shared__ float2 part[2][LN_WIDE / 32];
+    constexpr int N = Vec16<T>::N, P = N / 2;
+    const int nvec = a.d / N;
+    const float inv_d = 1.f / a.d;
+    const auto issue = [&](long long row, uint4* to) {
+        if (row < a.rows) {
+            wide_copy<T>(to, static_cast<const T*>(a.h) + row * a.h_stride, nvec);
+            wide_copy<T>(to + nvec, static_cast<const T*>(a.dy) + row * a.d, nvec);
+        }
+        cp_async_commit();
+    };
+    long long row = blockIdx.x;
+    issue(row, smem);
+    for (int turn = 0; row < a.rows; row += gridDim.x, turn ^= 1) {
+        const uint4* held = smem + turn * 2 * nvec;
+        const float mean = a.mean[row], rs = a.rstd[row];
+        issue(row + gridDim.x, smem + (turn ^ 1) * 2 * nvec);
+        cp_async_wait<1>();
+        const uint64_t minus = pack2(-mean, -mean), scale = pack2(rs, rs);
+        uint64_t s1 = 0, s2 = 0;
+        const auto both = [&](int v, uint64_t (&xh)[P], uint64_t (&g)[P]) {
+            uint64_t w[P];
+            weight_pairs<W, N>(a.w, 1.f, v, w);
+            vector_pairs<T>(held[v], xh);
+            vector_pairs<T>(held[nvec + v], g);
+#pragma unroll
+            for (int i = 0; i < P; ++i) {
+                xh[i] = mul2(add2(xh[i], minus), scale);
+                g[i] = mul2(g[i], w[i]);
+            }
+        };
+#pragma unroll 2
+        for (int v = threadIdx.x; v < nvec; v += LN_WIDE) {
+            uint64_t xh[P], g[P];
+            both(v, xh, g);
+#pragma unroll
+            for (int i = 0; i < P; ++i) {
+                s1 = add2(s1, g[i]);
+                s2 = fma2(g[i], xh[i], s2);
+            }
+        }
+        float a1, b1, a2, b2;
+        unpack2(s1, a1, b1);
+        unpack2(s2, a2, b2);
+        const float2 m = wide_sum2(a1 + b1, a2 + b2, part[turn]);
+        const float c1 = -m.x * inv_d, c2 = -m.y * inv_d;
+        const uint64_t shift = pack2(c1, c1), slope = pack2(c2, c2);
+#pragma unroll 2
+        for (int v = threadIdx.x; v < nvec; v += LN_WIDE) {
+            uint64_t xh[P], g[P];
+            both(v, xh, g);
+#pragma unroll
+            for (int i = 0; i < P; ++i) g[i] = mul2(fma2(xh[i], slope, add2(g[i], shift)), scale);
+            if (a.dh != nullptr) {
+                uint64_t e[P];
+                weight_pairs<T, N>(static_cast<const T*>(a.dh) + row * a.d, 0.f, v, e);
+#pragma unroll
+                for (int i = 0; i < P; ++i) g[i] = add2(g[i], e[i]);
+            }
+            reinterpret_cast<uint4*>(static_cast<T*>(a.dx) + row * a.d)[v] = pairs_vector<T>(g);
+        }
+    }
+}
+
 // ------------------------------------------------------------------------------------------ rows too long for registers
 
 constexpr int LN_LONG = 512;      // threads of each CTA of a cluster
@@ -795,6 +969,13 @@ template <class S> int launch_backward(const LnBwd& a, float* part, bool sums, i
     }
 }
 
+// Rows beyond 8192 of whole vectors go through shared memory where there are rows for all SMs and two of them fit (2000x20000 bf16: forward 72
+// us by clusters); `bytes`: of a row in all arrays that are held.  0: they do not.
+size_t wide_bytes(const void* kernel, long long rows, int d, int vec, int ve, size_t bytes) {
+    if (d <= 8192 || vec != ve || rows < sm_count()) return 0;
+    return ensure_dynamic_smem(kernel, 2 * bytes) == ADDER_OK ? 2 * bytes : 0;
+}
+
 // f(shape, cluster size) for the shape whose registers hold a row of d elements, in vectors of vec; false: none does.  Whole 16-byte
 // vectors go through the ring up to 8192 elements, 16 a thread.  Other rows, and longer ones, which a cluster shares, are held up to 32 a thread
 // by CTAs of one row; the backward pass (THREADS = 512) stays where it can, for the sums over the rows.
@@ -823,6 +1004,7 @@ template <class T, class W, int THREADS, class F> bool with_shape(int d, int vec
         else if (d <= 2048) f(LnShape<T, W, 128, VE, NV, STAGES, false, THREADS>(), 1);
         else if (d <= 4096) f(LnShape<T, W, 256, VE, NV, STAGES, false, THREADS>(), 1);
         else if (d <= 8192) f(LnShape<T, W, 512, VE, NV, 2, false, THREADS>(), 1);
+        else if (d <= 8 * 4096) f(LnShape<T, W, 256, VE, 16 / VE, 0, true>(), (d / VE + 256 * (16 / VE) - 1) / (256 * (16 / VE)));
         else f(LnShape<T, W, 256, VE, 32 / VE, 0, true>(), (d / VE + 256 * (32 / VE) - 1) / (256 * (32 / VE)));
     } else if (vec == 2) {
         if constexpr (sizeof(T) == 2) by_row(std::integral_constant<int, 2>());
@@ -889,6 +1071,9 @@ int adder_b200_layernorm_forward(const void* x, const void* residual, const void
         return with_weight_type<T>(weight_dtype, [&](auto* wt) {
             using W = std::remove_pointer_t<decltype(wt)>;
             int status = ADDER_OK;
+            const auto wide = ln_forward_wide_kernel<T, W>;
+            const size_t bytes = wide_bytes(reinterpret_cast<const void*>(wide), rows, (int)d, vec, Vec16<T>::N, d * sizeof(T) * (residual ? 2 : 1));
+            if (bytes > 0) return launch_clusters(wide, (unsigned)sm_count(), LN_WIDE, bytes, 1, s, a);
             const bool held = with_shape<T, W, 256>((int)d, vec, [&](auto shape, int parts) { status = launch_forward<decltype(shape)>(a, parts, s); });
             return held ? status : launch_clusters(ln_forward_long_kernel<T, W>, (unsigned)(rows * 8), LN_LONG, 0, 8, s, a);
         });
@@ -930,11 +1115,14 @@ int adder_b200_layernorm_backward(const void* dy, const void* dh, const void* h,
             using W = std::remove_pointer_t<decltype(wt)>;
             int status = ADDER_OK, groups = 0;
             float* part = static_cast<float*>(workspace);
-            const bool held = with_shape<T, W, 512>((int)d, vec, [&](auto shape, int parts) {
+            const auto wide = ln_dx_wide_kernel<T, W>;
+            const size_t bytes = wide_bytes(reinterpret_cast<const void*>(wide), rows, (int)d, vec, Vec16<T>::N, d * sizeof(T) * 2);
+            const bool held = bytes == 0 && with_shape<T, W, 512>((int)d, vec, [&](auto shape, int parts) {
                 status = launch_backward<decltype(shape)>(a, part, sums, parts, &groups, s);
             });
             if (!held) {
-                if (dx != nullptr) status = launch_clusters(ln_dx_long_kernel<T, W>, (unsigned)(rows * 8), LN_LONG, 0, 8, s, a);
+                if (dx != nullptr && bytes > 0) status = launch_clusters(wide, (unsigned)sm_count(), LN_WIDE, bytes, 1, s, a);
+                else if (dx != nullptr) status = launch_clusters(ln_dx_long_kernel<T, W>, (unsigned)(rows * 8), LN_LONG, 0, 8, s, a);
                 if (status == ADDER_OK && sums) status = vec == Vec16<T>::N ? launch_columns<T, Vec16<T>::N>(a, part, &groups, s) : launch_columns<T, 1>(a, part, &groups, s);
             }
             if (status != ADDER_OK || !sums) return status;

@@ -124,6 +124,23 @@ def test_rows_longer_than_a_block_holds(width, dtype):
         _near("db", grads[-1], *want["db"])
 
 
+@pytest.mark.parametrize("rows", [147, 148, 400])
+@pytest.mark.parametrize("width", [8200, 12000, 28000, 28672])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+def test_long_rows_enough_for_every_sm(rows, width, dtype):
+    """Two rows of one or two arrays in shared memory, or too much for it."""
+    for residual in (False, True):
+        x, r, w, b, dy, dh = _inputs(rows, (width,), dtype, torch.float32, residual, seed=width)
+        outs, grads = _run(x, r, w, b, dy, dh)
+        want = _exact(x, r, w, b, dy, dh if residual else None, 1e-5)
+        _near("y", outs[0], *want["y"])
+        if residual:
+            assert torch.equal(outs[1], want["h"])
+        _near("dx", grads[0], *want["dx"])
+        _near("dw", grads[-2], *want["dw"])
+        _near("db", grads[-1], *want["db"])
+
+
 def test_images_normalised_as_a_whole_and_other_ranks():
     from addernetcuda_b200.layernorm import FusedLayerNorm, layer_norm
     x, _, w, b, dy, _ = _inputs(6, (16, 7, 5), torch.float32, torch.float32, False)
