@@ -102,9 +102,9 @@ struct Best {
     float value, second;
     int vec;
 };
-// What the streaming threads hand over.
+// What the streaming threads hand over: joining it is left to the warp that finishes the row.
 struct LpHand {
-    float m[LP_TEAM / 32], s[LP_TEAM / 32], t[LP_TEAM / 32];
+    float m[LP_TEAM], s[LP_TEAM], t[LP_TEAM];
     Best best[LP_TEAM];
 };
 // What the CTAs of a cluster leave in the shared memory of the first.
@@ -585,8 +585,9 @@ __global__ void __launch_bounds__(THREADS == 32 ? 128 : LP_TEAM + 32, THREADS ==
             __syncwarp();
             bar_sync<LP_FULL>(buffer);
             const LpHand& in = hand[buffer];
-            const bool some = lane < LP_TEAM / 32;
-            float m = some ? in.m[lane] : -INFINITY, s = some ? in.s[lane] : 0.f, tt = some ? in.t[lane] : 0.f;
+            float m = in.m[lane], s = in.s[lane], tt = ENTROPY ? in.t[lane] : 0.f;
+#pragma unroll
+            for (int i = 1; i < LP_TEAM / 32; ++i) join(m, s, tt, in.m[32 * i + lane], in.s[32 * i + lane], ENTROPY ? in.t[32 * i + lane] : 0.f);
             finish_sums<T, ENTROPY>(r, one, lane, m, s, tt);
             uint64_t top = 0;
             if constexpr (TOP) {
@@ -696,11 +697,11 @@ __global__ void __launch_bounds__(THREADS == 32 ? 128 : LP_TEAM + 32, THREADS ==
             }
             write_row<ENTROPY, TOP>(a, row, lane, m, s, tt, top, target, at_target);
         } else {
-            join_lanes<ENTROPY>(m, s, tt, 32);
             __syncwarp();
             if (!CLUSTER) bar_sync<LP_EMPTY>(buffer);
             LpHand& out = hand[buffer];
-            if (lane == 0) { out.m[warp] = m; out.s[warp] = s; out.t[warp] = tt; }
+            out.m[t] = m; out.s[t] = s;
+            if (ENTROPY) out.t[t] = tt;
             if (TOP) out.best[t] = best;
             __syncwarp();
             bar_arrive<LP_FULL>(buffer);
@@ -971,9 +972,11 @@ int adder_b200_log_probs_backward(const void* logits, int dtype, long long rows,
         return ADDER_ERR_NULL_POINTER;
     const unsigned size = dtype == ADDER_TYPE_F32 ? 4 : 2;
     if (!aligned_to(logits, size) || !aligned_to(grad_logits, size)) return ADDER_ERR_ALIGNMENT;
-    const long long tile = 256LL * LP_UNROLL * (16 / size);      // elements that a CTA takes at once
     const bool warps = warp_rows(rows, classes);
-    const long long segments = warps ? 1 : (classes + tile - 1) / tile;
+    // A CTA takes two turns, whose loads and stores overlap (2048x128000 bf16 with an entropy 187 us with one, 161 with two, 164 with three), or
+    // one where there would be too few CTAs.
+    const long long turn = 256LL * LP_UNROLL * (16 / size), ones = (classes + turn - 1) / turn;
+    const long long segments = warps ? 1 : rows * ones >= 8LL * sm_count() ? (ones + 1) / 2 : ones;
     const long long grid = warps ? (rows + 3) / 4 : rows * segments;
     if (grid > 2147483647LL) return ADDER_ERR_UNSUPPORTED;
     const LpBwd a{logits, rows, row_stride, (int)classes, top_k, targets, ignore_index, stats, entropy, top_indices,
