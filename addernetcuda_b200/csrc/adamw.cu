@@ -195,7 +195,7 @@ template <class T, int BITS> struct Place {
     __device__ __forceinline__ Place(const Tensor& t, long long at)
         : p(static_cast<T*>(t.param) + at), g(static_cast<const T*>(t.grad) + at), m(static_cast<float*>(t.exp_avg) + at), v(static_cast<float*>(t.exp_avg_sq) + at) {}
     __device__ __forceinline__ void advance() { p += AW_TILE; g += AW_TILE; m += AW_TILE; v += AW_TILE; }
-    __device__ __forceinline__ bool whole() const { return aligned_to(p, 8 * sizeof(T)) && aligned_to(g, 16) && aligned_to(m, 32) && aligned_to(v, 32); }
+    __device__ __forceinline__ bool whole() const { return aligned_to(p, 8 * sizeof(T)) && aligned_to(g, 4) && aligned_to(m, 32) && aligned_to(v, 32); }
 };
 template <class T> struct Place<T, 8> {
     T* p;
@@ -209,7 +209,7 @@ template <class T> struct Place<T, 8> {
         p += AW_TILE; g += AW_TILE; m += AW_TILE; v += AW_TILE;
         sm += AW_TILE / AW_BLOCK; sv += AW_TILE / AW_BLOCK;
     }
-    __device__ __forceinline__ bool whole() const { return aligned_to(p, 8 * sizeof(T)) && aligned_to(g, 16) && aligned_to(m, 8) && aligned_to(v, 8); }
+    __device__ __forceinline__ bool whole() const { return aligned_to(p, 8 * sizeof(T)) && aligned_to(g, 4) && aligned_to(m, 8) && aligned_to(v, 8); }
 };
 // A warp's 256 elements of each tensor on their way through shared memory, STAGES tiles deep.  Lanes copy consecutive 16-byte words, so what
 // a lane reads may be another's copy: the warp waits for its copies together.  Offsets in a stage, in bytes.
@@ -229,11 +229,18 @@ template <class T, int BITS> struct Ring {
             asm volatile("cp.async.ca.shared.global [%0], [%1], 8;\n" ::"r"(to + 8 * lane), "l"(p + 8 * lane) : "memory");
         }
     }
+    // The same in words of 4 bytes, for gradients that lie one behind another in a bucket.
+    static __device__ __forceinline__ void copy_words(uint32_t to, const void* from, int lane) {
+#pragma unroll
+        for (int i = 0; i < E / 128; ++i)
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;\n" ::"r"(to + 128 * i + 4 * lane), "l"(static_cast<const char*>(from) + 128 * i + 4 * lane) : "memory");
+    }
     // `at` is of the warp's first element
     static __device__ __forceinline__ void fill(uint32_t stage, const Place<T, BITS>& at, int tile, int lane) {
         const int o = tile * AW_TILE;
         copy<E>(stage + P, at.p + o, lane);
-        copy<E>(stage + G, at.g + o, lane);
+        if (aligned_to(at.g, 16)) copy<E>(stage + G, at.g + o, lane);      // the same for all of a tensor
+        else copy_words(stage + G, at.g + o, lane);
         copy<F>(stage + M, at.m + o, lane);
         copy<F>(stage + V, at.v + o, lane);
         if constexpr (BITS == 8) {
