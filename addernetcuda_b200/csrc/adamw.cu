@@ -4,7 +4,11 @@
 //
 // Bound by memory: 28 bytes an element with fp32 parameters (p, g, m, v read, p, m, v written), 22 with 16-bit ones, 10 and 16 with 8-bit
 // states.  A CTA takes one chunk of one tensor; which one it finds by bisection in a table that travels in the launch's
-// parameters, so that nothing is copied to the device for it and a captured launch holds its own.
+// parameters, so that nothing is copied to the device for it and a captured launch holds its own.  A warp's next tiles are on their way
+// through shared memory while it computes.
+//
+// Measured (of a copy's rate): 101 M fp32 elements 428 us (all of it), 48 M bf16 ones 164 us (99 %), 25 M fp32 ones 113 us (94 %); 201 M bf16 with
+// 8-bit states 390 us (79 %), where instructions bound it as well: some 490 of a warp for 256 elements, issued in 84 % of the cycles (50 M elements).
 #include "kernels.h"
 #include "elements.cuh"
 #include <cmath>

@@ -6,10 +6,14 @@
 //             (selected: the target and the k largest)
 //
 // The forward reads the logits once: every thread keeps a maximum of its own with the two sums relative to it, which are rescaled when
-// it rises, and the threads' triples are joined at the end.  The largest k need no second pass over the row either: the k-th largest of
-// the threads' maxima is a lower bound of the k-th largest value, so all candidates lie with the few threads
-// whose maximum reaches it, and only their share of the row is read again.  The backward reads the logits and writes
-// the gradient.  Both are bound by memory for large rows; few rows are split over a cluster of CTAs that join through shared memory.
+// it rises, and the threads' triples are joined at the end, by a warp that does nothing else while the others stream the next row.  The
+// largest k need no second pass over the row either: the k-th largest of some of the threads' maxima is a lower bound of the k-th largest
+// value, so all candidates lie with the few threads whose maximum reaches it, and only their best group of vectors is read again.  The
+// backward reads the logits again and writes the gradient.
+//
+// What bounds them: memory, at 99 % of a copy's rate for the gradient (2048x128000 bf16: 161 us for 1.05 GB) and for the forward of fp32
+// logits (4096x32000: 81 us); the forward of 16-bit logits takes some 8 instructions a value and reaches 90 % (2048x128000
+// with entropy 89 us), and 81 % in shorter rows (4096x50257 bf16 78 us, 91 us with the 5 largest, 107 us with 20).  A few rows are split over a cluster of CTAs that join through shared memory (4x32000: 6 us, 10 us with the 20 largest).
 #include "kernels.h"
 #include "elements.cuh"
 #include <cooperative_groups.h>

@@ -14,7 +14,7 @@
  *   - every function that can fail returns an int status: ADDER_OK (0) or one of the ADDER_ERR_*
  *     codes below; nothing is printed and the process is never aborted (the reference prints and
  *     calls abort() on shapes it cannot tile, adder_cuda/adder.cu:294-297,:436-439);
- *   - kernels are atomic-free and deterministic: the same inputs give bit-identical outputs;
+ *   - kernels are deterministic: the same inputs give bit-identical outputs (no result is added up by atomics);
  *   - NCHW entry points take the layer geometry as (n, ci, h, w, co, k, stride, pad): batch, input
  *     channels, input height/width, output channels, square kernel size, stride, symmetric zero
  *     padding.  Output size is ho = (h - k + 2*pad) / stride + 1 (integer division), wo likewise,

@@ -167,6 +167,54 @@ def test_alignment_and_shared_storage():
         assert all(bool((b[gaps] == 7.0).all()) for b in bufs)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("bits", [32, 8])
+def test_large_tensors(dtype, bits):
+    """Several tiles a chunk, and tensors that end inside one."""
+    from addernetcuda_b200.optim import adamw_step
+    sizes = [20_000_003, 7, 65_537, 2_400_000]
+    if bits == 32:
+        p, g, m, v, steps = _make(sizes, dtype)
+        before = _copies(p, m, v, list(steps))
+        adamw_step(p, g, m, v, steps, **HYPER)
+        _check_step(p, g, m, v, steps, before)
+        return
+    p, g, m, v, sm, sv, steps = _eight(sizes, dtype)
+    before = _copies(p, m, v, sm, sv, list(steps))
+    adamw_step(p, g, m, v, steps, exp_avg_scales=sm, exp_avg_sq_scales=sv, **HYPER)
+    b1, b2 = HYPER["betas"]
+    for i, (p0, m0, v0, sm0, sv0, t0) in enumerate(zip(*before)):
+        m1, v1 = moments(g[i].float(), decode(m0, sm0, True), decode(v0, sv0, False), b1, b2)
+        for codes, scales, x, signed in ((m[i], sm[i], m1, True), (v[i], sv[i], v1, False)):
+            want, want_scales = encode(x, signed)
+            assert torch.equal(codes, want) and torch.equal(scales, want_scales), i
+        t = int(t0[0]) + 1
+        p1 = update64(p0, m1, v1, t, HYPER["lr"], b1, b2, HYPER["eps"], HYPER["weight_decay"])
+        size = HYPER["lr"] / (1 - b1 ** t) * m1.double().abs() / ((v1.double() / (1 - b2 ** t)).sqrt() + HYPER["eps"])
+        _near(f"p[{i}]", p[i], p1, U[dtype] * p1.abs() * (1 + 2.0 ** -8) + 32 * 2.0 ** -24 * size + 4 * 2.0 ** -24 * p1.abs())
+        assert steps[i].tolist() == [t, 0]
+
+
+@pytest.mark.parametrize("dtype", list(U), ids=str)
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("first", [1, 2, 3, 4, 6])
+def test_gradients_alone_at_other_addresses(dtype, bits, first):
+    """All else is aligned, as when gradients are views of a bucket: the same bits as from an aligned gradient."""
+    from addernetcuda_b200.optim import adamw_step
+    make = _make if bits == 32 else _eight
+    a, b = make(SIZES, dtype), make(SIZES, dtype)
+    grads = []
+    for g in b[1]:
+        buf = torch.full((g.numel() + 16,), float("nan"), device=DEV).to(dtype)      # what lies beside a gradient is not used
+        buf[first:first + g.numel()] = g
+        grads.append(buf[first:first + g.numel()])
+    for s, g in ((a, a[1]), (b, grads)):
+        kw = dict(exp_avg_scales=s[4], exp_avg_sq_scales=s[5]) if bits == 8 else {}
+        adamw_step(s[0], g, s[2], s[3], s[-1], **kw, **HYPER)
+    for x, y in zip([a[0], *a[2:]], [b[0], *b[2:]]):
+        assert all(torch.equal(t, u) for t, u in zip(list(x), list(y)))
+
+
 def test_other_memory_orders_and_mixed_types():
     from addernetcuda_b200.optim import adamw_step
     torch.manual_seed(0)

@@ -50,13 +50,13 @@ def _k(v):
     return (64 + v / 256) * 2.0 ** -24
 
 
-def _check(x, t, k=0, entropy=True, grads=True, ignore=-100):
+def _check(x, t, k=0, entropy=True, grads=True, ignore=-100, e=None):
     from addernetcuda_b200.logprobs import token_log_probs
     v = x.shape[-1]
     leaf = x.detach().requires_grad_(grads)
     r = token_log_probs(leaf, t, top_k=k, entropy=entropy, ignore_index=ignore)
     want = _exact(x, t, k, ignore)
-    e = _k(v)
+    e = e or _k(v)
     _close("log_prob", r.log_prob, want["log_prob"], e * (1 + want["log_prob"].abs()))
     if entropy:
         _close("entropy", r.entropy, want["entropy"], 2 * e * (1 + want["entropy"]))
@@ -109,6 +109,17 @@ def test_rows_split_over_a_cluster_or_not(rows):
         x, t = _logits(rows, v, torch.bfloat16, seed=rows)
         _check(x, t, 20)
         _check(x, t, 1, entropy=False)
+
+
+@pytest.mark.parametrize("v", [1000, 1025, 4000, 8191, 8192, 8193])
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_many_rows(v, dtype):
+    """Rows that one warp takes each: a lane adds up V / 32 values, so K = 64 + V / 32."""
+    e = (64 + v / 32) * 2.0 ** -24
+    for rows, k in ((3551, 5), (3552, 0), (4001, 20)):
+        x, t = _logits(rows, v, dtype, seed=v + k)
+        t[1::7] = -100
+        _check(x, t, k, entropy=k != 0, e=e)
 
 
 @pytest.mark.parametrize("v", [10, 1000, 5000, 50257])
