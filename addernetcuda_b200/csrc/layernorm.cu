@@ -1037,10 +1037,12 @@ template <class T, class F> int with_weight_type(int wtype, F&& f) {
     return f(static_cast<T*>(nullptr));
 }
 
+constexpr long long LN_MOST = (1LL << 30) - 65536;      // columns: both sums of all of them are counted in 32 bits
+
 int ln_check(long long rows, long long d, int dtype, int wtype) {
     if (rows < 0 || d <= 0) return ADDER_ERR_BAD_SHAPE;
     if (dtype < ADDER_TYPE_F32 || dtype > ADDER_TYPE_F16 || (wtype != dtype && wtype != ADDER_TYPE_F32)) return ADDER_ERR_UNSUPPORTED;
-    if (d > 2147483647LL - 65536 || rows > 2147483647LL / 8) return ADDER_ERR_UNSUPPORTED;
+    if (d > LN_MOST || rows > 2147483647LL / 8) return ADDER_ERR_UNSUPPORTED;
     return ADDER_OK;
 }
 
@@ -1085,7 +1087,7 @@ int adder_b200_layernorm_forward(const void* x, const void* residual, const void
 }
 
 size_t adder_b200_layernorm_backward_workspace_bytes(long long rows, long long d) {
-    if (rows <= 0 || d <= 0 || d > 2147483647LL - 65536) return 0;
+    if (rows <= 0 || d <= 0 || d > LN_MOST) return 0;
     return (size_t)std::max(ln_splits(rows, (int)d, 8), ln_most_parts(rows)) * 2 * d * sizeof(float);
 }
 

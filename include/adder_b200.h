@@ -249,7 +249,7 @@ ADDER_API int adder_b200_forward_affine(const float* x, const float* w, const fl
  *   h = x + residual, rounded to the type (h = x where residual is NULL);  y = (h - mean) / sqrt(var + eps) * weight + bias
  * x and residual have x_stride and residual_stride elements from row to row; y and h (written where there is a residual) are
  * contiguous.  weight and bias [d] are of weight_dtype, the same type or fp32, and may be NULL (1 and 0).  mean and rstd [rows], for the
- * backward call, may be NULL together.  Any alignment that the types need; 16-byte aligned rows run faster. */
+ * backward call, may be NULL together.  Any alignment that the types need; 16-byte aligned rows run faster.  d is at most 2^30 - 2^16. */
 ADDER_API int adder_b200_layernorm_forward(const void* x, const void* residual, const void* weight, const void* bias, void* y, void* h,
                                            float* mean, float* rstd, long long rows, long long d, long long x_stride,
                                            long long residual_stride, int dtype, int weight_dtype, float eps, void* stream);

@@ -325,3 +325,41 @@ def test_streams_and_captured_replays():
         want = _run(x2, r, w, b, dy, dh)
         for _, out in graphs:
             assert all(torch.equal(a, c) for a, c in zip(want[0] + want[1], out[0] + out[1]))
+
+
+def test_no_rows():
+    from addernetcuda_b200.layernorm import layer_norm
+    for dtype in (torch.float32, torch.bfloat16):
+        x = torch.randn(0, 33, device=DEV, dtype=dtype, requires_grad=True)
+        w, b = (torch.randn(33, device=DEV, requires_grad=True) for _ in range(2))
+        y, h = layer_norm(x, 33, w, b, residual=x.detach())
+        assert y.shape == h.shape == (0, 33)
+        dx, dw, db = torch.autograd.grad(y.sum() + h.sum(), (x, w, b))
+        assert dx.shape == (0, 33) and bool((dw == 0).all()) and bool((db == 0).all())
+
+
+@pytest.mark.parametrize("rows,d", [(530000, 4096), (2150000, 1001)])
+def test_offsets_beyond_32_bits(rows, d):
+    """The last rows of more than 2^31 elements: rows are summed up alike wherever they lie."""
+    from addernetcuda_b200.layernorm import layer_norm
+    assert rows * d > 2 ** 31
+    tail = torch.randn(8, d, device=DEV, dtype=torch.bfloat16)
+    x = torch.zeros(rows, d, device=DEV, dtype=torch.bfloat16)
+    x[-8:] = tail
+    w, b = (torch.randn(d, device=DEV) for _ in range(2))
+    y = layer_norm(x.requires_grad_(), d, w, b)
+    hd = tail.double()
+    want = (hd - hd.mean(1, keepdim=True)) / (hd.var(1, unbiased=False, keepdim=True) + 1e-5).sqrt()
+    k = (64 + 4 * d ** 0.5) * 2.0 ** -24
+    top = (want.abs() + 1) * w.double().abs() + b.double().abs()
+    off = (y[-8:].double() - (want * w.double() + b.double())).abs()
+    assert bool((off <= 2.0 ** -8 * (want * w.double() + b.double()).abs() + 2 * k * top).all())
+    dy = torch.zeros_like(x)
+    dy[-8:] = torch.randn(8, d, device=DEV)
+    dx, = torch.autograd.grad(y, x, dy)
+    g = dy[-8:].double() * w.double()
+    rstd = 1 / (hd.var(1, unbiased=False, keepdim=True) + 1e-5).sqrt()
+    ref = rstd * (g - g.mean(1, keepdim=True) - want * (g * want).mean(1, keepdim=True))
+    size = rstd * (g.abs() + g.abs().mean(1, keepdim=True) + (want.abs() + 1) * (g * want).abs().mean(1, keepdim=True))
+    assert bool(((dx[-8:].double() - ref).abs() <= 2.0 ** -8 * ref.abs() + 4 * k * size).all())
+    assert bool((dx[: 8] == 0).all())

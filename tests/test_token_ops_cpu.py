@@ -32,6 +32,10 @@ def test_layer_norm_entry_points_check_their_arguments():
     assert back(ws=None) == 5 and back(bytes=8) == 5
     assert lib.adder_b200_layernorm_backward_workspace_bytes(0, 8) == 0 and lib.adder_b200_layernorm_backward_workspace_bytes(2, 0) == 0
     assert lib.adder_b200_layernorm_backward_workspace_bytes(4, 8) >= 2 * 8 * 4
+    most = 2 ** 30 - 2 ** 16
+    assert call(d=most + 1) == back(d=most + 1) == back(d=2 ** 31) == call(d=2 ** 30)
+    assert call(d=most + 1) not in (0, call(d=0)) and back(d=most + 1) not in (0, back(d=0))
+    assert lib.adder_b200_layernorm_backward_workspace_bytes(1, most + 1) == 0 < lib.adder_b200_layernorm_backward_workspace_bytes(1, most)
 
 
 def test_log_probs_entry_points_check_their_arguments():
