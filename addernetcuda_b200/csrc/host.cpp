@@ -928,15 +928,13 @@ PyObject* py_adamw(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     }
     for (const auto& t : tensors)
         if (t.n > 0 && written.has(t.grad)) Py_RETURN_NONE;
-    {
-        pybind11::gil_scoped_release no_gil;
-        const c10::cuda::CUDAGuard guard(dev);
-        check(api.adamw_step(tensors.data(), (int)n, type, eight ? 8 : 32, lr, lr_device, b1, b2, eps, wd, scale_device,
-                             c10::cuda::getCurrentCUDAStream(dev.index()).stream()), "adder_b200_adamw_step");
-        for (const auto* list : {&p, &m, &v})
-            for (const at::Tensor* t : *list)
-                if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
-    }
+    // The lock stays: the lists own the tensors, and another thread may change a list.
+    const c10::cuda::CUDAGuard guard(dev);
+    check(api.adamw_step(tensors.data(), (int)n, type, eight ? 8 : 32, lr, lr_device, b1, b2, eps, wd, scale_device,
+                         c10::cuda::getCurrentCUDAStream(dev.index()).stream()), "adder_b200_adamw_step");
+    for (const auto* list : {&p, &m, &v})
+        for (const at::Tensor* t : *list)
+            if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
     Py_RETURN_TRUE;
     END_HANDLE_TH_ERRORS
 }

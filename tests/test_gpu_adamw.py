@@ -329,6 +329,41 @@ def test_without_the_host_path_the_results_are_the_same(monkeypatch):
             assert all(torch.equal(t, u) for t, u in zip(list(x), list(y)))
 
 
+def test_two_threads_at_once():
+    """Each with tensors, lists and a stream of its own, emptied and filled again between the steps."""
+    import threading
+
+    from addernetcuda_b200.optim import adamw_step
+    sets = [_make([1000, 3, 2048, 70000], torch.float32, seed=i) for i in range(2)]
+    want = [_make([1000, 3, 2048, 70000], torch.float32, seed=i) for i in range(2)]
+    for s in want:
+        for _ in range(50):
+            adamw_step(*s, **HYPER)
+    torch.cuda.synchronize()
+    failed = []
+
+    def work(s):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(50):
+                    lists = [list(ts) for ts in s[:4]]
+                    adamw_step(*lists, s[4], **HYPER)
+                    for ts in lists:
+                        ts.clear()
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=(s,)) for s in sets]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed
+    for s, w in zip(sets, want):
+        assert all(torch.equal(a, b) for x, y in zip(s, w) for a, b in zip(list(x), list(y)))
+
+
 def test_versions_tell_autograd_of_the_write():
     from addernetcuda_b200.optim import adamw_step
     p, g, m, v, steps = _make([8], torch.float32)
