@@ -122,6 +122,31 @@ def test_many_rows(v, dtype):
         _check(x, t, k, entropy=k != 0, e=e)
 
 
+@pytest.mark.parametrize("rows,v", [(2148, 1000003), (600000, 4000)])
+def test_offsets_beyond_32_bits(rows, v):
+    """The last rows of more than 2^31 logits."""
+    from addernetcuda_b200.logprobs import token_log_probs
+    assert rows * v > 2 ** 31
+    x = torch.zeros(rows, v, dtype=torch.bfloat16, device=DEV)
+    tail, t_tail = _logits(8, v, torch.bfloat16, seed=1)
+    x[-8:] = tail
+    t = torch.zeros(rows, dtype=torch.int64, device=DEV)
+    t[-8:] = t_tail
+    r = token_log_probs(x.requires_grad_(), t, top_k=3, entropy=True)
+    dx, = torch.autograd.grad([r.log_prob, r.entropy], x, [torch.ones_like(r.log_prob), torch.ones_like(r.entropy)])
+    tail.requires_grad_()
+    w = token_log_probs(tail, t_tail, top_k=3, entropy=True)
+    want, = torch.autograd.grad([w.log_prob, w.entropy], tail, [torch.ones_like(w.log_prob), torch.ones_like(w.entropy)])
+    e = (64 + v / 32) * 2.0 ** -24      # either variant, each within this of the exact value
+    assert torch.equal(r.top_indices[-8:], w.top_indices)
+    assert bool(((r.log_prob[-8:] - w.log_prob).abs() <= 2 * e * (1 + w.log_prob.abs())).all())
+    assert bool(((r.entropy[-8:] - w.entropy).abs() <= 4 * e * (1 + w.entropy)).all())
+    p = torch.log_softmax(tail.detach().double(), 1)
+    size = (torch.arange(v, device=DEV) == t_tail[:, None]) + p.exp() * (2 + p.abs() + w.entropy[:, None].double())
+    assert bool(((dx[-8:].double() - want.double()).abs() <= 2 * U[torch.bfloat16] * want.double().abs() + 4 * e * size).all())
+    assert bool((dx[rows // 2] == dx[0]).all())      # alike rows
+
+
 @pytest.mark.parametrize("v", [10, 1000, 5000, 50257])
 def test_ties_go_to_the_lowest_index(v):
     """Few different values, constant rows, zeros of both signs, runs and strides that meet one thread's share."""
