@@ -83,8 +83,8 @@ class _LayerNorm(torch.autograd.Function):
         h2, hs = _rows(h, rows, d)
         dx = torch.empty(h.shape, dtype=h.dtype, device=h.device) if need_x else None
         lib = _lib.load()
-        nbytes = lib.adder_b200_layernorm_backward_workspace_bytes(rows, d) if dw is not None or db is not None else 0
         with torch.cuda.device(h.device):
+            nbytes = lib.adder_b200_layernorm_backward_workspace_bytes(rows, d) if dw is not None or db is not None else 0
             ws = torch.empty(nbytes, dtype=torch.uint8, device=h.device) if nbytes else None
             _lib.check(lib.adder_b200_layernorm_backward(
                 dy.data_ptr(), _ptr(dh), h2.data_ptr(), _ptr(w), mean.data_ptr(), rstd.data_ptr(), _ptr(dx), _ptr(dw), _ptr(db),
