@@ -7,8 +7,8 @@
 // parameters, so that nothing is copied to the device for it and a captured launch holds its own.  A warp's next tiles are on their way
 // through shared memory while it computes.
 //
-// Measured (of a copy's rate): 101 M fp32 elements 428 us (all of it), 48 M bf16 ones 164 us (99 %), 25 M fp32 ones 113 us (94 %); 201 M bf16 with
-// 8-bit states 390 us (79 %), where instructions bound it as well: some 490 of a warp for 256 elements, issued in 84 % of the cycles (50 M elements).
+// Measured (of a copy's rate): 101 M fp32 elements 418 us and 48 M bf16 ones 160 us (all of it), 25 M fp32 ones 109 us (98 %); 201 M bf16 with 8-bit
+// states 390 us (79 %), where instructions bound it as well: some 490 of a warp for 256 elements, issued in 84 % of the cycles (50 M elements).
 #include "kernels.h"
 #include "elements.cuh"
 #include <cmath>
@@ -22,7 +22,8 @@ constexpr int AW_BLOCK = 256;                 // values that share a scale
 
 using Tensor = adder_b200_adamw_tensor;
 
-// 48 tensors fit in 4 KB of launch parameters, 480 in the 32 KB that there may be.
+// 48 tensors fit in 4 KB of launch parameters, 480 in the 32 KB that there may be.  The host takes longer to launch larger ones (9.1, 9.9 and 12.5
+// us a call with 48, 176 and 480), the kernel itself does not.
 template <int CAP> struct Table {
     Tensor t[CAP];
     int first[CAP + 1];      // first chunk of each tensor
@@ -479,10 +480,12 @@ int adder_b200_adamw_step(const adder_b200_adamw_tensor* tensors, int count, int
     h.eps = (float)eps; h.wd = (float)weight_decay;
     h.ln_b1 = (float)std::log(beta1); h.ln_b2 = (float)std::log(beta2);      // -inf for 0: 1 - 0^t = 1
     h.lr_device = lr_device; h.grad_scale = grad_scale;
-    // Small models get a CTA for every tile, so that all SMs take part; large ones up to 8 tiles a CTA, which fetches one while it computes
-    // another.
+    // Small models get a CTA for every tile, so that all SMs take part; larger ones up to 4 tiles a CTA, which fetches one while it computes
+    // another, and 8 with 8-bit states, which compute longer.  fp32 with 1, 2, 4 and 8 tiles, us: 0.5 M elements 6.3, 6.3, 7.3, 10.2; 1 M 8.7, 8.3,
+    // 8.3, 10.4; 3.1 M 17.4, 14.5, 12.4, 14.5; 25 M 119, 110, 109, 112.  bf16 with 8-bit states: 6 M 22.7, 18.6, 17.6, 20.6; 24 M 83, 64, 57, 55.
     int tiles = 1;
-    while (tiles < 8 && elements >= 8LL * sm_count() * tiles * AW_TILE) tiles *= 2;
+    while (tiles < 4 && elements >= 2LL * sm_count() * tiles * AW_TILE) tiles *= 2;
+    if (state_bits == 8 && elements >= 32LL * sm_count() * AW_TILE) tiles = 8;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     return with_type(dtype, [&](auto* type) {
         using T = std::remove_pointer_t<decltype(type)>;

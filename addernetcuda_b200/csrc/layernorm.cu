@@ -973,8 +973,8 @@ template <class S> int launch_backward(const LnBwd& a, float* part, bool sums, i
     }
 }
 
-// Rows beyond 8192 of whole vectors go through shared memory where there are rows for all SMs and two of them fit (2000x20000 bf16: forward 72
-// us by clusters); `bytes`: of a row in all arrays that are held.  0: they do not.
+// Rows beyond 8192 of whole vectors go through shared memory where there are rows for all SMs and two of them fit (2000x20000 bf16: forward 46
+// us, backward 105; by clusters 73 and 123); `bytes`: of a row in all arrays that are held.  0: they do not.
 size_t wide_bytes(const void* kernel, long long rows, int d, int vec, int ve, size_t bytes) {
     if (d <= 8192 || vec != ve || rows < sm_count()) return 0;
     return ensure_dynamic_smem(kernel, 2 * bytes) == ADDER_OK ? 2 * bytes : 0;
@@ -1132,7 +1132,8 @@ int adder_b200_layernorm_backward(const void* dy, const void* dh, const void* h,
                 if (status == ADDER_OK && sums) status = vec == Vec16<T>::N ? launch_columns<T, Vec16<T>::N>(a, part, &groups, s) : launch_columns<T, 1>(a, part, &groups, s);
             }
             if (status != ADDER_OK || !sums) return status;
-            // up to 16 parts one after another, more by 16 threads
+            // up to 16 parts one after another, more by 16 threads (whole backward pass: 16 parts of 4096 columns 9.3 us and 10.4 by 16; 592 of 1024 12.4
+            // one after another and 10.4)
             if (groups <= 16) ln_columns_finish_kernel<W, 1><<<(unsigned)((2 * d + 255) / 256), 256, 0, s>>>(part, groups, (int)d, static_cast<W*>(dweight), static_cast<W*>(dbias));
             else ln_columns_finish_kernel<W, 16><<<(unsigned)((2 * d + 15) / 16), 256, 0, s>>>(part, groups, (int)d, static_cast<W*>(dweight), static_cast<W*>(dbias));
             return launched();

@@ -924,9 +924,12 @@ template <class T, int THREADS, bool CLUSTER, bool ENTROPY, bool TOP> int launch
     }
 }
 
-// A warp a row: short rows, and longer ones where there are enough to fill the SMs (16384 x 4000 bf16: forward 33 us, by CTAs 94; backward see
-// below).
-bool warp_rows(long long rows, long long classes) { return classes <= 1024 || (classes <= 8192 && rows >= 24LL * sm_count()); }
+// A warp a row: short rows, and longer ones where there are enough to fill the SMs.  Forward and backward of bf16 with entropy, us by warps and by
+// CTAs: 2000x1024 11 and 20, 1184x2048 10 and 16, 1184x4096 14.5 and 16.5, 16384x4000 80 and 141, 3552x8000 37 and 41; on the other side
+// 296x2048 10.4 and 8.3, 600x4096 13.4 and 12.4, 1184x8192 18.6 and 17.7 (fp32 29 and 23).
+bool warp_rows(long long rows, long long classes) {
+    return classes <= 1024 || (classes <= 4096 && rows >= 8LL * sm_count()) || (classes <= 8192 && rows >= 24LL * sm_count());
+}
 
 template <class T, int THREADS, bool CLUSTER> int choose_forward(const LpFwd& a, int parts, cudaStream_t s) {
     if (a.entropy != nullptr)
@@ -955,7 +958,8 @@ int adder_b200_log_probs_forward(const void* logits, int dtype, long long rows, 
     return with_type(dtype, [&](auto* type) {
         using T = std::remove_pointer_t<decltype(type)>;
         if (warp_rows(rows, classes)) return choose_forward<T, 32, false>(a, 1, s);
-        // Few rows leave SMs idle: a row is then split over a cluster of up to 8 CTAs of at least 4096 elements.
+        // Few rows leave SMs idle: a row is then split over a cluster of up to 8 CTAs of at least 4096 elements (64x128000 bf16 by 4 CTAs 8.4 us,
+        // by one 12.4; 296x50257 by one 10.4, by two 12.2).
         int parts = 1;
         while (parts < 8 && rows * parts * 2 <= sm_count() * 4 && classes >= 8192LL * parts) parts *= 2;
         if (parts > 1) return choose_forward<T, LP_TEAM, true>(a, parts, s);
