@@ -7,6 +7,8 @@
 #include <torch/extension.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/forward_grad.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <ATen/cuda/CUDAContext.h>
@@ -441,6 +443,18 @@ NormResult norm_forward(const at::Tensor& x, const at::Tensor& r, const at::Tens
 
 using Optional = std::optional<at::Tensor>;
 
+// `grad` of an operator that is differentiable once, computed from the tensors in `from`.  Where the backward pass is itself recorded
+// (create_graph) it must not count as a constant: it gets a node that raises when it is differentiated.  The node's edges lead to what the
+// gradient depends on, so that a call for the gradients of some inputs alone comes by it, too.
+void once(const char* name, const at::Tensor& grad, std::initializer_list<const at::Tensor*> from) {
+    if (!grad.defined() || !at::GradMode::is_enabled()) return;
+    torch::autograd::edge_list edges;
+    for (const at::Tensor* t : from)
+        if (t->defined() && t->requires_grad()) edges.push_back(torch::autograd::impl::gradient_edge(*t));
+    if (edges.empty()) return;
+    torch::autograd::set_history(grad, std::make_shared<torch::autograd::Error>(std::string(name) + " is differentiable once", std::move(edges)));
+}
+
 struct LayerNorm : public torch::autograd::Function<LayerNorm> {
     static variable_list forward(AutogradContext* ctx, const Variable& x, const Optional& r, const Optional& w, const Optional& b, const Norm& n) {
         const at::Tensor none;
@@ -488,6 +502,10 @@ struct LayerNorm : public torch::autograd::Function<LayerNorm> {
         if (bytes > 0) ws = empty_on(h, {(int64_t)bytes}, at::kByte);
         check(api.layernorm_backward(ptr(dy), ptr(dh), ptr(h2), ptr(w), mean.const_data_ptr<float>(), rstd.const_data_ptr<float>(), ptr(dx), ptr(dw),
                                      ptr(db), ptr(ws), bytes, rows, d, stride, type, weight_type, current_stream(h)), "adder_b200_layernorm_backward");
+        const Variable& input = need_x || need_r ? h : none;      // h is an output as well, and asks for gradients whatever the inputs do
+        once("layer_norm", dx, {&dy, &dh, &input, &w});
+        once("layer_norm", dw, {&dy, &input});
+        once("layer_norm", db, {&dy});
         return {need_x ? dx : none, need_r ? dx : none, dw, db, none};
     }
 };
@@ -581,6 +599,7 @@ struct LogProbsNode : public torch::autograd::Function<LogProbsNode> {
                                      static_cast<const long long*>(ptr(indices)), stats.const_data_ptr<float>(), static_cast<const float*>(ptr(entropy)),
                                      static_cast<const float*>(ptr(g_lp)), static_cast<const float*>(ptr(g_ent)), static_cast<const float*>(ptr(g_top)),
                                      ptr(dx), current_stream(x)), "adder_b200_log_probs_backward");
+        once("token_log_probs", dx, {&x, &g_lp, &g_ent, &g_top});
         return {dx, none, none};
     }
 };

@@ -12,7 +12,6 @@ from typing import Optional, Sequence, Tuple, Union
 
 import torch
 import torch.nn as nn
-from torch.autograd.function import once_differentiable
 
 from . import _lib, _native, adder_cuda
 
@@ -37,6 +36,28 @@ def _ptr(t: Optional[torch.Tensor]):
 def _sizes(x: torch.Tensor, normalized_shape) -> Tuple[int, int]:
     d = math.prod(normalized_shape)
     return (x.numel() // d if d else 0), d
+
+
+class _Once(torch.autograd.Function):
+    """Hands on a gradient as what follows from `sources`, and raises where it is differentiated."""
+
+    @staticmethod
+    def forward(ctx, name, grad, *sources):
+        ctx.name = name
+        return grad.detach()
+
+    @staticmethod
+    def backward(ctx, _):
+        raise RuntimeError(f"{ctx.name} is differentiable once")
+
+
+def _once(name: str, grad: Optional[torch.Tensor], *sources) -> Optional[torch.Tensor]:
+    """`grad` of an operator that is differentiable once, computed from `sources`.  Where the backward pass is itself recorded
+    (create_graph) it must not count as a constant, so differentiating it raises."""
+    sources = [t for t in sources if t is not None and t.requires_grad]
+    if grad is None or not sources or not torch.is_grad_enabled():
+        return grad
+    return _Once.apply(name, grad, *sources)
 
 
 class _LayerNorm(torch.autograd.Function):
@@ -69,11 +90,21 @@ class _LayerNorm(torch.autograd.Function):
         return y, h
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy, dh=None):
         if dy is None and dh is None:
             return (None,) * 7
-        h, w, mean, rstd = ctx.saved_tensors
+        saved = ctx.saved_tensors
+        with torch.no_grad():
+            dx, dw, db = _LayerNorm.gradients(ctx, saved, dy, dh)
+        need_x, need_r = ctx.needs_input_grad[0], ctx.has_residual and ctx.needs_input_grad[1]
+        h = saved[0] if need_x or need_r else None      # it is an output as well, and asks for gradients whatever the inputs do
+        dx = _once("layer_norm", dx, dy, dh, h, saved[1])
+        return (dx if need_x else None, dx if need_r else None, _once("layer_norm", dw, dy, h), _once("layer_norm", db, dy),
+                None, None, None)
+
+    @staticmethod
+    def gradients(ctx, saved, dy, dh):
+        h, w, mean, rstd = saved
         rows, d, wcode = ctx.sizes
         need_x = ctx.needs_input_grad[0] or (ctx.has_residual and ctx.needs_input_grad[1])
         dw = torch.empty(w.shape, dtype=w.dtype, device=w.device) if w is not None and ctx.needs_input_grad[2] else None
@@ -90,8 +121,7 @@ class _LayerNorm(torch.autograd.Function):
                 dy.data_ptr(), _ptr(dh), h2.data_ptr(), _ptr(w), mean.data_ptr(), rstd.data_ptr(), _ptr(dx), _ptr(dw), _ptr(db),
                 _ptr(ws), nbytes, rows, d, hs, _lib.TYPE_CODES[h.dtype], wcode, adder_cuda._stream(h.device)),
                 "adder_b200_layernorm_backward")
-        return (dx if ctx.needs_input_grad[0] else None, dx if ctx.has_residual and ctx.needs_input_grad[1] else None, dw, db,
-                None, None, None)
+        return dx, dw, db
 
 
 def _check_input(t, name: str, dev=None) -> None:

@@ -11,10 +11,9 @@ from typing import NamedTuple, Optional
 
 import torch
 import torch.nn as nn
-from torch.autograd.function import once_differentiable
 
 from . import _lib, _native, adder_cuda
-from .layernorm import _check_input, _ptr, _rows
+from .layernorm import _check_input, _once, _ptr, _rows
 
 MAX_TOP_K = 32
 
@@ -57,11 +56,17 @@ class _LogProbs(torch.autograd.Function):
         return lp, ent, top, idx
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, g_lp, g_ent, g_top, _):
         if g_lp is None and g_ent is None and g_top is None:
             return (None,) * 6
-        logits, targets, stats, ent, idx = ctx.saved_tensors
+        saved = ctx.saved_tensors
+        with torch.no_grad():
+            dx = _LogProbs.gradient(ctx, saved, g_lp, g_ent, g_top)
+        return _once("token_log_probs", dx, saved[0], g_lp, g_ent, g_top), None, None, None, None, None
+
+    @staticmethod
+    def gradient(ctx, saved, g_lp, g_ent, g_top):
+        logits, targets, stats, ent, idx = saved
         top_k, ignore_index = ctx.args
         v = logits.shape[-1]
         rows = logits.numel() // v
@@ -73,7 +78,7 @@ class _LogProbs(torch.autograd.Function):
                 x.data_ptr(), _lib.TYPE_CODES[logits.dtype], rows, v, stride, _ptr(targets), ignore_index, top_k, _ptr(idx), stats.data_ptr(),
                 _ptr(ent), _ptr(g_lp), _ptr(g_ent), _ptr(g_top), dx.data_ptr(), adder_cuda._stream(logits.device)),
                 "adder_b200_log_probs_backward")
-        return dx, None, None, None, None, None
+        return dx
 
 
 def token_log_probs(logits: torch.Tensor, targets: Optional[torch.Tensor] = None, top_k: int = 0, entropy: bool = False,

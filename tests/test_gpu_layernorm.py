@@ -363,3 +363,49 @@ def test_offsets_beyond_32_bits(rows, d):
     size = rstd * (g.abs() + g.abs().mean(1, keepdim=True) + (want.abs() + 1) * (g * want).abs().mean(1, keepdim=True))
     assert bool(((dx[-8:].double() - ref).abs() <= 2.0 ** -8 * ref.abs() + 4 * k * size).all())
     assert bool((dx[: 8] == 0).all())
+
+
+@pytest.mark.parametrize("host_path", [True, False])
+@pytest.mark.parametrize("residual", [False, True])
+def test_gradients_are_not_taken_for_constants(host_path, residual, monkeypatch):
+    """A gradient of create_graph=True that depends on a leaf raises where it is differentiated, beside another term of the loss and for some
+    inputs alone; one that depends on nothing is a constant."""
+    from addernetcuda_b200 import _native
+    from addernetcuda_b200.layernorm import layer_norm
+    if not host_path:
+        monkeypatch.setattr(_native, "layer_norm", _native._absent)
+    x, r, w, b, dy, _ = _inputs(5, (24,), torch.float32, torch.float32, residual)
+
+    def call(leaves, upstream, of):
+        """Sum of the outputs weighted by `upstream`, and the gradients of it."""
+        out = layer_norm(leaves[0], 24, leaves[2], leaves[3], residual=leaves[1])
+        total = (out[0] * upstream).sum() + (out[1] * upstream).sum() if residual else (out * upstream).sum()
+        return total, torch.autograd.grad(total, of, create_graph=True)
+
+    for needed in ("x", "r", "w", "all"):
+        if needed == "r" and not residual:
+            continue
+        leaves = [t.clone().requires_grad_(needed in (n, "all")) if t is not None else None for t, n in ((x, "x"), (r, "r"), (w, "w"), (b, "b"))]
+        of = [t for t in leaves if t is not None and t.requires_grad]
+        for upstream in (dy, dy.clone().requires_grad_()):
+            total, grads = call(leaves, upstream, of)
+            plain = torch.autograd.grad((lambda o: (o[0] * dy).sum() + (o[1] * dy).sum() if residual else (o * dy).sum())(
+                layer_norm(leaves[0], 24, leaves[2], leaves[3], residual=leaves[1])), of)
+            assert all(torch.equal(g.detach(), p) for g, p in zip(grads, plain))
+            for g, leaf in zip(grads, of):
+                const = not upstream.requires_grad and (leaf is leaves[3] or needed == "w")
+                if const:
+                    assert not g.requires_grad
+                    continue
+                if leaf is leaves[3]:      # sums of the upstream gradient, the weights of which is its only leaf
+                    with pytest.raises(RuntimeError, match="differentiable once"):
+                        torch.autograd.grad(g.square().sum(), upstream, retain_graph=True)
+                    continue
+                with pytest.raises(RuntimeError, match="differentiable once"):
+                    (total + g.square().sum()).backward(retain_graph=True)
+                with pytest.raises(RuntimeError, match="differentiable once"):
+                    torch.autograd.grad(total + g.square().sum(), upstream if upstream.requires_grad else of[0], retain_graph=True)
+    only_b = [x, r, w, b.clone().requires_grad_()]
+    total, (g,) = call(only_b, dy, [only_b[3]])
+    (total + g.square().sum()).backward()
+    assert torch.equal(only_b[3].grad, g.detach())

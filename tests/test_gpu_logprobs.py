@@ -367,3 +367,28 @@ def test_streams_and_captured_replays():
         g.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(run(xs, ts), out))
+
+
+@pytest.mark.parametrize("host_path", [True, False])
+def test_gradients_are_not_taken_for_constants(host_path, monkeypatch):
+    """A gradient of create_graph=True raises where it is differentiated, beside another term of the loss and for some inputs alone."""
+    from addernetcuda_b200 import _native
+    from addernetcuda_b200.logprobs import token_log_probs
+    if not host_path:
+        monkeypatch.setattr(_native, "log_probs", _native._absent)
+    x, t = _logits(6, 40, torch.float32)
+    for weights in (torch.ones(6, device=DEV), torch.ones(6, device=DEV, requires_grad=True)):
+        for part in ("log_prob", "entropy", "top_log_probs"):
+            leaf = x.detach().requires_grad_()
+            out = getattr(token_log_probs(leaf, t, top_k=3, entropy=True), part)
+            total = (out * weights.view([6] + [1] * (out.dim() - 1))).sum()
+            g, = torch.autograd.grad(total, leaf, create_graph=True)
+            again = getattr(token_log_probs(leaf, t, top_k=3, entropy=True), part)
+            assert torch.equal(g.detach(), torch.autograd.grad(again.sum(), leaf)[0])
+            with pytest.raises(RuntimeError, match="differentiable once"):
+                (total + g.square().sum()).backward(retain_graph=True)
+            with pytest.raises(RuntimeError, match="differentiable once"):
+                torch.autograd.grad(total + g.square().sum(), leaf, retain_graph=True)
+            if weights.requires_grad:
+                with pytest.raises(RuntimeError, match="differentiable once"):
+                    torch.autograd.grad(g.square().sum(), weights)
