@@ -317,10 +317,11 @@ template <class S> __device__ __forceinline__ float2 ln_moments(const LnPairs<S>
     return make_float2(mean, sq);
 }
 
-// 1 / sqrt(x), the approximate one and a step of Newton's method.
+// 1 / sqrt(x), the approximate one and a step of Newton's method; 0 for a variance beyond the range and infinity for 0, which the step
+// would turn into NaN.
 __device__ __forceinline__ float inverse_root(float x) {
     const float r = rsqrtf(x);
-    return r * fmaf(-0.5f * x * r, r, 1.5f);
+    return r > 0.f && r < INFINITY ? r * fmaf(-0.5f * (x * r), r, 1.5f) : r;
 }
 
 // h = x + residual, rounded to what is stored: the norm is taken of that.

@@ -409,3 +409,19 @@ def test_gradients_are_not_taken_for_constants(host_path, residual, monkeypatch)
     total, (g,) = call(only_b, dy, [only_b[3]])
     (total + g.square().sum()).backward()
     assert torch.equal(only_b[3].grad, g.detach())
+
+
+@pytest.mark.parametrize("rows,width", [(3, 16), (3, 33), (3, 600), (3, 1001), (3, 2048), (3, 5000), (3, 20000), (300, 20000), (3, 20001), (3, 70000)])
+def test_variances_beyond_the_range_and_of_zero(rows, width):
+    """1 / sqrt(infinity) is 0: the norm of such a row is the bias, and no gradient goes through it.  1 / sqrt(0) is infinite."""
+    for dtype in (torch.float32, torch.bfloat16):
+        x, _, w, b, dy, _ = _inputs(rows, (width,), dtype, dtype, False)
+        sign = 1.0 - 2.0 * (torch.arange(width, device=DEV) % 2)
+        outs, grads = _run((3e19 * sign).expand(rows, width).to(dtype).contiguous(), None, w, b, dy, None)
+        assert torch.equal(outs[0], b.expand(rows, width))
+        assert not bool(grads[0].any()) and not bool(grads[1].any())
+        outs, _ = _run(x, None, w, b, dy, None, eps=float("inf"))
+        assert torch.equal(outs[0], b.expand(rows, width))
+        if width % 2 == 0:      # the mean is 0 in any order of addition, the squares are below the smallest number
+            outs, _ = _run((1e-30 * sign).expand(rows, width).to(dtype).contiguous(), None, w.abs(), None, dy, None, eps=0.0)
+            assert torch.equal(outs[0].float(), (sign * float("inf")).expand(rows, width))
