@@ -90,7 +90,7 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
     [n, 2], or n int32 tensors of two elements: the steps that each parameter has taken, counted up by the call, and a word that is 0
     between calls.  States are float32 with the strides of their parameters, or, where scales are given, uint8 codes with
     `scale_count(numel)` float32 scales (zeros of both are a state of zeros).  `lr` and `grad_scale` may be float32 CUDA tensors of
-    one element, read when the kernel runs.  No two of the tensors that are written may share memory: tensors that
+    one element, read when the kernel runs.  `eps` is 0 or at least 2^-126.  No two of the tensors that are written may share memory: tensors that
     start at the same address are refused, other overlaps are not looked for.  The whole step runs on the current stream."""
     if _native.adamw(params, grads, exp_avgs, exp_avg_sqs, steps, lr, betas[0], betas[1], eps, weight_decay, exp_avg_scales,
                      exp_avg_sq_scales, grad_scale):
@@ -191,7 +191,7 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f"invalid learning rate: {lr}")
         if not all(0.0 <= b < 1.0 for b in betas):
             raise ValueError(f"invalid betas: {betas}")
-        if not eps >= 0.0 or not weight_decay >= 0.0:
+        if not (eps == 0.0 or eps >= 2.0 ** -126) or not weight_decay >= 0.0:
             raise ValueError(f"invalid eps or weight_decay: {eps}, {weight_decay}")
         if state_bits not in (8, 32):
             raise ValueError(f"state_bits must be 8 or 32, got {state_bits}")

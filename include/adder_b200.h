@@ -302,7 +302,8 @@ typedef struct {
  *   g <- grad * grad_scale;  m <- beta1 m + (1 - beta1) g;  v <- beta2 v + (1 - beta2) g^2
  *   p <- p (1 - lr weight_decay) - lr / (1 - beta1^t) * m / (sqrt(v / (1 - beta2^t)) + eps)
  * lr_device and grad_scale, where not NULL, are one fp32 value each in device memory that is read when the kernel runs (lr then being
- * ignored), so that a captured step follows a schedule.  state_bits is 32 or 8.
+ * ignored), so that a captured step follows a schedule.  state_bits is 32 or 8.  eps is 0 or at least 2^-126; with 0 an element whose v
+ * is 0 is divided by 0.
  * 8-bit states: a block of 256 values is stored relative to its largest magnitude, which has the top code.  The code of a magnitude a is
  * bits 19 and up of the fp32 number a * (1 / largest * top) * 2^-127, rounded to nearest even, and its block's scale is
  * largest * (1 / top), every operation rounded to fp32: m has a sign and 3 exponent and 4 fraction bits (top = 248, codes 0-127, +128

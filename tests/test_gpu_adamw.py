@@ -478,3 +478,53 @@ def test_closure_and_missing_gradients():
 
     first = opt.step(closure)
     assert float(opt.step(closure)) < float(first)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("eps", [0.0, 1e-30])
+def test_second_moments_below_the_normal_range(dtype, eps):
+    """Gradients of 1e-20 to 1e-18 leave second moments of 2^-138 to 2^-124: the update by their root is as large as any other."""
+    from addernetcuda_b200.optim import adamw_step
+    b1, b2 = HYPER["betas"]
+    hyper = {**HYPER, "eps": eps, "weight_decay": 0.0}
+    gen = torch.Generator(device=DEV)
+    gen.manual_seed(3)
+    sizes = [5, 2048, 2051, 5000]
+    rnd = lambda n: torch.rand(n, device=DEV, generator=gen)      # noqa: E731
+    p = [(rnd(n) + 0.5).to(dtype) for n in sizes]
+    g = [(10.0 ** (-20 + 2 * rnd(n)) * (1 - 2 * (rnd(n) < 0.5).float())).to(dtype) for n in sizes]
+    m, v = ([torch.zeros(n, device=DEV) for n in sizes] for _ in range(2))
+    steps = torch.zeros(len(sizes), 2, dtype=torch.int32, device=DEV)
+    for t in (1, 2, 3):
+        before = _copies(p, m, v)
+        adamw_step(p, g, m, v, steps, **hyper)
+        for i, (p0, m0, v0) in enumerate(zip(*before)):
+            m1, v1 = moments(g[i].float(), m0, v0, b1, b2)
+            assert torch.equal(m[i], m1) and torch.equal(v[i], v1) and bool((v1 > 0).all())
+            p1 = update64(p0, m1, v1, t, hyper["lr"], b1, b2, eps, 0.0)
+            size = hyper["lr"] / (1 - b1 ** t) * m1.double().abs() / ((v1.double() / (1 - b2 ** t)).sqrt() + eps)
+            assert float(size.max()) > 0.5 * hyper["lr"]
+            _near(f"p[{i}]", p[i], p1, U[dtype] * p1.abs() * (1 + 2.0 ** -8) + 32 * 2.0 ** -24 * size + 4 * 2.0 ** -24 * p1.abs())
+    for a in m + g:      # a first moment of 0 moves nothing
+        a.zero_()
+    before = _copies(p)
+    adamw_step(p, g, m, v, steps, **hyper)
+    assert all(torch.equal(a, b) for a, b in zip(p, before[0]))
+
+
+def test_second_moments_below_the_normal_range_before_8_bit_states_are_stored():
+    """The update uses v as it is before it is stored.  8-bit steps have two kernels by eps: both sides of the rule."""
+    from addernetcuda_b200.optim import adamw_step
+    n, (b1, b2) = 256 * 9 + 5, HYPER["betas"]
+    gen = torch.Generator(device=DEV)
+    gen.manual_seed(4)
+    border = 2.0 ** -39 / (1 - b2) ** 0.5
+    for exponent, eps in ((-20, 0.0), (-20, 1e-30), (-12, 0.99 * border), (-12, border * (1 + 1e-6)), (-20, border * (1 + 1e-6))):
+        g = 10.0 ** (exponent + 2 * torch.rand(n, device=DEV, generator=gen))
+        p, m, v = torch.ones(n, device=DEV), torch.zeros(n, dtype=torch.uint8, device=DEV), torch.zeros(n, dtype=torch.uint8, device=DEV)
+        sm, sv, steps = torch.zeros(10, device=DEV), torch.zeros(10, device=DEV), torch.zeros(1, 2, dtype=torch.int32, device=DEV)
+        adamw_step([p], [g], [m], [v], steps, exp_avg_scales=[sm], exp_avg_sq_scales=[sv], **{**HYPER, "eps": eps, "weight_decay": 0.0})
+        m1, v1 = moments(g, torch.zeros(n, device=DEV), torch.zeros(n, device=DEV), b1, b2)
+        p1 = update64(torch.ones(n, device=DEV), m1, v1, 1, HYPER["lr"], b1, b2, eps, 0.0)
+        size = HYPER["lr"] / (1 - b1) * m1.double() / ((v1.double() / (1 - b2)).sqrt() + eps)
+        _near(f"p, eps {eps}", p, p1, (1 + 4) * 2.0 ** -24 * p1.abs() + 32 * 2.0 ** -24 * size)

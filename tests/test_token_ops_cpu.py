@@ -150,3 +150,15 @@ def test_codes_are_the_nearest_of_the_numbers_that_they_stand_for(signed, codes)
     assert np.array_equal(chosen[~small], best[~small])
     tie = (dist == best[:, None]).sum(1) == 2
     assert tie.sum() >= 10 and np.all(c[tie & ~small] % 2 == 0)
+
+
+def test_an_eps_below_the_normal_numbers_is_refused():
+    """Its reciprocal, where the second moment is 0, is beyond the range."""
+    from addernetcuda_b200.optim import AdamW, _Tensor
+    lib = _lib()
+    call = lambda eps: lib.adder_b200_adamw_step((_Tensor * 1)(_Tensor(P, P, P, P, None, None, P, 0)), 1, 0, 32, 1e-3, None, 0.9, 0.99, eps, 0.0, None, None)      # noqa: E731
+    assert call(1e-40) == call(2.0 ** -127) == call(1e-300) == 2 and call(0.0) == call(2.0 ** -126) == 0
+    p = [torch.nn.Parameter(torch.zeros(3))]
+    with pytest.raises(ValueError, match="eps"):
+        AdamW(p, eps=1e-40)
+    AdamW(p, eps=0.0), AdamW(p, eps=2.0 ** -126)
