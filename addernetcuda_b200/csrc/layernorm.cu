@@ -974,10 +974,12 @@ template <class S> int launch_backward(const LnBwd& a, float* part, bool sums, i
     }
 }
 
+constexpr int LN_HELD = 8192;      // columns up to which the backward pass keeps its sums of dw and db from row to row
+
 // Rows beyond 8192 of whole vectors go through shared memory where there are rows for all SMs and two of them fit (2000x20000 bf16: forward 46
 // us, backward 105; by clusters 73 and 123); `bytes`: of a row in all arrays that are held.  0: they do not.
 size_t wide_bytes(const void* kernel, long long rows, int d, int vec, int ve, size_t bytes) {
-    if (d <= 8192 || vec != ve || rows < sm_count()) return 0;
+    if (d <= LN_HELD || vec != ve || rows < sm_count()) return 0;
     return ensure_dynamic_smem(kernel, 2 * bytes) == ADDER_OK ? 2 * bytes : 0;
 }
 
@@ -992,7 +994,7 @@ template <class T, class W, int THREADS, class F> bool with_shape(int d, int vec
             if (d <= 128) return f(LnShape<T, W, 32, V, 4 / V, 0, false, 512>(), 1);
             if (d <= 512) return f(LnShape<T, W, 32, V, 16 / V, 0, false, 512>(), 1);
             if (d <= 2048) return f(LnShape<T, W, 128, V, 16 / V, 0, false, 512>(), 1);
-            if (d <= 8192) return f(LnShape<T, W, 512, V, 16 / V, 0, false, 512>(), 1);
+            if (d <= LN_HELD) return f(LnShape<T, W, 512, V, 16 / V, 0, false, 512>(), 1);
         }
         if (d <= 128) f(LnShape<T, W, 32, V, 4 / V, 0, false>(), 1);
         else if (d <= 512) f(LnShape<T, W, 32, V, 16 / V, 0, false>(), 1);
@@ -1008,7 +1010,7 @@ template <class T, class W, int THREADS, class F> bool with_shape(int d, int vec
         else if (d <= 1024) f(LnShape<T, W, 64, VE, NV, STAGES, false, THREADS>(), 1);
         else if (d <= 2048) f(LnShape<T, W, 128, VE, NV, STAGES, false, THREADS>(), 1);
         else if (d <= 4096) f(LnShape<T, W, 256, VE, NV, STAGES, false, THREADS>(), 1);
-        else if (d <= 8192) f(LnShape<T, W, 512, VE, NV, 2, false, THREADS>(), 1);
+        else if (d <= LN_HELD) f(LnShape<T, W, 512, VE, NV, 2, false, THREADS>(), 1);
         else if (d <= 8 * 4096) f(LnShape<T, W, 256, VE, 16 / VE, 0, true>(), (d / VE + 256 * (16 / VE) - 1) / (256 * (16 / VE)));
         else f(LnShape<T, W, 256, VE, 32 / VE, 0, true>(), (d / VE + 256 * (32 / VE) - 1) / (256 * (32 / VE)));
     } else if (vec == 2) {
@@ -1089,7 +1091,10 @@ int adder_b200_layernorm_forward(const void* x, const void* residual, const void
 
 size_t adder_b200_layernorm_backward_workspace_bytes(long long rows, long long d) {
     if (rows <= 0 || d <= 0 || d > LN_MOST) return 0;
-    return (size_t)std::max(ln_splits(rows, (int)d, 8), ln_most_parts(rows)) * 2 * d * sizeof(float);
+    // Up to LN_HELD columns the CTAs that stay write a part each; beyond, the splits of the pass over the columns do, which are most for
+    // the widest vectors.
+    const int parts = d <= LN_HELD ? ln_most_parts(rows) : ln_splits(rows, (int)d, 8);
+    return (size_t)parts * 2 * d * sizeof(float);
 }
 
 int adder_b200_layernorm_backward(const void* dy, const void* dh, const void* h, const void* weight, const float* mean, const float* rstd,

@@ -162,3 +162,14 @@ def test_an_eps_below_the_normal_numbers_is_refused():
     with pytest.raises(ValueError, match="eps"):
         AdamW(p, eps=1e-40)
     AdamW(p, eps=0.0), AdamW(p, eps=2.0 ** -126)
+
+
+def test_the_workspace_of_layer_norm_is_what_its_kernels_write():
+    """Rows beyond 8192 elements: sums of the splits of the rows, a small part of the input; shorter ones: sums of every CTA that stays."""
+    size = _lib().adder_b200_layernorm_backward_workspace_bytes
+    pair = lambda d: 2 * d * 4      # noqa: E731
+    assert size(592, 1 << 20) == pair(1 << 20)
+    for rows, d in ((64, 50176), (1000, 60000), (600, 1000000), (4096, 8193), (10 ** 6, 16384)):
+        assert pair(d) <= size(rows, d) <= max(pair(d), rows * d // 4) and size(rows, d) <= 512 * pair(d)
+        assert size(rows, d) % pair(d) == 0 and size(rows, d) // pair(d) <= -(-rows // 32)
+    assert size(4, 8192) == 4 * pair(8192) and size(10 ** 6, 8192) >= 128 * pair(8192)
