@@ -477,7 +477,8 @@ struct LayerNorm : public torch::autograd::Function<LayerNorm> {
         const Variable &h = saved[0], &w = saved[1], &mean = saved[2], &rstd = saved[3];
         int64_t stride;
         TORCH_CHECK(unwrapped(h) && type_code(h) == type && h.numel() == rows * d && plain(mean) && plain(rstd) && mean.numel() == rows &&
-                    rstd.numel() == rows && (!w.defined() || (unwrapped(w) && w.is_contiguous() && type_code(w) == weight_type && w.numel() == d)), SAVED);
+                    rstd.numel() == rows && mean.device() == h.device() && rstd.device() == h.device(), SAVED);
+        TORCH_CHECK(!w.defined() || (unwrapped(w) && w.is_contiguous() && type_code(w) == weight_type && w.numel() == d && w.device() == h.device()), SAVED);
         const c10::cuda::CUDAGuard guard(h.device());
         at::Tensor h2 = h;      // rows of consecutive elements
         if (!rows_of(h, 1, d, &stride) || h.dim() == 0 || h.size(-1) != d) {
@@ -577,10 +578,12 @@ struct LogProbsNode : public torch::autograd::Function<LogProbsNode> {
         const auto saved = ctx->get_saved_variables();
         const Variable &x = saved[0], &targets = saved[1], &stats = saved[2], &entropy = saved[3], &indices = saved[4];
         TORCH_CHECK(unwrapped(x) && type_code(x) == type && x.dim() >= 1 && x.size(-1) == classes && x.numel() == rows * classes && plain(stats) &&
-                    stats.numel() == 2 * rows && (!a[6] || (plain(entropy) && entropy.numel() == rows)), SAVED);
-        TORCH_CHECK((!a[5] || (unwrapped(targets) && targets.scalar_type() == at::kLong && targets.is_contiguous() && targets.numel() == rows)) &&
-                    (top_k == 0 || (unwrapped(indices) && indices.scalar_type() == at::kLong && indices.is_contiguous() &&
-                                    indices.numel() == rows * top_k)), SAVED);
+                    stats.numel() == 2 * rows && stats.device() == x.device() &&
+                    (!a[6] || (plain(entropy) && entropy.numel() == rows && entropy.device() == x.device())), SAVED);
+        const auto whole = [&](const Variable& t, int64_t count) {
+            return unwrapped(t) && t.scalar_type() == at::kLong && t.is_contiguous() && t.numel() == count && t.device() == x.device();
+        };
+        TORCH_CHECK((!a[5] || whole(targets, rows)) && (top_k == 0 || whole(indices, rows * top_k)), SAVED);
         const c10::cuda::CUDAGuard guard(x.device());
         for (at::Tensor* g : {&g_lp, &g_ent, &g_top})
             if (g->defined()) {

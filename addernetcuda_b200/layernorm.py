@@ -33,6 +33,24 @@ def _ptr(t: Optional[torch.Tensor]):
     return None if t is None else t.data_ptr()
 
 
+def _form(t: Optional[torch.Tensor]):
+    return None if t is None else (t.shape, t.dtype, t.device)
+
+
+def _save(ctx, *tensors) -> None:
+    ctx.forms = tuple(_form(t) for t in tensors)
+    ctx.save_for_backward(*tensors)
+
+
+def _saved(ctx):
+    """The saved tensors.  What a saved-tensor hook hands back need not be what it was given, and the kernels go by the sizes of the
+    forward call."""
+    tensors = ctx.saved_tensors
+    if tuple(_form(t) for t in tensors) != ctx.forms:
+        raise RuntimeError("the saved tensors came back in another form: the shapes, types and device of the forward are needed")
+    return tensors
+
+
 def _sizes(x: torch.Tensor, normalized_shape) -> Tuple[int, int]:
     d = math.prod(normalized_shape)
     return (x.numel() // d if d else 0), d
@@ -84,7 +102,7 @@ class _LayerNorm(torch.autograd.Function):
         ctx.bias_type = bias.dtype if bias is not None else None
         ctx.set_materialize_grads(False)
         if needs_grad:
-            ctx.save_for_backward(h if residual is not None else x, w, mean, rstd)
+            _save(ctx, h if residual is not None else x, w, mean, rstd)
         if residual is None:
             return y
         return y, h
@@ -93,7 +111,7 @@ class _LayerNorm(torch.autograd.Function):
     def backward(ctx, dy, dh=None):
         if dy is None and dh is None:
             return (None,) * 7
-        saved = ctx.saved_tensors
+        saved = _saved(ctx)
         with torch.no_grad():
             dx, dw, db = _LayerNorm.gradients(ctx, saved, dy, dh)
         need_x, need_r = ctx.needs_input_grad[0], ctx.has_residual and ctx.needs_input_grad[1]
@@ -104,7 +122,7 @@ class _LayerNorm(torch.autograd.Function):
 
     @staticmethod
     def gradients(ctx, saved, dy, dh):
-        h, w, mean, rstd = saved
+        h, (w, mean, rstd) = saved[0], (t.contiguous() if t is not None else None for t in saved[1:])
         rows, d, wcode = ctx.sizes
         need_x = ctx.needs_input_grad[0] or (ctx.has_residual and ctx.needs_input_grad[1])
         dw = torch.empty(w.shape, dtype=w.dtype, device=w.device) if w is not None and ctx.needs_input_grad[2] else None

@@ -13,7 +13,7 @@ import torch
 import torch.nn as nn
 
 from . import _lib, _native, adder_cuda
-from .layernorm import _check_input, _once, _ptr, _rows
+from .layernorm import _check_input, _once, _ptr, _rows, _save, _saved
 
 MAX_TOP_K = 32
 
@@ -50,7 +50,7 @@ class _LogProbs(torch.autograd.Function):
         ctx.args = (top_k, ignore_index)
         ctx.set_materialize_grads(False)
         if needs_grad:
-            ctx.save_for_backward(logits, targets, stats, ent, idx)
+            _save(ctx, logits, targets, stats, ent, idx)
         if idx is not None:
             ctx.mark_non_differentiable(idx)
         return lp, ent, top, idx
@@ -59,14 +59,14 @@ class _LogProbs(torch.autograd.Function):
     def backward(ctx, g_lp, g_ent, g_top, _):
         if g_lp is None and g_ent is None and g_top is None:
             return (None,) * 6
-        saved = ctx.saved_tensors
+        saved = _saved(ctx)
         with torch.no_grad():
             dx = _LogProbs.gradient(ctx, saved, g_lp, g_ent, g_top)
         return _once("token_log_probs", dx, saved[0], g_lp, g_ent, g_top), None, None, None, None, None
 
     @staticmethod
     def gradient(ctx, saved, g_lp, g_ent, g_top):
-        logits, targets, stats, ent, idx = saved
+        logits, (targets, stats, ent, idx) = saved[0], (t.contiguous() if t is not None else None for t in saved[1:])
         top_k, ignore_index = ctx.args
         v = logits.shape[-1]
         rows = logits.numel() // v

@@ -425,3 +425,36 @@ def test_variances_beyond_the_range_and_of_zero(rows, width):
         if width % 2 == 0:      # the mean is 0 in any order of addition, the squares are below the smallest number
             outs, _ = _run((1e-30 * sign).expand(rows, width).to(dtype).contiguous(), None, w.abs(), None, dy, None, eps=0.0)
             assert torch.equal(outs[0].float(), (sign * float("inf")).expand(rows, width))
+
+def _altered(number, change):
+    """Saved-tensor hooks that hand back `change` of the tensor that is saved as the `number`-th."""
+    saved = []
+
+    def pack(t):
+        saved.append(t)
+        return len(saved) - 1, t
+    return torch.autograd.graph.saved_tensors_hooks(pack, lambda kept: change(kept[1]) if kept[0] == number else kept[1])
+
+
+ALTERED = [lambda t: t.to(torch.float16 if t.is_floating_point() else torch.int32), lambda t: t.reshape(-1)[:-1], lambda t: t.cpu()]
+
+
+@pytest.mark.parametrize("host_path", [True, False])
+@pytest.mark.parametrize("residual", [False, True])
+def test_saved_tensors_that_come_back_in_another_form_are_refused(host_path, residual, monkeypatch):
+    from addernetcuda_b200 import _native
+    from addernetcuda_b200.layernorm import layer_norm
+    if not host_path:
+        monkeypatch.setattr(_native, "layer_norm", _native._absent)
+    x, r, w, b, dy, dh = _inputs(6, (40,), torch.float32, torch.float32, residual)
+    _, want = _run(x, r, w, b, dy, dh)
+    for number in range(4):
+        with _altered(number, lambda t: t.clone()):
+            _, got = _run(x, r, w, b, dy, dh)
+        assert all(torch.equal(p, q) for p, q in zip(got, want))
+        for change in ALTERED:
+            leaf = x.detach().requires_grad_()
+            with _altered(number, change):
+                out = layer_norm(leaf, 40, w, b, residual=r)
+            with pytest.raises(RuntimeError, match="saved tensors"):
+                torch.autograd.grad(out[0] if residual else out, leaf, dy)

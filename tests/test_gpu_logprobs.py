@@ -392,3 +392,37 @@ def test_gradients_are_not_taken_for_constants(host_path, monkeypatch):
             if weights.requires_grad:
                 with pytest.raises(RuntimeError, match="differentiable once"):
                     torch.autograd.grad(g.square().sum(), weights)
+
+def _altered(number, change):
+    """Saved-tensor hooks that hand back `change` of the tensor that is saved as the `number`-th."""
+    saved = []
+
+    def pack(t):
+        saved.append(t)
+        return len(saved) - 1, t
+    return torch.autograd.graph.saved_tensors_hooks(pack, lambda kept: change(kept[1]) if kept[0] == number else kept[1])
+
+
+ALTERED = [lambda t: t.to(torch.float16 if t.is_floating_point() else torch.int32), lambda t: t.reshape(-1)[:-1], lambda t: t.cpu()]
+
+
+@pytest.mark.parametrize("host_path", [True, False])
+def test_saved_tensors_that_come_back_in_another_form_are_refused(host_path, monkeypatch):
+    from addernetcuda_b200 import _native
+    from addernetcuda_b200.logprobs import token_log_probs
+    if not host_path:
+        monkeypatch.setattr(_native, "log_probs", _native._absent)
+    x, t = _logits(6, 40, torch.float32)
+
+    def run(hooks):
+        leaf = x.detach().requires_grad_()
+        with hooks:
+            r = token_log_probs(leaf, t, top_k=3, entropy=True)
+        return torch.autograd.grad(r.log_prob.sum() + r.entropy.sum() + r.top_log_probs.sum(), leaf)[0]
+
+    want = run(_altered(-1, None))
+    for number in range(5):
+        assert torch.equal(run(_altered(number, lambda s: s.clone())), want)
+        for change in ALTERED:
+            with pytest.raises(RuntimeError, match="saved tensors"):
+                run(_altered(number, change))
