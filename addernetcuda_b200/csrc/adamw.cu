@@ -464,6 +464,7 @@ int adder_b200_adamw_step(const adder_b200_adamw_tensor* tensors, int count, int
     if (state_bits != 32 && state_bits != 8) return ADDER_ERR_UNSUPPORTED;
     if (count == 0) return ADDER_OK;
     if (tensors == nullptr) return ADDER_ERR_NULL_POINTER;
+    if (!aligned_to(lr_device, 4) || !aligned_to(grad_scale, 4)) return ADDER_ERR_ALIGNMENT;
     const unsigned size = dtype == ADDER_TYPE_F32 ? 4 : 2;
     long long elements = 0;
     for (int i = 0; i < count; ++i) {

@@ -952,7 +952,9 @@ int adder_b200_log_probs_forward(const void* logits, int dtype, long long rows, 
     if (dtype < ADDER_TYPE_F32 || dtype > ADDER_TYPE_F16) return ADDER_ERR_UNSUPPORTED;
     if (rows == 0) return ADDER_OK;
     if (!logits || (log_prob && !targets) || (top_k > 0 && (!top_log_probs || !top_indices))) return ADDER_ERR_NULL_POINTER;
-    if (!aligned_to(logits, dtype == ADDER_TYPE_F32 ? 4 : 2) || !aligned_to(stats, 8)) return ADDER_ERR_ALIGNMENT;
+    if (!aligned_to(logits, dtype == ADDER_TYPE_F32 ? 4 : 2) || !aligned_to(targets, 8) || !aligned_to(top_indices, 8) || !aligned_to(stats, 8) ||
+        !aligned_to(log_prob, 4) || !aligned_to(entropy, 4) || !aligned_to(top_log_probs, 4))
+        return ADDER_ERR_ALIGNMENT;
     const LpFwd a{logits, rows, row_stride, (int)classes, top_k, targets, ignore_index, log_prob, entropy, stats, top_log_probs, top_indices};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     return with_type(dtype, [&](auto* type) {
@@ -979,7 +981,9 @@ int adder_b200_log_probs_backward(const void* logits, int dtype, long long rows,
         (grad_top && (top_k == 0 || !top_indices)))
         return ADDER_ERR_NULL_POINTER;
     const unsigned size = dtype == ADDER_TYPE_F32 ? 4 : 2;
-    if (!aligned_to(logits, size) || !aligned_to(grad_logits, size)) return ADDER_ERR_ALIGNMENT;
+    if (!aligned_to(logits, size) || !aligned_to(grad_logits, size) || !aligned_to(targets, 8) || !aligned_to(top_indices, 8) || !aligned_to(stats, 4) ||
+        !aligned_to(entropy, 4) || !aligned_to(grad_log_prob, 4) || !aligned_to(grad_entropy, 4) || !aligned_to(grad_top, 4))
+        return ADDER_ERR_ALIGNMENT;
     const bool warps = warp_rows(rows, classes);
     // A CTA takes two turns, whose loads and stores overlap (2048x128000 bf16 with an entropy 187 us with one, 161 with two, 164 with three), or
     // one where there would be too few CTAs.

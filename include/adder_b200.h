@@ -264,7 +264,7 @@ ADDER_API int adder_b200_layernorm_backward(const void* dy, const void* dh, cons
                                             int weight_dtype, void* stream);
 
 /* Of each row of logits (rows x classes of type dtype, row_stride elements from row to row, consecutive within one; any alignment
- * that the type needs), in fp32:
+ * that the type needs; stats is 8-byte aligned), in fp32:
  *   log_prob[row]  log softmax at targets[row]: 0 where the target is ignore_index, NaN where it is no class
  *   entropy[row]   -sum p log p
  *   top_log_probs, top_indices [row][top_k]  the top_k <= 32 largest, equal logits by index from the lowest

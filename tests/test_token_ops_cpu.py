@@ -173,3 +173,18 @@ def test_the_workspace_of_layer_norm_is_what_its_kernels_write():
         assert pair(d) <= size(rows, d) <= max(pair(d), rows * d // 4) and size(rows, d) <= 512 * pair(d)
         assert size(rows, d) % pair(d) == 0 and size(rows, d) // pair(d) <= -(-rows // 32)
     assert size(4, 8192) == 4 * pair(8192) and size(10 ** 6, 8192) >= 128 * pair(8192)
+
+
+def test_addresses_that_a_type_does_not_allow_are_refused():
+    """Targets, outputs, gradients and device scalars: a kernel that follows such an address faults."""
+    from addernetcuda_b200.optim import _Tensor
+    lib = _lib()
+    forward = dict(x=P, t=0, rows=2, classes=8, stride=8, targets=P, ignore=-100, k=2, lp=P, ent=P, stats=P, top=P, idx=P, s=None)
+    for name, by in (("targets", 4), ("lp", 2), ("ent", 2), ("stats", 4), ("top", 2), ("idx", 4)):
+        assert lib.adder_b200_log_probs_forward(*{**forward, name: P + by}.values()) == 4, name
+    backward = dict(x=P, t=0, rows=2, classes=8, stride=8, targets=P, ignore=-100, k=2, idx=P, stats=P, ent=P, g=P, ge=P, gt=P, dx=P, s=None)
+    for name, by in (("targets", 4), ("idx", 4), ("stats", 2), ("ent", 2), ("g", 2), ("ge", 2), ("gt", 2)):
+        assert lib.adder_b200_log_probs_backward(*{**backward, name: P + by}.values()) == 4, name
+    one = (_Tensor * 1)(_Tensor(P, P, P, P, None, None, P, 8))
+    for lr, scale in ((P + 2, None), (None, P + 1)):
+        assert lib.adder_b200_adamw_step(one, 1, 0, 32, 1e-3, lr, 0.9, 0.99, 1e-8, 0.0, scale, None) == 4
