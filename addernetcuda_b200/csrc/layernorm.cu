@@ -425,50 +425,46 @@ template <class S> __global__ void __launch_bounds__(S::THREADS, S::NV * S::VEC 
     }
 }
 
+// dx of rows that a cluster shares, a row each.
 template <class S> __global__ void __launch_bounds__(S::THREADS, S::NV * S::VEC > 16 ? 2 : 3) ln_dx_row_kernel(const LnBwd a) {
+    static_assert(S::CLUSTER && S::TEAMS == 1, "shorter rows go by CTAs that stay");
     __shared__ LnSums<S> sh;
-    cluster_arrive<S::CLUSTER>();
+    cluster_arrive<true>();
     using T = typename S::T;
-    const int t = threadIdx.x % S::G, team = threadIdx.x / S::G;
-    const int2 share = share_of<S::CLUSTER>(a.d / S::VEC);
+    const int t = threadIdx.x;
+    const int2 share = share_of<true>(a.d / S::VEC);
     const int v = share.x + t, v1 = share.y;
     const float inv_d = 1.f / a.d;
-    const long long parts = S::CLUSTER ? (long long)cg::this_cluster().num_blocks() : 1;
-    const long long row = blockIdx.x / parts * S::TEAMS + team;
+    const long long row = blockIdx.x / cg::this_cluster().num_blocks();
     LnPairs<S> xh, g, w;
-    float mean = 0.f, rs = 0.f;
-    if (row < a.rows) {
-        mean = a.mean[row]; rs = a.rstd[row];
-        ln_fetch<S>(xh, 0, static_cast<const T*>(a.h) + row * a.h_stride, v, v1);
-        ln_fetch<S>(g, 0, static_cast<const T*>(a.dy) + row * a.d, v, v1);
+    const float mean = a.mean[row], rs = a.rstd[row];
+    ln_fetch<S>(xh, 0, static_cast<const T*>(a.h) + row * a.h_stride, v, v1);
+    ln_fetch<S>(g, 0, static_cast<const T*>(a.dy) + row * a.d, v, v1);
+    cluster_wait<true>();
+    ln_weights<S>(w, a.w, 1.f, v, v1);
+    uint64_t s1 = 0, s2 = 0;
+    const uint64_t minus = pack2(-mean, -mean), scale = pack2(rs, rs);
+#pragma unroll
+    for (int i = 0; i < LnPairs<S>::P; ++i) {      // dy is 0 where there is no element
+        xh.p[i] = mul2(add2(xh.p[i], minus), scale);
+        g.p[i] = mul2(g.p[i], w.p[i]);
+        s1 = add2(s1, g.p[i]);
+        s2 = fma2(g.p[i], xh.p[i], s2);
     }
-    cluster_wait<S::CLUSTER>();
-    if (row < a.rows) {
-        ln_weights<S>(w, a.w, 1.f, v, v1);
-        uint64_t s1 = 0, s2 = 0;
-        const uint64_t minus = pack2(-mean, -mean), scale = pack2(rs, rs);
+    float a1, b1, a2, b2;
+    unpack2(s1, a1, b1);
+    unpack2(s2, a2, b2);
+    const float2 m = ln_sum2<S>(a1 + b1, a2 + b2, sh, 0, t, 0);
+    const float c1 = -m.x * inv_d, c2 = -m.y * inv_d;
+    const uint64_t shift = pack2(c1, c1), slope = pack2(c2, c2);
 #pragma unroll
-        for (int i = 0; i < LnPairs<S>::P; ++i) {      // dy is 0 where there is no element
-            xh.p[i] = mul2(add2(xh.p[i], minus), scale);
-            g.p[i] = mul2(g.p[i], w.p[i]);
-            s1 = add2(s1, g.p[i]);
-            s2 = fma2(g.p[i], xh.p[i], s2);
-        }
-        float a1, b1, a2, b2;
-        unpack2(s1, a1, b1);
-        unpack2(s2, a2, b2);
-        const float2 m = ln_sum2<S>(a1 + b1, a2 + b2, sh, team, t, 0);
-        const float c1 = -m.x * inv_d, c2 = -m.y * inv_d;
-        const uint64_t shift = pack2(c1, c1), slope = pack2(c2, c2);
+    for (int i = 0; i < LnPairs<S>::P; ++i) g.p[i] = mul2(fma2(xh.p[i], slope, add2(g.p[i], shift)), scale);
+    if (a.dh != nullptr) {
+        ln_fetch<S>(w, 0, static_cast<const T*>(a.dh) + row * a.d, v, v1);
 #pragma unroll
-        for (int i = 0; i < LnPairs<S>::P; ++i) g.p[i] = mul2(fma2(xh.p[i], slope, add2(g.p[i], shift)), scale);
-        if (a.dh != nullptr) {
-            ln_fetch<S>(w, 0, static_cast<const T*>(a.dh) + row * a.d, v, v1);
-#pragma unroll
-            for (int i = 0; i < LnPairs<S>::P; ++i) g.p[i] = add2(g.p[i], w.p[i]);
-        }
-        ln_store<S>(static_cast<T*>(a.dx) + row * a.d, g, v, v1);
+        for (int i = 0; i < LnPairs<S>::P; ++i) g.p[i] = add2(g.p[i], w.p[i]);
     }
+    ln_store<S>(static_cast<T*>(a.dx) + row * a.d, g, v, v1);
 }
 
 // dx of every row; with SUMS this thread's columns of dw and db, added up over its rows and then over the CTA's teams into
@@ -967,7 +963,7 @@ template <class S> int launch_backward(const LnBwd& a, float* part, bool sums, i
         return sums ? launch_stay_backward<S, true>(a, part, groups, s) : launch_stay_backward<S, false>(a, part, groups, s);
     } else {
         if (a.dx != nullptr) {
-            const int st = launch_clusters(ln_dx_row_kernel<S>, (unsigned)((a.rows + S::TEAMS - 1) / S::TEAMS * parts), S::THREADS, 0, parts, s, a);
+            const int st = launch_clusters(ln_dx_row_kernel<S>, (unsigned)(a.rows * parts), S::THREADS, 0, parts, s, a);
             if (st != ADDER_OK) return st;
         }
         return sums ? launch_columns<typename S::T, S::VEC>(a, part, groups, s) : ADDER_OK;
@@ -995,13 +991,14 @@ template <class T, class W, int THREADS, class F> bool with_shape(int d, int vec
             if (d <= 512) return f(LnShape<T, W, 32, V, 16 / V, 0, false, 512>(), 1);
             if (d <= 2048) return f(LnShape<T, W, 128, V, 16 / V, 0, false, 512>(), 1);
             if (d <= LN_HELD) return f(LnShape<T, W, 512, V, 16 / V, 0, false, 512>(), 1);
+        } else {
+            if (d <= 128) return f(LnShape<T, W, 32, V, 4 / V, 0, false>(), 1);
+            if (d <= 512) return f(LnShape<T, W, 32, V, 16 / V, 0, false>(), 1);
+            if (d <= 2048) return f(LnShape<T, W, 128, V, 16 / V, 0, false>(), 1);
+            if (d <= 4096) return f(LnShape<T, W, 128, V, 32 / V, 0, false>(), 1);
+            if (d <= 8192) return f(LnShape<T, W, 256, V, 32 / V, 0, false>(), 1);
         }
-        if (d <= 128) f(LnShape<T, W, 32, V, 4 / V, 0, false>(), 1);
-        else if (d <= 512) f(LnShape<T, W, 32, V, 16 / V, 0, false>(), 1);
-        else if (d <= 2048) f(LnShape<T, W, 128, V, 16 / V, 0, false>(), 1);
-        else if (d <= 4096) f(LnShape<T, W, 128, V, 32 / V, 0, false>(), 1);
-        else if (d <= 8192) f(LnShape<T, W, 256, V, 32 / V, 0, false>(), 1);
-        else f(LnShape<T, W, 256, V, 32 / V, 0, true>(), (d / V + 256 * (32 / V) - 1) / (256 * (32 / V)));
+        f(LnShape<T, W, 256, V, 32 / V, 0, true>(), (d / V + 256 * (32 / V) - 1) / (256 * (32 / V)));
     };
     if (d > 8 * 8192) return false;
     if (vec == VE) {
