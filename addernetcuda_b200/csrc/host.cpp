@@ -422,6 +422,9 @@ bool norm_of(const at::Tensor& x, const at::Tensor* r, const at::Tensor* w, cons
     return true;
 }
 
+// A gradient as its memory stands: contiguous, and no lazy negation (which a view of a conjugate's imaginary part is).
+at::Tensor whole_gradient(const at::Tensor& g) { return (g.is_neg() ? g.resolve_neg() : g).contiguous(); }
+
 void* ptr(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
 struct NormResult { at::Tensor y, h, mean, rstd; };
@@ -486,8 +489,8 @@ struct LayerNorm : public torch::autograd::Function<LayerNorm> {
             stride = d;
         }
         if (!dy.defined()) dy = at::zeros_like(h, at::MemoryFormat::Contiguous);
-        dy = dy.contiguous();
-        if (dh.defined()) dh = dh.contiguous();
+        dy = whole_gradient(dy);
+        if (dh.defined()) dh = whole_gradient(dh);
         for (const at::Tensor* g : {&dy, &dh})
             TORCH_CHECK(!g->defined() || (g->scalar_type() == h.scalar_type() && g->device() == h.device() && g->sizes() == h.sizes()),
                         "the gradient must have the type, device and shape of the output");
@@ -587,7 +590,7 @@ struct LogProbsNode : public torch::autograd::Function<LogProbsNode> {
         const c10::cuda::CUDAGuard guard(x.device());
         for (at::Tensor* g : {&g_lp, &g_ent, &g_top})
             if (g->defined()) {
-                *g = g->contiguous();
+                *g = whole_gradient(*g);
                 TORCH_CHECK(g->scalar_type() == at::kFloat && g->device() == x.device() && g->numel() == (g == &g_top ? rows * top_k : rows),
                             "the gradient must be a float32 tensor of the output's shape and device");
             }

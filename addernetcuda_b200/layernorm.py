@@ -18,6 +18,7 @@ from . import _lib, _native, adder_cuda
 
 def _rows(t: torch.Tensor, rows: int, d: int):
     """(tensor, elements from row to row) of t as `rows` rows of d consecutive elements; a copy only where it is no such view."""
+    t = t.resolve_neg()
     if t.is_contiguous():
         return t, d
     try:
@@ -27,6 +28,11 @@ def _rows(t: torch.Tensor, rows: int, d: int):
     if d > 1 and v.stride(1) != 1:
         return t.contiguous(), d
     return v, v.stride(0)
+
+
+def _whole(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    """t as its memory stands: contiguous, and no lazy negation (which a view of a conjugate's imaginary part is)."""
+    return None if t is None else t.resolve_neg().contiguous()
 
 
 def _ptr(t: Optional[torch.Tensor]):
@@ -89,8 +95,7 @@ class _LayerNorm(torch.autograd.Function):
         h = torch.empty_like(y) if residual is not None else None
         mean = torch.empty(rows, device=dev) if needs_grad else None
         rstd = torch.empty(rows, device=dev) if needs_grad else None
-        w = weight.contiguous() if weight is not None else None
-        b = bias.contiguous() if bias is not None else None
+        w, b = _whole(weight), _whole(bias)
         wtype = w if w is not None else b if b is not None else x
         with torch.cuda.device(dev):
             _lib.check(_lib.load().adder_b200_layernorm_forward(
@@ -122,13 +127,13 @@ class _LayerNorm(torch.autograd.Function):
 
     @staticmethod
     def gradients(ctx, saved, dy, dh):
-        h, (w, mean, rstd) = saved[0], (t.contiguous() if t is not None else None for t in saved[1:])
+        h, (w, mean, rstd) = saved[0], map(_whole, saved[1:])
         rows, d, wcode = ctx.sizes
         need_x = ctx.needs_input_grad[0] or (ctx.has_residual and ctx.needs_input_grad[1])
         dw = torch.empty(w.shape, dtype=w.dtype, device=w.device) if w is not None and ctx.needs_input_grad[2] else None
         db = torch.empty(ctx.shape, dtype=ctx.bias_type, device=h.device) if ctx.bias_type is not None and ctx.needs_input_grad[3] else None
-        dy = dy.contiguous() if dy is not None else torch.zeros(h.shape, dtype=h.dtype, device=h.device)
-        dh = dh.contiguous() if dh is not None else None
+        dy = _whole(dy) if dy is not None else torch.zeros(h.shape, dtype=h.dtype, device=h.device)
+        dh = _whole(dh)
         h2, hs = _rows(h, rows, d)
         dx = torch.empty(h.shape, dtype=h.dtype, device=h.device) if need_x else None
         lib = _lib.load()

@@ -13,7 +13,7 @@ import torch
 import torch.nn as nn
 
 from . import _lib, _native, adder_cuda
-from .layernorm import _check_input, _once, _ptr, _rows, _save, _saved
+from .layernorm import _check_input, _once, _ptr, _rows, _save, _saved, _whole
 
 MAX_TOP_K = 32
 
@@ -66,12 +66,12 @@ class _LogProbs(torch.autograd.Function):
 
     @staticmethod
     def gradient(ctx, saved, g_lp, g_ent, g_top):
-        logits, (targets, stats, ent, idx) = saved[0], (t.contiguous() if t is not None else None for t in saved[1:])
+        logits, (targets, stats, ent, idx) = saved[0], map(_whole, saved[1:])
         top_k, ignore_index = ctx.args
         v = logits.shape[-1]
         rows = logits.numel() // v
         x, stride = _rows(logits, rows, v)
-        g_lp, g_ent, g_top = (g.contiguous() if g is not None else None for g in (g_lp, g_ent, g_top))
+        g_lp, g_ent, g_top = map(_whole, (g_lp, g_ent, g_top))
         dx = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
         with torch.cuda.device(logits.device):
             _lib.check(_lib.load().adder_b200_log_probs_backward(
@@ -107,7 +107,7 @@ def token_log_probs(logits: torch.Tensor, targets: Optional[torch.Tensor] = None
             raise TypeError(f"targets must be int64 or int32, got {targets.dtype}")
         if targets.shape != logits.shape[:-1]:
             raise ValueError(f"targets have shape {tuple(targets.shape)}, expected {tuple(logits.shape[:-1])}")
-        targets = targets.to(torch.int64).contiguous()
+        targets = _whole(targets.to(torch.int64))
     top_k = int(top_k)
     if not 0 <= top_k <= min(MAX_TOP_K, logits.shape[-1]):
         raise ValueError(f"top_k must be between 0 and {min(MAX_TOP_K, logits.shape[-1])}, got {top_k}")

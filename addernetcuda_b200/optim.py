@@ -58,6 +58,8 @@ def _check(t, name: str, dev, dtype, like=None, numel=None) -> None:
         raise RuntimeError(f"tensors are on different devices ({dev} and {t.device})")
     if t.dtype != dtype:
         raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    if t.is_neg() and not name.startswith("grads"):
+        raise ValueError(f"{name} must not be a lazily negated view")
     if like is not None and (t.shape != like.shape or _strides(t) != _strides(like)):
         raise ValueError(f"{name} must have the shape and strides of its parameter: {tuple(t.shape)} {t.stride()}, "
                          f"expected {tuple(like.shape)} {like.stride()}")
@@ -124,7 +126,7 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
         _check(g, f"grads[{i}]", dev, p.dtype)
         if g.shape != p.shape:
             raise ValueError(f"grads[{i}] has shape {tuple(g.shape)}, expected {tuple(p.shape)}")
-        if _strides(g) != _strides(p):
+        if _strides(g) != _strides(p) or g.is_neg():
             g = torch.empty_like(p).copy_(g)
             kept.append(g)
         _check(exp_avgs[i], f"exp_avgs[{i}]", dev, state_type, like=p)

@@ -528,3 +528,18 @@ def test_second_moments_below_the_normal_range_before_8_bit_states_are_stored():
         p1 = update64(torch.ones(n, device=DEV), m1, v1, 1, HYPER["lr"], b1, b2, eps, 0.0)
         size = HYPER["lr"] / (1 - b1) * m1.double() / ((v1.double() / (1 - b2)).sqrt() + eps)
         _near(f"p, eps {eps}", p, p1, (1 + 4) * 2.0 ** -24 * p1.abs() + 32 * 2.0 ** -24 * size)
+
+
+def test_lazily_negated_gradients():
+    from addernetcuda_b200.optim import adamw_step
+    negated = lambda v: torch.complex(torch.zeros_like(v), v).conj().imag      # noqa: E731
+    p, g, m, v, steps = _make([1, 1, 40], torch.float32)
+    before = _copies(p, m, v, list(steps))
+    lazy = [negated(t) for t in g]
+    assert all(t.is_neg() for t in lazy) and lazy[0].is_contiguous()
+    adamw_step(p, lazy, m, v, steps, **HYPER)
+    _check_step(p, [-t for t in g], m, v, steps, before)
+    with pytest.raises(ValueError, match="lazily negated"):
+        adamw_step([lazy[0]], [g[0]], m[:1], v[:1], steps[:1], **HYPER)
+    with pytest.raises(ValueError, match="lazily negated"):
+        adamw_step(p[:1], g[:1], [negated(m[0])], v[:1], steps[:1], **HYPER)

@@ -458,3 +458,27 @@ def test_saved_tensors_that_come_back_in_another_form_are_refused(host_path, res
                 out = layer_norm(leaf, 40, w, b, residual=r)
             with pytest.raises(RuntimeError, match="saved tensors"):
                 torch.autograd.grad(out[0] if residual else out, leaf, dy)
+
+
+def _negated(t):
+    """-t, as a lazily negated view of one element or of strided ones."""
+    return torch.complex(torch.zeros_like(t), t).conj().imag
+
+
+@pytest.mark.parametrize("host_path", [True, False])
+def test_lazily_negated_tensors(host_path, monkeypatch):
+    from addernetcuda_b200 import _native
+    from addernetcuda_b200.layernorm import layer_norm
+    if not host_path:
+        monkeypatch.setattr(_native, "layer_norm", _native._absent)
+    x = torch.randn(1, 1, device=DEV)
+    assert _negated(x).is_neg() and _negated(x).is_contiguous()
+    _, h = layer_norm(_negated(x), 1, residual=_negated(2 * x))
+    assert torch.equal(h, -3 * x)
+    w, b = torch.full((1,), 2.0, device=DEV), torch.full((1,), 3.0, device=DEV)
+    assert float(layer_norm(x, 1, _negated(w), _negated(b))) == -3.0
+    for rows, width in ((1, 1), (3, 1), (4, 8)):
+        x, _, w, b, dy, _ = _inputs(rows, (width,), torch.float32, torch.float32, False)
+        _, want = _run(-x, None, w, b, -dy, None)
+        _, got = _run(_negated(x), None, w, b, _negated(dy), None)
+        assert all(torch.equal(p, q) for p, q in zip(got, want))

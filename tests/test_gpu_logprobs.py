@@ -426,3 +426,25 @@ def test_saved_tensors_that_come_back_in_another_form_are_refused(host_path, mon
         for change in ALTERED:
             with pytest.raises(RuntimeError, match="saved tensors"):
                 run(_altered(number, change))
+
+
+@pytest.mark.parametrize("host_path", [True, False])
+def test_lazily_negated_tensors(host_path, monkeypatch):
+    """The imaginary part of a conjugate is one; with one row its strides do not tell."""
+    from addernetcuda_b200 import _native
+    from addernetcuda_b200.logprobs import token_log_probs
+    if not host_path:
+        monkeypatch.setattr(_native, "log_probs", _native._absent)
+    for rows in (1, 3):
+        x, t = _logits(rows, 40, torch.float32)
+        leaf = x.detach().requires_grad_()
+        negated = lambda v: torch.complex(torch.zeros_like(v), v).conj().imag      # noqa: E731
+        up = [torch.rand(rows, device=DEV), torch.rand(rows, device=DEV), torch.rand(rows, 1, device=DEV)]
+
+        def gradient(upstream):
+            r = token_log_probs(leaf, t, top_k=1, entropy=True)
+            return torch.autograd.grad([r.log_prob, r.entropy, r.top_log_probs], leaf, upstream)[0]
+
+        got, want = gradient([negated(u) for u in up]), gradient([-u for u in up])
+        assert torch.equal(got, want)
+        assert torch.equal(token_log_probs(negated(x), t).log_prob, token_log_probs(-x, t).log_prob)
