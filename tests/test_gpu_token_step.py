@@ -174,3 +174,53 @@ def test_loss_and_accuracy_of_an_evaluation():
     labels = torch.cat([y for _, y in batches]).to(DEV)
     assert got["loss"] == pytest.approx(float(-logp.gather(1, labels[:, None]).mean()), rel=1e-5)
     assert got["entropy"] == pytest.approx(float(-(logp.exp() * logp).sum(1).mean()), rel=1e-5, abs=1e-6)
+
+
+class Classifier(torch.nn.Module):
+    """A norm and a product of this library's and elementwise operations, whose sums have one order: the same bits in every run.  63 columns, so
+    that gradients one behind another in a bucket do not begin at 16 bytes."""
+
+    def __init__(self):
+        super().__init__()
+        gen = torch.Generator()
+        gen.manual_seed(5)
+        self.norm = FusedLayerNorm(63)
+        self.scale = torch.nn.Parameter(0.3 * torch.randn(67, 63, generator=gen))
+        self.shift = torch.nn.Parameter(torch.zeros(67))
+
+    def forward(self, x):
+        return (self.norm(x)[:, None] * self.scale).sum(-1) + self.shift
+
+
+@pytest.mark.parametrize("optimizer", ["adamw", "adamw8"])
+def test_training_steps_captured_or_not_and_with_gradients_in_buckets_give_the_same_bits(optimizer, tmp_path):
+    import torch.distributed as dist
+    from addernetcuda_b200.ddp import BucketedDDP
+
+    def train(use_graph, with_ddp):
+        net = Classifier().to(DEV)
+        ddp = BucketedDDP(net) if with_ddp else None
+        ts = TrainStep(net, (24, 63), 67, lr=3e-3, weight_decay=0.01, ddp=ddp, use_graph=use_graph, device=DEV, optimizer=optimizer, criterion=TokenCrossEntropy())
+        gen = torch.Generator(device=DEV)
+        gen.manual_seed(6)
+        losses = []
+        for i in range(4):
+            x, y = torch.randn(24, 63, device=DEV, generator=gen), torch.randint(0, 67, (24,), device=DEV, generator=gen)
+            for _ in range(1 if use_graph or i else 4):      # a captured step is preceded by three eager ones on the first batch
+                losses.append(ts.step(x, y).clone())
+        if with_ddp:
+            assert any(p.grad.data_ptr() % 16 for p in net.parameters())
+        assert all(s["step"].tolist() == [7, 0] for s in ts.opt.state.values())
+        states = [s[k] for s in ts.opt.state.values() for k in ("exp_avg", "exp_avg_sq")]
+        assert optimizer == "adamw" or any(t.dtype == torch.uint8 for t in states)
+        return losses[-4:], [p.detach() for p in net.parameters()] + states
+
+    dist.init_process_group("gloo", init_method=f"file://{tmp_path}/store", rank=0, world_size=1)
+    try:
+        runs = [train(use_graph, with_ddp) for with_ddp in (False, True) for use_graph in (False, True)]
+    finally:
+        dist.destroy_process_group()
+    assert float(runs[0][0][-1]) != float(runs[0][0][-2])
+    for losses, tensors in runs[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(losses, runs[0][0]))
+        assert all(torch.equal(a, b) for a, b in zip(tensors, runs[0][1]))
