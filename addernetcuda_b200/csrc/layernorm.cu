@@ -9,8 +9,9 @@
 // backward pass, its sums of dw and db, which are added up over the CTAs by a second kernel, always in the same order.
 //
 // Measured (of a copy's rate): 8192x4096 bf16 with a residual stream forward 51 us (81 %), backward 50 us (82 %: some 5 us of it the second
-// kernel); 16384x2048 fp32 48 us (86 %) and 68 us (90 %); 2000x20000 bf16 46 us (53 %) and 106 us (35 %: long rows read h and dy once
-// more for dw and db); 8192x1001 bf16, whose rows allow no vectors, 31 us and 41 us (32 and 24 %: two bytes at a time).
+// kernel); 16384x2048 fp32 48 us (86 %) and 68 us (90 %); 2000x20000 bf16 47 us (53 %: one CTA an SM goes over
+// shared memory three times, with barriers between) and 106 us (35 %: long rows read h and dy once more for dw and db); 8192x1001 bf16, whose rows
+// allow no vectors, 31 us and 41 us (32 and 24 %: two bytes at a time).
 #include "kernels.h"
 #include "elements.cuh"
 #include <cooperative_groups.h>

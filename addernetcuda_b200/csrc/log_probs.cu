@@ -13,7 +13,13 @@
 //
 // What bounds them: memory, at 99 % of a copy's rate for the gradient (2048x128000 bf16: 161 us for 1.05 GB) and for the forward of fp32
 // logits (4096x32000: 81 us); the forward of 16-bit logits takes some 8 instructions a value and reaches 90 % (2048x128000
-// with entropy 89 us), and 81 % in shorter rows (4096x50257 bf16 78 us, 91 us with the 5 largest, 107 us with 20).  A few rows are split over a cluster of CTAs that join through shared memory (4x32000: 6 us, 10 us with the 20 largest).
+// with entropy 89 us), and 81 % with 50257 classes (4096 rows 77 us; 91 us with the 5 largest, 107 with 20, 126 with 32, which one warp a CTA
+// finds while eight stream).  A few rows are split over a cluster of CTAs that join through shared memory (4x32000: 6 us, 10 us with the 20
+// largest).  Rows by warps wait for loads and joins: 16384x1000 fp32 18.6 us (54 %), 16384x4000 bf16 with entropy 38 us (53 %), 16384x1000
+// bf16 20.6 us (24 %) and with the 5 largest 31.9 (16 %): a warp looks for them alone, after its row.
+// The gradient goes by vectors where a row of logits and its row of dx lie alike modulo 16 bytes.  Elsewhere (most rows of a padded buffer
+// whose row stride is not the number of classes) it goes element by element: 2048x50257 in rows of 50304 288 us bf16 and 260 fp32, where
+// dense rows take 74 and 126.
 #include "kernels.h"
 #include "elements.cuh"
 #include <cooperative_groups.h>
@@ -960,8 +966,10 @@ int adder_b200_log_probs_forward(const void* logits, int dtype, long long rows, 
     return with_type(dtype, [&](auto* type) {
         using T = std::remove_pointer_t<decltype(type)>;
         if (warp_rows(rows, classes)) return choose_forward<T, 32, false>(a, 1, s);
-        // Few rows leave SMs idle: a row is then split over a cluster of up to 8 CTAs of at least 4096 elements (64x128000 bf16 by 4 CTAs 8.4 us,
-        // by one 12.4; 296x50257 by one 10.4, by two 12.2).
+        // Few rows leave SMs idle: a row is then split over a cluster of up to 8 CTAs of at least 4096 elements, as long as there are no more than
+        // 4 CTAs an SM.  bf16 with entropy by 1, 2, 4 and 8 CTAs, us: 4x32000 6.3, 6.3, 6.3, 5.8 (4 are taken); 64x128000 12.4, 8.3, 8.4, 9.0 (8);
+        // 128x50257 8.3, 8.3, 8.6, 12.4 (4); 296x50257 10.4, 12.2, 16.5, 23.4 (2).  From some 2 CTAs an SM on a split costs more than it gives, so
+        // the last three take 4 to 18 % more than the best.
         int parts = 1;
         while (parts < 8 && rows * parts * 2 <= sm_count() * 4 && classes >= 8192LL * parts) parts *= 2;
         if (parts > 1) return choose_forward<T, LP_TEAM, true>(a, parts, s);

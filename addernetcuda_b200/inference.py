@@ -112,7 +112,7 @@ def validate(batches: Iterable[Tuple[torch.Tensor, torch.Tensor]], model: nn.Mod
 def evaluate(batches: Iterable[Tuple[torch.Tensor, torch.Tensor]], model: nn.Module, device=None, topk=(1, 5), ignore_index: int = -100):
     """Top-k accuracies in percent, mean loss (-log p of the label) and mean entropy of `model`'s (CUDA) outputs over (inputs, labels)
     batches: one pass over the logits [..., classes] of each batch, one host synchronisation in all.  Equal logits rank by index;
-    labels equal to `ignore_index` do not count."""
+    labels equal to `ignore_index` do not count.  `topk` goes up to 32."""
     model.eval()
     device = device if device is not None else next(model.parameters()).device
     total = None

@@ -164,7 +164,8 @@ def layer_norm(x: torch.Tensor, normalized_shape: Union[int, Sequence[int]], wei
 
     Without `residual` h is x, and y is returned.  With it h = x + residual, rounded to the type of both, and (y, h) is returned.
     `weight` and `bias` have the shape `normalized_shape` and x's type or float32 (both the same).  x and residual may be
-    any views; those whose rows are not consecutive are copied.  Differentiable once, with respect to x, residual, weight and bias."""
+    any views; those whose rows are not consecutive are copied.  Differentiable once, with respect to x, residual, weight and bias: a
+    gradient of create_graph=True raises where it is differentiated.  At most 2^28 - 1 rows of at most 2^30 - 2^16 elements."""
     shape = (normalized_shape,) if isinstance(normalized_shape, int) else tuple(normalized_shape)
     out = _native.layer_norm(x, residual, weight, bias, shape, eps)
     if out is not None:

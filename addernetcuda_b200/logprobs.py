@@ -89,9 +89,11 @@ def token_log_probs(logits: torch.Tensor, targets: Optional[torch.Tensor] = None
       entropy       -sum p log p of each row, with `entropy=True`;
       top_log_probs, top_indices   of the `top_k` (at most 32) most probable classes, equal logits by index from the lowest.
 
-    All but the indices are float32 and differentiable once with respect to the logits.  -inf marks classes that are out; where none is left
+    All but the indices are float32 and differentiable once with respect to the logits (a gradient of create_graph=True raises where it
+    is differentiated).  -inf marks classes that are out; where none is left
     the log probabilities are -inf, the entropy and the gradient 0.  A row with a NaN or +inf gives NaN, and indices of -1.  Logits may be
-    a view such as [..., :classes] of a padded buffer; views whose rows are not consecutive are copied."""
+    a view such as [..., :classes] of a padded buffer; views whose rows are not consecutive are copied.  The gradient of such a view takes two
+    to four times as long as that of dense rows, unless row stride and classes differ by a multiple of 16 bytes."""
     out = _native.log_probs(logits, targets, top_k, entropy, ignore_index)
     if out is not None:
         return TokenLogProbs(*out)

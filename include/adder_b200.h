@@ -249,13 +249,15 @@ ADDER_API int adder_b200_forward_affine(const float* x, const float* w, const fl
  *   h = x + residual, rounded to the type (h = x where residual is NULL);  y = (h - mean) / sqrt(var + eps) * weight + bias
  * x and residual have x_stride and residual_stride elements from row to row; y and h (written where there is a residual) are
  * contiguous.  weight and bias [d] are of weight_dtype, the same type or fp32, and may be NULL (1 and 0).  mean and rstd [rows], for the
- * backward call, may be NULL together.  Any alignment that the types need; 16-byte aligned rows run faster.  d is at most 2^30 - 2^16. */
+ * backward call, may be NULL together.  Any alignment that the types need; 16-byte aligned rows run faster.  d is at most 2^30 - 2^16,
+ * rows at most 2^28 - 1.  A row whose variance overflows has rstd 0, and y is the bias. */
 ADDER_API int adder_b200_layernorm_forward(const void* x, const void* residual, const void* weight, const void* bias, void* y, void* h,
                                            float* mean, float* rstd, long long rows, long long d, long long x_stride,
                                            long long residual_stride, int dtype, int weight_dtype, float eps, void* stream);
 
 /* Gradients from dy (and dh, that of h itself, or NULL): dx [rows][d], which is the gradient of x and of the residual, and
- * dweight, dbias [d], sums over the rows in an order that depends on the sizes alone.  Each of the three may be NULL.  dy, dh and dx are
+ * dweight, dbias [d], sums over the rows in an order that depends on the sizes, h_stride and the alignment of the buffers, which choose the
+ * kernel, and on nothing else.  Each of the three may be NULL.  dy, dh and dx are
  * contiguous, h (x where there was no residual) has h_stride.  The workspace serves dweight and dbias. */
 ADDER_API size_t adder_b200_layernorm_backward_workspace_bytes(long long rows, long long d);
 ADDER_API int adder_b200_layernorm_backward(const void* dy, const void* dh, const void* h, const void* weight, const float* mean,
@@ -277,7 +279,8 @@ ADDER_API int adder_b200_log_probs_forward(const void* logits, int dtype, long l
 
 /* grad_logits (contiguous, of the logits' type) <- the gradient of sum(grad_log_prob * log_prob + grad_entropy * entropy +
  * grad_top * top_log_probs), from the forward's inputs, stats, entropy and top_indices.  Gradients that are NULL count as zeros.  Rows of
- * nothing but -inf get zeros; rows with a NaN, or whose target is no class while grad_log_prob is given, NaN. */
+ * nothing but -inf get zeros; rows with a NaN, or whose target is no class while grad_log_prob is given, NaN.  Fast where a row of logits
+ * and its row of grad_logits lie alike modulo 16 bytes, as all do where row_stride and classes are alike modulo 16 bytes of elements. */
 ADDER_API int adder_b200_log_probs_backward(const void* logits, int dtype, long long rows, long long classes, long long row_stride,
                                             const long long* targets, long long ignore_index, int top_k, const long long* top_indices,
                                             const float* stats, const float* entropy, const float* grad_log_prob,
