@@ -121,7 +121,7 @@ def evaluate(batches: Iterable[Tuple[torch.Tensor, torch.Tensor]], model: nn.Mod
         out = model(inputs)
         r = token_log_probs(out, labels, top_k=min(max(topk), out.shape[-1]), entropy=True, ignore_index=ignore_index)
         counts = labels != ignore_index
-        hit = (r.top_indices == labels.unsqueeze(-1)) & counts.unsqueeze(-1)
+        hit = (r.top_indices == labels.unsqueeze(-1)) & (counts & (labels >= 0)).unsqueeze(-1)      # -1: the classes of a row with a NaN
         sums = torch.stack([counts.sum().double(), -r.log_prob.double().sum(), torch.where(counts, r.entropy, 0.0).double().sum(),
                             *(hit[..., :k].sum().double() for k in topk)])
         total = sums if total is None else total + sums

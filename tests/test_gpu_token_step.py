@@ -224,3 +224,10 @@ def test_training_steps_captured_or_not_and_with_gradients_in_buckets_give_the_s
     for losses, tensors in runs[1:]:
         assert all(torch.equal(a, b) for a, b in zip(losses, runs[0][0]))
         assert all(torch.equal(a, b) for a, b in zip(tensors, runs[0][1]))
+
+
+def test_a_label_that_is_no_class_is_no_hit_on_a_row_without_classes():
+    from addernetcuda_b200.inference import evaluate
+    logits = torch.tensor([[1.0, 2.0, 3.0], [float("nan"), 0.0, 0.0], [5.0, 1.0, 0.0], [0.0, 9.0, 1.0]])
+    got = evaluate([(logits, torch.tensor([2, -1, 0, -100]))], torch.nn.Identity(), DEV, topk=(1, 2))
+    assert got["topk"] == pytest.approx((200 / 3, 200 / 3)) and got["loss"] != got["loss"]
