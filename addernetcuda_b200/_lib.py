@@ -76,6 +76,18 @@ SIGNATURES = {
                                      [c_void_p] * 6),
     "adder_b200_log_probs_backward": (c_int, [c_void_p, c_int, c_longlong, c_longlong, c_longlong, c_void_p, c_longlong, c_int] +
                                       [c_void_p] * 8),
+    "adder_b200_rmsnorm_forward": (c_int, [c_void_p] * 6 + [c_longlong] * 4 + [c_int, c_int, c_float, c_void_p]),
+    "adder_b200_rmsnorm_forward_8bit": (c_int, [c_void_p] * 6 + [c_longlong] * 5 + [c_int, c_int, c_float, c_void_p]),
+    "adder_b200_rmsnorm_backward_workspace_bytes": (c_size_t, [c_longlong, c_longlong]),
+    "adder_b200_rmsnorm_backward": (c_int, [c_void_p] * 8 + [c_size_t] + [c_longlong] * 3 + [c_int, c_int, c_void_p]),
+    "adder_b200_quantize_rows": (c_int, [c_void_p] * 3 + [c_longlong] * 4 + [c_int, c_void_p]),
+    "adder_b200_quantize_weight": (c_int, [c_void_p] * 3 + [c_longlong] * 4 + [c_int, c_void_p]),
+    "adder_b200_linear_8bit": (c_int, [c_void_p] * 6 + [c_longlong] * 5 + [c_int, c_void_p]),
+    "adder_b200_distillation_forward": (c_int, [c_void_p, c_int, c_longlong, c_longlong, c_longlong, c_void_p, c_int, c_void_p, c_int, c_float,
+                                                c_void_p, c_longlong] + [c_void_p] * 5),
+    "adder_b200_distillation_backward": (c_int, [c_void_p, c_int, c_longlong, c_longlong, c_longlong, c_void_p, c_int, c_float, c_void_p,
+                                                 c_longlong] + [c_void_p] * 6),
+    "adder_b200_verify_drafts": (c_int, [c_void_p, c_void_p, c_int] + [c_void_p] * 5 + [c_longlong] * 7 + [c_void_p]),
     "adder_b200_adamw_step": (c_int, [c_void_p, c_int, c_int, c_int, c_double, c_void_p] + [c_double] * 4 + [c_void_p, c_void_p]),
     "adder_b200_adamw_state_values": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_longlong, c_void_p]),
     "adder_b200_device_status": (c_int, [POINTER(c_int), c_int]),

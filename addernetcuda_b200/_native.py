@@ -1,7 +1,7 @@
 """The C++ host path of the eager layer calls (csrc/host.cpp), loaded on the first call with a CUDA tensor.
 
-`layer`, `conv`, `layer_with_stats`, `layer_affine`, `affine`, `column`, `layer_norm`, `log_probs` and `adamw` return None for whatever
-they do not take - the layers anything but contiguous fp32 CUDA tensors of a geometry the kernels are built for, the others anything but
+`layer`, `conv`, `layer_with_stats`, `layer_affine`, `affine`, `column`, `layer_norm`, `log_probs`, `adamw`, `rms_norm`, `rms_norm_8bit`,
+`linear_8bit`, `distillation` and `verify_drafts` return None for whatever they do not take - the layers anything but contiguous fp32 CUDA tensors of a geometry the kernels are built for, the others anything but
 CUDA tensors of their types in rows or, `adamw`, contiguous - and callers then go on in Python, which handles the rest or raises.  They always call the product library; inside a `_lib.tuning()` block they return None.
 """
 from __future__ import annotations
@@ -22,8 +22,12 @@ _NAMES = ("adder_b200_status_string", "adder_b200_forward", "adder_b200_forward_
           "adder_b200_conv_backward_input_workspace_bytes", "adder_b200_conv_backward_input_with_workspace",
           "adder_b200_conv_backward_weight_workspace_bytes", "adder_b200_conv_backward_weight",
           "adder_b200_layernorm_forward", "adder_b200_layernorm_backward_workspace_bytes", "adder_b200_layernorm_backward",
-          "adder_b200_log_probs_forward", "adder_b200_log_probs_backward", "adder_b200_adamw_step")
-_ENTRIES = ("layer", "conv", "layer_with_stats", "layer_affine", "affine", "column", "layer_norm", "log_probs", "adamw")
+          "adder_b200_log_probs_forward", "adder_b200_log_probs_backward", "adder_b200_adamw_step",
+          "adder_b200_rmsnorm_forward", "adder_b200_rmsnorm_forward_8bit", "adder_b200_rmsnorm_backward_workspace_bytes", "adder_b200_rmsnorm_backward",
+          "adder_b200_quantize_rows", "adder_b200_linear_8bit", "adder_b200_distillation_forward", "adder_b200_distillation_backward",
+          "adder_b200_verify_drafts")
+_ENTRIES = ("layer", "conv", "layer_with_stats", "layer_affine", "affine", "column", "layer_norm", "log_probs", "adamw",
+            "rms_norm", "rms_norm_8bit", "linear_8bit", "distillation", "verify_drafts")
 _mod = None
 
 
@@ -81,4 +85,5 @@ def _first_call(name):
     return call
 
 
-layer, conv, layer_with_stats, layer_affine, affine, column, layer_norm, log_probs, adamw = (_first_call(n) for n in _ENTRIES)
+(layer, conv, layer_with_stats, layer_affine, affine, column, layer_norm, log_probs, adamw, rms_norm, rms_norm_8bit, linear_8bit,
+ distillation, verify_drafts) = (_first_call(n) for n in _ENTRIES)

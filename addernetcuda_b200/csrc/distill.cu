@@ -1,0 +1,415 @@
+// Distillation from a teacher's top logits: how far a row's softmax is from the teacher's, and its gradient.
+//
+//   forward   t = softmax(z / T) over the k classes i_j that the teacher names, p = softmax(x / T), M = max x
+//             D = sum_j t_j (ln t_j - ln p_{i_j}),  ln p_i = (x_i - M) / T - ln sum e^((x - M) / T);  log softmax(x) at a target class
+//   backward  dx_i = g_D / T (p_i - sum_{j: i_j = i} t_j) + g_L ([i = target] - softmax(x)_i)
+//
+// The forward reads the logits once: every thread keeps a maximum of its own with the sums relative to it (two where the target's
+// probability at temperature 1 is asked for beside another temperature), which are rescaled when it rises and joined at the end.  It leaves M,
+// the sums and t for the backward, which reads the logits again and writes the gradient.
+#include "kernels.h"
+#include "launch.cuh"
+#include "softmax.cuh"
+#include <cooperative_groups.h>
+
+namespace adder {
+namespace {
+
+namespace cg = cooperative_groups;
+
+constexpr int DS_MAX_K = 256, DS_TEAM = 256, DS_UNROLL = 4;
+
+struct DsFwd {
+    const void* x;
+    long long rows, stride;
+    int classes, k;
+    const void* teacher;             // [rows][k]
+    int teacher_type;
+    const long long* indices;        // [rows][k]
+    const long long* targets;        // [rows], or null
+    long long ignore;
+    float inv_t;                     // 1 / T
+    float scale;                     // log2(e) / T
+    float* divergence;               // [rows]
+    float* log_prob;                 // [rows], with targets
+    float* stats;                    // [rows][3]: M and both sums; or null
+    float* mass;                     // [rows][k]: t; or null
+};
+
+// Largest value m with sums of 2^((x - m) scale) and, with BOTH, of 2^((x - m) log2 e).
+template <bool BOTH> struct DsSums {
+    float m = -INFINITY;
+    uint64_t s = 0, s1 = 0;      // pairs
+
+    __device__ __forceinline__ void raise(float top, float scale) {
+        const float f = m == -INFINITY ? 0.f : exp2_fast((m - top) * scale);
+        s = mul2(s, pack2(f, f));
+        if (BOTH) {
+            const float f1 = m == -INFINITY ? 0.f : exp2_fast((m - top) * LOG2E);
+            s1 = mul2(s1, pack2(f1, f1));
+        }
+        m = top;
+    }
+    __device__ __forceinline__ void add(float a, float b, float scale) {
+        const uint64_t d = add2(pack2(a, b), pack2(-m, -m));
+        float lo, hi;
+        unpack2(mul2(d, pack2(scale, scale)), lo, hi);
+        s = add2(s, pack2(exp2_fast(lo), exp2_fast(hi)));
+        if (BOTH) {
+            unpack2(mul2(d, pack2(LOG2E, LOG2E)), lo, hi);
+            s1 = add2(s1, pack2(exp2_fast(lo), exp2_fast(hi)));
+        }
+    }
+};
+struct DsPart {
+    float m, s, s1;
+};
+// Sums relative to the larger maximum.  Equal maxima (both -inf among them) need no factor; a NaN stays one.
+__device__ __forceinline__ DsPart ds_join(DsPart a, DsPart b, float scale) {
+    const float m = max_nan(a.m, b.m);
+    const float da = a.m == m ? 0.f : a.m - m, db = b.m == m ? 0.f : b.m - m;
+    return {m, a.s * exp2_fast(da * scale) + b.s * exp2_fast(db * scale), a.s1 * exp2_fast(da * LOG2E) + b.s1 * exp2_fast(db * LOG2E)};
+}
+__device__ __forceinline__ DsPart ds_join_lanes(DsPart p, float scale) {
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) {
+        const DsPart o{__shfl_xor_sync(0xffffffffu, p.m, off), __shfl_xor_sync(0xffffffffu, p.s, off), __shfl_xor_sync(0xffffffffu, p.s1, off)};
+        p = ds_join(p, o, scale);
+    }
+    return p;
+}
+
+// Values of a vector into the sums.
+template <class T, int U, bool BOTH> __device__ __forceinline__ void ds_take(const uint4 (&q)[U], DsSums<BOTH>& run, float scale) {
+    constexpr int VE = Vec16<T>::N;
+    uint32_t w;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const uint32_t a = max_word<T>(max_word<T>(q[u].x, q[u].y), max_word<T>(q[u].z, q[u].w));
+        w = u == 0 ? a : max_word<T>(w, a);
+    }
+    const float top = word_max<T>(w);
+    if (!(top <= run.m)) run.raise(top, scale);      // a NaN, too
+    if (run.m == -INFINITY) return;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        float f[VE];
+        Vec16<T>::unpack(q[u], f);
+#pragma unroll
+        for (int i = 0; i < VE; i += 2) run.add(f[i], f[i + 1], scale);
+    }
+}
+
+__device__ __forceinline__ float ds_value(const void* p, int type, long long i) {
+    if (type == ADDER_TYPE_F32) return static_cast<const float*>(p)[i];
+    return type == ADDER_TYPE_BF16 ? to_float(static_cast<const __nv_bfloat16*>(p)[i]) : to_float(static_cast<const __half*>(p)[i]);
+}
+
+// THREADS threads a row (32: a warp, four of them a CTA); with CLUSTER a row is shared out over the CTAs of a cluster.
+template <class T, int THREADS, bool CLUSTER, bool BOTH> __global__ void __launch_bounds__(THREADS == 32 ? 128 : THREADS) ds_forward_kernel(const DsFwd a) {
+    constexpr int VE = Vec16<T>::N, WARPS = THREADS / 32;
+    __shared__ DsPart parts_of[WARPS], ranks_of[8];
+    const int t = threadIdx.x % THREADS, lane = t & 31;
+    const int parts = CLUSTER ? (int)cg::this_cluster().num_blocks() : 1, rank = CLUSTER ? (int)cg::this_cluster().block_rank() : 0;
+    const long long row = THREADS == 32 ? (long long)blockIdx.x * 4 + threadIdx.x / 32 : blockIdx.x / parts;
+    if (CLUSTER) asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");
+    if (THREADS == 32 && row >= a.rows) return;
+    const T* x = static_cast<const T*>(a.x) + row * a.stride;
+    const int mis = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T)), head = min(a.classes, mis == 0 ? 0 : VE - mis);
+    const int nvec = (a.classes - head) / VE, singles = rank == 0 ? a.classes - nvec * VE : 0;
+    const int v0 = (int)((long long)nvec * rank / parts), v1 = (int)((long long)nvec * (rank + 1) / parts);
+    const uint4* vec = reinterpret_cast<const uint4*>(x + head);
+
+    DsSums<BOTH> run;
+    int v = v0 + t;
+    for (; v + (DS_UNROLL - 1) * THREADS < v1; v += DS_UNROLL * THREADS) {
+        uint4 q[DS_UNROLL];
+#pragma unroll
+        for (int u = 0; u < DS_UNROLL; ++u) q[u] = __ldg(vec + v + u * THREADS);
+        ds_take<T, DS_UNROLL>(q, run, a.scale);
+    }
+    for (; v < v1; v += THREADS) {
+        uint4 q[1] = {__ldg(vec + v)};
+        ds_take<T, 1>(q, run, a.scale);
+    }
+    if (t < singles) {
+        const float one = to_float(x[t < head ? t : t + nvec * VE]);
+        if (!(one <= run.m)) run.raise(one, a.scale);
+        if (run.m != -INFINITY) run.add(one, -INFINITY, a.scale);
+    }
+    float lo, hi, lo1, hi1;
+    unpack2(run.s, lo, hi);
+    unpack2(run.s1, lo1, hi1);
+    DsPart all{run.m, lo + hi, lo1 + hi1};
+    all = ds_join_lanes(all, a.scale);
+    if constexpr (THREADS > 32) {
+        if (lane == 0) parts_of[t >> 5] = all;
+        __syncthreads();
+        all = lane < WARPS ? parts_of[lane] : DsPart{-INFINITY, 0.f, 0.f};
+        all = ds_join_lanes(all, a.scale);
+    }
+    if constexpr (CLUSTER) {
+        asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+        if (t == 0) cg::this_cluster().map_shared_rank(ranks_of, 0)[rank] = all;
+        cg::this_cluster().sync();
+        if (rank != 0) return;
+        all = lane < parts ? ranks_of[lane] : DsPart{-INFINITY, 0.f, 0.f};
+        all = ds_join_lanes(all, a.scale);
+    }
+    // The teacher's classes, by one warp.
+    if (t >= 32) return;
+    const auto z = [&](int j) { return ds_value(a.teacher, a.teacher_type, row * a.k + j); };
+    const long long* at = a.indices + row * a.k;
+    float top = -INFINITY;
+    bool broken = false;
+    for (int j = lane; j < a.k; j += 32) {
+        const long long i = at[j];
+        broken |= i >= a.classes || i < -1;
+        if (i >= 0) top = max_nan(top, z(j));
+    }
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, off));
+    broken = __any_sync(0xffffffffu, broken) || top == INFINITY || top != top;
+    const bool empty = top == -INFINITY;
+    float sum = 0.f;
+    for (int j = lane; j < a.k; j += 32)
+        if (at[j] >= 0 && !empty) sum += exp2_fast((z(j) - top) * a.scale);
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+    const float log_mass = logf(sum), log_sum = logf(all.s);
+    float d = 0.f;
+    for (int j = lane; j < a.k; j += 32) {
+        const long long i = at[j];
+        float share = 0.f;
+        if (i >= 0 && i < a.classes && !empty) {
+            const float e = (z(j) - top) * a.inv_t, log_t = e - log_mass;
+            share = exp2_fast((z(j) - top) * a.scale) / sum;
+            if (share > 0.f) {
+                const float xi = to_float(x[i]);
+                d += share * (log_t - ((xi - all.m) * a.inv_t - log_sum));
+            }
+        }
+        if (a.mass != nullptr) a.mass[row * a.k + j] = broken ? NAN : share;
+    }
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) d += __shfl_xor_sync(0xffffffffu, d, off);
+    if (lane == 0) {
+        const bool nothing = all.m == -INFINITY;
+        a.divergence[row] = broken ? NAN : empty ? 0.f : nothing ? INFINITY : d;
+        if (a.targets != nullptr) {
+            const long long target = a.targets[row];
+            const float s1 = BOTH ? all.s1 : all.s;
+            a.log_prob[row] = target == a.ignore ? 0.f : target < 0 || target >= a.classes ? NAN : nothing ? -INFINITY : to_float(x[target]) - all.m - logf(s1);
+        }
+        if (a.stats != nullptr) {
+            a.stats[3 * row] = all.m;
+            a.stats[3 * row + 1] = all.s;
+            a.stats[3 * row + 2] = BOTH ? all.s1 : all.s;
+        }
+    }
+}
+
+struct DsBwd {
+    const void* x;
+    long long rows, stride;
+    int classes, k;
+    const long long* indices;
+    const long long* targets;        // or null
+    long long ignore;
+    float inv_t, scale;
+    const float* stats;
+    const float* mass;
+    const float* g_divergence;       // [rows], or null
+    const float* g_log_prob;         // [rows], or null
+    void* dx;
+    int segments;                    // of a row
+};
+
+// What a row's elements have in common: dx = soft 2^((x - m) scale) + hard 2^((x - m) log2 e)
+template <bool BOTH> struct DsSlope {
+    float m, soft, hard, scale;
+    __device__ __forceinline__ uint64_t pair(float a, float b) const {
+        const uint64_t d = add2(pack2(a, b), pack2(-m, -m));
+        float lo, hi;
+        unpack2(mul2(d, pack2(scale, scale)), lo, hi);
+        uint64_t r = mul2(pack2(exp2_fast(lo), exp2_fast(hi)), pack2(soft, soft));
+        if (BOTH) {
+            unpack2(mul2(d, pack2(LOG2E, LOG2E)), lo, hi);
+            r = fma2(pack2(exp2_fast(lo), exp2_fast(hi)), pack2(hard, hard), r);
+        }
+        return r;
+    }
+    __device__ __forceinline__ float one(float a) const {
+        float lo, hi;
+        unpack2(pair(a, a), lo, hi);
+        return lo;
+    }
+};
+
+template <class T, int THREADS, bool BOTH> __global__ void __launch_bounds__(THREADS == 32 ? 128 : THREADS) ds_backward_kernel(const DsBwd a) {
+    constexpr int VE = Vec16<T>::N;
+    const int t = threadIdx.x % THREADS;
+    const long long row = THREADS == 32 ? (long long)blockIdx.x * 4 + threadIdx.x / 32 : blockIdx.x / a.segments;
+    const int segment = THREADS == 32 ? 0 : (int)(blockIdx.x % a.segments);
+    if (row >= a.rows) return;
+    const T* x = static_cast<const T*>(a.x) + row * a.stride;
+    T* dx = static_cast<T*>(a.dx) + row * (long long)a.classes;
+    const int mis = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
+    const bool same = (reinterpret_cast<uintptr_t>(dx) & 15) == (reinterpret_cast<uintptr_t>(x) & 15);
+    const int head = min(a.classes, mis == 0 ? 0 : VE - mis), nvec = (a.classes - head) / VE;
+    const int v0 = (int)((long long)nvec * segment / a.segments), v1 = (int)((long long)nvec * (segment + 1) / a.segments);
+    const uint4* vec = reinterpret_cast<const uint4*>(x + head);
+    uint4 q[DS_UNROLL];
+    if (same) {      // on their way while the row's numbers are looked up
+#pragma unroll
+        for (int u = 0; u < DS_UNROLL; ++u)
+            if (v0 + t + u * THREADS < v1) q[u] = __ldg(vec + v0 + t + u * THREADS);
+    }
+    const float m = a.stats[3 * row], s = a.stats[3 * row + 1], s1 = a.stats[3 * row + 2];
+    const bool nothing = m == -INFINITY;
+    const float gd = a.g_divergence != nullptr ? a.g_divergence[row] * a.inv_t : 0.f;
+    const long long target = a.targets != nullptr && a.g_log_prob != nullptr ? a.targets[row] : a.ignore;
+    const float gl = target == a.ignore ? 0.f : target < 0 || target >= a.classes ? NAN : a.g_log_prob[row];
+    // A row without classes of the teacher's has no part of the divergence; one with a NaN among them is NaN.
+    const float* mass = a.mass + row * a.k;
+    const long long* at = a.indices + row * a.k;
+    float some = 0.f;
+    for (int j = threadIdx.x & 31; j < a.k; j += 32) some = max_nan(some, mass[j]);
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) some = max_nan(some, __shfl_xor_sync(0xffffffffu, some, off));
+    DsSlope<BOTH> slope;
+    slope.m = m;
+    slope.scale = a.scale;
+    const float soft = some == 0.f ? 0.f : some != some ? NAN : gd;
+    slope.soft = soft / s;
+    slope.hard = -gl / s1;
+    if (!BOTH) slope.soft += slope.hard;
+
+    int begin, end;
+    if (same) {
+        uint4* out = reinterpret_cast<uint4*>(dx + head);
+        for (int v = v0 + t; v < v1; v += THREADS * DS_UNROLL) {
+            if (v != v0 + t) {
+#pragma unroll
+                for (int u = 0; u < DS_UNROLL; ++u)
+                    if (v + u * THREADS < v1) q[u] = __ldg(vec + v + u * THREADS);
+            }
+#pragma unroll
+            for (int u = 0; u < DS_UNROLL; ++u)
+                if (v + u * THREADS < v1) {
+                    float f[VE];
+                    Vec16<T>::unpack(q[u], f);
+#pragma unroll
+                    for (int i = 0; i < VE; i += 2) unpack2(nothing ? 0ull : slope.pair(f[i], f[i + 1]), f[i], f[i + 1]);
+                    __stcs(out + v + u * THREADS, Vec16<T>::pack(f));
+                }
+        }
+        begin = segment == 0 ? 0 : head + v0 * VE;
+        end = segment == a.segments - 1 ? a.classes : head + v1 * VE;
+        if (segment == 0 && t < head) dx[t] = from_float<T>(nothing ? 0.f : slope.one(to_float(x[t])));
+        const int tail = head + nvec * VE + t;
+        if (segment == a.segments - 1 && tail < a.classes) dx[tail] = from_float<T>(nothing ? 0.f : slope.one(to_float(x[tail])));
+    } else {
+        begin = (int)((long long)a.classes * segment / a.segments);
+        end = (int)((long long)a.classes * (segment + 1) / a.segments);
+        for (int i = begin + t; i < end; i += THREADS) dx[i] = from_float<T>(nothing ? 0.f : slope.one(to_float(x[i])));
+    }
+    if (nothing) return;
+    // The named classes, written again in whole: where several names are one class, each writes the same sum.
+    if constexpr (THREADS == 32) __syncwarp(); else __syncthreads();
+    for (int j = t; j <= a.k; j += THREADS) {
+        const long long i = j < a.k ? at[j] : (gl != 0.f ? target : -1);
+        if (i < begin || i >= end) continue;
+        float g = i == target ? gl : 0.f;
+        for (int l = 0; l < a.k; ++l)
+            if (at[l] == i) g -= soft * mass[l];
+        dx[i] = from_float<T>(slope.one(to_float(x[i])) + g);
+    }
+}
+
+// A warp a row: short rows, and longer ones where there are enough to fill the SMs.
+bool ds_warp_rows(long long rows, long long classes) {
+    return classes <= 1024 || (classes <= 4096 && rows >= 8LL * sm_count()) || (classes <= 8192 && rows >= 24LL * sm_count());
+}
+
+template <class T, bool BOTH> int launch_distill_forward(const DsFwd& a, cudaStream_t s) {
+    if (ds_warp_rows(a.rows, a.classes)) {
+        ds_forward_kernel<T, 32, false, BOTH><<<(unsigned)((a.rows + 3) / 4), 128, 0, s>>>(a);
+        return launched();
+    }
+    int parts = 1;      // few rows are split over clusters, as long as there are no more than 4 CTAs an SM
+    while (parts < 8 && a.rows * parts * 2 <= sm_count() * 4 && a.classes >= 8192LL * parts) parts *= 2;
+    if (parts > 1) return launch_clusters(ds_forward_kernel<T, DS_TEAM, true, BOTH>, (unsigned)(a.rows * parts), DS_TEAM, 0, parts, s, a);
+    ds_forward_kernel<T, DS_TEAM, false, BOTH><<<(unsigned)a.rows, DS_TEAM, 0, s>>>(a);
+    return launched();
+}
+
+int ds_check(long long rows, long long classes, long long row_stride, int dtype, int k, float temperature) {
+    if (rows < 0 || classes <= 0 || k < 1 || (rows > 1 && row_stride < 0) || !(temperature > 0.f) || temperature == INFINITY) return ADDER_ERR_BAD_SHAPE;
+    if (classes > 2147483647LL - 1024 || rows > 2147483647LL / 8 || k > DS_MAX_K || dtype < ADDER_TYPE_F32 || dtype > ADDER_TYPE_F16) return ADDER_ERR_UNSUPPORTED;
+    return ADDER_OK;
+}
+
+}  // namespace
+}  // namespace adder
+
+using namespace adder;
+
+extern "C" {
+
+int adder_b200_distillation_forward(const void* logits, int dtype, long long rows, long long classes, long long row_stride, const void* teacher,
+                                    int teacher_dtype, const long long* indices, int k, float temperature, const long long* targets,
+                                    long long ignore_index, float* divergence, float* log_prob, float* stats, float* mass, void* stream) {
+    const int st = ds_check(rows, classes, row_stride, dtype, k, temperature);
+    if (st != ADDER_OK) return st;
+    if (teacher_dtype < ADDER_TYPE_F32 || teacher_dtype > ADDER_TYPE_F16) return ADDER_ERR_UNSUPPORTED;
+    if (rows == 0) return ADDER_OK;
+    if (!logits || !teacher || !indices || !divergence || !targets != !log_prob || !stats != !mass) return ADDER_ERR_NULL_POINTER;
+    if (!aligned_to(logits, dtype == ADDER_TYPE_F32 ? 4 : 2) || !aligned_to(teacher, teacher_dtype == ADDER_TYPE_F32 ? 4 : 2) || !aligned_to(indices, 8) ||
+        !aligned_to(targets, 8) || !aligned_to(divergence, 4) || !aligned_to(log_prob, 4) || !aligned_to(stats, 4) || !aligned_to(mass, 4))
+        return ADDER_ERR_ALIGNMENT;
+    const DsFwd a{logits, rows, row_stride, (int)classes, k, teacher, teacher_dtype, indices, targets, ignore_index, (float)(1.0 / temperature),
+                  (float)(1.4426950408889634 / temperature), divergence, log_prob, stats, mass};
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const bool both = targets != nullptr && temperature != 1.f;
+    return with_type(dtype, [&](auto* type) {
+        using T = std::remove_pointer_t<decltype(type)>;
+        return both ? launch_distill_forward<T, true>(a, s) : launch_distill_forward<T, false>(a, s);
+    });
+}
+
+int adder_b200_distillation_backward(const void* logits, int dtype, long long rows, long long classes, long long row_stride,
+                                     const long long* indices, int k, float temperature, const long long* targets, long long ignore_index,
+                                     const float* stats, const float* mass, const float* grad_divergence, const float* grad_log_prob,
+                                     void* grad_logits, void* stream) {
+    const int st = ds_check(rows, classes, row_stride, dtype, k, temperature);
+    if (st != ADDER_OK) return st;
+    if (rows == 0) return ADDER_OK;
+    if (!logits || !indices || !stats || !mass || !grad_logits || (grad_log_prob && !targets)) return ADDER_ERR_NULL_POINTER;
+    const unsigned size = dtype == ADDER_TYPE_F32 ? 4 : 2;
+    if (!aligned_to(logits, size) || !aligned_to(grad_logits, size) || !aligned_to(indices, 8) || !aligned_to(targets, 8) || !aligned_to(stats, 4) ||
+        !aligned_to(mass, 4) || !aligned_to(grad_divergence, 4) || !aligned_to(grad_log_prob, 4))
+        return ADDER_ERR_ALIGNMENT;
+    const bool warps = ds_warp_rows(rows, classes), both = grad_log_prob != nullptr && temperature != 1.f;
+    // A CTA takes two turns, whose loads and stores overlap, or one where there would be too few CTAs.
+    const long long turn = (long long)DS_TEAM * DS_UNROLL * (16 / size), ones = (classes + turn - 1) / turn;
+    const long long segments = warps ? 1 : rows * ones >= 8LL * sm_count() ? (ones + 1) / 2 : ones;
+    const long long grid = warps ? (rows + 3) / 4 : rows * segments;
+    if (grid > 2147483647LL) return ADDER_ERR_UNSUPPORTED;
+    const DsBwd a{logits, rows, row_stride, (int)classes, k, indices, targets, ignore_index, (float)(1.0 / temperature),
+                  (float)(1.4426950408889634 / temperature), stats, mass, grad_divergence, grad_log_prob, grad_logits, (int)segments};
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    return with_type(dtype, [&](auto* type) {
+        using T = std::remove_pointer_t<decltype(type)>;
+        if (warps) {
+            if (both) ds_backward_kernel<T, 32, true><<<(unsigned)grid, 128, 0, s>>>(a);
+            else ds_backward_kernel<T, 32, false><<<(unsigned)grid, 128, 0, s>>>(a);
+        } else {
+            if (both) ds_backward_kernel<T, DS_TEAM, true><<<(unsigned)grid, DS_TEAM, 0, s>>>(a);
+            else ds_backward_kernel<T, DS_TEAM, false><<<(unsigned)grid, DS_TEAM, 0, s>>>(a);
+        }
+        return launched();
+    });
+}
+
+}  // extern "C"

@@ -1,0 +1,234 @@
+// Verification of drafted tokens against the target's probabilities, from given random numbers.
+//
+//   a sequence has L drafted tokens t_i, each drawn from probabilities q_i, and the target's probabilities p_0 .. p_L
+//   n = the first i with not (u_i q_i(t_i) < p_i(t_i)), or L;  then one more token, of weights w(c):
+//     max(p_n(c) - q_n(c), 0) where n < L (p_n(c), without t_n, where the drafter gives no probabilities), or p_L(c) where n = L
+//   token = the first c with sum_{c' <= c} w(c') > u sum w  and  w(c) > 0
+//
+// The sums are held in 64 bits: differences of two fp32 values are exact there, and a border between two classes moves by some 1e-16 of the
+// whole, so the token does not depend on the order of a sum in practice (in 32 bits it would, for one draw in a hundred of 128000 classes).
+//
+// A sequence's row is split over a cluster of CTAs and their warps, a segment of consecutive classes a warp.  Every CTA finds n for itself,
+// sums its segments and leaves the sums with all CTAs of the cluster; then the warp whose segment holds the border reads that again.
+// Bound by memory: of all rows only those of p_n and q_n are read; for few sequences by latency: four loads that wait for one another (the
+// token, its probabilities, the row, the segment again).
+#include "kernels.h"
+#include "elements.cuh"
+#include "launch.cuh"
+#include <cooperative_groups.h>
+
+namespace adder {
+namespace {
+
+namespace cg = cooperative_groups;
+
+constexpr int DV_THREADS = 256, DV_WARPS = DV_THREADS / 32, DV_MOST_PARTS = 8;
+
+struct DvArgs {
+    const void* p;                 // [sequences][drafts + 1][classes]
+    const void* q;                 // [sequences][drafts][classes], or null: the drafter is certain of its tokens
+    const long long* tokens;       // [sequences][drafts]
+    const float* u;                // [sequences][drafts + 1]
+    const long long* lengths;      // [sequences], or null
+    long long* out;                // [sequences][drafts + 1]
+    long long* accepted;           // [sequences]
+    long long p_sequence, p_place, q_sequence, q_place;      // strides
+    int drafts, classes;
+};
+
+template <class T, int N> __device__ __forceinline__ void dv_load(const T* p, float (&f)[N]) {
+    if constexpr (N == 1) f[0] = to_float(*p);
+    else Vec16<T>::unpack(__ldg(reinterpret_cast<const uint4*>(p)), f);
+}
+__device__ __forceinline__ double dv_positive(double w) { return w > 0.0 ? w : 0.0; }      // a NaN counts as 0
+// Inclusive sums over the lanes of a warp.
+__device__ __forceinline__ double dv_scan(double v, int lane) {
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+        const double o = __shfl_up_sync(0xffffffffu, v, off);
+        if (lane >= off) v += o;
+    }
+    return v;
+}
+
+// VEC consecutive classes a lane at a time.
+template <class T, int VEC> __global__ void __launch_bounds__(DV_THREADS) dv_kernel(const DvArgs a) {
+    __shared__ double sums[2][DV_MOST_PARTS * DV_WARPS];
+    __shared__ int first_refused;
+    cg::cluster_group cluster = cg::this_cluster();
+    const int parts = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+    const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
+    const long long b = blockIdx.x / parts;
+    const long long* tokens = a.tokens + b * a.drafts;
+    const float* u = a.u + b * (a.drafts + 1);
+    const T* p = static_cast<const T*>(a.p) + b * a.p_sequence;
+    const T* q = a.q != nullptr ? static_cast<const T*>(a.q) + b * a.q_sequence : nullptr;
+    const int length = a.lengths == nullptr ? a.drafts : (int)max(0LL, min((long long)a.drafts, a.lengths[b]));
+
+    if (warp == 0) {
+        int n = length;
+        for (int base = 0; base < length; base += 32) {
+            const int i = base + lane;
+            bool stands = true;
+            if (i < length) {
+                const long long token = tokens[i];
+                stands = false;      // what is no class does not stand
+                if (token >= 0 && token < a.classes) {
+                    const double pt = to_float(p[i * a.p_place + token]), qt = q == nullptr ? 1.0 : (double)to_float(q[i * a.q_place + token]);
+                    stands = (double)u[i] * qt < pt;
+                }
+            }
+            const unsigned refused = ~__ballot_sync(0xffffffffu, stands);
+            if (refused != 0) {
+                n = base + __ffs(refused) - 1;
+                break;
+            }
+        }
+        if (lane == 0) first_refused = n;
+    }
+    __syncthreads();
+    const int n = first_refused;
+    const T* p_row = p + n * a.p_place;
+    const T* q_row = n < length && q != nullptr ? q + n * a.q_place : nullptr;
+    const int gone = n < length && q == nullptr && tokens[n] >= 0 && tokens[n] < a.classes ? (int)tokens[n] : -1;
+    const int segments = parts * DV_WARPS, segment = rank * DV_WARPS + warp, nvec = a.classes / VEC;
+    const int v0 = (int)((long long)nvec * segment / segments), v1 = (int)((long long)nvec * (segment + 1) / segments);
+
+    // Weights of the classes of vector v; with `whole` those of p alone.
+    const auto weights = [&](int v, bool whole, double (&w)[VEC]) {
+        float f[VEC];
+        dv_load<T, VEC>(p_row + (size_t)v * VEC, f);
+        if (q_row == nullptr || whole) {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) w[j] = !whole && v * VEC + j == gone ? 0.0 : dv_positive(f[j]);
+        } else {
+            float g[VEC];
+            dv_load<T, VEC>(q_row + (size_t)v * VEC, g);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) w[j] = dv_positive((double)f[j] - (double)g[j]);
+        }
+    };
+    // Sums of all segments in the lanes of every warp, two a lane: what lies before them, and theirs.
+    double before = 0.0, mine[2], total = 0.0;
+    const auto sum_up = [&](bool whole, int turn) {
+        double s = 0.0;
+#pragma unroll 4
+        for (int v = v0 + lane; v < v1; v += 32) {
+            double w[VEC], part = 0.0;
+            weights(v, whole, w);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) part += w[j];
+            s += part;
+        }
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
+        if (lane < parts) cluster.map_shared_rank(&sums[turn][0], lane)[segment] = s;
+        cluster.sync();
+#pragma unroll
+        for (int i = 0; i < 2; ++i) mine[i] = 2 * lane + i < segments ? sums[turn][2 * lane + i] : 0.0;
+        const double all = dv_scan(mine[0] + mine[1], lane);
+        before = __shfl_up_sync(0xffffffffu, all, 1);
+        if (lane == 0) before = 0.0;
+        total = __shfl_sync(0xffffffffu, all, 31);
+    };
+    cluster.sync();      // all CTAs of the cluster have begun
+    sum_up(false, 0);
+    bool whole = false;
+    if (total == 0.0) {      // p nowhere above q: rounding alone, or probabilities that are none
+        whole = true;
+        sum_up(true, 1);
+    }
+    const double want = (double)u[a.drafts] * total;
+    if (rank == 0) {
+        for (int i = t; i <= a.drafts; i += DV_THREADS) {
+            if (i < n) a.out[b * (a.drafts + 1) + i] = tokens[i];
+            else if (i > n) a.out[b * (a.drafts + 1) + i] = -1;
+        }
+        if (t == 0) a.accepted[b] = n;
+    }
+    if (!(total > 0.0) || total > 1.7e308) {      // no class has a weight, or one has no finite one
+        if (rank == 0 && t == 0) a.out[b * (a.drafts + 1) + n] = -1;
+        return;
+    }
+    // The segment that holds the border, or, where rounding or u >= 1 leaves none, the last with a weight.
+    const double end0 = before + mine[0], end1 = end0 + mine[1];
+    const unsigned in0 = __ballot_sync(0xffffffffu, mine[0] > 0.0 && end0 > want), in1 = __ballot_sync(0xffffffffu, mine[1] > 0.0 && end1 > want);
+    const unsigned some0 = __ballot_sync(0xffffffffu, mine[0] > 0.0), some1 = __ballot_sync(0xffffffffu, mine[1] > 0.0);
+    int chosen;
+    if ((in0 | in1) != 0) {
+        const int l = __ffs(in0 | in1) - 1;
+        chosen = 2 * l + ((in0 >> l) & 1 ? 0 : 1);
+    } else {
+        const int l = 31 - __clz(some0 | some1);
+        chosen = 2 * l + ((some1 >> l) & 1);
+    }
+    if (chosen != segment) return;
+    double reached = __shfl_sync(0xffffffffu, (chosen & 1) ? end0 : before, chosen >> 1);
+    int last = -1, found = -1;
+    for (int base = v0; base < v1; base += 32) {
+        const int v = base + lane;
+        double w[VEC], own = 0.0;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) w[j] = 0.0;
+        if (v < v1) weights(v, whole, w);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) own += w[j];
+        const double upto = dv_scan(own, lane);
+        double at = reached + (upto - own);
+        int hit = -1;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            at += w[j];
+            if (w[j] > 0.0) {
+                last = v * VEC + j;
+                if (hit < 0 && at > want) hit = v * VEC + j;
+            }
+        }
+        const unsigned who = __ballot_sync(0xffffffffu, hit >= 0);
+        if (who != 0) {
+            found = __shfl_sync(0xffffffffu, hit, __ffs(who) - 1);
+            break;
+        }
+        reached += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    last = __reduce_max_sync(0xffffffffu, last);
+    if (lane == 0) a.out[b * (a.drafts + 1) + n] = found >= 0 ? found : last;
+}
+
+template <class T, int VEC> int launch_drafts(const DvArgs& a, long long sequences, cudaStream_t s) {
+    // A CTA takes at least some 2048 classes, and there are up to four an SM.
+    int parts = 1;
+    while (parts < DV_MOST_PARTS && a.classes >= 4096LL * parts && sequences * parts * 2 <= 4LL * sm_count()) parts *= 2;
+    return launch_clusters(dv_kernel<T, VEC>, (unsigned)(sequences * parts), DV_THREADS, 0, parts, s, a);
+}
+
+}  // namespace
+}  // namespace adder
+
+using namespace adder;
+
+extern "C" int adder_b200_verify_drafts(const void* target, const void* draft, int dtype, const long long* tokens, const float* uniforms,
+                                        const long long* lengths, long long* out_tokens, long long* accepted, long long sequences, long long drafts,
+                                        long long classes, long long target_sequence_stride, long long target_place_stride,
+                                        long long draft_sequence_stride, long long draft_place_stride, void* stream) {
+    if (sequences < 0 || drafts < 0 || classes <= 0) return ADDER_ERR_BAD_SHAPE;
+    if (target_sequence_stride < 0 || target_place_stride < 0 || draft_sequence_stride < 0 || draft_place_stride < 0) return ADDER_ERR_BAD_SHAPE;
+    if (dtype < ADDER_TYPE_F32 || dtype > ADDER_TYPE_F16) return ADDER_ERR_UNSUPPORTED;
+    if (classes > 2147483647LL - 1024 || drafts > 65535 || sequences > 2147483647LL / DV_MOST_PARTS) return ADDER_ERR_UNSUPPORTED;
+    if (sequences == 0) return ADDER_OK;
+    if (!target || !uniforms || !out_tokens || !accepted || (drafts > 0 && !tokens)) return ADDER_ERR_NULL_POINTER;
+    const unsigned size = dtype == ADDER_TYPE_F32 ? 4 : 2;
+    if (!aligned_to(target, size) || !aligned_to(draft, size) || !aligned_to(tokens, 8) || !aligned_to(lengths, 8) || !aligned_to(out_tokens, 8) ||
+        !aligned_to(accepted, 8) || !aligned_to(uniforms, 4))
+        return ADDER_ERR_ALIGNMENT;
+    const DvArgs a{target, draft, tokens, uniforms, lengths, out_tokens, accepted, target_sequence_stride, target_place_stride,
+                   draft_sequence_stride, draft_place_stride, (int)drafts, (int)classes};
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    return with_type(dtype, [&](auto* type) {
+        using T = std::remove_pointer_t<decltype(type)>;
+        constexpr int VE = Vec16<T>::N;
+        bool vectors = classes % VE == 0 && aligned_to(target, 16) && aligned_to(draft, 16);
+        for (long long stride : {target_sequence_stride, target_place_stride, draft_sequence_stride, draft_place_stride}) vectors = vectors && stride % VE == 0;
+        return vectors ? launch_drafts<T, VE>(a, sequences, s) : launch_drafts<T, 1>(a, sequences, s);
+    });
+}

@@ -10,6 +10,7 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/CUDAEvent.h>
@@ -19,6 +20,7 @@
 
 #include <array>
 #include <atomic>
+#include <cmath>
 #include <mutex>
 
 #include "../../include/adder_b200.h"
@@ -46,6 +48,15 @@ struct Api {      // entry points of the loaded libadder_b200.so
     decltype(&adder_b200_layernorm_backward) layernorm_backward = nullptr;
     decltype(&adder_b200_log_probs_forward) log_probs_forward = nullptr;
     decltype(&adder_b200_log_probs_backward) log_probs_backward = nullptr;
+    decltype(&adder_b200_rmsnorm_forward) rmsnorm_forward = nullptr;
+    decltype(&adder_b200_rmsnorm_forward_8bit) rmsnorm_forward_8bit = nullptr;
+    decltype(&adder_b200_rmsnorm_backward_workspace_bytes) rmsnorm_backward_workspace_bytes = nullptr;
+    decltype(&adder_b200_rmsnorm_backward) rmsnorm_backward = nullptr;
+    decltype(&adder_b200_quantize_rows) quantize_rows = nullptr;
+    decltype(&adder_b200_linear_8bit) linear_8bit = nullptr;
+    decltype(&adder_b200_distillation_forward) distillation_forward = nullptr;
+    decltype(&adder_b200_distillation_backward) distillation_backward = nullptr;
+    decltype(&adder_b200_verify_drafts) verify_drafts = nullptr;
     decltype(&adder_b200_adamw_step) adamw_step = nullptr;
 };
 // Written once, by the first bind to the product library, which is never unloaded: autograd nodes made by this path call through it
@@ -610,6 +621,191 @@ struct LogProbsNode : public torch::autograd::Function<LogProbsNode> {
     }
 };
 
+struct RmsResult { at::Tensor y, h, rstd; };
+
+RmsResult rms_forward(const at::Tensor& x, const at::Tensor& r, const at::Tensor& w, const Norm& n, bool keep) {
+    const c10::cuda::CUDAGuard guard(x.device());
+    RmsResult out;
+    out.y = empty_on(x, x.sizes(), x.scalar_type());
+    if (r.defined()) out.h = empty_on(x, x.sizes(), x.scalar_type());
+    if (keep) out.rstd = empty_on(x, {n.rows});
+    check(api.rmsnorm_forward(ptr(x), ptr(r), ptr(w), ptr(out.y), ptr(out.h), static_cast<float*>(ptr(out.rstd)), n.rows, n.d, n.x_stride,
+                              n.r_stride, n.type, n.weight_type, (float)n.eps, current_stream(x)), "adder_b200_rmsnorm_forward");
+    return out;
+}
+
+struct RmsNorm : public torch::autograd::Function<RmsNorm> {
+    static variable_list forward(AutogradContext* ctx, const Variable& x, const Optional& r, const Optional& w, const Norm& n) {
+        const at::Tensor none;
+        auto out = rms_forward(x, r.value_or(none), w.value_or(none), n, true);
+        ctx->save_for_backward({r ? out.h : x, w.value_or(none), out.rstd});
+        ctx->saved_data["sizes"] = std::vector<int64_t>{n.rows, n.d, n.type, n.weight_type, r.has_value()};
+        ctx->set_materialize_grads(false);
+        return r ? variable_list{out.y, out.h} : variable_list{out.y};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const Variable none;
+        const auto sizes = ctx->saved_data["sizes"].toIntVector();
+        const int64_t rows = sizes[0], d = sizes[1];
+        const int type = (int)sizes[2], weight_type = (int)sizes[3];
+        const bool has_r = sizes[4];
+        at::Tensor dy = grads[0], dh = has_r ? grads[1] : none;
+        if (!dy.defined() && !dh.defined()) return {none, none, none, none};
+        const auto saved = ctx->get_saved_variables();
+        const Variable &h = saved[0], &w = saved[1], &rstd = saved[2];
+        int64_t stride;
+        TORCH_CHECK(unwrapped(h) && type_code(h) == type && h.numel() == rows * d && plain(rstd) && rstd.numel() == rows && rstd.device() == h.device(), SAVED);
+        TORCH_CHECK(!w.defined() || (unwrapped(w) && w.is_contiguous() && type_code(w) == weight_type && w.numel() == d && w.device() == h.device()), SAVED);
+        const c10::cuda::CUDAGuard guard(h.device());
+        at::Tensor h2 = h;      // rows of consecutive elements
+        if (!rows_of(h, 1, d, &stride) || h.dim() == 0 || h.size(-1) != d) {
+            h2 = h.contiguous();
+            stride = d;
+        }
+        if (!dy.defined()) dy = at::zeros_like(h, at::MemoryFormat::Contiguous);
+        dy = whole_gradient(dy);
+        if (dh.defined()) dh = whole_gradient(dh);
+        for (const at::Tensor* g : {&dy, &dh})
+            TORCH_CHECK(!g->defined() || (g->scalar_type() == h.scalar_type() && g->device() == h.device() && g->sizes() == h.sizes()),
+                        "the gradient must have the type, device and shape of the output");
+        int edge = 0;
+        const bool need_x = ctx->needs_input_grad(edge++), need_r = has_r && ctx->needs_input_grad(edge++);
+        const bool need_w = w.defined() && ctx->needs_input_grad(edge++);
+        at::Tensor dx, dw, ws;
+        if (need_x || need_r) dx = empty_on(h, h.sizes(), h.scalar_type());
+        if (need_w) dw = empty_on(h, w.sizes(), w.scalar_type());
+        const size_t bytes = need_w ? api.rmsnorm_backward_workspace_bytes(rows, d) : 0;
+        if (bytes > 0) ws = empty_on(h, {(int64_t)bytes}, at::kByte);
+        check(api.rmsnorm_backward(ptr(dy), ptr(dh), ptr(h2), ptr(w), rstd.const_data_ptr<float>(), ptr(dx), ptr(dw), ptr(ws), bytes, rows, d, stride,
+                                   type, weight_type, current_stream(h)), "adder_b200_rmsnorm_backward");
+        const Variable& input = need_x || need_r ? h : none;      // h is an output as well, and asks for gradients whatever the inputs do
+        once("rms_norm", dx, {&dy, &dh, &input, &w});
+        once("rms_norm", dw, {&dy, &input});
+        return {need_x ? dx : none, need_r ? dx : none, dw, none};
+    }
+};
+
+struct Distill {      // a checked call
+    int64_t rows, classes, stride, ignore;
+    int type, teacher_type, k;
+    double temperature;
+};
+
+bool whole_long(const at::Tensor& t, const at::Device& dev) {
+    return unwrapped(t) && t.scalar_type() == at::kLong && t.is_contiguous() && t.device() == dev;
+}
+
+bool distill_of(const at::Tensor& x, const at::Tensor& teacher, const at::Tensor& indices, const at::Tensor* targets, Distill* n) {
+    n->type = type_code(x);
+    n->teacher_type = type_code(teacher);
+    if (n->type < 0 || n->teacher_type < 0 || !unwrapped(x) || x.dim() < 1 || x.numel() == 0) return false;
+    n->classes = x.size(-1);
+    n->rows = x.numel() / n->classes;
+    if (!rows_of(x, 1, n->classes, &n->stride) || !(n->temperature > 0.0) || !std::isfinite(n->temperature)) return false;
+    const auto lead = x.sizes().slice(0, x.dim() - 1);
+    if (!unwrapped(teacher) || !teacher.is_contiguous() || teacher.device() != x.device() || teacher.dim() != x.dim() ||
+        teacher.sizes().slice(0, lead.size()) != lead || teacher.size(-1) < 1 || teacher.size(-1) > 256 || (at::GradMode::is_enabled() && teacher.requires_grad()))
+        return false;
+    n->k = (int)teacher.size(-1);
+    return whole_long(indices, x.device()) && indices.sizes() == teacher.sizes() && (targets == nullptr || (whole_long(*targets, x.device()) && targets->sizes() == lead));
+}
+
+struct DistillResult { at::Tensor divergence, log_prob, stats, mass; };
+
+DistillResult distill_forward(const at::Tensor& x, const at::Tensor& teacher, const at::Tensor& indices, const at::Tensor& targets, const Distill& n, bool keep) {
+    const c10::cuda::CUDAGuard guard(x.device());
+    DistillResult out;
+    const auto lead = x.sizes().slice(0, x.dim() - 1);
+    out.divergence = empty_on(x, lead);
+    if (targets.defined()) out.log_prob = empty_on(x, lead);
+    if (keep) {
+        out.stats = empty_on(x, {n.rows, 3});
+        out.mass = empty_on(x, {n.rows, n.k});
+    }
+    check(api.distillation_forward(ptr(x), n.type, n.rows, n.classes, n.stride, ptr(teacher), n.teacher_type,
+                                   static_cast<const long long*>(ptr(indices)), n.k, (float)n.temperature, static_cast<const long long*>(ptr(targets)), n.ignore, static_cast<float*>(ptr(out.divergence)),
+                                   static_cast<float*>(ptr(out.log_prob)), static_cast<float*>(ptr(out.stats)), static_cast<float*>(ptr(out.mass)),
+                                   current_stream(x)), "adder_b200_distillation_forward");
+    return out;
+}
+
+struct DistillNode : public torch::autograd::Function<DistillNode> {
+    static variable_list forward(AutogradContext* ctx, const Variable& x, const at::Tensor& teacher, const at::Tensor& indices, const Optional& targets,
+                                 const Distill& n) {
+        const at::Tensor none;
+        auto out = distill_forward(x, teacher, indices, targets.value_or(none), n, true);
+        ctx->save_for_backward({x, indices, targets.value_or(none), out.stats, out.mass});
+        ctx->saved_data["args"] = std::vector<int64_t>{n.rows, n.classes, n.ignore, n.type, n.k, targets.has_value()};
+        ctx->saved_data["temperature"] = n.temperature;
+        ctx->set_materialize_grads(false);
+        variable_list list{out.divergence};
+        if (targets) list.push_back(out.log_prob);
+        return list;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const Variable none;
+        const auto a = ctx->saved_data["args"].toIntVector();
+        const int64_t rows = a[0], classes = a[1], ignore = a[2];
+        const int type = (int)a[3], k = (int)a[4];
+        at::Tensor g_div = grads[0], g_lp = a[5] ? grads[1] : none;
+        if (!g_div.defined() && !g_lp.defined()) return {none, none, none, none, none};
+        const auto saved = ctx->get_saved_variables();
+        const Variable &x = saved[0], &indices = saved[1], &targets = saved[2], &stats = saved[3], &mass = saved[4];
+        TORCH_CHECK(unwrapped(x) && type_code(x) == type && x.dim() >= 1 && x.size(-1) == classes && x.numel() == rows * classes && plain(stats) &&
+                    stats.numel() == 3 * rows && stats.device() == x.device() && plain(mass) && mass.numel() == rows * k && mass.device() == x.device(), SAVED);
+        TORCH_CHECK(whole_long(indices, x.device()) && indices.numel() == rows * k && (!a[5] || (whole_long(targets, x.device()) && targets.numel() == rows)), SAVED);
+        const c10::cuda::CUDAGuard guard(x.device());
+        for (at::Tensor* g : {&g_div, &g_lp})
+            if (g->defined()) {
+                *g = whole_gradient(*g);
+                TORCH_CHECK(g->scalar_type() == at::kFloat && g->device() == x.device() && g->numel() == rows,
+                            "the gradient must be a float32 tensor of the output's shape and device");
+            }
+        at::Tensor x2 = x;
+        int64_t stride;
+        if (!rows_of(x, 1, classes, &stride)) {
+            x2 = x.contiguous();
+            stride = classes;
+        }
+        at::Tensor dx = empty_on(x, x.sizes(), x.scalar_type());
+        check(api.distillation_backward(ptr(x2), type, rows, classes, stride, static_cast<const long long*>(ptr(indices)), k,
+                                        (float)ctx->saved_data["temperature"].toDouble(), static_cast<const long long*>(ptr(targets)), ignore,
+                                        stats.const_data_ptr<float>(), mass.const_data_ptr<float>(), static_cast<const float*>(ptr(g_div)),
+                                        static_cast<const float*>(ptr(g_lp)), ptr(dx), current_stream(x)), "adder_b200_distillation_backward");
+        once("distillation", dx, {&x, &g_div, &g_lp});
+        return {dx, none, none, none, none};
+    }
+};
+
+// Codes whose rows begin at multiples of 16 bytes.
+struct Codes {
+    at::Tensor values;
+    int64_t stride;
+};
+Codes empty_codes(const at::Tensor& like, at::IntArrayRef sizes) {
+    c10::SmallVector<int64_t, 5> whole(sizes.begin(), sizes.end());
+    const int64_t d = whole.back(), stride = (d + 15) / 16 * 16;
+    whole.back() = stride;
+    at::Tensor t = empty_on(like, whole, at::kFloat8_e4m3fn);
+    return {stride == d ? t : t.slice(-1, 0, d), stride};
+}
+at::Tensor empty_scales(const at::Tensor& like, at::IntArrayRef sizes) {
+    c10::SmallVector<int64_t, 5> whole(sizes.begin(), sizes.end());
+    whole.back() = (whole.back() + 127) / 128;
+    return empty_on(like, whole);
+}
+// Codes as the product takes them; false: they have to be copied, or are none.
+bool codes_of(const at::Tensor& values, const at::Tensor& scales, int64_t* rows, int64_t* stride) {
+    if (!unwrapped(values) || values.scalar_type() != at::kFloat8_e4m3fn || values.dim() < 1 || values.numel() == 0 || !plain(scales) ||
+        scales.device() != values.device() || scales.dim() != values.dim())
+        return false;
+    const int64_t d = values.size(-1);
+    *rows = values.numel() / d;
+    if (!rows_of(values, 1, d, stride)) return false;
+    if (*rows == 1) *stride = (d + 15) / 16 * 16;
+    return *stride % 16 == 0 && *stride >= d && ((uintptr_t)values.data_ptr() & 15) == 0 && scales.size(-1) == (d + 127) / 128;
+}
+
 // ------------------------------------------------------------------------------------------ Python entry points
 
 const at::Tensor* tensor_arg(PyObject* o) { return THPVariable_CheckExact(o) ? &THPVariable_Unpack(o) : nullptr; }
@@ -842,6 +1038,194 @@ PyObject* py_log_probs(PyObject*, PyObject* const* args, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// rms_norm(x, residual or None, weight or None, shape, eps) -> y, or (y, h) with a residual, or None
+PyObject* py_rms_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 5 || !available()) Py_RETURN_NONE;
+    const at::Tensor *x = tensor_arg(args[0]), *r, *w;
+    double eps;
+    if (x == nullptr || !optional_tensor(args[1], &r) || !optional_tensor(args[2], &w) || !PyTuple_CheckExact(args[3]) || !double_arg(args[4], &eps))
+        Py_RETURN_NONE;
+    c10::SmallVector<int64_t, 5> shape(PyTuple_GET_SIZE(args[3]));
+    for (size_t i = 0; i < shape.size(); ++i)
+        if (!int_arg(PyTuple_GET_ITEM(args[3], i), &shape[i])) Py_RETURN_NONE;
+    Norm c;
+    if (!norm_of(*x, r, w, nullptr, shape, eps, &c)) Py_RETURN_NONE;
+    at::Tensor y, h;
+    {
+        pybind11::gil_scoped_release no_gil;
+        bool node = false;
+        if (at::GradMode::is_enabled())
+            for (const at::Tensor* t : {x, r, w}) node = node || (t != nullptr && t->requires_grad());
+        if (node) {
+            auto out = RmsNorm::apply(*x, optional(r), optional(w), c);
+            y = out[0];
+            if (r != nullptr) h = out[1];
+        } else {
+            const at::Tensor none;
+            auto out = rms_forward(*x, r != nullptr ? *r : none, w != nullptr ? *w : none, c, false);
+            y = out.y; h = out.h;
+        }
+    }
+    if (r == nullptr) return THPVariable_Wrap(std::move(y));
+    return Py_BuildValue("(NN)", THPVariable_Wrap(std::move(y)), THPVariable_Wrap(std::move(h)));
+    END_HANDLE_TH_ERRORS
+}
+
+// rms_norm_8bit(x, weight or None, eps, residual or None) -> (values, scales, h or None), or None
+PyObject* py_rms_norm_8bit(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 4 || !available()) Py_RETURN_NONE;
+    const at::Tensor *x = tensor_arg(args[0]), *r, *w;
+    double eps;
+    if (x == nullptr || !optional_tensor(args[1], &w) || !double_arg(args[2], &eps) || !optional_tensor(args[3], &r) || x->dim() < 1) Py_RETURN_NONE;
+    Norm c;
+    if (!norm_of(*x, r, w, nullptr, x->sizes().slice(x->dim() - 1), eps, &c)) Py_RETURN_NONE;
+    if (at::GradMode::is_enabled())
+        for (const at::Tensor* t : {x, r, w})
+            if (t != nullptr && t->requires_grad()) Py_RETURN_NONE;
+    Codes y;
+    at::Tensor scales, h;
+    {
+        pybind11::gil_scoped_release no_gil;
+        const c10::cuda::CUDAGuard guard(x->device());
+        const at::Tensor none;
+        y = empty_codes(*x, x->sizes());
+        scales = empty_scales(*x, x->sizes());
+        if (r != nullptr) h = empty_on(*x, x->sizes(), x->scalar_type());
+        check(api.rmsnorm_forward_8bit(ptr(*x), ptr(r != nullptr ? *r : none), ptr(w != nullptr ? *w : none), ptr(y.values), scales.mutable_data_ptr<float>(), ptr(h),
+                                       c.rows, c.d, c.x_stride, c.r_stride, y.stride, c.type, c.weight_type, (float)eps, current_stream(*x)),
+              "adder_b200_rmsnorm_forward_8bit");
+    }
+    return Py_BuildValue("(NNN)", THPVariable_Wrap(std::move(y.values)), THPVariable_Wrap(std::move(scales)), wrap_or_none(std::move(h)));
+    END_HANDLE_TH_ERRORS
+}
+
+// Both tensors of a pair such as Rows8
+bool pair_arg(PyObject* o, const at::Tensor** a, const at::Tensor** b) {
+    if (!PyTuple_Check(o) || PyTuple_GET_SIZE(o) != 2) return false;
+    *a = tensor_arg(PyTuple_GET_ITEM(o, 0));
+    *b = tensor_arg(PyTuple_GET_ITEM(o, 1));
+    return *a != nullptr && *b != nullptr;
+}
+
+// linear_8bit(x or (values, scales), (values, scales), bias or None, dtype or None) -> y, or None
+PyObject* py_linear_8bit(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 4 || !available()) Py_RETURN_NONE;
+    const at::Tensor *x = tensor_arg(args[0]), *xv = nullptr, *xs = nullptr, *wv, *ws, *bias;
+    if ((x == nullptr && !pair_arg(args[0], &xv, &xs)) || !pair_arg(args[1], &wv, &ws) || !optional_tensor(args[2], &bias)) Py_RETURN_NONE;
+    at::ScalarType out_type = x != nullptr ? x->scalar_type() : at::kBFloat16;
+    if (args[3] != Py_None) {
+        if (!THPDtype_Check(args[3])) Py_RETURN_NONE;
+        out_type = reinterpret_cast<THPDtype*>(args[3])->scalar_type;
+    }
+    const int out_code = out_type == at::kFloat ? ADDER_TYPE_F32 : out_type == at::kBFloat16 ? ADDER_TYPE_BF16 : out_type == at::kHalf ? ADDER_TYPE_F16 : -1;
+    int64_t outer, w_stride, rows, x_stride;
+    if (out_code < 0 || !codes_of(*wv, *ws, &outer, &w_stride) || wv->dim() != 2 || ws->size(0) != (outer + 127) / 128) Py_RETURN_NONE;
+    const int64_t inner = wv->size(1);
+    const at::Tensor& first = x != nullptr ? *x : *xv;
+    if (first.dim() < 1 || first.size(-1) != inner || first.device() != wv->device()) Py_RETURN_NONE;
+    const auto lead = first.sizes().slice(0, first.dim() - 1);
+    int type = 0;
+    if (x != nullptr) {
+        type = type_code(*x);
+        if (type < 0 || !unwrapped(*x) || x->numel() == 0 || !rows_of(*x, 1, inner, &x_stride) || needs_node(*x, *x)) Py_RETURN_NONE;
+        rows = x->numel() / inner;
+    } else if (!codes_of(*xv, *xs, &rows, &x_stride) || xs->sizes().slice(0, lead.size()) != lead) {
+        Py_RETURN_NONE;
+    }
+    if (bias != nullptr && (!unwrapped(*bias) || !bias->is_contiguous() || bias->device() != wv->device() || bias->scalar_type() != out_type || bias->dim() != 1 ||
+                            bias->size(0) != outer || needs_node(*bias, *bias)))
+        Py_RETURN_NONE;
+    at::Tensor y;
+    {
+        pybind11::gil_scoped_release no_gil;
+        const c10::cuda::CUDAGuard guard(wv->device());
+        const cudaStream_t stream = current_stream(*wv);
+        at::Tensor values, scales;
+        if (x != nullptr) {
+            Codes codes = empty_codes(*x, {rows, inner});
+            values = codes.values;
+            scales = empty_scales(*x, {rows, inner});
+            check(api.quantize_rows(ptr(*x), static_cast<unsigned char*>(ptr(values)), scales.mutable_data_ptr<float>(), rows, inner, x_stride, codes.stride, type, stream),
+                  "adder_b200_quantize_rows");
+            x_stride = codes.stride;
+        } else {
+            values = *xv;
+            scales = *xs;
+        }
+        c10::SmallVector<int64_t, 5> sizes(lead.begin(), lead.end());
+        sizes.push_back(outer);
+        y = empty_on(*wv, sizes, out_type);
+        const at::Tensor none;
+        check(api.linear_8bit(static_cast<const unsigned char*>(ptr(values)), scales.const_data_ptr<float>(), static_cast<const unsigned char*>(ptr(*wv)),
+                              ws->const_data_ptr<float>(), ptr(bias != nullptr ? *bias : none), ptr(y), rows, inner, outer, x_stride, w_stride, out_code, stream),
+              "adder_b200_linear_8bit");
+    }
+    return THPVariable_Wrap(std::move(y));
+    END_HANDLE_TH_ERRORS
+}
+
+// distillation(logits, teacher, indices, temperature, targets or None, ignore_index) -> (divergence, log_prob or None), or None
+PyObject* py_distillation(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 6 || !available()) Py_RETURN_NONE;
+    const at::Tensor *x = tensor_arg(args[0]), *teacher = tensor_arg(args[1]), *indices = tensor_arg(args[2]), *targets;
+    Distill c;
+    if (x == nullptr || teacher == nullptr || indices == nullptr || !double_arg(args[3], &c.temperature) || !optional_tensor(args[4], &targets) ||
+        !int_arg(args[5], &c.ignore) || !distill_of(*x, *teacher, *indices, targets, &c))
+        Py_RETURN_NONE;
+    at::Tensor divergence, log_prob;
+    {
+        pybind11::gil_scoped_release no_gil;
+        if (at::GradMode::is_enabled() && x->requires_grad()) {
+            auto list = DistillNode::apply(*x, *teacher, *indices, optional(targets), c);
+            divergence = list[0];
+            if (targets != nullptr) log_prob = list[1];
+        } else {
+            const at::Tensor none;
+            auto r = distill_forward(*x, *teacher, *indices, targets != nullptr ? *targets : none, c, false);
+            divergence = r.divergence; log_prob = r.log_prob;
+        }
+    }
+    return Py_BuildValue("(NN)", THPVariable_Wrap(std::move(divergence)), wrap_or_none(std::move(log_prob)));
+    END_HANDLE_TH_ERRORS
+}
+
+// verify_drafts(target_probs, draft_probs or None, draft_tokens, uniforms, lengths or None) -> (tokens, accepted), or None
+PyObject* py_verify_drafts(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 5 || !available()) Py_RETURN_NONE;
+    const at::Tensor *p = tensor_arg(args[0]), *q, *tokens = tensor_arg(args[2]), *u = tensor_arg(args[3]), *lengths;
+    if (p == nullptr || !optional_tensor(args[1], &q) || tokens == nullptr || u == nullptr || !optional_tensor(args[4], &lengths)) Py_RETURN_NONE;
+    const int type = type_code(*p);
+    if (type < 0 || !unwrapped(*p) || p->dim() != 3 || p->numel() == 0) Py_RETURN_NONE;
+    const int64_t b = p->size(0), places = p->size(1), classes = p->size(2);
+    const std::array<int64_t, 3> of_draft{b, places - 1, classes};
+    if (q != nullptr && (!unwrapped(*q) || q->device() != p->device() || q->scalar_type() != p->scalar_type() || q->sizes() != at::IntArrayRef(of_draft))) Py_RETURN_NONE;
+    for (const at::Tensor* t : {p, q})
+        if (t != nullptr && classes > 1 && t->stride(2) != 1) Py_RETURN_NONE;
+    if (!whole_long(*tokens, p->device()) || tokens->dim() != 2 || tokens->size(0) != b || tokens->size(1) != places - 1 || !plain(*u) || u->device() != p->device() ||
+        u->dim() != 2 || u->size(0) != b || u->size(1) != places)
+        Py_RETURN_NONE;
+    if (lengths != nullptr && (!whole_long(*lengths, p->device()) || lengths->dim() != 1 || lengths->size(0) != b)) Py_RETURN_NONE;
+    at::Tensor out, accepted;
+    {
+        pybind11::gil_scoped_release no_gil;
+        const c10::cuda::CUDAGuard guard(p->device());
+        const at::Tensor none;
+        out = empty_on(*p, {b, places}, at::kLong);
+        accepted = empty_on(*p, {b}, at::kLong);
+        check(api.verify_drafts(ptr(*p), ptr(q != nullptr ? *q : none), type, static_cast<const long long*>(ptr(*tokens)), u->const_data_ptr<float>(),
+                                lengths != nullptr ? static_cast<const long long*>(ptr(*lengths)) : nullptr, static_cast<long long*>(ptr(out)),
+                                static_cast<long long*>(ptr(accepted)), b, places - 1, classes, p->stride(0), p->stride(1), q != nullptr ? q->stride(0) : 0,
+                                q != nullptr ? q->stride(1) : 0, current_stream(*p)), "adder_b200_verify_drafts");
+    }
+    return Py_BuildValue("(NN)", THPVariable_Wrap(std::move(out)), THPVariable_Wrap(std::move(accepted)));
+    END_HANDLE_TH_ERRORS
+}
+
 // The addresses that one step writes to: no two may be equal.
 class Addresses {
 public:
@@ -997,6 +1381,15 @@ PyObject* py_bind(PyObject*, PyObject* const* args, Py_ssize_t n) {
         get("adder_b200_layernorm_backward", &a.layernorm_backward);
         get("adder_b200_log_probs_forward", &a.log_probs_forward);
         get("adder_b200_log_probs_backward", &a.log_probs_backward);
+        get("adder_b200_rmsnorm_forward", &a.rmsnorm_forward);
+        get("adder_b200_rmsnorm_forward_8bit", &a.rmsnorm_forward_8bit);
+        get("adder_b200_rmsnorm_backward_workspace_bytes", &a.rmsnorm_backward_workspace_bytes);
+        get("adder_b200_rmsnorm_backward", &a.rmsnorm_backward);
+        get("adder_b200_quantize_rows", &a.quantize_rows);
+        get("adder_b200_linear_8bit", &a.linear_8bit);
+        get("adder_b200_distillation_forward", &a.distillation_forward);
+        get("adder_b200_distillation_backward", &a.distillation_backward);
+        get("adder_b200_verify_drafts", &a.verify_drafts);
         get("adder_b200_adamw_step", &a.adamw_step);
         api = a;
     }
@@ -1012,6 +1405,8 @@ PyObject* py_bind(PyObject*, PyObject* const* args, Py_ssize_t n) {
 PyMethodDef methods[] = {ADDER_METHOD("bind", py_bind), ADDER_METHOD("layer", py_layer), ADDER_METHOD("conv", py_conv), ADDER_METHOD("layer_with_stats", py_layer_with_stats),
                          ADDER_METHOD("layer_affine", py_layer_affine), ADDER_METHOD("affine", py_affine), ADDER_METHOD("column", py_column),
                          ADDER_METHOD("layer_norm", py_layer_norm), ADDER_METHOD("log_probs", py_log_probs), ADDER_METHOD("adamw", py_adamw),
+                         ADDER_METHOD("rms_norm", py_rms_norm), ADDER_METHOD("rms_norm_8bit", py_rms_norm_8bit), ADDER_METHOD("linear_8bit", py_linear_8bit),
+                         ADDER_METHOD("distillation", py_distillation), ADDER_METHOD("verify_drafts", py_verify_drafts),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_adder_host", nullptr, -1, methods};
 

@@ -21,7 +21,7 @@
 // whose row stride is not the number of classes) it goes element by element: 2048x50257 in rows of 50304 288 us bf16 and 260 fp32, where
 // dense rows take 74 and 126.
 #include "kernels.h"
-#include "elements.cuh"
+#include "softmax.cuh"
 #include <cooperative_groups.h>
 #include <type_traits>
 
@@ -35,18 +35,6 @@ constexpr int LP_TEAM = 256;            // threads that stream one row; a CTA ha
 constexpr int LP_UNROLL = 4;            // backward: vectors that a thread has in flight
 constexpr int LP_GROUP = 4, LP_STAGES = 2;      // forward: vectors of a thread that are taken together, groups of them on their way or in use
 constexpr float LP_FLOOR = -200.f;      // 2^-200 is 0 in fp32: stands for exponents of -inf where 0 * -inf would be NaN
-constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
-
-__device__ __forceinline__ float max_nan(float a, float b) {
-    float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ float exp2_fast(float x) {
-    float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
-}
 
 // A key orders elements by value, then by index from the lowest: no two are equal.  0 is below all of them.
 __device__ __forceinline__ uint64_t key_of(float v, uint32_t index) {
@@ -143,31 +131,6 @@ __device__ __forceinline__ void join(float& m, float& s, float& t, float m2, flo
     t = (t + s * d1) * f1 + (t2 + s2 * d2) * f2;
     s = s * f1 + s2 * f2;
     m = M;
-}
-
-template <class T> __device__ __forceinline__ uint32_t max_pair(uint32_t a, uint32_t b);
-template <> __device__ __forceinline__ uint32_t max_pair<__nv_bfloat16>(uint32_t a, uint32_t b) {
-    uint32_t r;
-    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-    return r;
-}
-template <> __device__ __forceinline__ uint32_t max_pair<__half>(uint32_t a, uint32_t b) {
-    uint32_t r;
-    asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-    return r;
-}
-// The largest of a vector's values, NaN if one is: as a word of its type, so that 16-bit values are compared in pairs.
-template <class T> __device__ __forceinline__ uint32_t max_word(uint32_t a, uint32_t b) {
-    if constexpr (sizeof(T) == 4) return __float_as_uint(max_nan(__uint_as_float(a), __uint_as_float(b)));
-    else return max_pair<T>(a, b);
-}
-template <class T> __device__ __forceinline__ float word_max(uint32_t w) {
-    if constexpr (sizeof(T) == 4) {
-        return __uint_as_float(w);
-    } else {
-        const float2 p = unpack_pair<T>(w);
-        return max_nan(p.x, p.y);
-    }
 }
 
 // A thread's maximum m with s = sum 2^d and t = sum 2^d d over its values x, d = x log2(e) - ref.  ref is m log2(e) rounded (one fused

@@ -7,6 +7,7 @@ What the reference's test.py does around a trained network, without its dataset 
     map it is (running statistics are constants), applied together with the residual add and ReLU of the
     block in ONE kernel behind each adder layer (the adder output is not linear in the weights, so the
     affine map cannot move into them; it becomes the layer's epilogue instead);
+  * `quantize_linear` puts the multiply-based linear layers' weights in 8 bits, for products on the fp8 tensor cores;
   * `accuracy` / `validate` are test.py:68-126: top-1 / top-5 over batches, no gradients; `evaluate` gives them with the mean loss and
     entropy from one pass over the logits.
 """
@@ -18,6 +19,7 @@ import torch
 import torch.nn as nn
 
 from . import _lib, _native, adder_cuda
+from .linear8 import Linear8bit
 from .logprobs import token_log_probs
 
 
@@ -75,6 +77,25 @@ def fold_batchnorm(model: nn.Module) -> nn.Module:
         for name, child in list(module.named_children()):
             if isinstance(child, nn.BatchNorm2d):
                 setattr(module, name, FoldedBatchNorm2d(child))
+            else:
+                convert(child)
+
+    convert(model)
+    return model
+
+
+def quantize_linear(model: nn.Module) -> nn.Module:
+    """Replace, in place, every multiply-based linear layer of `model` (on CUDA) - nn.Linear, and 1x1 nn.Conv2d of stride 1 and one group without
+    padding, as the `fc` of `addernetcuda_b200.resnet` - by a `linear8.Linear8bit` with its weight in 8 bits, and put the model in evaluation
+    mode.  Adder layers stay as they are: their |x - w| is no product.  Subclasses of the two stay, too."""
+    model.eval()
+
+    def convert(module: nn.Module):
+        for name, child in list(module.named_children()):
+            pointwise = type(child) is nn.Conv2d and child.kernel_size == (1, 1) and child.stride == (1, 1) and child.groups == 1 and \
+                child.padding in ((0, 0), "valid")
+            if type(child) is nn.Linear or pointwise:
+                setattr(module, name, Linear8bit(child))
             else:
                 convert(child)
 

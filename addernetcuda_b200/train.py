@@ -19,7 +19,9 @@ class TrainStep:
 
     `optimizer` is "sgd" (with `momentum`), "adamw" or "adamw8" (`optim.AdamW` with states in 32 or 8 bits), or a function of the
     parameters that returns a torch.optim.Optimizer; `criterion` a module of (logits, labels), nn.CrossEntropyLoss where it is None
-    (`logprobs.TokenCrossEntropy` is this library's own).
+    (`logprobs.TokenCrossEntropy` is this library's own).  With a `teacher`, a network of the same classes on the same device, which is put
+    in evaluation mode and runs without gradients, the criterion is called with its best classes, too: (logits, labels, teacher_logits,
+    teacher_indices), `criterion.top_k` of them; `distill.DistillationLoss()` where it is None.
 
     step(images, labels) copies the batch into the static buffers (from pinned host memory when the
     inputs are CPU tensors), runs the step (graph replay when `use_graph`), and returns the loss as
@@ -28,7 +30,7 @@ class TrainStep:
 
     def __init__(self, model: nn.Module, batch_shape, num_classes: int, lr: float = 0.1, momentum: float = 0.9,
                  weight_decay: float = 0.0, ddp=None, use_graph: bool = True, device="cuda:0", optimizer="sgd",
-                 criterion: Optional[nn.Module] = None):
+                 criterion: Optional[nn.Module] = None, teacher: Optional[nn.Module] = None):
         from . import strict_fp32
         strict_fp32()          # the benchmark configurations are fp32 end to end
         self.model = model
@@ -38,6 +40,10 @@ class TrainStep:
         self.labels = torch.zeros(batch_shape[0], dtype=torch.long, device=self.device)
         self.num_classes = num_classes
         self.opt = self._make_optimizer(optimizer, lr, momentum, weight_decay)
+        self.teacher = teacher.eval() if teacher is not None else None
+        if criterion is None and teacher is not None:
+            from .distill import DistillationLoss
+            criterion = DistillationLoss()
         self.criterion = criterion if criterion is not None else nn.CrossEntropyLoss()
         self.loss = torch.zeros((), device=self.device)
         self.logits: Optional[torch.Tensor] = None
@@ -63,7 +69,7 @@ class TrainStep:
         else:
             self.opt.zero_grad(set_to_none=True)
         logits = self.model(self.images)
-        loss = self.criterion(logits, self.labels)
+        loss = self.criterion(logits, self.labels, *self._teaching())
         loss.backward()
         if self.ddp is not None:
             self.ddp.finish()
@@ -71,6 +77,16 @@ class TrainStep:
             self.opt.step()
         self.logits = logits.detach()
         self.loss.copy_(loss.detach())
+
+    def _teaching(self) -> tuple:
+        """The teacher's best classes of the batch: their log probabilities, which serve as logits, and indices."""
+        if self.teacher is None:
+            return ()
+        from .logprobs import token_log_probs
+        with torch.no_grad():
+            logits = self.teacher(self.images)
+            best = token_log_probs(logits, top_k=min(self.criterion.top_k, logits.shape[-1]))
+        return best.top_log_probs, best.top_indices
 
     def warmup(self, iters: int = 3) -> None:
         """Eager iterations on a side stream (required before capture); they do update the weights."""

@@ -286,6 +286,71 @@ ADDER_API int adder_b200_log_probs_backward(const void* logits, int dtype, long 
                                             const float* stats, const float* entropy, const float* grad_log_prob,
                                             const float* grad_entropy, const float* grad_top, void* grad_logits, void* stream);
 
+/* RMS norm of rows of d elements: h = x + residual, rounded to the element type (x where residual is NULL, and h then may be NULL),
+ * y = h / sqrt(mean(h^2) + eps) * weight.  x and residual have x_stride and residual_stride elements from row to row, consecutive within one;
+ * y and h are contiguous.  weight [d] is of weight_dtype (dtype or fp32), NULL: 1.  rstd [rows] is kept for the backward call, or NULL.
+ * Sums are fp32; rows whose squares overflow give 0, as 1 / infinity does. */
+ADDER_API int adder_b200_rmsnorm_forward(const void* x, const void* residual, const void* weight, void* y, void* h, float* rstd, long long rows,
+                                         long long d, long long x_stride, long long residual_stride, int dtype, int weight_dtype, float eps,
+                                         void* stream);
+/* The same with y in 8 bits: values[row][values_stride] e4m3 codes, scales[row][ceil(d / 128)], y = code * scale.  With a the largest
+ * magnitude of 128 columns of a row, before any rounding of y to fewer than 32 bits: scale = a * (1 / 448), code = e4m3(y * (1 / a * 448)), each
+ * operation rounded to fp32 and the code to nearest even; zeros where a < 2^-100.  128 columns with a NaN or an infinity stand for NaN. */
+ADDER_API int adder_b200_rmsnorm_forward_8bit(const void* x, const void* residual, const void* weight, void* values, float* scales, void* h,
+                                              long long rows, long long d, long long x_stride, long long residual_stride,
+                                              long long values_stride, int dtype, int weight_dtype, float eps, void* stream);
+/* Gradients from dy (and dh, that of h itself, or NULL): dx [rows][d], that of x and of the residual, and dweight [d], whose workspace it
+ * is; either may be NULL.  dy, dh and dx are contiguous, h (x where there was no residual) has h_stride. */
+ADDER_API size_t adder_b200_rmsnorm_backward_workspace_bytes(long long rows, long long d);
+ADDER_API int adder_b200_rmsnorm_backward(const void* dy, const void* dh, const void* h, const void* weight, const float* rstd, void* dx,
+                                          void* dweight, void* workspace, size_t workspace_bytes, long long rows, long long d,
+                                          long long h_stride, int dtype, int weight_dtype, void* stream);
+
+/* Tensors in 8 bits, in the form of adder_b200_rmsnorm_forward_8bit: rows with a scale for each 128 columns (scales[rows][ceil(d / 128)]),
+ * a weight with one for each 128 x 128 (scales[ceil(rows / 128)][ceil(d / 128)]).  values_stride >= d. */
+ADDER_API int adder_b200_quantize_rows(const void* x, unsigned char* values, float* scales, long long rows, long long d, long long x_stride,
+                                       long long values_stride, int dtype, void* stream);
+ADDER_API int adder_b200_quantize_weight(const void* w, unsigned char* values, float* scales, long long rows, long long d, long long w_stride,
+                                         long long values_stride, int dtype, void* stream);
+/* y[tokens][outer] (contiguous, of type dtype) = x w^T + bias of two tensors in 8 bits, x [tokens][inner] with a scale for each 128 columns
+ * (contiguous), w [outer][inner] with one for each 128 x 128; bias [outer] of type dtype, or NULL.  Sums are fp32, y is rounded once.
+ * x and w begin at multiples of 16 bytes, and so do their rows (x_stride, w_stride); what lies behind a row's last column is not read
+ * as a value. */
+ADDER_API int adder_b200_linear_8bit(const unsigned char* x, const float* x_scales, const unsigned char* w, const float* w_scales,
+                                     const void* bias, void* y, long long tokens, long long inner, long long outer, long long x_stride,
+                                     long long w_stride, int dtype, void* stream);
+
+/* Distillation from a teacher's k <= 256 best classes of each row.  With t = softmax(teacher / temperature) over the classes indices[row][k]
+ * (-1: none, which may stand anywhere; a class may stand twice) and p = softmax(logits / temperature) over all of the row:
+ *   divergence[row]  sum of t (ln t - ln p): 0 where the teacher names no class or all its logits are -inf, +inf where p is 0 and t is not, NaN
+ *                    where an index is no class or below -1, or a logit of the teacher's is NaN or +inf
+ *   log_prob[row]    log softmax(logits) at targets[row]: 0 where the target is ignore_index, NaN where it is no class; with targets alone
+ * logits as those of adder_b200_log_probs_forward.  stats[row][3] and mass[row][k] (t) are kept for the backward call; both or neither. */
+ADDER_API int adder_b200_distillation_forward(const void* logits, int dtype, long long rows, long long classes, long long row_stride,
+                                              const void* teacher, int teacher_dtype, const long long* indices, int k, float temperature,
+                                              const long long* targets, long long ignore_index, float* divergence, float* log_prob,
+                                              float* stats, float* mass, void* stream);
+/* grad_logits (contiguous, of the logits' type) <- the gradient of sum(grad_divergence * divergence + grad_log_prob * log_prob); gradients
+ * that are NULL count as zeros.  Rows of nothing but -inf get zeros. */
+ADDER_API int adder_b200_distillation_backward(const void* logits, int dtype, long long rows, long long classes, long long row_stride,
+                                               const long long* indices, int k, float temperature, const long long* targets,
+                                               long long ignore_index, const float* stats, const float* mass, const float* grad_divergence,
+                                               const float* grad_log_prob, void* grad_logits, void* stream);
+
+/* Drafted tokens of sequences against a target's probabilities.  target[sequence][drafts + 1][classes] and draft[sequence][drafts][classes]
+ * (of one type, consecutive classes, the other strides in elements; draft NULL: a drafter that gives its tokens probability 1),
+ * tokens[sequence][drafts], uniforms[sequence][drafts + 1] in [0, 1), lengths[sequence] drafts each (NULL: all; clipped to 0 .. drafts):
+ *   accepted[sequence]            the first i with not (uniforms[i] * draft_i(tokens[i]) < target_i(tokens[i])), or the length
+ *   out_tokens[sequence][drafts + 1]  the accepted tokens, one more, and -1 behind it
+ * The one more is the first class c of positive weight with sum of weights up to c > uniforms[drafts] * their whole sum, of weights
+ * max(target_n - draft_n, 0) where token n was refused (target_n but for that token with draft NULL; target_n where those are all 0), else
+ * target_n; the last class of positive weight where there is no such one, -1 where no weight is positive or their sum is not finite.  Sums are
+ * 64-bit.  A token that is no class is refused; a probability that is NaN counts as 0. */
+ADDER_API int adder_b200_verify_drafts(const void* target, const void* draft, int dtype, const long long* tokens, const float* uniforms,
+                                       const long long* lengths, long long* out_tokens, long long* accepted, long long sequences,
+                                       long long drafts, long long classes, long long target_sequence_stride, long long target_place_stride,
+                                       long long draft_sequence_stride, long long draft_place_stride, void* stream);
+
 /* One tensor of an optimizer step: n elements, all pointers to device memory.
  * param and grad have the step's element type; exp_avg and exp_avg_sq are fp32, or with 8-bit states one code a value with a scale for
  * each 256 consecutive values (ceil(n / 256) of them; NULL with 32-bit states).  step points to two ints: the steps that this tensor
