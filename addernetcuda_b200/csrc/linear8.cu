@@ -186,10 +186,17 @@ __device__ __forceinline__ void l8_read(uint32_t (&r)[16], uint32_t addr) {
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
                    "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]) : "r"(addr));
 }
+__device__ __forceinline__ void l8_read(uint32_t (&r)[32], uint32_t addr) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,"
+                 "%28,%29,%30,%31}, [%32];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+                   "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]),
+                   "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]) : "r"(addr));
+}
 // Keeps the uses of r behind the wait.
-__device__ __forceinline__ void l8_hold(uint32_t (&r)[16]) {
+template <int N> __device__ __forceinline__ void l8_hold(uint32_t (&r)[N]) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) asm volatile("" : "+r"(r[i]));
+    for (int i = 0; i < N; ++i) asm volatile("" : "+r"(r[i]));
 }
 __device__ __forceinline__ uint64_t l8_pair(uint32_t lo, uint32_t hi) {
     uint64_t p;
@@ -203,7 +210,7 @@ __device__ __forceinline__ uint64_t l8_pair(uint32_t lo, uint32_t hi) {
 // and each has the sums of its 128 tokens in 256 columns of its tensor memory, twice: while one block's sums are being made, eight warps read
 // those of the block before, multiply them by its scales and add them up in registers (a row and 128 columns a thread, so that both scales are
 // one number a thread).
-constexpr int L8P_STAGES = 6, L8P_THREADS = 320, L8P_STAGING = 4096;
+constexpr int L8P_STAGES = 6, L8P_THREADS = 384, L8P_STAGING = 4096;
 constexpr uint32_t L8P_SMEM = L8P_STAGES * 2 * L8_SLAB + 8 * L8P_STAGING + 1024;
 
 template <class T> __global__ void __launch_bounds__(L8P_THREADS, 1)
@@ -240,52 +247,56 @@ linear8_pair_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_cons
         n0 = in / rows * 256;
     };
     bool ok = true;
-
-    if (wid == 8) {      // ---- copies
-        if (l8_elect()) {
-            l8_prefetch_map(&x_map);
-            l8_prefetch_map(&w_map);
-            int stage = 0, turn = 0;
-            for (int tile = blockIdx.x >> 1; tile < tiles && ok; tile += pairs) {
-                int m0, n0;
-                place(tile, m0, n0);
-                for (int b = 0; b < a.blocks; ++b) {
-                    if (!mbar_wait(&empty[stage], (turn & 1) ^ 1)) { ok = false; break; }
-                    const uint32_t bar = l8_map_shared(&full[stage], 0), to = smem0 + stage * 2 * L8_SLAB;
-                    if (rank == 0) mbar_arrive_expect_tx(&full[stage], 4 * L8_SLAB);
-                    l8_load<2>(to, &x_map, bar, b * E4M3_BLOCK, m0 + (int)rank * 128);
-                    l8_load<2>(to + L8_SLAB, &w_map, bar, b * E4M3_BLOCK, n0 + (int)rank * 128);
-                    if (++stage == L8P_STAGES) { stage = 0; ++turn; }
-                }
-            }
-            if (!ok) {      // no copy is left in flight
-                gave_up = 1;
-                for (int i = 0; i < L8P_STAGES && rank == 0; ++i) {
-                    const int t = i < stage ? turn : turn - 1;
-                    if (t >= 0) mbar_wait(&full[i], t & 1);
-                }
-            }
-        }
-        __syncwarp();
-    } else if (wid == 9) {      // ---- products
-        if (rank == 0) {
-            int stage = 0, turn = 0, it = 0;
-            for (int tile = blockIdx.x >> 1; tile < tiles && ok; tile += pairs)
-                for (int b = 0; b < a.blocks; ++b, ++it) {
-                    if (!l8_wait(&taken[it & 1], ((it >> 1) & 1) ^ 1) || !l8_wait(&full[stage], turn & 1)) { ok = false; break; }
-                    l8_after_sync();
-                    if (l8_elect()) {
-                        const uint32_t at = smem0 + stage * 2 * L8_SLAB;
-                        l8_multiply<2>(tmem + (it & 1) * 256, l8_desc(at), l8_desc(at + L8_SLAB), l8_instruction(256, 256));
-                        l8_commit<2>(&empty[stage]);
-                        l8_commit<2>(&made[it & 1]);
+    // registers: 384 threads begin with 168 each, 64512 in all; the eight warps of the sums take 224, the other four keep 56
+    if (wid >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        if (wid == 8) {      // ---- copies
+            if (l8_elect()) {
+                l8_prefetch_map(&x_map);
+                l8_prefetch_map(&w_map);
+                int stage = 0, turn = 0;
+                for (int tile = blockIdx.x >> 1; tile < tiles && ok; tile += pairs) {
+                    int m0, n0;
+                    place(tile, m0, n0);
+                    for (int b = 0; b < a.blocks; ++b) {
+                        if (!mbar_wait(&empty[stage], (turn & 1) ^ 1)) { ok = false; break; }
+                        const uint32_t bar = l8_map_shared(&full[stage], 0), to = smem0 + stage * 2 * L8_SLAB;
+                        if (rank == 0) mbar_arrive_expect_tx(&full[stage], 4 * L8_SLAB);
+                        l8_load<2>(to, &x_map, bar, b * E4M3_BLOCK, m0 + (int)rank * 128);
+                        l8_load<2>(to + L8_SLAB, &w_map, bar, b * E4M3_BLOCK, n0 + (int)rank * 128);
+                        if (++stage == L8P_STAGES) { stage = 0; ++turn; }
                     }
-                    __syncwarp();
-                    if (++stage == L8P_STAGES) { stage = 0; ++turn; }
                 }
-            if (!ok && lane == 0) gave_up = 1;
+                if (!ok) {      // no copy is left in flight
+                    gave_up = 1;
+                    for (int i = 0; i < L8P_STAGES && rank == 0; ++i) {
+                        const int t = i < stage ? turn : turn - 1;
+                        if (t >= 0) mbar_wait(&full[i], t & 1);
+                    }
+                }
+            }
+            __syncwarp();
+        } else if (wid == 9) {      // ---- products
+            if (rank == 0) {
+                int stage = 0, turn = 0, it = 0;
+                for (int tile = blockIdx.x >> 1; tile < tiles && ok; tile += pairs)
+                    for (int b = 0; b < a.blocks; ++b, ++it) {
+                        if (!l8_wait(&taken[it & 1], ((it >> 1) & 1) ^ 1) || !l8_wait(&full[stage], turn & 1)) { ok = false; break; }
+                        l8_after_sync();
+                        if (l8_elect()) {
+                            const uint32_t at = smem0 + stage * 2 * L8_SLAB;
+                            l8_multiply<2>(tmem + (it & 1) * 256, l8_desc(at), l8_desc(at + L8_SLAB), l8_instruction(256, 256));
+                            l8_commit<2>(&empty[stage]);
+                            l8_commit<2>(&made[it & 1]);
+                        }
+                        __syncwarp();
+                        if (++stage == L8P_STAGES) { stage = 0; ++turn; }
+                    }
+                if (!ok && lane == 0) gave_up = 1;
+            }
         }
     } else {      // ---- sums
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
         const int quarter = wid & 3, half = wid >> 2;
         const uint32_t from = tmem + ((uint32_t)quarter << 21) + half * 128;
         const uint32_t taken_at = l8_map_shared(taken, 0);
@@ -310,19 +321,20 @@ linear8_pair_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_cons
                 l8_after_sync();
                 const uint64_t s2 = pack2(scale, scale);
                 const uint32_t at = from + (it & 1) * 256;
-                uint32_t r[2][16];
-                l8_read(r[0], at);
+                uint32_t r[2][32];
 #pragma unroll
-                for (int c = 0; c < 8; ++c) {
+                for (int h = 0; h < 2; ++h) {
+                    l8_read(r[0], at + 64 * h);
+                    l8_read(r[1], at + 64 * h + 32);
                     l8_wait_loads();
-                    l8_hold(r[c & 1]);
-                    if (c < 7) l8_read(r[(c + 1) & 1], at + 16 * (c + 1));
+                    l8_hold(r[0]);
+                    l8_hold(r[1]);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) acc[8 * c + i] = fma2(l8_pair(r[c & 1][2 * i], r[c & 1][2 * i + 1]), s2, acc[8 * c + i]);
+                    for (int i = 0; i < 32; ++i) acc[32 * h + i] = fma2(l8_pair(r[i / 16][2 * i % 32], r[i / 16][2 * i % 32 + 1]), s2, acc[32 * h + i]);
                 }
                 l8_before_sync();
                 __syncwarp();
-                if (lane == 0) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(taken_at + 8 * (it & 1)) : "memory");
+                if (lane == 0) asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(taken_at + 8 * (it & 1)) : "memory");
             }
             if (!ok) {
                 if (lane == 0) gave_up = 1;
@@ -376,25 +388,70 @@ linear8_pair_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_cons
 
 // ---- few tokens: 128 outputs x N tokens a CTA, the columns' blocks shared out over a cluster
 
-// The weight's rows are the rows of the products, so that few tokens fill the tensor core; its bytes are what counts.  Four warps add up the blocks'
-// sums in registers, an output a thread; then the CTAs of a cluster share out the tokens, and each adds up its own in the order of the CTAs.
-constexpr int L8S_THREADS = 192;
-
+// The weight's rows are the rows of the products, so that few tokens fill the tensor core; its bytes are what counts.  Four warps (eight for 128
+// tokens) add up the blocks' sums in registers, an output and up to 64 tokens a thread; then the CTAs of a cluster share out the tokens, and each
+// adds up its own in the order of the CTAs.
 template <int N> struct L8Small {
-    static constexpr int STAGES = N <= 16 ? 6 : N <= 32 ? 5 : N <= 64 ? 4 : 3;      // two CTAs an SM
-    static constexpr int BUFFERS = N <= 64 ? 4 : 2;                                 // of sums
-    static constexpr int COLUMNS = N * BUFFERS;
+    static constexpr int HALVES = N == 128 ? 2 : 1, COLUMNS = N / HALVES;           // of tokens, of a warp
+    static constexpr int SUMS = 128 * HALVES, THREADS = SUMS + 64;                  // threads that add up; two warps more
+    static constexpr int CTAS = N == 128 ? 1 : 2;                                   // an SM
+    static constexpr int STAGES = N <= 16 ? 6 : N <= 32 ? 5 : N <= 64 ? 4 : 6;
+    static constexpr int BUFFERS = 4;                                               // of sums
     static constexpr uint32_t STAGE = L8_SLAB + N * 128, SMEM = STAGES * STAGE + 1024;
 };
 
-template <class T, int N> __global__ void __launch_bounds__(L8S_THREADS, 2)
+// The CTAs of a cluster share out a thread's tokens: each gets the others' sums of its own, [CTA][tokens / 4][thread][4], so that the lanes of a warp
+// store side by side (a lane's tokens side by side took three times as long), and adds them up in the order of the CTAs.
+template <class T, int COLUMNS, int PARTS, int THREADS> __device__ __forceinline__ void l8_join(const float (&acc)[COLUMNS], float* sums, uint32_t rank, int tokens, T* out,
+                                                                                                int outer, bool writes, float bias) {
+    constexpr int SHARE = COLUMNS / PARTS, V = SHARE < 4 ? SHARE : 4;
+    float* const mine = sums + threadIdx.x * V;
+    if (threadIdx.x < THREADS) {
+#pragma unroll
+        for (int r = 0; r < PARTS; ++r) {
+            const uint32_t to = l8_map_shared(mine + rank * THREADS * SHARE, r);
+#pragma unroll
+            for (int c = 0; c < SHARE; c += V) {
+                const float* f = acc + r * SHARE + c;
+                if constexpr (V == 4)
+                    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to + 4 * c * THREADS), "f"(f[0]), "f"(f[1]), "f"(f[2]), "f"(f[3]) : "memory");
+                else
+                    asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(to + 4 * c * THREADS), "f"(f[0]), "f"(f[1]) : "memory");
+            }
+        }
+    }
+    l8_cluster_sync();
+    if (!writes) return;
+#pragma unroll
+    for (int c = 0; c < SHARE; c += V) {
+        float f[V] = {};
+#pragma unroll
+        for (int r = 0; r < PARTS; ++r) {
+            const float* from = mine + (r * SHARE + c) * THREADS;
+            if constexpr (V == 4) {
+                const float4 v = *reinterpret_cast<const float4*>(from);
+                f[0] += v.x; f[1] += v.y; f[2] += v.z; f[3] += v.w;
+            } else {
+                const float2 v = *reinterpret_cast<const float2*>(from);
+                f[0] += v.x; f[1] += v.y;
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const int m = (int)rank * SHARE + c + j;
+            if (m < tokens) out[(long long)m * outer] = from_float<T>(f[j] + bias);
+        }
+    }
+}
+
+template <class T, int N> __global__ void __launch_bounds__(L8Small<N>::THREADS, L8Small<N>::CTAS)
 linear8_small_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap w_map, const L8Args a, int* error_flag) {
     using S = L8Small<N>;
     extern __shared__ uint8_t raw[];
     __shared__ uint64_t full[S::STAGES], empty[S::STAGES], made[S::BUFFERS], taken[S::BUFFERS];
     __shared__ uint32_t tmem_base;
     __shared__ int gave_up;
-    __shared__ __align__(16) float scales[4][2][N];      // of each warp: a block's scales of all tokens, times the weight's
+    __shared__ __align__(16) float scales[S::SUMS / 32][2][S::COLUMNS];      // of each warp: a block's scales of all tokens, times the weight's
     const int wid = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t smem0 = (smem_u32(raw) + 1023u) & ~1023u;
     float* const parts_of = reinterpret_cast<float*>(raw + (smem0 - smem_u32(raw)));
@@ -407,11 +464,11 @@ linear8_small_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_con
     if (threadIdx.x == 0) {
         gave_up = 0;
         for (int s = 0; s < S::STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
-        for (int b = 0; b < S::BUFFERS; ++b) { mbar_init(&made[b], 1); mbar_init(&taken[b], 4); }
+        for (int b = 0; b < S::BUFFERS; ++b) { mbar_init(&made[b], 1); mbar_init(&taken[b], S::SUMS / 32); }
         mbar_fence_init();
     }
-    if (wid == 5) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base)), "r"(S::COLUMNS) : "memory");
+    if (wid == S::SUMS / 32 + 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base)), "r"(N * S::BUFFERS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
     l8_before_sync();
@@ -419,11 +476,12 @@ linear8_small_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_con
     l8_after_sync();
     const uint32_t tmem = tmem_base;
     bool ok = true;
-    float acc[N];
+    uint64_t pairs[S::COLUMNS / 2];
 #pragma unroll
-    for (int i = 0; i < N; ++i) acc[i] = 0.f;
+    for (int i = 0; i < S::COLUMNS / 2; ++i) pairs[i] = 0;
+    const int half = wid / 4 * S::COLUMNS;      // the first token of a thread that adds up
 
-    if (wid == 4) {      // ---- copies
+    if (wid == S::SUMS / 32) {      // ---- copies
         if (l8_elect()) {
             l8_prefetch_map(&w_map);
             l8_prefetch_map(&x_map);
@@ -445,7 +503,7 @@ linear8_small_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_con
             }
         }
         __syncwarp();
-    } else if (wid == 5) {      // ---- products
+    } else if (wid == S::SUMS / 32 + 1) {      // ---- products
         int stage = 0, turn = 0;
         for (int it = 0; it < b1 - b0; ++it) {
             const int buffer = it % S::BUFFERS;
@@ -462,16 +520,16 @@ linear8_small_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_con
         }
         if (!ok && lane == 0) gave_up = 1;
     } else {      // ---- sums
-        const uint32_t from = tmem + ((uint32_t)wid << 21);
+        const uint32_t from = tmem + ((uint32_t)(wid & 3) << 21) + half;
         const float* ws = a.ws + (long long)(n0 / E4M3_BLOCK) * a.blocks;
-        constexpr int MINE = (N + 31) / 32;
+        constexpr int MINE = (S::COLUMNS + 31) / 32, PART = S::COLUMNS < 32 ? 16 : 32, READS = S::COLUMNS / PART;
         float next[MINE], w_next = 0.f;      // tokens lane, lane + 32, ...
         const auto fetch = [&](int b) {
             w_next = ws[b];
 #pragma unroll
             for (int i = 0; i < MINE; ++i) {
-                const int m = m0 + lane + 32 * i;
-                next[i] = lane + 32 * i < N && m < a.tokens ? a.xs[(long long)m * a.blocks + b] : 0.f;
+                const int c = lane + 32 * i, m = m0 + half + c;
+                next[i] = c < S::COLUMNS && m < a.tokens ? a.xs[(long long)m * a.blocks + b] : 0.f;
             }
         };
         if (b0 < b1) fetch(b0);
@@ -480,65 +538,55 @@ linear8_small_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_con
             float* sc = scales[wid][it & 1];
 #pragma unroll
             for (int i = 0; i < MINE; ++i)
-                if (lane + 32 * i < N) sc[lane + 32 * i] = next[i] * w_next;
+                if (lane + 32 * i < S::COLUMNS) sc[lane + 32 * i] = next[i] * w_next;
             if (b0 + it + 1 < b1) fetch(b0 + it + 1);
             __syncwarp();
             if (!l8_wait(&made[buffer], (it / S::BUFFERS) & 1)) { ok = false; break; }
             l8_after_sync();
+            uint32_t r[READS][PART];
 #pragma unroll
-            for (int c = 0; c < N; c += 16) {
-                uint32_t r[16];
-                l8_read(r, from + buffer * N + c);
-                l8_wait_loads();
-                l8_hold(r);
+            for (int i = 0; i < READS; ++i) l8_read(r[i], from + buffer * N + i * PART);
+            l8_wait_loads();
 #pragma unroll
-                for (int i = 0; i < 16; i += 4) {
-                    const float4 s = *reinterpret_cast<const float4*>(sc + c + i);
-                    acc[c + i] = fmaf(__uint_as_float(r[i]), s.x, acc[c + i]);
-                    acc[c + i + 1] = fmaf(__uint_as_float(r[i + 1]), s.y, acc[c + i + 1]);
-                    acc[c + i + 2] = fmaf(__uint_as_float(r[i + 2]), s.z, acc[c + i + 2]);
-                    acc[c + i + 3] = fmaf(__uint_as_float(r[i + 3]), s.w, acc[c + i + 3]);
-                }
-            }
+            for (int i = 0; i < READS; ++i) l8_hold(r[i]);
             l8_before_sync();
             __syncwarp();
             if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&taken[buffer])) : "memory");
+#pragma unroll
+            for (int c = 0; c < S::COLUMNS; c += 4) {
+                const ulonglong2 s2 = *reinterpret_cast<const ulonglong2*>(sc + c);
+                const uint32_t* v = &r[c / PART][c % PART];
+                pairs[c / 2] = fma2(l8_pair(v[0], v[1]), s2.x, pairs[c / 2]);
+                pairs[c / 2 + 1] = fma2(l8_pair(v[2], v[3]), s2.y, pairs[c / 2 + 1]);
+            }
         }
         if (!ok && lane == 0) gave_up = 1;
     }
     // Everything loaded has been multiplied and everything multiplied has been added: the stages are free.
-    const int n = n0 + (int)threadIdx.x;
-    const bool writes = threadIdx.x < 128 && n < a.outer;
+    const int n = n0 + (int)(threadIdx.x & 127), m = m0 + half;
+    const bool writes = threadIdx.x < S::SUMS && n < a.outer;
     const float bias = writes && a.bias != nullptr ? to_float(static_cast<const T*>(a.bias)[n]) : 0.f;
-    T* out = static_cast<T*>(a.y) + n;
+    T* out = static_cast<T*>(a.y) + (long long)m * a.outer + n;
+    float acc[S::COLUMNS];
+#pragma unroll
+    for (int i = 0; i < S::COLUMNS / 2; ++i) unpack2(pairs[i], acc[2 * i], acc[2 * i + 1]);
     if (parts == 1) {
 #pragma unroll
-        for (int c = 0; c < N; ++c)
-            if (writes && m0 + c < a.tokens) out[(long long)(m0 + c) * a.outer] = from_float<T>(acc[c] + bias);
+        for (int c = 0; c < S::COLUMNS; ++c)
+            if (writes && m + c < a.tokens) out[(long long)c * a.outer] = from_float<T>(acc[c] + bias);
     } else {
         __syncthreads();
         l8_cluster_sync();      // ... of all CTAs
-        const int share = N / (int)parts;
-        if (threadIdx.x < 128) {
-#pragma unroll
-            for (int c = 0; c < N; ++c) {
-                const uint32_t to = l8_map_shared(parts_of + ((int)rank * share + c % share) * 128 + threadIdx.x, c / share);
-                asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to), "f"(acc[c]) : "memory");
-            }
+        switch (parts) {
+            case 2: l8_join<T, S::COLUMNS, 2, S::SUMS>(acc, parts_of, rank, a.tokens - m, out, a.outer, writes, bias); break;
+            case 4: l8_join<T, S::COLUMNS, 4, S::SUMS>(acc, parts_of, rank, a.tokens - m, out, a.outer, writes, bias); break;
+            default: l8_join<T, S::COLUMNS, 8, S::SUMS>(acc, parts_of, rank, a.tokens - m, out, a.outer, writes, bias); break;
         }
-        l8_cluster_sync();
-        if (writes)
-            for (int c = 0; c < share; ++c) {
-                const int m = m0 + (int)rank * share + c;
-                float sum = parts_of[c * 128 + threadIdx.x];
-                for (uint32_t r = 1; r < parts; ++r) sum += parts_of[(r * share + c) * 128 + threadIdx.x];
-                if (m < a.tokens) out[(long long)m * a.outer] = from_float<T>(sum + bias);
-            }
     }
     l8_before_sync();
     __syncthreads();
     if (threadIdx.x == 0 && gave_up) *error_flag = 1;
-    if (wid == 5) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::COLUMNS));
+    if (wid == S::SUMS / 32 + 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(N * S::BUFFERS));
 }
 
 struct L8Call {
@@ -572,8 +620,8 @@ template <class T, int N> int launch_linear8_small(L8Call c, int* flag, cudaStre
     const long long tiles = (long long)c.a.m_tiles * c.a.n_tiles;
     if (tiles > 2147483647LL / 8) return ADDER_ERR_UNSUPPORTED;
     int parts = 1;      // as long as all CTAs are resident at once and have two blocks each
-    while (parts < 8 && tiles * parts * 2 <= 2LL * sm_count() && c.a.blocks >= 4 * parts) parts *= 2;
-    return launch_clusters(kernel, (unsigned)(tiles * parts), L8S_THREADS, S::SMEM, parts, s, x_map, w_map, c.a, flag);
+    while (parts < 8 && tiles * parts * 2 <= (long long)S::CTAS * sm_count() && c.a.blocks >= 4 * parts) parts *= 2;
+    return launch_clusters(kernel, (unsigned)(tiles * parts), S::THREADS, S::SMEM, parts, s, x_map, w_map, c.a, flag);
 }
 
 template <class T> int launch_linear8(const L8Call& c, cudaStream_t s) {
