@@ -119,7 +119,18 @@ struct L8Args {
     void* y;
     int tokens, outer, blocks;      // blocks of 128 columns
     int m_tiles, n_tiles;
+    bool whole_fours;               // scales may be read four at a time
 };
+// Scales of blocks b to b + 3, as far as there are that many.
+__device__ __forceinline__ void l8_four(const float* p, int b, int blocks, bool whole, float (&f)[4]) {
+    if (whole) {
+        const float4 v = __ldg(reinterpret_cast<const float4*>(p + b));
+        f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[i] = p[min(b + i, blocks - 1)];
+    }
+}
 
 constexpr uint32_t L8_SLAB = 128 * 128;      // bytes of 128 rows of a block
 
@@ -247,9 +258,9 @@ linear8_pair_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_cons
         n0 = in / rows * 256;
     };
     bool ok = true;
-    // registers: 384 threads begin with 168 each, 64512 in all; the eight warps of the sums take 224, the other four keep 56
+    // registers: 384 threads begin with 168 each, 64512 in all; the eight warps of the sums take 240, the other four keep 24
     if (wid >= 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 24;");
         if (wid == 8) {      // ---- copies
             if (l8_elect()) {
                 l8_prefetch_map(&x_map);
@@ -277,26 +288,26 @@ linear8_pair_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_cons
             }
             __syncwarp();
         } else if (wid == 9) {      // ---- products
-            if (rank == 0) {
+            // one thread: its products of a block follow the word that a buffer is free by a wait alone (by the whole warp, which asked for
+            // the copies last, it took 500 clocks, and the product 8192x4096x16384 525 us)
+            if (rank == 0 && l8_elect()) {
                 int stage = 0, turn = 0, it = 0;
                 for (int tile = blockIdx.x >> 1; tile < tiles && ok; tile += pairs)
                     for (int b = 0; b < a.blocks; ++b, ++it) {
-                        if (!l8_wait(&taken[it & 1], ((it >> 1) & 1) ^ 1) || !l8_wait(&full[stage], turn & 1)) { ok = false; break; }
+                        if (!mbar_wait(&full[stage], turn & 1) || !mbar_wait(&taken[it & 1], ((it >> 1) & 1) ^ 1)) { ok = false; break; }
                         l8_after_sync();
-                        if (l8_elect()) {
-                            const uint32_t at = smem0 + stage * 2 * L8_SLAB;
-                            l8_multiply<2>(tmem + (it & 1) * 256, l8_desc(at), l8_desc(at + L8_SLAB), l8_instruction(256, 256));
-                            l8_commit<2>(&empty[stage]);
-                            l8_commit<2>(&made[it & 1]);
-                        }
-                        __syncwarp();
+                        const uint32_t at = smem0 + stage * 2 * L8_SLAB;
+                        l8_multiply<2>(tmem + (it & 1) * 256, l8_desc(at), l8_desc(at + L8_SLAB), l8_instruction(256, 256));
+                        l8_commit<2>(&made[it & 1]);
+                        l8_commit<2>(&empty[stage]);
                         if (++stage == L8P_STAGES) { stage = 0; ++turn; }
                     }
-                if (!ok && lane == 0) gave_up = 1;
+                if (!ok) gave_up = 1;
             }
+            __syncwarp();
         }
     } else {      // ---- sums
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 240;");
         const int quarter = wid & 3, half = wid >> 2;
         const uint32_t from = tmem + ((uint32_t)quarter << 21) + half * 128;
         const uint32_t taken_at = l8_map_shared(taken, 0);
@@ -313,28 +324,54 @@ linear8_pair_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_cons
             uint64_t acc[64];
 #pragma unroll
             for (int i = 0; i < 64; ++i) acc[i] = 0;
-            float x_next = xs[0], w_next = ws[0];
-            for (int b = 0; b < a.blocks; ++b, ++it) {
-                const float scale = x_next * w_next;
-                if (b + 1 < a.blocks) { x_next = xs[b + 1]; w_next = ws[b + 1]; }
-                if (!l8_wait(&made[it & 1], (it >> 1) & 1)) { ok = false; break; }
+            // Scales of four blocks at a time, the next four on their way: a warp's rows lie in 32 lines, of which hardly any L1 is left to keep one
+            float s[4], x4[4], w4[4];
+            const auto fetch = [&](int b) {
+                l8_four(xs, b, a.blocks, a.whole_fours, x4);
+                l8_four(ws, b, a.blocks, a.whole_fours, w4);
+            };
+            fetch(0);
+            // 32 columns at a time, the next ones on their way while some are added: without that all warps wait for their loads, and then
+            // for one another's additions
+            uint32_t r[2][32];
+            const auto arrived = [&](int part) {
+                l8_wait_loads();
+                l8_hold(r[part & 1]);
+            };
+            if (!l8_wait(&made[it & 1], (it >> 1) & 1)) ok = false;
+            else {
                 l8_after_sync();
-                const uint64_t s2 = pack2(scale, scale);
-                const uint32_t at = from + (it & 1) * 256;
-                uint32_t r[2][32];
+                l8_read(r[0], from + (it & 1) * 256);
+            }
+            for (int b = 0; b < a.blocks && ok; ++b, ++it) {
+                if ((b & 3) == 0) {
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    l8_read(r[0], at + 64 * h);
-                    l8_read(r[1], at + 64 * h + 32);
-                    l8_wait_loads();
-                    l8_hold(r[0]);
-                    l8_hold(r[1]);
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) acc[32 * h + i] = fma2(l8_pair(r[i / 16][2 * i % 32], r[i / 16][2 * i % 32 + 1]), s2, acc[32 * h + i]);
+                    for (int i = 0; i < 4; ++i) s[i] = x4[i] * w4[i];
+                    if (b + 4 < a.blocks) fetch(b + 4);
                 }
+                const uint64_t s2 = pack2(s[0], s[0]);
+                s[0] = s[1]; s[1] = s[2]; s[2] = s[3];
+                const uint32_t at = from + (it & 1) * 256;
+                const auto add = [&](int part) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) acc[16 * part + i] = fma2(l8_pair(r[part & 1][2 * i], r[part & 1][2 * i + 1]), s2, acc[16 * part + i]);
+                };
+#pragma unroll
+                for (int part = 0; part < 3; ++part) {
+                    arrived(part);
+                    l8_read(r[(part + 1) & 1], at + 32 * (part + 1));
+                    add(part);
+                }
+                arrived(3);
                 l8_before_sync();
                 __syncwarp();
                 if (lane == 0) asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(taken_at + 8 * (it & 1)) : "memory");
+                if (b + 1 < a.blocks) {
+                    if (!l8_wait(&made[(it + 1) & 1], ((it + 1) >> 1) & 1)) ok = false;
+                    l8_after_sync();
+                    l8_read(r[0], from + ((it + 1) & 1) * 256);
+                }
+                add(3);
             }
             if (!ok) {
                 if (lane == 0) gave_up = 1;
@@ -504,21 +541,21 @@ linear8_small_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_con
         }
         __syncwarp();
     } else if (wid == S::SUMS / 32 + 1) {      // ---- products
-        int stage = 0, turn = 0;
-        for (int it = 0; it < b1 - b0; ++it) {
-            const int buffer = it % S::BUFFERS;
-            if (!l8_wait(&taken[buffer], ((it / S::BUFFERS) & 1) ^ 1) || !l8_wait(&full[stage], turn & 1)) { ok = false; break; }
-            l8_after_sync();
-            if (l8_elect()) {
+        if (l8_elect()) {
+            int stage = 0, turn = 0;
+            for (int it = 0; it < b1 - b0; ++it) {
+                const int buffer = it % S::BUFFERS;
+                if (!mbar_wait(&full[stage], turn & 1) || !mbar_wait(&taken[buffer], ((it / S::BUFFERS) & 1) ^ 1)) { ok = false; break; }
+                l8_after_sync();
                 const uint32_t at = smem0 + stage * S::STAGE;
                 l8_multiply<1>(tmem + buffer * N, l8_desc(at), l8_desc(at + L8_SLAB), l8_instruction(128, N));
-                l8_commit<1>(&empty[stage]);
                 l8_commit<1>(&made[buffer]);
+                l8_commit<1>(&empty[stage]);
+                if (++stage == S::STAGES) { stage = 0; ++turn; }
             }
-            __syncwarp();
-            if (++stage == S::STAGES) { stage = 0; ++turn; }
+            if (!ok) gave_up = 1;
         }
-        if (!ok && lane == 0) gave_up = 1;
+        __syncwarp();
     } else {      // ---- sums
         const uint32_t from = tmem + ((uint32_t)(wid & 3) << 21) + half;
         const float* ws = a.ws + (long long)(n0 / E4M3_BLOCK) * a.blocks;
@@ -699,7 +736,8 @@ int adder_b200_linear_8bit(const unsigned char* x, const float* x_scales, const 
     if (!aligned_to(x, 16) || !aligned_to(w, 16) || x_stride % 16 != 0 || w_stride % 16 != 0 || !aligned_to(x_scales, 4) || !aligned_to(w_scales, 4) ||
         !aligned_to(bias, size) || !aligned_to(y, size))
         return ADDER_ERR_ALIGNMENT;
-    const L8Call c{x, w, x_stride, w_stride, inner, {x_scales, w_scales, bias, y, (int)tokens, (int)outer, (int)((inner + E4M3_BLOCK - 1) / E4M3_BLOCK), 0, 0}};
+    const L8Call c{x, w, x_stride, w_stride, inner, {x_scales, w_scales, bias, y, (int)tokens, (int)outer, (int)((inner + E4M3_BLOCK - 1) / E4M3_BLOCK), 0, 0,
+                    (inner + E4M3_BLOCK - 1) / E4M3_BLOCK % 4 == 0 && aligned_to(x_scales, 16) && aligned_to(w_scales, 16)}};
     return with_type(dtype, [&](auto* type) { return launch_linear8<std::remove_pointer_t<decltype(type)>>(c, static_cast<cudaStream_t>(stream)); });
 }
 
