@@ -423,24 +423,29 @@ linear8_pair_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_cons
     if (wid == 9) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
 }
 
-// ---- few tokens: 128 outputs x N tokens a CTA, the columns' blocks shared out over a cluster
+// ---- fewer tokens: a tile of 128 outputs x N tokens a CTA, the columns' blocks shared out over a cluster
 
-// The weight's rows are the rows of the products, so that few tokens fill the tensor core; its bytes are what counts.  Four warps (eight for 128
-// tokens) add up the blocks' sums in registers, an output and up to 64 tokens a thread; then the CTAs of a cluster share out the tokens, and each
-// adds up its own in the order of the CTAs.
+// Up to 32 tokens the weight's rows are the rows of the products, so that few tokens fill the tensor core; its bytes are what counts.  Four warps
+// add up the blocks' sums in registers, an output and all tokens a thread, whose scales lie in shared memory.  That costs as much of its bandwidth
+// as reading N numbers a thread: with 128 tokens a block took 1330 clocks.  So N = 128 has the tokens as the rows, as a pair has: eight warps, a token
+// and 64 outputs a thread, one number as scale (512x4096x4096 28.8 us before).  In the end the CTAs of a cluster share out a thread's sums, and
+// each adds up its own in the order of the CTAs.
 template <int N> struct L8Small {
-    static constexpr int HALVES = N == 128 ? 2 : 1, COLUMNS = N / HALVES;           // of tokens, of a warp
-    static constexpr int SUMS = 128 * HALVES, THREADS = SUMS + 64;                  // threads that add up; two warps more
-    static constexpr int CTAS = N == 128 ? 1 : 2;                                   // an SM
-    static constexpr int STAGES = N <= 16 ? 6 : N <= 32 ? 5 : N <= 64 ? 4 : 6;
+    static constexpr bool ROWS = N == 128;                                          // tokens are rows
+    static constexpr int COLUMNS = ROWS ? 64 : N;                                   // a thread's sums
+    static constexpr int SUMS = ROWS ? 256 : 128, THREADS = SUMS + 64;              // threads that add up; two warps more
+    static constexpr int CTAS = ROWS ? 1 : 2;                                       // an SM
+    static constexpr int STAGES = N <= 16 ? 6 : N <= 32 ? 5 : 6;
     static constexpr int BUFFERS = 4;                                               // of sums
     static constexpr uint32_t STAGE = L8_SLAB + N * 128, SMEM = STAGES * STAGE + 1024;
+    // in the end the stages hold what the CTAs of a cluster hand over, and rows of y on their way out
+    static_assert(SUMS * COLUMNS * 4 + (ROWS ? SUMS * (COLUMNS + 4) * 4 : 0) <= STAGES * STAGE);
 };
 
-// The CTAs of a cluster share out a thread's tokens: each gets the others' sums of its own, [CTA][tokens / 4][thread][4], so that the lanes of a warp
-// store side by side (a lane's tokens side by side took three times as long), and adds them up in the order of the CTAs.
-template <class T, int COLUMNS, int PARTS, int THREADS> __device__ __forceinline__ void l8_join(const float (&acc)[COLUMNS], float* sums, uint32_t rank, int tokens, T* out,
-                                                                                                int outer, bool writes, float bias) {
+// The CTAs of a cluster share out a thread's sums: each gets the others' of its own part, [CTA][sums / V][thread][V], so that the lanes of a warp
+// store side by side (a lane's sums side by side took three times as long), and adds them up in the order of the CTAs.  store(first, values)
+// takes V of them.
+template <int COLUMNS, int PARTS, int THREADS, class Store> __device__ __forceinline__ void l8_join(const float (&acc)[COLUMNS], float* sums, uint32_t rank, Store&& store) {
     constexpr int SHARE = COLUMNS / PARTS, V = SHARE < 4 ? SHARE : 4;
     float* const mine = sums + threadIdx.x * V;
     if (threadIdx.x < THREADS) {
@@ -458,7 +463,7 @@ template <class T, int COLUMNS, int PARTS, int THREADS> __device__ __forceinline
         }
     }
     l8_cluster_sync();
-    if (!writes) return;
+    if (threadIdx.x >= THREADS) return;
 #pragma unroll
     for (int c = 0; c < SHARE; c += V) {
         float f[V] = {};
@@ -473,11 +478,7 @@ template <class T, int COLUMNS, int PARTS, int THREADS> __device__ __forceinline
                 f[0] += v.x; f[1] += v.y;
             }
         }
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const int m = (int)rank * SHARE + c + j;
-            if (m < tokens) out[(long long)m * outer] = from_float<T>(f[j] + bias);
-        }
+        store((int)rank * SHARE + c, f);
     }
 }
 
@@ -488,7 +489,7 @@ linear8_small_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_con
     __shared__ uint64_t full[S::STAGES], empty[S::STAGES], made[S::BUFFERS], taken[S::BUFFERS];
     __shared__ uint32_t tmem_base;
     __shared__ int gave_up;
-    __shared__ __align__(16) float scales[S::SUMS / 32][2][S::COLUMNS];      // of each warp: a block's scales of all tokens, times the weight's
+    __shared__ __align__(16) float scales[S::ROWS ? 1 : 4][2][S::ROWS ? 4 : N];      // of each warp: a block's scales of all tokens, times the weight's
     const int wid = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t smem0 = (smem_u32(raw) + 1023u) & ~1023u;
     float* const parts_of = reinterpret_cast<float*>(raw + (smem0 - smem_u32(raw)));
@@ -516,7 +517,8 @@ linear8_small_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_con
     uint64_t pairs[S::COLUMNS / 2];
 #pragma unroll
     for (int i = 0; i < S::COLUMNS / 2; ++i) pairs[i] = 0;
-    const int half = wid / 4 * S::COLUMNS;      // the first token of a thread that adds up
+    // what a thread adds up: row m or n of the tile, and COLUMNS columns from `first` on
+    const int line = threadIdx.x & 127, first = S::ROWS ? (wid >> 2) * S::COLUMNS : 0;
 
     if (wid == S::SUMS / 32) {      // ---- copies
         if (l8_elect()) {
@@ -547,8 +549,8 @@ linear8_small_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_con
                 const int buffer = it % S::BUFFERS;
                 if (!mbar_wait(&full[stage], turn & 1) || !mbar_wait(&taken[buffer], ((it / S::BUFFERS) & 1) ^ 1)) { ok = false; break; }
                 l8_after_sync();
-                const uint32_t at = smem0 + stage * S::STAGE;
-                l8_multiply<1>(tmem + buffer * N, l8_desc(at), l8_desc(at + L8_SLAB), l8_instruction(128, N));
+                const uint32_t w = l8_desc(smem0 + stage * S::STAGE), x = l8_desc(smem0 + stage * S::STAGE + L8_SLAB);
+                l8_multiply<1>(tmem + buffer * N, S::ROWS ? x : w, S::ROWS ? w : x, l8_instruction(128, N));
                 l8_commit<1>(&made[buffer]);
                 l8_commit<1>(&empty[stage]);
                 if (++stage == S::STAGES) { stage = 0; ++turn; }
@@ -557,26 +559,31 @@ linear8_small_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_con
         }
         __syncwarp();
     } else {      // ---- sums
-        const uint32_t from = tmem + ((uint32_t)(wid & 3) << 21) + half;
+        const uint32_t from = tmem + ((uint32_t)(wid & 3) << 21) + first;
         const float* ws = a.ws + (long long)(n0 / E4M3_BLOCK) * a.blocks;
-        constexpr int MINE = (S::COLUMNS + 31) / 32, PART = S::COLUMNS < 32 ? 16 : 32, READS = S::COLUMNS / PART;
-        float next[MINE], w_next = 0.f;      // tokens lane, lane + 32, ...
+        const bool fours = a.whole_fours && b0 % 4 == 0;
+        constexpr int PART = S::COLUMNS < 32 ? 16 : 32, READS = S::COLUMNS / PART;
+        const int token = m0 + (S::ROWS ? line : lane);      // whose scales this thread reads: four blocks', and the next four on their way
+        const bool reads = token < a.tokens && (S::ROWS || lane < N);
+        float scale[4], x4[4] = {0.f, 0.f, 0.f, 0.f}, w4[4];
         const auto fetch = [&](int b) {
-            w_next = ws[b];
-#pragma unroll
-            for (int i = 0; i < MINE; ++i) {
-                const int c = lane + 32 * i, m = m0 + half + c;
-                next[i] = c < S::COLUMNS && m < a.tokens ? a.xs[(long long)m * a.blocks + b] : 0.f;
-            }
+            l8_four(ws, b, a.blocks, fours, w4);
+            if (reads) l8_four(a.xs + (long long)token * a.blocks, b, a.blocks, fours, x4);
         };
-        if (b0 < b1) fetch(b0);
+        fetch(b0);
         for (int it = 0; it < b1 - b0; ++it) {
             const int buffer = it % S::BUFFERS;
-            float* sc = scales[wid][it & 1];
+            if ((it & 3) == 0) {
 #pragma unroll
-            for (int i = 0; i < MINE; ++i)
-                if (lane + 32 * i < S::COLUMNS) sc[lane + 32 * i] = next[i] * w_next;
-            if (b0 + it + 1 < b1) fetch(b0 + it + 1);
+                for (int j = 0; j < 4; ++j) scale[j] = x4[j] * w4[j];
+                if (b0 + it + 4 < b1) fetch(b0 + it + 4);
+            }
+            const float* sc = scales[S::ROWS ? 0 : wid][it & 1];
+            if constexpr (!S::ROWS) {
+                if (lane < N) scales[wid][it & 1][lane] = scale[0];
+            }
+            const uint64_t same = pack2(scale[0], scale[0]);
+            scale[0] = scale[1]; scale[1] = scale[2]; scale[2] = scale[3];
             __syncwarp();
             if (!l8_wait(&made[buffer], (it / S::BUFFERS) & 1)) { ok = false; break; }
             l8_after_sync();
@@ -588,11 +595,12 @@ linear8_small_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_con
             for (int i = 0; i < READS; ++i) l8_hold(r[i]);
             l8_before_sync();
             __syncwarp();
-            if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&taken[buffer])) : "memory");
+            if (lane == 0) asm volatile("mbarrier.arrive.relaxed.cta.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&taken[buffer])) : "memory");
 #pragma unroll
             for (int c = 0; c < S::COLUMNS; c += 4) {
-                const ulonglong2 s2 = *reinterpret_cast<const ulonglong2*>(sc + c);
                 const uint32_t* v = &r[c / PART][c % PART];
+                ulonglong2 s2 = make_ulonglong2(same, same);
+                if constexpr (!S::ROWS) s2 = *reinterpret_cast<const ulonglong2*>(sc + c);
                 pairs[c / 2] = fma2(l8_pair(v[0], v[1]), s2.x, pairs[c / 2]);
                 pairs[c / 2 + 1] = fma2(l8_pair(v[2], v[3]), s2.y, pairs[c / 2 + 1]);
             }
@@ -600,24 +608,72 @@ linear8_small_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_con
         if (!ok && lane == 0) gave_up = 1;
     }
     // Everything loaded has been multiplied and everything multiplied has been added: the stages are free.
-    const int n = n0 + (int)(threadIdx.x & 127), m = m0 + half;
-    const bool writes = threadIdx.x < S::SUMS && n < a.outer;
-    const float bias = writes && a.bias != nullptr ? to_float(static_cast<const T*>(a.bias)[n]) : 0.f;
-    T* out = static_cast<T*>(a.y) + (long long)m * a.outer + n;
     float acc[S::COLUMNS];
 #pragma unroll
     for (int i = 0; i < S::COLUMNS / 2; ++i) unpack2(pairs[i], acc[2 * i], acc[2 * i + 1]);
-    if (parts == 1) {
+    const T* bias = static_cast<const T*>(a.bias);
+    const bool vectors = (long long)a.outer * sizeof(T) % 16 == 0 && (reinterpret_cast<uintptr_t>(a.y) & 15) == 0;
+    // Where the rows of y are no whole vectors, those of a warp go through shared memory, so that neighbouring lanes store a row's elements
+    // (a row a lane, element by element, 333x2000x5003 took 29.4 us).
+    constexpr int PITCH = S::COLUMNS + 4 / sizeof(T);
+    T* const mine = reinterpret_cast<T*>(parts_of + S::SUMS * S::COLUMNS) + wid * 32 * PITCH;
+    const auto store = [&](int c, auto& f) {
+        constexpr int V = sizeof(f) / sizeof(float);
+        if constexpr (S::ROWS) {
+            const int m = m0 + line, n = n0 + first + c;
+            if (m >= a.tokens) return;
+            T* out = static_cast<T*>(a.y) + (long long)m * a.outer + n;
+            if (bias != nullptr) {
 #pragma unroll
-        for (int c = 0; c < S::COLUMNS; ++c)
-            if (writes && m + c < a.tokens) out[(long long)c * a.outer] = from_float<T>(acc[c] + bias);
+                for (int j = 0; j < V; ++j) f[j] += n + j < a.outer ? to_float(bias[n + j]) : 0.f;
+            }
+            if (!vectors) {      // through shared memory: see below
+#pragma unroll
+                for (int j = 0; j < V; ++j) mine[lane * PITCH + c + j] = from_float<T>(f[j]);
+            } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+                for (int j = 0; j < V; j += 4)
+                    if (n + j < a.outer) *reinterpret_cast<float4*>(out + j) = make_float4(f[j], f[j + 1], f[j + 2], f[j + 3]);
+            } else if constexpr (V == 8) {
+                if (n < a.outer) *reinterpret_cast<uint4*>(out) = Vec16<T>::pack(f);
+            } else {
+                if (n < a.outer) *reinterpret_cast<uint2*>(out) = make_uint2(pack_pair<T>(f[0], f[1]), pack_pair<T>(f[2], f[3]));
+            }
+        } else {
+            const int n = n0 + line;
+            if (n >= a.outer) return;
+            const float shift = bias != nullptr ? to_float(bias[n]) : 0.f;
+#pragma unroll
+            for (int j = 0; j < V; ++j)
+                if (m0 + c + j < a.tokens) static_cast<T*>(a.y)[(long long)(m0 + c + j) * a.outer + n] = from_float<T>(f[j] + shift);
+        }
+    };
+    if (parts == 1) {
+        if (threadIdx.x < S::SUMS) {
+#pragma unroll
+            for (int c = 0; c < S::COLUMNS; c += 8) {
+                float f[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) f[j] = acc[c + j];
+                store(c, f);
+            }
+        }
     } else {
         __syncthreads();
         l8_cluster_sync();      // ... of all CTAs
         switch (parts) {
-            case 2: l8_join<T, S::COLUMNS, 2, S::SUMS>(acc, parts_of, rank, a.tokens - m, out, a.outer, writes, bias); break;
-            case 4: l8_join<T, S::COLUMNS, 4, S::SUMS>(acc, parts_of, rank, a.tokens - m, out, a.outer, writes, bias); break;
-            default: l8_join<T, S::COLUMNS, 8, S::SUMS>(acc, parts_of, rank, a.tokens - m, out, a.outer, writes, bias); break;
+            case 2: l8_join<S::COLUMNS, 2, S::SUMS>(acc, parts_of, rank, store); break;
+            case 4: l8_join<S::COLUMNS, 4, S::SUMS>(acc, parts_of, rank, store); break;
+            default: l8_join<S::COLUMNS, 8, S::SUMS>(acc, parts_of, rank, store); break;
+        }
+    }
+    if (S::ROWS && !vectors && threadIdx.x < S::SUMS) {
+        __syncwarp();
+        const int share = S::COLUMNS / (int)parts, c0 = (int)rank * share, m1 = m0 + (wid & 3) * 32, rows = min(32, a.tokens - m1);
+        T* out = static_cast<T*>(a.y) + (long long)m1 * a.outer + n0 + first + c0;
+        for (int i = lane; i < rows * share; i += 32) {      // share: a power of two
+            const int row = i >> (31 - __clz(share)), c = i & (share - 1);
+            if (n0 + first + c0 + c < a.outer) out[(long long)row * a.outer + c] = mine[row * PITCH + c0 + c];
         }
     }
     l8_before_sync();
@@ -668,9 +724,10 @@ template <class T> int launch_linear8(const L8Call& c, cudaStream_t s) {
     const int tokens = c.a.tokens;
     if (tokens <= 16) return launch_linear8_small<T, 16>(c, flag, s);
     if (tokens <= 32) return launch_linear8_small<T, 32>(c, flag, s);
-    if (tokens <= 64) return launch_linear8_small<T, 64>(c, flag, s);
-    const long long pair_tiles = (long long)((tokens + 255) / 256) * ((c.a.outer + 255) / 256);
-    if (tokens <= 128 || pair_tiles < sm_count() / 2) return launch_linear8_small<T, 128>(c, flag, s);
+    // Turns of all SMs: a pair's takes some 1.6 times as long as a CTA's of 128 x 128.
+    const long long pair_tiles = (long long)((tokens + 255) / 256) * ((c.a.outer + 255) / 256), small_tiles = (long long)((tokens + 127) / 128) * ((c.a.outer + 127) / 128);
+    const long long pair_turns = (pair_tiles + sm_count() / 2 - 1) / (sm_count() / 2), small_turns = (small_tiles + sm_count() - 1) / sm_count();
+    if (tokens <= 128 || 5 * small_turns <= 8 * pair_turns) return launch_linear8_small<T, 128>(c, flag, s);
     return launch_linear8_pair<T>(c, flag, s);
 }
 
