@@ -40,7 +40,19 @@ template <class T, int N> __device__ __forceinline__ void dv_load(const T* p, fl
     if constexpr (N == 1) f[0] = to_float(*p);
     else Vec16<T>::unpack(__ldg(reinterpret_cast<const uint4*>(p)), f);
 }
-__device__ __forceinline__ double dv_positive(double w) { return w > 0.0 ? w : 0.0; }      // a NaN counts as 0
+// f - g where that is positive, else 0 (a NaN, too), as what fp32 makes of it and what that leaves out: nothing for two fp16 values of up to 1, and
+// for bf16 where one is less than 2^16 times the other; beyond, the difference is rounded, to 2^-25 of itself.  Differences of fp32 values are
+// rounded more often, so what is left out counts (the operations after d are exact as long as nothing overflows).
+template <class T> __device__ __forceinline__ float dv_difference(float f, float g, float& left) {
+    const float d = f - g;
+    left = 0.f;
+    if constexpr (sizeof(T) == 4) {
+        const float b = d - f;
+        const float e = (f - (d - b)) - (g + b);
+        if (d > 0.f && d < INFINITY) left = e;
+    }
+    return fmaxf(d, 0.f);
+}
 // Inclusive sums over the lanes of a warp.
 __device__ __forceinline__ double dv_scan(double v, int lane) {
 #pragma unroll
@@ -54,6 +66,7 @@ __device__ __forceinline__ double dv_scan(double v, int lane) {
 // VEC consecutive classes a lane at a time.
 template <class T, int VEC> __global__ void __launch_bounds__(DV_THREADS) dv_kernel(const DvArgs a) {
     __shared__ double sums[2][DV_MOST_PARTS * DV_WARPS];
+    __shared__ double part_of[DV_WARPS];
     __shared__ int first_refused;
     cg::cluster_group cluster = cg::this_cluster();
     const int parts = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
@@ -94,34 +107,46 @@ template <class T, int VEC> __global__ void __launch_bounds__(DV_THREADS) dv_ker
     const int segments = parts * DV_WARPS, segment = rank * DV_WARPS + warp, nvec = a.classes / VEC;
     const int v0 = (int)((long long)nvec * segment / segments), v1 = (int)((long long)nvec * (segment + 1) / segments);
 
-    // Weights of the classes of vector v; with `whole` those of p alone.
-    const auto weights = [&](int v, bool whole, double (&w)[VEC]) {
+    // Weights of the classes of vector v, and what fp32 leaves out of them; with `whole` those of p alone.
+    const auto weights = [&](int v, bool whole, float (&w)[VEC], float (&left)[VEC]) {
         float f[VEC];
         dv_load<T, VEC>(p_row + (size_t)v * VEC, f);
         if (q_row == nullptr || whole) {
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) w[j] = !whole && v * VEC + j == gone ? 0.0 : dv_positive(f[j]);
+            for (int j = 0; j < VEC; ++j) {
+                w[j] = !whole && v * VEC + j == gone ? 0.f : fmaxf(f[j], 0.f);
+                left[j] = 0.f;
+            }
         } else {
             float g[VEC];
             dv_load<T, VEC>(q_row + (size_t)v * VEC, g);
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) w[j] = dv_positive((double)f[j] - (double)g[j]);
+            for (int j = 0; j < VEC; ++j) w[j] = dv_difference<T>(f[j], g[j], left[j]);
         }
+    };
+    // Sum of the weights of vectors from to to - 1, in every lane of a warp.
+    const auto sum_of = [&](int from, int to, bool whole) {
+        double s = 0.0;
+        float rest = 0.f;
+#pragma unroll 4
+        for (int v = from + lane; v < to; v += 32) {
+            float w[VEC], left[VEC];
+            weights(v, whole, w, left);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                s += (double)w[j];
+                rest += left[j];
+            }
+        }
+        s += (double)rest;
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
+        return s;
     };
     // Sums of all segments in the lanes of every warp, two a lane: what lies before them, and theirs.
     double before = 0.0, mine[2], total = 0.0;
     const auto sum_up = [&](bool whole, int turn) {
-        double s = 0.0;
-#pragma unroll 4
-        for (int v = v0 + lane; v < v1; v += 32) {
-            double w[VEC], part = 0.0;
-            weights(v, whole, w);
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) part += w[j];
-            s += part;
-        }
-#pragma unroll
-        for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
+        const double s = sum_of(v0, v1, whole);
         if (lane < parts) cluster.map_shared_rank(&sums[turn][0], lane)[segment] = s;
         cluster.sync();
 #pragma unroll
@@ -162,24 +187,43 @@ template <class T, int VEC> __global__ void __launch_bounds__(DV_THREADS) dv_ker
         const int l = 31 - __clz(some0 | some1);
         chosen = 2 * l + ((some1 >> l) & 1);
     }
-    if (chosen != segment) return;
-    double reached = __shfl_sync(0xffffffffu, (chosen & 1) ? end0 : before, chosen >> 1);
+    // Its CTA reads the segment again, a part a warp, and the warp whose part holds the border (or the last weight) once more.
+    if (chosen / DV_WARPS != rank) return;
+    const int c0 = (int)((long long)nvec * chosen / segments), c1 = (int)((long long)nvec * (chosen + 1) / segments);
+    const auto edge = [&](int i) { return c0 + (int)((long long)(c1 - c0) * i / DV_WARPS); };
+    const double mass = sum_of(edge(warp), edge(warp + 1), whole);
+    if (lane == 0) part_of[warp] = mass;
+    __syncthreads();
+    double reached = __shfl_sync(0xffffffffu, (chosen & 1) ? end0 : before, chosen >> 1), at_last = reached;
+    int holder = -1, last_part = -1;
+    for (int i = 0; i < DV_WARPS && holder < 0; ++i) {
+        const double w = part_of[i];
+        if (w > 0.0) {
+            last_part = i;
+            at_last = reached;
+            if (reached + w > want) holder = i;
+        }
+        reached += w;
+    }
+    if (warp != last_part) return;      // the holder where there is one
+    reached = at_last;
     int last = -1, found = -1;
-    for (int base = v0; base < v1; base += 32) {
+    for (int base = edge(warp); base < edge(warp + 1); base += 32) {
         const int v = base + lane;
-        double w[VEC], own = 0.0;
+        float w[VEC], left[VEC];
+        double own = 0.0;
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) w[j] = 0.0;
-        if (v < v1) weights(v, whole, w);
+        for (int j = 0; j < VEC; ++j) w[j] = left[j] = 0.f;
+        if (v < edge(warp + 1)) weights(v, whole, w, left);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) own += w[j];
+        for (int j = 0; j < VEC; ++j) own += (double)w[j] + (double)left[j];
         const double upto = dv_scan(own, lane);
         double at = reached + (upto - own);
         int hit = -1;
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
-            at += w[j];
-            if (w[j] > 0.0) {
+            at += (double)w[j] + (double)left[j];
+            if (w[j] > 0.f) {
                 last = v * VEC + j;
                 if (hit < 0 && at > want) hit = v * VEC + j;
             }
