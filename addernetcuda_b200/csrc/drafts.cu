@@ -40,18 +40,25 @@ template <class T, int N> __device__ __forceinline__ void dv_load(const T* p, fl
     if constexpr (N == 1) f[0] = to_float(*p);
     else Vec16<T>::unpack(__ldg(reinterpret_cast<const uint4*>(p)), f);
 }
-// f - g where that is positive, else 0 (a NaN, too), as what fp32 makes of it and what that leaves out: nothing for two fp16 values of up to 1, and
-// for bf16 where one is less than 2^16 times the other; beyond, the difference is rounded, to 2^-25 of itself.  Differences of fp32 values are
-// rounded more often, so what is left out counts (the operations after d are exact as long as nothing overflows).
+// Weights below fp32's smallest normal number count as nothing, NaN too.
+constexpr float DV_LEAST = 0x1p-126f;
+// A weight of at least that in 64 bits, by its bits: a conversion takes 16 clocks of a scheduler (64x6x128000 20.6 us with them).  Infinity becomes 2^128.
+__device__ __forceinline__ double dv_double(float w) {
+    const uint32_t u = __float_as_uint(w);
+    return __hiloint2double((int)((u >> 3) + 0x38000000u), (int)(u << 29));
+}
+// f - g, and what fp32 leaves out of it: nothing for two fp16 values of up to 1, and for bf16 where one is less than 2^16 times the other; beyond, the
+// difference is rounded, to 2^-25 of itself.  Differences of fp32 values are rounded more often, so what is left out counts (the operations
+// after d are exact as long as nothing overflows).
 template <class T> __device__ __forceinline__ float dv_difference(float f, float g, float& left) {
     const float d = f - g;
     left = 0.f;
     if constexpr (sizeof(T) == 4) {
         const float b = d - f;
         const float e = (f - (d - b)) - (g + b);
-        if (d > 0.f && d < INFINITY) left = e;
+        if (d >= DV_LEAST && d < INFINITY) left = e;
     }
-    return fmaxf(d, 0.f);
+    return d;
 }
 // Inclusive sums over the lanes of a warp.
 __device__ __forceinline__ double dv_scan(double v, int lane) {
@@ -114,7 +121,7 @@ template <class T, int VEC> __global__ void __launch_bounds__(DV_THREADS) dv_ker
         if (q_row == nullptr || whole) {
 #pragma unroll
             for (int j = 0; j < VEC; ++j) {
-                w[j] = !whole && v * VEC + j == gone ? 0.f : fmaxf(f[j], 0.f);
+                w[j] = !whole && v * VEC + j == gone ? 0.f : f[j];
                 left[j] = 0.f;
             }
         } else {
@@ -126,7 +133,7 @@ template <class T, int VEC> __global__ void __launch_bounds__(DV_THREADS) dv_ker
     };
     // Sum of the weights of vectors from to to - 1, in every lane of a warp.
     const auto sum_of = [&](int from, int to, bool whole) {
-        double s = 0.0;
+        double sum[2] = {0.0, 0.0};
         float rest = 0.f;
 #pragma unroll 4
         for (int v = from + lane; v < to; v += 32) {
@@ -134,11 +141,11 @@ template <class T, int VEC> __global__ void __launch_bounds__(DV_THREADS) dv_ker
             weights(v, whole, w, left);
 #pragma unroll
             for (int j = 0; j < VEC; ++j) {
-                s += (double)w[j];
+                if (w[j] >= DV_LEAST) sum[j & 1] += dv_double(w[j]);
                 rest += left[j];
             }
         }
-        s += (double)rest;
+        double s = sum[0] + sum[1] + (double)rest;
 #pragma unroll
         for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
         return s;
@@ -171,7 +178,7 @@ template <class T, int VEC> __global__ void __launch_bounds__(DV_THREADS) dv_ker
         }
         if (t == 0) a.accepted[b] = n;
     }
-    if (!(total > 0.0) || total > 1.7e308) {      // no class has a weight, or one has no finite one
+    if (!(total > 0.0) || total >= 0x1p128) {      // no class has a weight, or one has no finite one
         if (rank == 0 && t == 0) a.out[b * (a.drafts + 1) + n] = -1;
         return;
     }
@@ -216,14 +223,16 @@ template <class T, int VEC> __global__ void __launch_bounds__(DV_THREADS) dv_ker
         for (int j = 0; j < VEC; ++j) w[j] = left[j] = 0.f;
         if (v < edge(warp + 1)) weights(v, whole, w, left);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) own += (double)w[j] + (double)left[j];
+        for (int j = 0; j < VEC; ++j) {
+            if (w[j] >= DV_LEAST) own += dv_double(w[j]) + (double)left[j];
+        }
         const double upto = dv_scan(own, lane);
         double at = reached + (upto - own);
         int hit = -1;
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
-            at += (double)w[j] + (double)left[j];
-            if (w[j] > 0.f) {
+            if (w[j] >= DV_LEAST) {
+                at += dv_double(w[j]) + (double)left[j];
                 last = v * VEC + j;
                 if (hit < 0 && at > want) hit = v * VEC + j;
             }

@@ -55,8 +55,8 @@ def verify_drafts(target_probs: torch.Tensor, draft_probs: Optional[torch.Tensor
     max(target_probs[n] - draft_probs[n], 0) (without draft probabilities: from target_probs[n] without the refused token), and from
     target_probs[n] where all n drafts stand, or where nothing is left of the difference: the first class c of positive weight whose sum of
     weights up to c is above uniforms[drafts] times their whole sum.  Sums are taken in 64 bits.  Probabilities need not sum to 1; what is
-    not positive, NaN included, weighs nothing; a token that is no class is refused; where no class has a weight, or their sum is not
-    finite, -1 is drawn.  Places behind a sequence's length are not looked at, but for the one at it.  Without a gradient."""
+    below 2^-126, NaN included, weighs nothing; a token that is no class is refused; where no class has a weight, or their sum is not finite
+    in float32, -1 is drawn.  Places behind a sequence's length are not looked at, but for the one at it.  Without a gradient."""
     out = _native.verify_drafts(target_probs, draft_probs, draft_tokens, uniforms, lengths)
     if out is not None:
         return VerifiedDrafts(*out)

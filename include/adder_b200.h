@@ -344,8 +344,8 @@ ADDER_API int adder_b200_distillation_backward(const void* logits, int dtype, lo
  *   out_tokens[sequence][drafts + 1]  the accepted tokens, one more, and -1 behind it
  * The one more is the first class c of positive weight with sum of weights up to c > uniforms[drafts] * their whole sum, of weights
  * max(target_n - draft_n, 0) where token n was refused (target_n but for that token with draft NULL; target_n where those are all 0), else
- * target_n; the last class of positive weight where there is no such one, -1 where no weight is positive or their sum is not finite.  Sums are
- * 64-bit.  A token that is no class is refused; a probability that is NaN counts as 0. */
+ * target_n; the last class of positive weight where there is no such one, -1 where no weight is positive or their sum is 2^128 or more.  Sums are
+ * 64-bit.  A token that is no class is refused; a weight that is NaN or below 2^-126 counts as 0. */
 ADDER_API int adder_b200_verify_drafts(const void* target, const void* draft, int dtype, const long long* tokens, const float* uniforms,
                                        const long long* lengths, long long* out_tokens, long long* accepted, long long sequences,
                                        long long drafts, long long classes, long long target_sequence_stride, long long target_place_stride,
