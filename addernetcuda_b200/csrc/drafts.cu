@@ -22,7 +22,8 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int DV_THREADS = 256, DV_WARPS = DV_THREADS / 32, DV_MOST_PARTS = 8;
+constexpr int DV_THREADS = 512, DV_WARPS = DV_THREADS / 32, DV_MOST_PARTS = 8;
+constexpr int DV_EACH = DV_MOST_PARTS * DV_WARPS / 32;      // segments a lane
 
 struct DvArgs {
     const void* p;                 // [sequences][drafts + 1][classes]
@@ -78,6 +79,7 @@ template <class T, int VEC> __global__ void __launch_bounds__(DV_THREADS) dv_ker
     cg::cluster_group cluster = cg::this_cluster();
     const int parts = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
     const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
     const long long b = blockIdx.x / parts;
     const long long* tokens = a.tokens + b * a.drafts;
     const float* u = a.u + b * (a.drafts + 1);
@@ -150,20 +152,24 @@ template <class T, int VEC> __global__ void __launch_bounds__(DV_THREADS) dv_ker
         for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
         return s;
     };
-    // Sums of all segments in the lanes of every warp, two a lane: what lies before them, and theirs.
-    double before = 0.0, mine[2], total = 0.0;
+    // Sums of all segments in the lanes of every warp, DV_EACH a lane: what lies before them, and theirs.
+    double before = 0.0, mine[DV_EACH], total = 0.0;
     const auto sum_up = [&](bool whole, int turn) {
         const double s = sum_of(v0, v1, whole);
+        if (turn == 0) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");      // all CTAs of the cluster have begun
         if (lane < parts) cluster.map_shared_rank(&sums[turn][0], lane)[segment] = s;
         cluster.sync();
+        double own = 0.0;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) mine[i] = 2 * lane + i < segments ? sums[turn][2 * lane + i] : 0.0;
-        const double all = dv_scan(mine[0] + mine[1], lane);
+        for (int i = 0; i < DV_EACH; ++i) {
+            mine[i] = DV_EACH * lane + i < segments ? sums[turn][DV_EACH * lane + i] : 0.0;
+            own += mine[i];
+        }
+        const double all = dv_scan(own, lane);
         before = __shfl_up_sync(0xffffffffu, all, 1);
         if (lane == 0) before = 0.0;
         total = __shfl_sync(0xffffffffu, all, 31);
     };
-    cluster.sync();      // all CTAs of the cluster have begun
     sum_up(false, 0);
     bool whole = false;
     if (total == 0.0) {      // p nowhere above q: rounding alone, or probabilities that are none
@@ -182,76 +188,65 @@ template <class T, int VEC> __global__ void __launch_bounds__(DV_THREADS) dv_ker
         if (rank == 0 && t == 0) a.out[b * (a.drafts + 1) + n] = -1;
         return;
     }
-    // The segment that holds the border, or, where rounding or u >= 1 leaves none, the last with a weight.
-    const double end0 = before + mine[0], end1 = end0 + mine[1];
-    const unsigned in0 = __ballot_sync(0xffffffffu, mine[0] > 0.0 && end0 > want), in1 = __ballot_sync(0xffffffffu, mine[1] > 0.0 && end1 > want);
-    const unsigned some0 = __ballot_sync(0xffffffffu, mine[0] > 0.0), some1 = __ballot_sync(0xffffffffu, mine[1] > 0.0);
-    int chosen;
-    if ((in0 | in1) != 0) {
-        const int l = __ffs(in0 | in1) - 1;
-        chosen = 2 * l + ((in0 >> l) & 1 ? 0 : 1);
-    } else {
-        const int l = 31 - __clz(some0 | some1);
-        chosen = 2 * l + ((some1 >> l) & 1);
+    // The segment that holds the border, or, where rounding or u >= 1 leaves none, the last with a weight; and what lies before it.
+    double reached = before, before_last = before;
+    int holds = -1, some = -1;
+#pragma unroll
+    for (int i = 0; i < DV_EACH; ++i) {
+        if (mine[i] > 0.0 && holds < 0) {
+            some = i;
+            before_last = reached;
+            if (reached + mine[i] > want) holds = i;
+        }
+        reached += mine[i];
     }
-    // Its CTA reads the segment again, a part a warp, and the warp whose part holds the border (or the last weight) once more.
+    const unsigned holders = __ballot_sync(0xffffffffu, holds >= 0), weighty = __ballot_sync(0xffffffffu, some >= 0);
+    const int from_lane = holders != 0 ? __ffs(holders) - 1 : 31 - __clz(weighty);
+    const int chosen = DV_EACH * from_lane + __shfl_sync(0xffffffffu, some, from_lane);      // the holding one where there is one
+    reached = __shfl_sync(0xffffffffu, before_last, from_lane);
+    // Its CTA reads the segment again, a part a warp and consecutive vectors a lane; the lane whose vectors hold the border (or the last weight) goes
+    // over them once more.
     if (chosen / DV_WARPS != rank) return;
     const int c0 = (int)((long long)nvec * chosen / segments), c1 = (int)((long long)nvec * (chosen + 1) / segments);
-    const auto edge = [&](int i) { return c0 + (int)((long long)(c1 - c0) * i / DV_WARPS); };
-    const double mass = sum_of(edge(warp), edge(warp + 1), whole);
-    if (lane == 0) part_of[warp] = mass;
-    __syncthreads();
-    double reached = __shfl_sync(0xffffffffu, (chosen & 1) ? end0 : before, chosen >> 1), at_last = reached;
-    int holder = -1, last_part = -1;
-    for (int i = 0; i < DV_WARPS && holder < 0; ++i) {
-        const double w = part_of[i];
-        if (w > 0.0) {
-            last_part = i;
-            at_last = reached;
-            if (reached + w > want) holder = i;
-        }
-        reached += w;
-    }
-    if (warp != last_part) return;      // the holder where there is one
-    reached = at_last;
-    int last = -1, found = -1;
-    for (int base = edge(warp); base < edge(warp + 1); base += 32) {
-        const int v = base + lane;
+    const int p0 = c0 + (int)((long long)(c1 - c0) * warp / DV_WARPS), p1 = c0 + (int)((long long)(c1 - c0) * (warp + 1) / DV_WARPS), each = (p1 - p0 + 31) / 32;
+    const int l0 = min(p1, p0 + lane * each), l1 = min(p1, l0 + each);
+    double own = 0.0;
+    for (int v = l0; v < l1; ++v) {
         float w[VEC], left[VEC];
-        double own = 0.0;
+        weights(v, whole, w, left);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) w[j] = left[j] = 0.f;
-        if (v < edge(warp + 1)) weights(v, whole, w, left);
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
+        for (int j = 0; j < VEC; ++j)
             if (w[j] >= DV_LEAST) own += dv_double(w[j]) + (double)left[j];
-        }
-        const double upto = dv_scan(own, lane);
-        double at = reached + (upto - own);
-        int hit = -1;
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-            if (w[j] >= DV_LEAST) {
-                at += dv_double(w[j]) + (double)left[j];
-                last = v * VEC + j;
-                if (hit < 0 && at > want) hit = v * VEC + j;
-            }
-        }
-        const unsigned who = __ballot_sync(0xffffffffu, hit >= 0);
-        if (who != 0) {
-            found = __shfl_sync(0xffffffffu, hit, __ffs(who) - 1);
-            break;
-        }
-        reached += __shfl_sync(0xffffffffu, upto, 31);
     }
-    last = __reduce_max_sync(0xffffffffu, last);
-    if (lane == 0) a.out[b * (a.drafts + 1) + n] = found >= 0 ? found : last;
+    const double upto = dv_scan(own, lane);
+    if (lane == 31) part_of[warp] = upto;
+    __syncthreads();
+    const double mass = lane < DV_WARPS ? part_of[lane] : 0.0, end = reached + dv_scan(mass, lane);
+    const unsigned hold = __ballot_sync(0xffffffffu, mass > 0.0 && end > want), any = __ballot_sync(0xffffffffu, mass > 0.0);
+    const int part = hold != 0 ? __ffs(hold) - 1 : 31 - __clz(any);
+    reached = __shfl_sync(0xffffffffu, end - mass, part);
+    if (warp != part) return;
+    const unsigned hold_lane = __ballot_sync(0xffffffffu, own > 0.0 && reached + upto > want), any_lane = __ballot_sync(0xffffffffu, own > 0.0);
+    if (lane != (hold_lane != 0 ? __ffs(hold_lane) - 1 : 31 - __clz(any_lane))) return;
+    double at = reached + (upto - own);
+    int token = -1;
+    for (int v = l0; v < l1 && !(at > want && token >= 0); ++v) {
+        float w[VEC], left[VEC];
+        weights(v, whole, w, left);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j)
+            if (w[j] >= DV_LEAST && !(at > want && token >= 0)) {
+                at += dv_double(w[j]) + (double)left[j];
+                token = v * VEC + j;
+            }
+    }
+    a.out[b * (a.drafts + 1) + n] = token;
 }
 
 template <class T, int VEC> int launch_drafts(const DvArgs& a, long long sequences, cudaStream_t s) {
-    // A CTA takes at least some 2048 classes, and there are up to four an SM.
+    // A CTA takes at least some 2048 classes, and there are up to two an SM.
     int parts = 1;
-    while (parts < DV_MOST_PARTS && a.classes >= 4096LL * parts && sequences * parts * 2 <= 4LL * sm_count()) parts *= 2;
+    while (parts < DV_MOST_PARTS && a.classes >= 4096LL * parts && sequences * parts * 2 <= 2LL * sm_count()) parts *= 2;
     return launch_clusters(dv_kernel<T, VEC>, (unsigned)(sequences * parts), DV_THREADS, 0, parts, s, a);
 }
 
