@@ -87,6 +87,7 @@ template <class T, int VEC> __global__ void __launch_bounds__(DV_THREADS) dv_ker
     const T* q = a.q != nullptr ? static_cast<const T*>(a.q) + b * a.q_sequence : nullptr;
     const int length = a.lengths == nullptr ? a.drafts : (int)max(0LL, min((long long)a.drafts, a.lengths[b]));
 
+    const float u_last = u[a.drafts];
     if (warp == 0) {
         int n = length;
         for (int base = 0; base < length; base += 32) {
@@ -113,8 +114,9 @@ template <class T, int VEC> __global__ void __launch_bounds__(DV_THREADS) dv_ker
     const T* p_row = p + n * a.p_place;
     const T* q_row = n < length && q != nullptr ? q + n * a.q_place : nullptr;
     const int gone = n < length && q == nullptr && tokens[n] >= 0 && tokens[n] < a.classes ? (int)tokens[n] : -1;
-    const int segments = parts * DV_WARPS, segment = rank * DV_WARPS + warp, nvec = a.classes / VEC;
-    const int v0 = (int)((long long)nvec * segment / segments), v1 = (int)((long long)nvec * (segment + 1) / segments);
+    const int segments = parts * DV_WARPS, segment = rank * DV_WARPS + warp, nvec = a.classes / VEC, shift = 31 - __clz(segments);      // a power of two
+    const auto segment_begin = [&](int i) { return (int)((long long)nvec * i >> shift); };
+    const int v0 = segment_begin(segment), v1 = segment_begin(segment + 1);
 
     // Weights of the classes of vector v, and what fp32 leaves out of them; with `whole` those of p alone.
     const auto weights = [&](int v, bool whole, float (&w)[VEC], float (&left)[VEC]) {
@@ -176,7 +178,7 @@ template <class T, int VEC> __global__ void __launch_bounds__(DV_THREADS) dv_ker
         whole = true;
         sum_up(true, 1);
     }
-    const double want = (double)u[a.drafts] * total;
+    const double want = (double)u_last * total;
     if (rank == 0) {
         for (int i = t; i <= a.drafts; i += DV_THREADS) {
             if (i < n) a.out[b * (a.drafts + 1) + i] = tokens[i];
@@ -207,7 +209,7 @@ template <class T, int VEC> __global__ void __launch_bounds__(DV_THREADS) dv_ker
     // Its CTA reads the segment again, a part a warp and consecutive vectors a lane; the lane whose vectors hold the border (or the last weight) goes
     // over them once more.
     if (chosen / DV_WARPS != rank) return;
-    const int c0 = (int)((long long)nvec * chosen / segments), c1 = (int)((long long)nvec * (chosen + 1) / segments);
+    const int c0 = segment_begin(chosen), c1 = segment_begin(chosen + 1);
     const int p0 = c0 + (int)((long long)(c1 - c0) * warp / DV_WARPS), p1 = c0 + (int)((long long)(c1 - c0) * (warp + 1) / DV_WARPS), each = (p1 - p0 + 31) / 32;
     const int l0 = min(p1, p0 + lane * each), l1 = min(p1, l0 + each);
     double own = 0.0;
