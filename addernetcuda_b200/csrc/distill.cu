@@ -11,6 +11,7 @@
 #include "launch.cuh"
 #include "softmax.cuh"
 #include <cooperative_groups.h>
+#include <type_traits>
 
 namespace adder {
 namespace {
@@ -36,15 +37,30 @@ struct DsFwd {
     float* mass;                     // [rows][k]: t; or null
 };
 
-// Largest value m with sums of 2^((x - m) scale) and, with BOTH, of 2^((x - m) log2 e).
-template <bool BOTH> struct DsSums {
+// What a row's second sum, at temperature 1, is made of: nothing (ONE: none is asked for, or the temperature is 1), an exponential of its own
+// (OWN), or the first one's squared (SQUARE: T = 2) or its fourth power (FOURTH: T = 4).  The exponential unit takes 8 clocks of a scheduler for a
+// warp's values and memory 11, so a second exponential costs time and two products do not (2048x128000 bf16: 145 us with OWN).
+enum DsSecond { ONE, OWN, SQUARE, FOURTH };
+template <int SECOND> __device__ __forceinline__ uint64_t ds_second(uint64_t d, uint64_t e) {
+    if constexpr (SECOND == OWN) {
+        float lo, hi;
+        unpack2(mul2(d, pack2(LOG2E, LOG2E)), lo, hi);
+        return pack2(exp2_fast(lo), exp2_fast(hi));
+    } else {
+        const uint64_t square = mul2(e, e);
+        return SECOND == SQUARE ? square : mul2(square, square);
+    }
+}
+
+// Largest value m with sums of 2^((x - m) scale) and, but with ONE, of 2^((x - m) log2 e).
+template <int SECOND> struct DsSums {
     float m = -INFINITY;
     uint64_t s = 0, s1 = 0;      // pairs
 
     __device__ __forceinline__ void raise(float top, float scale) {
         const float f = m == -INFINITY ? 0.f : exp2_fast((m - top) * scale);
         s = mul2(s, pack2(f, f));
-        if (BOTH) {
+        if (SECOND != ONE) {
             const float f1 = m == -INFINITY ? 0.f : exp2_fast((m - top) * LOG2E);
             s1 = mul2(s1, pack2(f1, f1));
         }
@@ -54,11 +70,9 @@ template <bool BOTH> struct DsSums {
         const uint64_t d = add2(pack2(a, b), pack2(-m, -m));
         float lo, hi;
         unpack2(mul2(d, pack2(scale, scale)), lo, hi);
-        s = add2(s, pack2(exp2_fast(lo), exp2_fast(hi)));
-        if (BOTH) {
-            unpack2(mul2(d, pack2(LOG2E, LOG2E)), lo, hi);
-            s1 = add2(s1, pack2(exp2_fast(lo), exp2_fast(hi)));
-        }
+        const uint64_t e = pack2(exp2_fast(lo), exp2_fast(hi));
+        s = add2(s, e);
+        if constexpr (SECOND != ONE) s1 = add2(s1, ds_second<SECOND>(d, e));
     }
 };
 struct DsPart {
@@ -80,7 +94,7 @@ __device__ __forceinline__ DsPart ds_join_lanes(DsPart p, float scale) {
 }
 
 // Values of a vector into the sums.
-template <class T, int U, bool BOTH> __device__ __forceinline__ void ds_take(const uint4 (&q)[U], DsSums<BOTH>& run, float scale) {
+template <class T, int U, int SECOND> __device__ __forceinline__ void ds_take(const uint4 (&q)[U], DsSums<SECOND>& run, float scale) {
     constexpr int VE = Vec16<T>::N;
     uint32_t w;
 #pragma unroll
@@ -105,10 +119,18 @@ __device__ __forceinline__ float ds_value(const void* p, int type, long long i) 
     return type == ADDER_TYPE_BF16 ? to_float(static_cast<const __nv_bfloat16*>(p)[i]) : to_float(static_cast<const __half*>(p)[i]);
 }
 
+// The teacher's classes of a row, looked up while the row is read: their logits by the teacher and of the row, and their indices, -1 where there is
+// none.
+struct DsNamed {
+    float z[DS_MAX_K], x[DS_MAX_K];
+    int at[DS_MAX_K];
+};
+
 // THREADS threads a row (32: a warp, four of them a CTA); with CLUSTER a row is shared out over the CTAs of a cluster.
-template <class T, int THREADS, bool CLUSTER, bool BOTH> __global__ void __launch_bounds__(THREADS == 32 ? 128 : THREADS) ds_forward_kernel(const DsFwd a) {
+template <class T, int THREADS, bool CLUSTER, int SECOND> __global__ void __launch_bounds__(THREADS == 32 ? 128 : THREADS) ds_forward_kernel(const DsFwd a) {
     constexpr int VE = Vec16<T>::N, WARPS = THREADS / 32;
     __shared__ DsPart parts_of[WARPS], ranks_of[8];
+    __shared__ DsNamed named_of[THREADS == 32 ? 4 : 1];
     const int t = threadIdx.x % THREADS, lane = t & 31;
     const int parts = CLUSTER ? (int)cg::this_cluster().num_blocks() : 1, rank = CLUSTER ? (int)cg::this_cluster().block_rank() : 0;
     const long long row = THREADS == 32 ? (long long)blockIdx.x * 4 + threadIdx.x / 32 : blockIdx.x / parts;
@@ -120,17 +142,51 @@ template <class T, int THREADS, bool CLUSTER, bool BOTH> __global__ void __launc
     const int v0 = (int)((long long)nvec * rank / parts), v1 = (int)((long long)nvec * (rank + 1) / parts);
     const uint4* vec = reinterpret_cast<const uint4*>(x + head);
 
-    DsSums<BOTH> run;
-    int v = v0 + t;
-    for (; v + (DS_UNROLL - 1) * THREADS < v1; v += DS_UNROLL * THREADS) {
-        uint4 q[DS_UNROLL];
-#pragma unroll
-        for (int u = 0; u < DS_UNROLL; ++u) q[u] = __ldg(vec + v + u * THREADS);
-        ds_take<T, DS_UNROLL>(q, run, a.scale);
+    DsNamed& named = named_of[THREADS == 32 ? threadIdx.x / 32 : 0];
+    bool broken = false;
+    if (rank == 0) {
+        for (int j = t; j < a.k; j += THREADS) {
+            const long long i = a.indices[row * a.k + j];
+            broken |= i >= a.classes || i < -1;
+            const bool in = i >= 0 && i < a.classes;
+            named.at[j] = in ? (int)i : -1;
+            named.z[j] = ds_value(a.teacher, a.teacher_type, row * a.k + j);
+            if (in) named.x[j] = to_float(x[i]);
+        }
     }
-    for (; v < v1; v += THREADS) {
-        uint4 q[1] = {__ldg(vec + v)};
-        ds_take<T, 1>(q, run, a.scale);
+    long long target = a.ignore;
+    float x_target = 0.f;
+    if (a.targets != nullptr && t == 0) {
+        target = a.targets[row];
+        if (target >= 0 && target < a.classes) x_target = to_float(x[target]);
+    }
+    DsSums<SECOND> run;
+    // a thread's next vectors are on their way while it works on some
+    uint4 q[2][DS_UNROLL];
+    const auto fetch = [&](int v, uint4 (&to)[DS_UNROLL]) {
+#pragma unroll
+        for (int u = 0; u < DS_UNROLL; ++u) {
+            if (v + u * THREADS < v1) to[u] = __ldg(vec + v + u * THREADS);
+        }
+    };
+    fetch(v0 + t, q[0]);
+    const auto take = [&](int v, const uint4 (&from)[DS_UNROLL]) {
+        if (v + (DS_UNROLL - 1) * THREADS < v1) {
+            ds_take<T, DS_UNROLL>(from, run, a.scale);
+            return;
+        }
+#pragma unroll
+        for (int u = 0; u < DS_UNROLL - 1; ++u)
+            if (v + u * THREADS < v1) {
+                const uint4 one[1] = {from[u]};
+                ds_take<T, 1>(one, run, a.scale);
+            }
+    };
+    for (int v = v0 + t; v < v1; v += 2 * DS_UNROLL * THREADS) {
+        fetch(v + DS_UNROLL * THREADS, q[1]);
+        take(v, q[0]);
+        fetch(v + 2 * DS_UNROLL * THREADS, q[0]);
+        take(v + DS_UNROLL * THREADS, q[1]);
     }
     if (t < singles) {
         const float one = to_float(x[t < head ? t : t + nvec * VE]);
@@ -157,37 +213,33 @@ template <class T, int THREADS, bool CLUSTER, bool BOTH> __global__ void __launc
         all = ds_join_lanes(all, a.scale);
     }
     // The teacher's classes, by one warp.
-    if (t >= 32) return;
-    const auto z = [&](int j) { return ds_value(a.teacher, a.teacher_type, row * a.k + j); };
-    const long long* at = a.indices + row * a.k;
-    float top = -INFINITY;
-    bool broken = false;
-    for (int j = lane; j < a.k; j += 32) {
-        const long long i = at[j];
-        broken |= i >= a.classes || i < -1;
-        if (i >= 0) top = max_nan(top, z(j));
+    if constexpr (THREADS > 32) {
+        broken = __syncthreads_or(broken);
+        if (t >= 32) return;
+    } else {
+        broken = __any_sync(0xffffffffu, broken);
+        __syncwarp();
     }
+    float top = -INFINITY;
+    for (int j = lane; j < a.k; j += 32)
+        if (named.at[j] >= 0) top = max_nan(top, named.z[j]);
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, off));
-    broken = __any_sync(0xffffffffu, broken) || top == INFINITY || top != top;
+    broken |= top == INFINITY || top != top;
     const bool empty = top == -INFINITY;
     float sum = 0.f;
     for (int j = lane; j < a.k; j += 32)
-        if (at[j] >= 0 && !empty) sum += exp2_fast((z(j) - top) * a.scale);
+        if (named.at[j] >= 0 && !empty) sum += exp2_fast((named.z[j] - top) * a.scale);
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
     const float log_mass = logf(sum), log_sum = logf(all.s);
     float d = 0.f;
     for (int j = lane; j < a.k; j += 32) {
-        const long long i = at[j];
         float share = 0.f;
-        if (i >= 0 && i < a.classes && !empty) {
-            const float e = (z(j) - top) * a.inv_t, log_t = e - log_mass;
-            share = exp2_fast((z(j) - top) * a.scale) / sum;
-            if (share > 0.f) {
-                const float xi = to_float(x[i]);
-                d += share * (log_t - ((xi - all.m) * a.inv_t - log_sum));
-            }
+        if (named.at[j] >= 0 && !empty) {
+            const float e = (named.z[j] - top) * a.inv_t;
+            share = exp2_fast((named.z[j] - top) * a.scale) / sum;
+            if (share > 0.f) d += share * (e - log_mass - ((named.x[j] - all.m) * a.inv_t - log_sum));
         }
         if (a.mass != nullptr) a.mass[row * a.k + j] = broken ? NAN : share;
     }
@@ -197,14 +249,13 @@ template <class T, int THREADS, bool CLUSTER, bool BOTH> __global__ void __launc
         const bool nothing = all.m == -INFINITY;
         a.divergence[row] = broken ? NAN : empty ? 0.f : nothing ? INFINITY : d;
         if (a.targets != nullptr) {
-            const long long target = a.targets[row];
-            const float s1 = BOTH ? all.s1 : all.s;
-            a.log_prob[row] = target == a.ignore ? 0.f : target < 0 || target >= a.classes ? NAN : nothing ? -INFINITY : to_float(x[target]) - all.m - logf(s1);
+            const float s1 = SECOND != ONE ? all.s1 : all.s;
+            a.log_prob[row] = target == a.ignore ? 0.f : target < 0 || target >= a.classes ? NAN : nothing ? -INFINITY : x_target - all.m - logf(s1);
         }
         if (a.stats != nullptr) {
             a.stats[3 * row] = all.m;
             a.stats[3 * row + 1] = all.s;
-            a.stats[3 * row + 2] = BOTH ? all.s1 : all.s;
+            a.stats[3 * row + 2] = SECOND != ONE ? all.s1 : all.s;
         }
     }
 }
@@ -226,18 +277,16 @@ struct DsBwd {
 };
 
 // What a row's elements have in common: dx = soft 2^((x - m) scale) + hard 2^((x - m) log2 e)
-template <bool BOTH> struct DsSlope {
+template <int SECOND> struct DsSlope {
     float m, soft, hard, scale;
     __device__ __forceinline__ uint64_t pair(float a, float b) const {
         const uint64_t d = add2(pack2(a, b), pack2(-m, -m));
         float lo, hi;
         unpack2(mul2(d, pack2(scale, scale)), lo, hi);
-        uint64_t r = mul2(pack2(exp2_fast(lo), exp2_fast(hi)), pack2(soft, soft));
-        if (BOTH) {
-            unpack2(mul2(d, pack2(LOG2E, LOG2E)), lo, hi);
-            r = fma2(pack2(exp2_fast(lo), exp2_fast(hi)), pack2(hard, hard), r);
-        }
-        return r;
+        const uint64_t e = pack2(exp2_fast(lo), exp2_fast(hi));
+        const uint64_t r = mul2(e, pack2(soft, soft));
+        if constexpr (SECOND != ONE) return fma2(ds_second<SECOND>(d, e), pack2(hard, hard), r);
+        else return r;
     }
     __device__ __forceinline__ float one(float a) const {
         float lo, hi;
@@ -246,12 +295,13 @@ template <bool BOTH> struct DsSlope {
     }
 };
 
-template <class T, int THREADS, bool BOTH> __global__ void __launch_bounds__(THREADS == 32 ? 128 : THREADS) ds_backward_kernel(const DsBwd a) {
+template <class T, int THREADS, int SECOND> __global__ void __launch_bounds__(THREADS == 32 ? 128 : THREADS) ds_backward_kernel(const DsBwd a) {
     constexpr int VE = Vec16<T>::N;
     const int t = threadIdx.x % THREADS;
-    const long long row = THREADS == 32 ? (long long)blockIdx.x * 4 + threadIdx.x / 32 : blockIdx.x / a.segments;
+    // from the last row on: what the forward read last is still in L2
+    const long long row = a.rows - 1 - (THREADS == 32 ? (long long)blockIdx.x * 4 + threadIdx.x / 32 : blockIdx.x / a.segments);
     const int segment = THREADS == 32 ? 0 : (int)(blockIdx.x % a.segments);
-    if (row >= a.rows) return;
+    if (row < 0) return;
     const T* x = static_cast<const T*>(a.x) + row * a.stride;
     T* dx = static_cast<T*>(a.dx) + row * (long long)a.classes;
     const int mis = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
@@ -277,13 +327,13 @@ template <class T, int THREADS, bool BOTH> __global__ void __launch_bounds__(THR
     for (int j = threadIdx.x & 31; j < a.k; j += 32) some = max_nan(some, mass[j]);
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) some = max_nan(some, __shfl_xor_sync(0xffffffffu, some, off));
-    DsSlope<BOTH> slope;
+    DsSlope<SECOND> slope;
     slope.m = m;
     slope.scale = a.scale;
     const float soft = some == 0.f ? 0.f : some != some ? NAN : gd;
     slope.soft = soft / s;
     slope.hard = -gl / s1;
-    if (!BOTH) slope.soft += slope.hard;
+    if (SECOND == ONE) slope.soft += slope.hard;
 
     int begin, end;
     if (same) {
@@ -332,16 +382,24 @@ bool ds_warp_rows(long long rows, long long classes) {
     return classes <= 1024 || (classes <= 4096 && rows >= 8LL * sm_count()) || (classes <= 8192 && rows >= 24LL * sm_count());
 }
 
-template <class T, bool BOTH> int launch_distill_forward(const DsFwd& a, cudaStream_t s) {
+template <class T, int SECOND> int launch_distill_forward(const DsFwd& a, cudaStream_t s) {
     if (ds_warp_rows(a.rows, a.classes)) {
-        ds_forward_kernel<T, 32, false, BOTH><<<(unsigned)((a.rows + 3) / 4), 128, 0, s>>>(a);
+        ds_forward_kernel<T, 32, false, SECOND><<<(unsigned)((a.rows + 3) / 4), 128, 0, s>>>(a);
         return launched();
     }
     int parts = 1;      // few rows are split over clusters, as long as there are no more than 4 CTAs an SM
     while (parts < 8 && a.rows * parts * 2 <= sm_count() * 4 && a.classes >= 8192LL * parts) parts *= 2;
-    if (parts > 1) return launch_clusters(ds_forward_kernel<T, DS_TEAM, true, BOTH>, (unsigned)(a.rows * parts), DS_TEAM, 0, parts, s, a);
-    ds_forward_kernel<T, DS_TEAM, false, BOTH><<<(unsigned)a.rows, DS_TEAM, 0, s>>>(a);
+    if (parts > 1) return launch_clusters(ds_forward_kernel<T, DS_TEAM, true, SECOND>, (unsigned)(a.rows * parts), DS_TEAM, 0, parts, s, a);
+    ds_forward_kernel<T, DS_TEAM, false, SECOND><<<(unsigned)a.rows, DS_TEAM, 0, s>>>(a);
     return launched();
+}
+
+// f(std::integral_constant<int, DsSecond>) by the temperature, and by whether the probabilities at temperature 1 are asked for.
+template <class F> int with_second(float temperature, bool asked, F&& f) {
+    if (!asked || temperature == 1.f) return f(std::integral_constant<int, ONE>());
+    if (temperature == 2.f) return f(std::integral_constant<int, SQUARE>());
+    if (temperature == 4.f) return f(std::integral_constant<int, FOURTH>());
+    return f(std::integral_constant<int, OWN>());
 }
 
 int ds_check(long long rows, long long classes, long long row_stride, int dtype, int k, float temperature) {
@@ -371,10 +429,9 @@ int adder_b200_distillation_forward(const void* logits, int dtype, long long row
     const DsFwd a{logits, rows, row_stride, (int)classes, k, teacher, teacher_dtype, indices, targets, ignore_index, (float)(1.0 / temperature),
                   (float)(1.4426950408889634 / temperature), divergence, log_prob, stats, mass};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const bool both = targets != nullptr && temperature != 1.f;
     return with_type(dtype, [&](auto* type) {
         using T = std::remove_pointer_t<decltype(type)>;
-        return both ? launch_distill_forward<T, true>(a, s) : launch_distill_forward<T, false>(a, s);
+        return with_second(temperature, targets != nullptr, [&](auto second) { return launch_distill_forward<T, decltype(second)::value>(a, s); });
     });
 }
 
@@ -390,7 +447,7 @@ int adder_b200_distillation_backward(const void* logits, int dtype, long long ro
     if (!aligned_to(logits, size) || !aligned_to(grad_logits, size) || !aligned_to(indices, 8) || !aligned_to(targets, 8) || !aligned_to(stats, 4) ||
         !aligned_to(mass, 4) || !aligned_to(grad_divergence, 4) || !aligned_to(grad_log_prob, 4))
         return ADDER_ERR_ALIGNMENT;
-    const bool warps = ds_warp_rows(rows, classes), both = grad_log_prob != nullptr && temperature != 1.f;
+    const bool warps = ds_warp_rows(rows, classes);
     // A CTA takes two turns, whose loads and stores overlap, or one where there would be too few CTAs.
     const long long turn = (long long)DS_TEAM * DS_UNROLL * (16 / size), ones = (classes + turn - 1) / turn;
     const long long segments = warps ? 1 : rows * ones >= 8LL * sm_count() ? (ones + 1) / 2 : ones;
@@ -401,14 +458,12 @@ int adder_b200_distillation_backward(const void* logits, int dtype, long long ro
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     return with_type(dtype, [&](auto* type) {
         using T = std::remove_pointer_t<decltype(type)>;
-        if (warps) {
-            if (both) ds_backward_kernel<T, 32, true><<<(unsigned)grid, 128, 0, s>>>(a);
-            else ds_backward_kernel<T, 32, false><<<(unsigned)grid, 128, 0, s>>>(a);
-        } else {
-            if (both) ds_backward_kernel<T, DS_TEAM, true><<<(unsigned)grid, DS_TEAM, 0, s>>>(a);
-            else ds_backward_kernel<T, DS_TEAM, false><<<(unsigned)grid, DS_TEAM, 0, s>>>(a);
-        }
-        return launched();
+        return with_second(temperature, grad_log_prob != nullptr, [&](auto second) {
+            constexpr int SECOND = decltype(second)::value;
+            if (warps) ds_backward_kernel<T, 32, SECOND><<<(unsigned)grid, 128, 0, s>>>(a);
+            else ds_backward_kernel<T, DS_TEAM, SECOND><<<(unsigned)grid, DS_TEAM, 0, s>>>(a);
+            return launched();
+        });
     });
 }
 
