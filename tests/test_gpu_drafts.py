@@ -118,6 +118,19 @@ def test_special_values():
     _check(p, None, tokens, u)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("scale", [1e-3, 3.0, 200.0])
+def test_weights_that_are_no_probabilities(dtype, scale):
+    """Sums far below and above 1, and single weights of several."""
+    for v in (37, 5000, 40001):
+        torch.manual_seed(v)
+        p = (scale * torch.rand(12, 3, v, device=DEV)).to(dtype)
+        q = (scale * torch.rand(12, 2, v, device=DEV)).to(dtype)
+        tokens = torch.randint(0, v, (12, 2), device=DEV)
+        _check(p, q, tokens, torch.rand(12, 3, device=DEV))
+        _check(p, None, tokens, torch.rand(12, 3, device=DEV))
+
+
 def test_views_and_places_behind_the_length():
     from addernetcuda_b200.drafts import verify_drafts
     p, q, tokens, u = _inputs(6, 3, 1024, torch.bfloat16, seed=3)
