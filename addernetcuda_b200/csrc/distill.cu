@@ -119,33 +119,84 @@ __device__ __forceinline__ float ds_value(const void* p, int type, long long i) 
     return type == ADDER_TYPE_BF16 ? to_float(static_cast<const __nv_bfloat16*>(p)[i]) : to_float(static_cast<const __half*>(p)[i]);
 }
 
-// The teacher's classes of a row, looked up while the row is read: their logits by the teacher and of the row, and their indices, -1 where there is
-// none.
+// A row as a team sees it: vectors v0 to v1 - 1 (shared out over a cluster), and up to VE - 1 single elements before and behind all
+// vectors, which are rank 0's.
+template <class T> struct DsRow {
+    static constexpr int VE = Vec16<T>::N;
+    const T* x;
+    const uint4* vec;
+    int head, nvec, singles, v0, v1;
+
+    __device__ __forceinline__ void set(const DsFwd& a, long long row, int rank, int parts) {
+        x = static_cast<const T*>(a.x) + row * a.stride;
+        const int mis = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
+        head = min(a.classes, mis == 0 ? 0 : VE - mis);
+        nvec = (a.classes - head) / VE;
+        singles = rank == 0 ? a.classes - nvec * VE : 0;
+        v0 = parts == 1 ? 0 : (int)((long long)nvec * rank / parts);
+        v1 = parts == 1 ? nvec : (int)((long long)nvec * (rank + 1) / parts);
+        vec = reinterpret_cast<const uint4*>(x + head);
+    }
+    __device__ __forceinline__ int single(int i) const { return i < head ? i : i + nvec * VE; }
+};
+
+// A thread's share of a row, every THREADS-th vector, the next ones on their way while it works on some.
+template <class T, int THREADS, int SECOND> struct DsReader {
+    uint4 q[2][DS_UNROLL];
+
+    __device__ __forceinline__ void fetch(const DsRow<T>& r, int v, uint4 (&to)[DS_UNROLL]) {
+#pragma unroll
+        for (int u = 0; u < DS_UNROLL; ++u)
+            if (v + u * THREADS < r.v1) to[u] = __ldg(r.vec + v + u * THREADS);
+    }
+    __device__ __forceinline__ void take(const DsRow<T>& r, int v, const uint4 (&from)[DS_UNROLL], DsSums<SECOND>& run, float scale) {
+        if (v + (DS_UNROLL - 1) * THREADS < r.v1) {
+            ds_take<T, DS_UNROLL>(from, run, scale);
+            return;
+        }
+#pragma unroll
+        for (int u = 0; u < DS_UNROLL - 1; ++u)
+            if (v + u * THREADS < r.v1) {
+                const uint4 one[1] = {from[u]};
+                ds_take<T, 1>(one, run, scale);
+            }
+    }
+    __device__ __forceinline__ void begin(const DsRow<T>& r, int t) { fetch(r, r.v0 + t, q[0]); }
+    // The sums of a row that has begun.
+    __device__ __forceinline__ DsPart read(const DsRow<T>& r, int t, float scale) {
+        DsSums<SECOND> run;
+        for (int v = r.v0 + t; v < r.v1; v += 2 * DS_UNROLL * THREADS) {
+            fetch(r, v + DS_UNROLL * THREADS, q[1]);
+            take(r, v, q[0], run, scale);
+            fetch(r, v + 2 * DS_UNROLL * THREADS, q[0]);
+            take(r, v + DS_UNROLL * THREADS, q[1], run, scale);
+        }
+        if (t < r.singles) {
+            const float one = to_float(r.x[r.single(t)]);
+            if (!(one <= run.m)) run.raise(one, scale);
+            if (run.m != -INFINITY) run.add(one, -INFINITY, scale);
+        }
+        float lo, hi, lo1, hi1;
+        unpack2(run.s, lo, hi);
+        unpack2(run.s1, lo1, hi1);
+        return {run.m, lo + hi, lo1 + hi1};
+    }
+};
+
+// What the teacher says of a row, looked up by a warp: its classes' logits by the teacher and of the row, their indices (-1: none), and the target.
 struct DsNamed {
     float z[DS_MAX_K], x[DS_MAX_K];
     int at[DS_MAX_K];
 };
+template <class T> struct DsTold {
+    bool broken;
+    long long target;
+    float x_target;
 
-// THREADS threads a row (32: a warp, four of them a CTA); with CLUSTER a row is shared out over the CTAs of a cluster.
-template <class T, int THREADS, bool CLUSTER, int SECOND> __global__ void __launch_bounds__(THREADS == 32 ? 128 : THREADS) ds_forward_kernel(const DsFwd a) {
-    constexpr int VE = Vec16<T>::N, WARPS = THREADS / 32;
-    __shared__ DsPart parts_of[WARPS], ranks_of[8];
-    __shared__ DsNamed named_of[THREADS == 32 ? 4 : 1];
-    const int t = threadIdx.x % THREADS, lane = t & 31;
-    const int parts = CLUSTER ? (int)cg::this_cluster().num_blocks() : 1, rank = CLUSTER ? (int)cg::this_cluster().block_rank() : 0;
-    const long long row = THREADS == 32 ? (long long)blockIdx.x * 4 + threadIdx.x / 32 : blockIdx.x / parts;
-    if (CLUSTER) asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");
-    if (THREADS == 32 && row >= a.rows) return;
-    const T* x = static_cast<const T*>(a.x) + row * a.stride;
-    const int mis = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T)), head = min(a.classes, mis == 0 ? 0 : VE - mis);
-    const int nvec = (a.classes - head) / VE, singles = rank == 0 ? a.classes - nvec * VE : 0;
-    const int v0 = (int)((long long)nvec * rank / parts), v1 = (int)((long long)nvec * (rank + 1) / parts);
-    const uint4* vec = reinterpret_cast<const uint4*>(x + head);
-
-    DsNamed& named = named_of[THREADS == 32 ? threadIdx.x / 32 : 0];
-    bool broken = false;
-    if (rank == 0) {
-        for (int j = t; j < a.k; j += THREADS) {
+    __device__ __forceinline__ void look_up(const DsFwd& a, long long row, const T* x, int lane, DsNamed& named) {
+        broken = false;
+        target = a.targets != nullptr ? a.targets[row] : a.ignore;
+        for (int j = lane; j < a.k; j += 32) {
             const long long i = a.indices[row * a.k + j];
             broken |= i >= a.classes || i < -1;
             const bool in = i >= 0 && i < a.classes;
@@ -153,80 +204,20 @@ template <class T, int THREADS, bool CLUSTER, int SECOND> __global__ void __laun
             named.z[j] = ds_value(a.teacher, a.teacher_type, row * a.k + j);
             if (in) named.x[j] = to_float(x[i]);
         }
-    }
-    long long target = a.ignore;
-    float x_target = 0.f;
-    if (a.targets != nullptr && t == 0) {
-        target = a.targets[row];
-        if (target >= 0 && target < a.classes) x_target = to_float(x[target]);
-    }
-    DsSums<SECOND> run;
-    // a thread's next vectors are on their way while it works on some
-    uint4 q[2][DS_UNROLL];
-    const auto fetch = [&](int v, uint4 (&to)[DS_UNROLL]) {
-#pragma unroll
-        for (int u = 0; u < DS_UNROLL; ++u) {
-            if (v + u * THREADS < v1) to[u] = __ldg(vec + v + u * THREADS);
-        }
-    };
-    fetch(v0 + t, q[0]);
-    const auto take = [&](int v, const uint4 (&from)[DS_UNROLL]) {
-        if (v + (DS_UNROLL - 1) * THREADS < v1) {
-            ds_take<T, DS_UNROLL>(from, run, a.scale);
-            return;
-        }
-#pragma unroll
-        for (int u = 0; u < DS_UNROLL - 1; ++u)
-            if (v + u * THREADS < v1) {
-                const uint4 one[1] = {from[u]};
-                ds_take<T, 1>(one, run, a.scale);
-            }
-    };
-    for (int v = v0 + t; v < v1; v += 2 * DS_UNROLL * THREADS) {
-        fetch(v + DS_UNROLL * THREADS, q[1]);
-        take(v, q[0]);
-        fetch(v + 2 * DS_UNROLL * THREADS, q[0]);
-        take(v + DS_UNROLL * THREADS, q[1]);
-    }
-    if (t < singles) {
-        const float one = to_float(x[t < head ? t : t + nvec * VE]);
-        if (!(one <= run.m)) run.raise(one, a.scale);
-        if (run.m != -INFINITY) run.add(one, -INFINITY, a.scale);
-    }
-    float lo, hi, lo1, hi1;
-    unpack2(run.s, lo, hi);
-    unpack2(run.s1, lo1, hi1);
-    DsPart all{run.m, lo + hi, lo1 + hi1};
-    all = ds_join_lanes(all, a.scale);
-    if constexpr (THREADS > 32) {
-        if (lane == 0) parts_of[t >> 5] = all;
-        __syncthreads();
-        all = lane < WARPS ? parts_of[lane] : DsPart{-INFINITY, 0.f, 0.f};
-        all = ds_join_lanes(all, a.scale);
-    }
-    if constexpr (CLUSTER) {
-        asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
-        if (t == 0) cg::this_cluster().map_shared_rank(ranks_of, 0)[rank] = all;
-        cg::this_cluster().sync();
-        if (rank != 0) return;
-        all = lane < parts ? ranks_of[lane] : DsPart{-INFINITY, 0.f, 0.f};
-        all = ds_join_lanes(all, a.scale);
-    }
-    // The teacher's classes, by one warp.
-    if constexpr (THREADS > 32) {
-        broken = __syncthreads_or(broken);
-        if (t >= 32) return;
-    } else {
+        x_target = target >= 0 && target < a.classes ? to_float(x[target]) : 0.f;
         broken = __any_sync(0xffffffffu, broken);
         __syncwarp();
     }
+};
+
+// A row's outputs from its sums, by the warp that has looked up what the teacher says.
+template <class T, int SECOND> __device__ __forceinline__ void ds_finish(const DsFwd& a, long long row, const DsPart& all, const DsTold<T>& told, const DsNamed& named, int lane) {
     float top = -INFINITY;
     for (int j = lane; j < a.k; j += 32)
         if (named.at[j] >= 0) top = max_nan(top, named.z[j]);
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, off));
-    broken |= top == INFINITY || top != top;
-    const bool empty = top == -INFINITY;
+    const bool broken = told.broken || top == INFINITY || top != top, empty = top == -INFINITY;
     float sum = 0.f;
     for (int j = lane; j < a.k; j += 32)
         if (named.at[j] >= 0 && !empty) sum += exp2_fast((named.z[j] - top) * a.scale);
@@ -247,17 +238,107 @@ template <class T, int THREADS, bool CLUSTER, int SECOND> __global__ void __laun
     for (int off = 16; off > 0; off >>= 1) d += __shfl_xor_sync(0xffffffffu, d, off);
     if (lane == 0) {
         const bool nothing = all.m == -INFINITY;
+        const float s1 = SECOND != ONE ? all.s1 : all.s;
         a.divergence[row] = broken ? NAN : empty ? 0.f : nothing ? INFINITY : d;
-        if (a.targets != nullptr) {
-            const float s1 = SECOND != ONE ? all.s1 : all.s;
-            a.log_prob[row] = target == a.ignore ? 0.f : target < 0 || target >= a.classes ? NAN : nothing ? -INFINITY : x_target - all.m - logf(s1);
-        }
+        if (a.targets != nullptr)
+            a.log_prob[row] = told.target == a.ignore ? 0.f : told.target < 0 || told.target >= a.classes ? NAN : nothing ? -INFINITY : told.x_target - all.m - logf(s1);
         if (a.stats != nullptr) {
             a.stats[3 * row] = all.m;
             a.stats[3 * row + 1] = all.s;
-            a.stats[3 * row + 2] = SECOND != ONE ? all.s1 : all.s;
+            a.stats[3 * row + 2] = s1;
         }
     }
+}
+
+// A warp a row, four of them a CTA.
+template <class T, int SECOND> __global__ void __launch_bounds__(128) ds_warp_kernel(const DsFwd a) {
+    __shared__ DsNamed named_of[4];
+    const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+    const long long row = (long long)blockIdx.x * 4 + warp;
+    if (row >= a.rows) return;
+    DsRow<T> r;
+    r.set(a, row, 0, 1);
+    DsReader<T, 32, SECOND> reader;
+    reader.begin(r, lane);
+    DsTold<T> told;
+    told.look_up(a, row, r.x, lane, named_of[warp]);
+    ds_finish<T, SECOND>(a, row, ds_join_lanes(reader.read(r, lane, a.scale), a.scale), told, named_of[warp], lane);
+}
+
+// A CTA's rows one after another: DS_TEAM threads read them, and a warp more finishes each while the others read the next (2048x50257 bf16 with 64 classes
+// of the teacher's: 47 us where a CTA of DS_TEAM threads did one row and all of it).
+constexpr int DS_STREAM = DS_TEAM + 32;
+enum { DS_EMPTY = 1, DS_FULL = 3 };      // named barriers, two of each; 0 is __syncthreads
+__device__ __forceinline__ void ds_sync(int id) { asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(DS_STREAM) : "memory"); }
+__device__ __forceinline__ void ds_arrive(int id) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "n"(DS_STREAM) : "memory"); }
+
+template <class T, int SECOND> __global__ void __launch_bounds__(DS_STREAM, 4) ds_stream_kernel(const DsFwd a) {
+    constexpr int WARPS = DS_TEAM / 32;
+    __shared__ DsPart parts_of[2][WARPS];
+    __shared__ DsNamed named;
+    const int t = threadIdx.x, lane = t & 31;
+    long long row = blockIdx.x;
+    DsRow<T> r;
+    r.set(a, row, 0, 1);
+    if (t < DS_TEAM) {
+        DsReader<T, DS_TEAM, SECOND> reader;
+        reader.begin(r, t);
+        for (int turn = 0; row < a.rows; turn ^= 1) {
+            DsPart mine = reader.read(r, t, a.scale);
+            row += gridDim.x;
+            if (row < a.rows) {
+                r.set(a, row, 0, 1);
+                reader.begin(r, t);
+            }
+            mine = ds_join_lanes(mine, a.scale);
+            ds_sync(DS_EMPTY + turn);      // the row before the last is finished
+            if (lane == 0) parts_of[turn][t >> 5] = mine;
+            __syncwarp();
+            ds_arrive(DS_FULL + turn);
+        }
+        return;
+    }
+    ds_arrive(DS_EMPTY);
+    ds_arrive(DS_EMPTY + 1);
+    for (int turn = 0; row < a.rows; turn ^= 1, row += gridDim.x) {
+        r.set(a, row, 0, 1);
+        DsTold<T> told;
+        told.look_up(a, row, r.x, lane, named);
+        ds_sync(DS_FULL + turn);
+        const DsPart all = lane < WARPS ? parts_of[turn][lane] : DsPart{-INFINITY, 0.f, 0.f};
+        __syncwarp();
+        // those that will wait for it: the rows after the next
+        if (row + 2 * (long long)gridDim.x < a.rows) ds_arrive(DS_EMPTY + turn);
+        ds_finish<T, SECOND>(a, row, ds_join_lanes(all, a.scale), told, named, lane);
+        __syncwarp();
+    }
+}
+
+// Few rows: each is shared out over a cluster of CTAs.
+template <class T, int SECOND> __global__ void __launch_bounds__(DS_TEAM) ds_cluster_kernel(const DsFwd a) {
+    constexpr int WARPS = DS_TEAM / 32;
+    __shared__ DsPart parts_of[WARPS], ranks_of[8];
+    __shared__ DsNamed named;
+    const int t = threadIdx.x, lane = t & 31, parts = (int)cg::this_cluster().num_blocks(), rank = (int)cg::this_cluster().block_rank();
+    const long long row = blockIdx.x / parts;
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+    DsRow<T> r;
+    r.set(a, row, rank, parts);
+    DsReader<T, DS_TEAM, SECOND> reader;
+    reader.begin(r, t);
+    DsTold<T> told;
+    if (rank == 0 && t < 32) told.look_up(a, row, r.x, lane, named);
+    const DsPart mine = ds_join_lanes(reader.read(r, t, a.scale), a.scale);
+    if (lane == 0) parts_of[t >> 5] = mine;
+    __syncthreads();
+    DsPart all = lane < WARPS ? parts_of[lane] : DsPart{-INFINITY, 0.f, 0.f};
+    all = ds_join_lanes(all, a.scale);
+    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");      // all CTAs of the cluster have begun
+    if (t == 0) cg::this_cluster().map_shared_rank(ranks_of, 0)[rank] = all;
+    cg::this_cluster().sync();
+    if (rank != 0 || t >= 32) return;
+    all = lane < parts ? ranks_of[lane] : DsPart{-INFINITY, 0.f, 0.f};
+    ds_finish<T, SECOND>(a, row, ds_join_lanes(all, a.scale), told, named, lane);
 }
 
 struct DsBwd {
@@ -384,13 +465,14 @@ bool ds_warp_rows(long long rows, long long classes) {
 
 template <class T, int SECOND> int launch_distill_forward(const DsFwd& a, cudaStream_t s) {
     if (ds_warp_rows(a.rows, a.classes)) {
-        ds_forward_kernel<T, 32, false, SECOND><<<(unsigned)((a.rows + 3) / 4), 128, 0, s>>>(a);
+        ds_warp_kernel<T, SECOND><<<(unsigned)((a.rows + 3) / 4), 128, 0, s>>>(a);
         return launched();
     }
     int parts = 1;      // few rows are split over clusters, as long as there are no more than 4 CTAs an SM
     while (parts < 8 && a.rows * parts * 2 <= sm_count() * 4 && a.classes >= 8192LL * parts) parts *= 2;
-    if (parts > 1) return launch_clusters(ds_forward_kernel<T, DS_TEAM, true, SECOND>, (unsigned)(a.rows * parts), DS_TEAM, 0, parts, s, a);
-    ds_forward_kernel<T, DS_TEAM, false, SECOND><<<(unsigned)a.rows, DS_TEAM, 0, s>>>(a);
+    if (parts > 1) return launch_clusters(ds_cluster_kernel<T, SECOND>, (unsigned)(a.rows * parts), DS_TEAM, 0, parts, s, a);
+    const long long most = 4LL * sm_count();
+    ds_stream_kernel<T, SECOND><<<(unsigned)(a.rows < most ? a.rows : most), DS_STREAM, 0, s>>>(a);
     return launched();
 }
 
