@@ -9,7 +9,7 @@
 // the sums and t for the backward, which reads the logits again and writes the gradient.
 #include "kernels.h"
 #include "launch.cuh"
-#include "softmax.cuh"
+#include "logit_rows.cuh"
 #include <cooperative_groups.h>
 #include <type_traits>
 
@@ -18,7 +18,8 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int DS_MAX_K = 256, DS_TEAM = 256, DS_UNROLL = 4;
+constexpr int DS_MAX_K = 256, DS_TEAM = LP_TEAM;
+constexpr int DS_UNROLL = 4;            // backward: vectors that a thread has in flight
 
 struct DsFwd {
     const void* x;
@@ -103,7 +104,7 @@ template <class T, int U, int SECOND> __device__ __forceinline__ void ds_take(co
         w = u == 0 ? a : max_word<T>(w, a);
     }
     const float top = word_max<T>(w);
-    if (!(top <= run.m)) run.raise(top, scale);      // a NaN, too
+    if (top > run.m || top != top) run.raise(top, scale);      // a NaN stays
     if (run.m == -INFINITY) return;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -119,63 +120,45 @@ __device__ __forceinline__ float ds_value(const void* p, int type, long long i) 
     return type == ADDER_TYPE_BF16 ? to_float(static_cast<const __nv_bfloat16*>(p)[i]) : to_float(static_cast<const __half*>(p)[i]);
 }
 
-// A row as a team sees it: vectors v0 to v1 - 1 (shared out over a cluster), and up to VE - 1 single elements before and behind all
-// vectors, which are rank 0's.
-template <class T> struct DsRow {
-    static constexpr int VE = Vec16<T>::N;
-    const T* x;
-    const uint4* vec;
-    int head, nvec, singles, v0, v1;
-
-    __device__ __forceinline__ void set(const DsFwd& a, long long row, int rank, int parts) {
-        x = static_cast<const T*>(a.x) + row * a.stride;
-        const int mis = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
-        head = min(a.classes, mis == 0 ? 0 : VE - mis);
-        nvec = (a.classes - head) / VE;
-        singles = rank == 0 ? a.classes - nvec * VE : 0;
-        v0 = parts == 1 ? 0 : (int)((long long)nvec * rank / parts);
-        v1 = parts == 1 ? nvec : (int)((long long)nvec * (rank + 1) / parts);
-        vec = reinterpret_cast<const uint4*>(x + head);
-    }
-    __device__ __forceinline__ int single(int i) const { return i < head ? i : i + nvec * VE; }
-};
-
-// A thread's share of a row, every THREADS-th vector, the next ones on their way while it works on some.
+// The sums of a row's share of a thread, every THREADS-th vector, on their way through shared memory (double-buffered in registers instead, the forward
+// of 2048x128000 bf16 took 104 us).
 template <class T, int THREADS, int SECOND> struct DsReader {
-    uint4 q[2][DS_UNROLL];
+    using Stream = LpStream<T, THREADS>;
+    Stream stream;
+    uint32_t from;
 
-    __device__ __forceinline__ void fetch(const DsRow<T>& r, int v, uint4 (&to)[DS_UNROLL]) {
+    __device__ __forceinline__ void begin(const DsFwd& a, uint4* ring, long long row, long long step, int t, int rank, int parts) {
+        stream.first = stream.at = from = smem_u32(ring) + threadIdx.x * 16;
+        stream.row = row;
+        stream.step = step;
+        stream.set_row(a, t, rank, parts);
 #pragma unroll
-        for (int u = 0; u < DS_UNROLL; ++u)
-            if (v + u * THREADS < r.v1) to[u] = __ldg(r.vec + v + u * THREADS);
+        for (int i = 0; i < LP_STAGES - 1; ++i) stream.issue(a, t, rank, parts);
     }
-    __device__ __forceinline__ void take(const DsRow<T>& r, int v, const uint4 (&from)[DS_UNROLL], DsSums<SECOND>& run, float scale) {
-        if (v + (DS_UNROLL - 1) * THREADS < r.v1) {
-            ds_take<T, DS_UNROLL>(from, run, scale);
-            return;
-        }
-#pragma unroll
-        for (int u = 0; u < DS_UNROLL - 1; ++u)
-            if (v + u * THREADS < r.v1) {
-                const uint4 one[1] = {from[u]};
-                ds_take<T, 1>(one, run, scale);
-            }
-    }
-    __device__ __forceinline__ void begin(const DsRow<T>& r, int t) { fetch(r, r.v0 + t, q[0]); }
-    // The sums of a row that has begun.
-    __device__ __forceinline__ DsPart read(const DsRow<T>& r, int t, float scale) {
+    __device__ __forceinline__ DsPart read(const DsFwd& a, const LpRow<T>& r, int t, int rank, int parts) {
+        const float one = t < r.singles ? to_float(r.x[r.single(t)]) : -INFINITY;
         DsSums<SECOND> run;
-        for (int v = r.v0 + t; v < r.v1; v += 2 * DS_UNROLL * THREADS) {
-            fetch(r, v + DS_UNROLL * THREADS, q[1]);
-            take(r, v, q[0], run, scale);
-            fetch(r, v + 2 * DS_UNROLL * THREADS, q[0]);
-            take(r, v + DS_UNROLL * THREADS, q[1], run, scale);
+        int v = r.v0 + t;
+        for (int g = r.groups(THREADS); g > 0; --g) {
+            stream.issue(a, t, rank, parts);
+            cp_async_wait<LP_STAGES - 1>();
+            if (v + (LP_GROUP - 1) * THREADS < r.v1) {
+                uint4 q[LP_GROUP];
+#pragma unroll
+                for (int u = 0; u < LP_GROUP; ++u) q[u] = read16(from + u * Stream::SLOT);
+                ds_take<T, LP_GROUP>(q, run, a.scale);
+            } else {
+#pragma unroll 1
+                for (int u = 0; u < LP_GROUP - 1 && v + u * THREADS < r.v1; ++u) {
+                    const uint4 q[1] = {read16(from + u * Stream::SLOT)};
+                    ds_take<T, 1>(q, run, a.scale);
+                }
+            }
+            from = from == stream.first + Stream::RING - Stream::STAGE ? stream.first : from + Stream::STAGE;
+            v += LP_GROUP * THREADS;
         }
-        if (t < r.singles) {
-            const float one = to_float(r.x[r.single(t)]);
-            if (!(one <= run.m)) run.raise(one, scale);
-            if (run.m != -INFINITY) run.add(one, -INFINITY, scale);
-        }
+        if (one > run.m || one != one) run.raise(one, a.scale);
+        if (t < r.singles && run.m != -INFINITY) run.add(one, -INFINITY, a.scale);
         float lo, hi, lo1, hi1;
         unpack2(run.s, lo, hi);
         unpack2(run.s1, lo1, hi1);
@@ -252,17 +235,18 @@ template <class T, int SECOND> __device__ __forceinline__ void ds_finish(const D
 
 // A warp a row, four of them a CTA.
 template <class T, int SECOND> __global__ void __launch_bounds__(128) ds_warp_kernel(const DsFwd a) {
+    extern __shared__ uint4 ring[];
     __shared__ DsNamed named_of[4];
     const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
     const long long row = (long long)blockIdx.x * 4 + warp;
     if (row >= a.rows) return;
-    DsRow<T> r;
+    LpRow<T> r;
     r.set(a, row, 0, 1);
     DsReader<T, 32, SECOND> reader;
-    reader.begin(r, lane);
+    reader.begin(a, ring, row, a.rows, lane, 0, 1);
     DsTold<T> told;
     told.look_up(a, row, r.x, lane, named_of[warp]);
-    ds_finish<T, SECOND>(a, row, ds_join_lanes(reader.read(r, lane, a.scale), a.scale), told, named_of[warp], lane);
+    ds_finish<T, SECOND>(a, row, ds_join_lanes(reader.read(a, r, lane, 0, 1), a.scale), told, named_of[warp], lane);
 }
 
 // A CTA's rows one after another: DS_TEAM threads read them, and a warp more finishes each while the others read the next (2048x50257 bf16 with 64 classes
@@ -274,23 +258,18 @@ __device__ __forceinline__ void ds_arrive(int id) { asm volatile("bar.arrive %0,
 
 template <class T, int SECOND> __global__ void __launch_bounds__(DS_STREAM, 4) ds_stream_kernel(const DsFwd a) {
     constexpr int WARPS = DS_TEAM / 32;
+    extern __shared__ uint4 ring[];
     __shared__ DsPart parts_of[2][WARPS];
     __shared__ DsNamed named;
     const int t = threadIdx.x, lane = t & 31;
     long long row = blockIdx.x;
-    DsRow<T> r;
-    r.set(a, row, 0, 1);
+    LpRow<T> r;
     if (t < DS_TEAM) {
         DsReader<T, DS_TEAM, SECOND> reader;
-        reader.begin(r, t);
-        for (int turn = 0; row < a.rows; turn ^= 1) {
-            DsPart mine = reader.read(r, t, a.scale);
-            row += gridDim.x;
-            if (row < a.rows) {
-                r.set(a, row, 0, 1);
-                reader.begin(r, t);
-            }
-            mine = ds_join_lanes(mine, a.scale);
+        reader.begin(a, ring, row, gridDim.x, t, 0, 1);
+        for (int turn = 0; row < a.rows; turn ^= 1, row += gridDim.x) {
+            r.set(a, row, 0, 1);
+            const DsPart mine = ds_join_lanes(reader.read(a, r, t, 0, 1), a.scale);
             ds_sync(DS_EMPTY + turn);      // the row before the last is finished
             if (lane == 0) parts_of[turn][t >> 5] = mine;
             __syncwarp();
@@ -317,18 +296,19 @@ template <class T, int SECOND> __global__ void __launch_bounds__(DS_STREAM, 4) d
 // Few rows: each is shared out over a cluster of CTAs.
 template <class T, int SECOND> __global__ void __launch_bounds__(DS_TEAM) ds_cluster_kernel(const DsFwd a) {
     constexpr int WARPS = DS_TEAM / 32;
+    extern __shared__ uint4 ring[];
     __shared__ DsPart parts_of[WARPS], ranks_of[8];
     __shared__ DsNamed named;
     const int t = threadIdx.x, lane = t & 31, parts = (int)cg::this_cluster().num_blocks(), rank = (int)cg::this_cluster().block_rank();
     const long long row = blockIdx.x / parts;
     asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
-    DsRow<T> r;
+    LpRow<T> r;
     r.set(a, row, rank, parts);
     DsReader<T, DS_TEAM, SECOND> reader;
-    reader.begin(r, t);
+    reader.begin(a, ring, row, a.rows, t, rank, parts);
     DsTold<T> told;
     if (rank == 0 && t < 32) told.look_up(a, row, r.x, lane, named);
-    const DsPart mine = ds_join_lanes(reader.read(r, t, a.scale), a.scale);
+    const DsPart mine = ds_join_lanes(reader.read(a, r, t, rank, parts), a.scale);
     if (lane == 0) parts_of[t >> 5] = mine;
     __syncthreads();
     DsPart all = lane < WARPS ? parts_of[lane] : DsPart{-INFINITY, 0.f, 0.f};
@@ -464,16 +444,17 @@ bool ds_warp_rows(long long rows, long long classes) {
 }
 
 template <class T, int SECOND> int launch_distill_forward(const DsFwd& a, cudaStream_t s) {
-    if (ds_warp_rows(a.rows, a.classes)) {
-        ds_warp_kernel<T, SECOND><<<(unsigned)((a.rows + 3) / 4), 128, 0, s>>>(a);
-        return launched();
-    }
+    const auto launch = [&](auto kernel, long long grid, int threads, size_t ring, int parts) {
+        const int st = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), ring);
+        return st != ADDER_OK ? st : launch_clusters(kernel, (unsigned)grid, threads, ring, parts, s, a);
+    };
+    if (ds_warp_rows(a.rows, a.classes)) return launch(ds_warp_kernel<T, SECOND>, (a.rows + 3) / 4, 128, LpStream<T, 32>::RING, 1);
+    constexpr size_t ring = LpStream<T, DS_TEAM>::RING;
     int parts = 1;      // few rows are split over clusters, as long as there are no more than 4 CTAs an SM
     while (parts < 8 && a.rows * parts * 2 <= sm_count() * 4 && a.classes >= 8192LL * parts) parts *= 2;
-    if (parts > 1) return launch_clusters(ds_cluster_kernel<T, SECOND>, (unsigned)(a.rows * parts), DS_TEAM, 0, parts, s, a);
+    if (parts > 1) return launch(ds_cluster_kernel<T, SECOND>, a.rows * parts, DS_TEAM, ring, parts);
     const long long most = 4LL * sm_count();
-    ds_stream_kernel<T, SECOND><<<(unsigned)(a.rows < most ? a.rows : most), DS_STREAM, 0, s>>>(a);
-    return launched();
+    return launch(ds_stream_kernel<T, SECOND>, a.rows < most ? a.rows : most, DS_STREAM, ring, 1);
 }
 
 // f(std::integral_constant<int, DsSecond>) by the temperature, and by whether the probabilities at temperature 1 are asked for.

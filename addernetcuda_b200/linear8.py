@@ -120,6 +120,15 @@ def _aligned(values: torch.Tensor):
     return out, stride
 
 
+def _padded(values: torch.Tensor) -> torch.Tensor:
+    """The same codes [rows, columns], laid out as `_codes` does."""
+    if values.shape[0] <= 1 or values.stride() == (-(-values.shape[1] // 16) * 16, 1):
+        return values
+    out, _ = _codes(values.shape[:1], values.shape[1], values.device)
+    out.view(torch.uint8).copy_(values.contiguous().view(torch.uint8))
+    return out
+
+
 def linear_8bit(x: Union[torch.Tensor, Rows8], weight: Weight8, bias: Optional[torch.Tensor] = None,
                 dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """x @ weight.T + bias with both factors in 8 bits: [..., weight rows] of `dtype`.
@@ -189,6 +198,16 @@ class Linear8bit(nn.Module):
         self.register_buffer("values", values)
         self.register_buffer("scales", scales)
         self.register_buffer("bias", None if layer.bias is None else layer.bias.detach().float())
+
+    def _apply(self, fn, recurse=True):
+        # a module's .half(), .float() and the like are for parameters: what is held here keeps its types, and follows to a device alone
+        kept = dict(self._buffers)
+        super()._apply(fn, recurse)
+        for name, t in kept.items():
+            if t is not None and self._buffers[name].dtype != t.dtype:
+                self._buffers[name] = t.to(self._buffers[name].device)
+        self._buffers["values"] = _padded(self._buffers["values"])
+        return self
 
     def forward(self, x):
         if self.convolution:

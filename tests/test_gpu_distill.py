@@ -151,6 +151,19 @@ def test_special_rows(classes, dtype):
     assert lp[8].isnan() and torch.isfinite(d[8]) and grad[8].isnan().all()
 
 
+@pytest.mark.parametrize("classes", [40, 3000, 40000])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_nan_stays(classes, dtype):
+    """Beside nothing but -inf, and wherever in the row it stands."""
+    places = [0, 1, 7, classes // 2, classes - 2, classes - 1]
+    x, z, at, targets, g, gl = _inputs(2 * len(places), classes, 4, dtype, seed=6, empty=False)
+    x[::2] = float("-inf")
+    for i, place in enumerate(places):
+        x[2 * i:2 * i + 2, place] = float("nan")
+    r, grad = _call(x, z, at, 2.0, targets, g, gl)
+    assert r.divergence.isnan().all() and r.log_prob[:-1].isnan().all() and grad.isnan().all()
+
+
 def test_far_values():
     """Logits of 1e4 and beyond, and a mask of the type's lowest value."""
     for dtype in (torch.float32, torch.bfloat16):

@@ -244,6 +244,10 @@ def test_layers_of_networks():
     again = torch.nn.Sequential(torch.nn.Linear(100, 300), torch.nn.ReLU(), torch.nn.Linear(300, 17, bias=False)).to(DEV)
     quantize_linear(again).load_state_dict(net.state_dict())
     assert torch.equal(again(x), got)
+    for moved in (net.half(), net.cpu().cuda()):      # types of parameters; another device and back
+        assert moved[0].values.dtype == torch.float8_e4m3fn and moved[0].scales.dtype == torch.float32 and moved[0].values.stride(0) == 112
+        assert torch.equal(moved(x), got)
+    assert net(x.half()).dtype == torch.float16
     conv = torch.nn.Conv2d(40, 24, 1).to(DEV)
     image = torch.randn(3, 40, 5, 7, device=DEV)
     y = Linear8bit(conv)(image)
