@@ -120,6 +120,7 @@ struct L8Args {
     int tokens, outer, blocks;      // blocks of 128 columns
     int m_tiles, n_tiles;
     bool whole_fours;               // scales may be read four at a time
+    bool whole_rows;                // rows of y are whole 16-byte vectors
 };
 // Scales of blocks b to b + 3, as far as there are that many.
 __device__ __forceinline__ void l8_four(const float* p, int b, int blocks, bool whole, float (&f)[4]) {
@@ -221,11 +222,12 @@ __device__ __forceinline__ uint64_t l8_pair(uint32_t lo, uint32_t hi) {
 // and each has the sums of its 128 tokens in 256 columns of its tensor memory, twice: while one block's sums are being made, eight warps read
 // those of the block before, multiply them by its scales and add them up in registers (a row and 128 columns a thread, so that both scales are
 // one number a thread).
-constexpr int L8P_STAGES = 6, L8P_THREADS = 384, L8P_STAGING = 4096;
-constexpr uint32_t L8P_SMEM = L8P_STAGES * 2 * L8_SLAB + 8 * L8P_STAGING + 1024;
+constexpr int L8P_STAGES = 5, L8P_THREADS = 384, L8P_STAGING = 4096;      // staging: bytes of a part of a warp's rows, two of them
+constexpr uint32_t L8P_SMEM = L8P_STAGES * 2 * L8_SLAB + 16 * L8P_STAGING + 1024;
 
 template <class T> __global__ void __launch_bounds__(L8P_THREADS, 1)
-linear8_pair_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap w_map, const L8Args a, int* error_flag) {
+linear8_pair_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap y_map, const L8Args a,
+                    int* error_flag) {
     extern __shared__ uint8_t raw[];
     __shared__ uint64_t full[L8P_STAGES], empty[L8P_STAGES], made[2], taken[2];
     __shared__ uint32_t tmem_base;
@@ -311,7 +313,6 @@ linear8_pair_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_cons
         const int quarter = wid & 3, half = wid >> 2;
         const uint32_t from = tmem + ((uint32_t)quarter << 21) + half * 128;
         const uint32_t taken_at = l8_map_shared(taken, 0);
-        uint8_t* const mine = staging + wid * L8P_STAGING;
         int it = 0;
         for (int tile = blockIdx.x >> 1; tile < tiles && ok; tile += pairs) {
             int m0, n0;
@@ -377,14 +378,18 @@ linear8_pair_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_cons
                 if (lane == 0) gave_up = 1;
                 break;
             }
-            // Through shared memory, 128 bytes of each row at a time, so that a row's part is stored by neighbouring lanes.
+            // Through shared memory, 128 bytes of each row at a time, in the swizzle of the copy that stores them while the next tile's sums begin (by the
+            // warps' own stores a tile took 3500 clocks, a tenth of its time).  Rows of y that are no whole vectors are stored by the warps,
+            // neighbouring lanes a row's elements.
             constexpr int C = 128 / sizeof(T), V = 16 / sizeof(T);      // columns of a part, of a vector
             const int rows = min(32, a.tokens - m0);
-            const bool vectors = (long long)a.outer * sizeof(T) % 16 == 0 && (reinterpret_cast<uintptr_t>(a.y) & 15) == 0;
 #pragma unroll
             for (int p = 0; p < 128 / C; ++p) {
                 const int c0 = n0 + p * C;
                 if (c0 >= a.outer) break;
+                uint8_t* const mine = staging + (2 * wid + (p & 1)) * L8P_STAGING;
+                if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");      // the part before the last has been read
+                __syncwarp();
 #pragma unroll
                 for (int v = 0; v < C / V; ++v) {
                     float f[V];
@@ -396,25 +401,27 @@ linear8_pair_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_cons
                     }
                     *reinterpret_cast<uint4*>(mine + lane * 128 + ((v ^ (lane & 7)) * 16)) = Vec16<T>::pack(f);
                 }
-                __syncwarp();
-                T* out = static_cast<T*>(a.y) + (long long)m0 * a.outer + c0;
-                if (vectors) {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const int row = i * 4 + lane / 8, v = lane & 7;
-                        if (row < rows && c0 + v * V < a.outer)
-                            *reinterpret_cast<uint4*>(out + (long long)row * a.outer + v * V) = *reinterpret_cast<const uint4*>(mine + row * 128 + ((v ^ (row & 7)) * 16));
+                if (a.whole_rows) {
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0 && rows > 0) {
+                        asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];" ::"l"(&y_map), "r"(smem_u32(mine)), "r"(c0), "r"(m0) : "memory");
+                        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
                     }
                 } else {
+                    __syncwarp();
+                    T* out = static_cast<T*>(a.y) + (long long)m0 * a.outer + c0;
                     for (int row = 0; row < rows; ++row)
 #pragma unroll
                         for (int c = lane; c < C; c += 32)
                             if (c0 + c < a.outer)
                                 out[(long long)row * a.outer + c] = *reinterpret_cast<const T*>(mine + row * 128 + (((c / V) ^ (row & 7)) * 16) + c % V * sizeof(T));
+                    __syncwarp();
                 }
-                __syncwarp();
             }
         }
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+        __syncwarp();
     }
     l8_before_sync();
     __syncthreads();
@@ -612,7 +619,7 @@ linear8_small_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_con
 #pragma unroll
     for (int i = 0; i < S::COLUMNS / 2; ++i) unpack2(pairs[i], acc[2 * i], acc[2 * i + 1]);
     const T* bias = static_cast<const T*>(a.bias);
-    const bool vectors = (long long)a.outer * sizeof(T) % 16 == 0 && (reinterpret_cast<uintptr_t>(a.y) & 15) == 0;
+    const bool vectors = a.whole_rows;
     // Where the rows of y are no whole vectors, those of a warp go through shared memory, so that neighbouring lanes store a row's elements
     // (a row a lane, element by element, 333x2000x5003 took 29.4 us).
     constexpr int PITCH = S::COLUMNS + 4 / sizeof(T);
@@ -685,12 +692,15 @@ linear8_small_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_con
 struct L8Call {
     const uint8_t *x, *w;
     long long x_stride, w_stride, inner;
+    int type;
     L8Args a;
 };
 
 template <class T> int launch_linear8_pair(L8Call c, int* flag, cudaStream_t s) {
-    CUtensorMap x_map, w_map;
+    CUtensorMap x_map, w_map, y_map;
     if (!make_byte_rows_map(&x_map, c.x, c.a.tokens, c.inner, c.x_stride, 128) || !make_byte_rows_map(&w_map, c.w, c.a.outer, c.inner, c.w_stride, 128)) return ADDER_ERR_CUDA;
+    y_map = x_map;
+    if (c.a.whole_rows && !make_rows_map(&y_map, c.a.y, c.type, c.a.tokens, c.a.outer, 32)) return ADDER_ERR_CUDA;
     c.a.m_tiles = (c.a.tokens + 255) / 256;
     c.a.n_tiles = (c.a.outer + 255) / 256;
     const auto kernel = linear8_pair_kernel<T>;
@@ -698,7 +708,7 @@ template <class T> int launch_linear8_pair(L8Call c, int* flag, cudaStream_t s) 
     if (st != ADDER_OK) return st;
     const long long tiles = (long long)c.a.m_tiles * c.a.n_tiles;
     if (tiles > 2147483647LL / 8) return ADDER_ERR_UNSUPPORTED;
-    return launch_clusters(kernel, 2 * (unsigned)std::min((long long)sm_count() / 2, tiles), L8P_THREADS, L8P_SMEM, 2, s, x_map, w_map, c.a, flag);
+    return launch_clusters(kernel, 2 * (unsigned)std::min((long long)sm_count() / 2, tiles), L8P_THREADS, L8P_SMEM, 2, s, x_map, w_map, y_map, c.a, flag);
 }
 
 template <class T, int N> int launch_linear8_small(L8Call c, int* flag, cudaStream_t s) {
@@ -793,8 +803,9 @@ int adder_b200_linear_8bit(const unsigned char* x, const float* x_scales, const 
     if (!aligned_to(x, 16) || !aligned_to(w, 16) || x_stride % 16 != 0 || w_stride % 16 != 0 || !aligned_to(x_scales, 4) || !aligned_to(w_scales, 4) ||
         !aligned_to(bias, size) || !aligned_to(y, size))
         return ADDER_ERR_ALIGNMENT;
-    const L8Call c{x, w, x_stride, w_stride, inner, {x_scales, w_scales, bias, y, (int)tokens, (int)outer, (int)((inner + E4M3_BLOCK - 1) / E4M3_BLOCK), 0, 0,
-                    (inner + E4M3_BLOCK - 1) / E4M3_BLOCK % 4 == 0 && aligned_to(x_scales, 16) && aligned_to(w_scales, 16)}};
+    const L8Call c{x, w, x_stride, w_stride, inner, dtype, {x_scales, w_scales, bias, y, (int)tokens, (int)outer, (int)((inner + E4M3_BLOCK - 1) / E4M3_BLOCK), 0, 0,
+                    (inner + E4M3_BLOCK - 1) / E4M3_BLOCK % 4 == 0 && aligned_to(x_scales, 16) && aligned_to(w_scales, 16),
+                    outer * size % 16 == 0 && aligned_to(y, 16)}};
     return with_type(dtype, [&](auto* type) { return launch_linear8<std::remove_pointer_t<decltype(type)>>(c, static_cast<cudaStream_t>(stream)); });
 }
 

@@ -24,6 +24,9 @@ bool make_nchw_tensor_map(CUtensorMap* map, const float* base, int N, int C, int
 // Encodes a 2-d map over `rows` rows of `columns` bytes that begin `stride` bytes apart, for boxes of 128 bytes x box_rows in the 128-byte
 // swizzle that the tensor core reads; what lies outside arrives as zeros.  base and stride are multiples of 16.
 bool make_byte_rows_map(CUtensorMap* map, const void* base, long long rows, long long columns, long long stride, int box_rows);
+// The same for storing rows of elements of type dtype (ADDER_TYPE_*), contiguous, in boxes of 128 bytes x box_rows; a row is a multiple of 16
+// bytes.
+bool make_rows_map(CUtensorMap* map, void* base, int dtype, long long rows, long long columns, int box_rows);
 
 // Address (on the current device) of the int that kernels set when a bounded wait gives up.
 int device_error_flag(int** flag);

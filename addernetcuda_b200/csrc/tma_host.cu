@@ -62,6 +62,20 @@ bool make_byte_rows_map(CUtensorMap* map, const void* base, long long rows, long
                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+bool make_rows_map(CUtensorMap* map, void* base, int dtype, long long rows, long long columns, int box_rows) {
+    EncodeTiledFn enc = encoder();
+    if (enc == nullptr) return false;
+    const int size = dtype == ADDER_TYPE_F32 ? 4 : 2;
+    const cuuint64_t dims[2] = {(cuuint64_t)columns, (cuuint64_t)rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)columns * size};
+    const cuuint32_t box[2] = {(cuuint32_t)(128 / size), (cuuint32_t)box_rows};
+    const cuuint32_t estr[2] = {1, 1};
+    const CUtensorMapDataType type = dtype == ADDER_TYPE_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : dtype == ADDER_TYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                                                                           : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    return enc(map, type, 2, base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 int device_error_flag(int** flag) {
     int dev = -1;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return ADDER_ERR_CUDA;
