@@ -7,6 +7,10 @@
 // The forward reads the logits once: every thread keeps a maximum of its own with the sums relative to it (two where the target's
 // probability at temperature 1 is asked for beside another temperature), which are rescaled when it rises and joined at the end.  It leaves M,
 // the sums and t for the backward, which reads the logits again and writes the gradient.
+//
+// What bounds it: memory (2048x128000 bf16: forward 89 us, 90 % of a copy's rate, with the label's probability at T = 2 or 4 96 us; backward 165 us,
+// 97 %), the exponential unit where two exponentials are taken (T = 3 with labels 149 us), and a row's beginning and end in shorter ones (2048x50257
+// with 64 classes of the teacher's 44 us, 71 %).  256x1000 fp32, a warp a row, waits for its loads: 6.8 us forward, 6.8 backward.
 #include "kernels.h"
 #include "launch.cuh"
 #include "logit_rows.cuh"

@@ -9,9 +9,11 @@
 // whole, so the token does not depend on the order of a sum in practice (in 32 bits it would, for one draw in a hundred of 128000 classes).
 //
 // A sequence's row is split over a cluster of CTAs and their warps, a segment of consecutive classes a warp.  Every CTA finds n for itself,
-// sums its segments and leaves the sums with all CTAs of the cluster; then the warp whose segment holds the border reads that again.
-// Bound by memory: of all rows only those of p_n and q_n are read; for few sequences by latency: four loads that wait for one another (the
-// token, its probabilities, the row, the segment again).
+// sums its segments and leaves the sums with all CTAs of the cluster; then the CTA whose segment holds the border reads that again, a part a warp.
+//
+// What bounds it: of all rows only those of p_n and q_n are read, in lines that nothing has touched before, behind three loads that wait for one
+// another (the tokens, their probabilities, the row), and the segment's second reading waits for the sums.  One sequence of 32000 fp32 classes 6.4 us;
+// 64 of 128000 bf16 16.4 us, where the bytes alone take 5 (with 512 threads a CTA or 256, and with additions in fp32 instead of 64 bits, the same).
 #include "kernels.h"
 #include "elements.cuh"
 #include "launch.cuh"

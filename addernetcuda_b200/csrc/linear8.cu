@@ -2,8 +2,13 @@
 //
 //   y[m][n] = sum over blocks b of 128 columns:  xs[m][b] ws[n / 128][b] sum over k in b of xc[m][k] wc[n][k]   [+ bias[n]]
 //
-// codes are e4m3; their products and the sums of a block are exact or nearly so in fp32, and each block's sum is multiplied by its two scales
+// Codes are e4m3; their products and the sums of a block are exact or nearly so in fp32, and each block's sum is multiplied by its two scales
 // and added up in fp32.  y is rounded once.
+//
+// What bounds it.  Few tokens: the weight's bytes (8x4096x32000 24.7 us, 81 % of a copy's rate; 1x4096x4096 7.7 us, of which the weight takes 2.6: a
+// launch, the first copies and the join of a cluster).  Many tokens: products and sums in turn (8192x4096x16384 505 us, 2.17 PFLOP/s, 66 % of twice
+// the measured bf16 rate; alone, without the sums, 421): a block of 256 x 256 takes a pair 512 clocks of products, and its sums 650 of eight warps, of
+// which 400 are their additions.  Between them a wave or two of tiles: 512x4096x4096 15.7 us, 1024x4096x4096 21.6, 4096x4096x4096 69.5.
 #include <algorithm>
 #include "kernels.h"
 #include "e4m3.cuh"
@@ -411,11 +416,21 @@ linear8_pair_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_cons
                 } else {
                     __syncwarp();
                     T* out = static_cast<T*>(a.y) + (long long)m0 * a.outer + c0;
-                    for (int row = 0; row < rows; ++row)
+                    for (int r0 = 0; r0 < rows; r0 += 8) {
+                        T held[8][C / 32];
 #pragma unroll
-                        for (int c = lane; c < C; c += 32)
-                            if (c0 + c < a.outer)
-                                out[(long long)row * a.outer + c] = *reinterpret_cast<const T*>(mine + row * 128 + (((c / V) ^ (row & 7)) * 16) + c % V * sizeof(T));
+                        for (int i = 0; i < 8; ++i)
+#pragma unroll
+                            for (int k = 0; k < C / 32; ++k) {
+                                const int row = r0 + i, c = lane + 32 * k;
+                                held[i][k] = *reinterpret_cast<const T*>(mine + row * 128 + (((c / V) ^ (row & 7)) * 16) + c % V * sizeof(T));
+                            }
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+#pragma unroll
+                            for (int k = 0; k < C / 32; ++k)
+                                if (r0 + i < rows && c0 + lane + 32 * k < a.outer) out[(long long)(r0 + i) * a.outer + lane + 32 * k] = held[i][k];
+                    }
                     __syncwarp();
                 }
             }
@@ -734,7 +749,9 @@ template <class T> int launch_linear8(const L8Call& c, cudaStream_t s) {
     const int tokens = c.a.tokens;
     if (tokens <= 16) return launch_linear8_small<T, 16>(c, flag, s);
     if (tokens <= 32) return launch_linear8_small<T, 32>(c, flag, s);
-    // Turns of all SMs: a pair's takes some 1.6 times as long as a CTA's of 128 x 128.
+    // Turns of all SMs: a pair's takes some 1.6 times as long as that of CTAs of 128 x 128.  us by those and by pairs: 512x4096x4096 15.7 and 20.3,
+    // 200x4096x4096 13.0 and 19.9, 300x4096x11008 31.5 and 37.1; on the other side 700x4096x4096 28.8 and 20.7, 160x4096x32000 58 and 38,
+    // 2048x512x2048 11.3 and 8.3.
     const long long pair_tiles = (long long)((tokens + 255) / 256) * ((c.a.outer + 255) / 256), small_tiles = (long long)((tokens + 127) / 128) * ((c.a.outer + 127) / 128);
     const long long pair_turns = (pair_tiles + sm_count() / 2 - 1) / (sm_count() / 2), small_turns = (small_tiles + sm_count() - 1) / sm_count();
     if (tokens <= 128 || 5 * small_turns <= 8 * pair_turns) return launch_linear8_small<T, 128>(c, flag, s);
