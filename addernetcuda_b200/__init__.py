@@ -5,8 +5,9 @@
     import resnet20              # the reference's model file, unchanged
 
 Sub-modules: `adder` (adder2d, adder2d_function, adder), `adder_cuda` (the extension's entry
-points plus the fused forward/backward), `resnet` (ResNet-20/50 builders), `batchnorm` and `layernorm` (norms with the residual
-add in their pass), `logprobs` (log probabilities, entropy, top classes, cross entropy), `optim` (AdamW, states in 32 or 8 bits),
+points plus the fused forward/backward), `resnet` (ResNet-20/50 builders), `batchnorm`, `layernorm` and `rmsnorm` (norms with the
+residual add in their pass), `logprobs` (log probabilities, entropy, top classes, cross entropy), `linear8` (products in 8 bits),
+`distill` (distillation from a teacher's best classes), `drafts` (verification of drafted tokens), `optim` (AdamW, states in 32 or 8 bits),
 `train` (the training step), `ddp` (bucketed gradient all-reduce for batch-sharded training), `build` (nvcc build of the C-ABI
 library).
 """
