@@ -282,7 +282,7 @@ template <class T, int SECOND> __global__ void __launch_bounds__(DS_STREAM, 4) d
         return;
     }
     ds_arrive(DS_EMPTY);
-    ds_arrive(DS_EMPTY + 1);
+    if (row + gridDim.x < a.rows) ds_arrive(DS_EMPTY + 1);      // where there is one row, nobody waits for this
     for (int turn = 0; row < a.rows; turn ^= 1, row += gridDim.x) {
         r.set(a, row, 0, 1);
         DsTold<T> told;

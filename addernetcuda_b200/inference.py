@@ -87,20 +87,25 @@ def fold_batchnorm(model: nn.Module) -> nn.Module:
 def quantize_linear(model: nn.Module) -> nn.Module:
     """Replace, in place, every multiply-based linear layer of `model` (on CUDA) - nn.Linear, and 1x1 nn.Conv2d of stride 1 and one group without
     padding, as the `fc` of `addernetcuda_b200.resnet` - by a `linear8.Linear8bit` with its weight in 8 bits, and put the model in evaluation
-    mode.  Adder layers stay as they are: their |x - w| is no product.  Subclasses of the two stay, too."""
+    mode.  Adder layers stay as they are: their |x - w| is no product.  Subclasses of the two stay, too.  A layer that stands in several places
+    is replaced by one; a model that is itself such a layer by what is returned."""
     model.eval()
+    made = {}
 
-    def convert(module: nn.Module):
-        for name, child in list(module.named_children()):
-            pointwise = type(child) is nn.Conv2d and child.kernel_size == (1, 1) and child.stride == (1, 1) and child.groups == 1 and \
-                child.padding in ((0, 0), "valid")
-            if type(child) is nn.Linear or pointwise:
-                setattr(module, name, Linear8bit(child))
-            else:
-                convert(child)
+    def replacement(child: nn.Module):
+        pointwise = type(child) is nn.Conv2d and child.kernel_size == (1, 1) and child.stride == (1, 1) and child.groups == 1 and \
+            child.padding in ((0, 0), "valid")
+        if type(child) is not nn.Linear and not pointwise:
+            return None
+        if child not in made:
+            made[child] = Linear8bit(child).eval()
+        return made[child]
 
-    convert(model)
-    return model
+    for module in list(model.modules()):
+        for name, child in list(module._modules.items()):
+            if child is not None and replacement(child) is not None:
+                setattr(module, name, replacement(child))
+    return replacement(model) or model
 
 
 def accuracy(output: torch.Tensor, target: torch.Tensor, topk: Sequence[int] = (1,)):

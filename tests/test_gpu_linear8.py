@@ -81,7 +81,8 @@ def _near(y, x, w, bias):
 
 SIZES = [(1, 128, 128), (1, 1, 1), (1, 4096, 1000), (2, 100, 3), (7, 300, 129), (8, 512, 4096), (16, 128, 250), (17, 129, 127), (31, 1000, 640), (33, 256, 2000),
          (64, 2048, 513), (65, 384, 1024), (100, 130, 1001), (127, 640, 255), (128, 1024, 2048), (129, 96, 384), (200, 2000, 5003), (256, 512, 1536),
-         (300, 4096, 500), (513, 250, 777), (1000, 1280, 3000), (1024, 512, 4096), (2050, 384, 1100)]
+         (300, 4096, 500), (513, 250, 777), (1000, 1280, 3000), (1024, 512, 4096), (2050, 384, 1100), (2048, 64, 5000), (2000, 300, 2999), (60, 200, 1),
+         (3, 100000, 70), (150, 1, 9000)]
 
 
 @pytest.mark.parametrize("m,k,n", SIZES)
@@ -248,6 +249,10 @@ def test_layers_of_networks():
         assert moved[0].values.dtype == torch.float8_e4m3fn and moved[0].scales.dtype == torch.float32 and moved[0].values.stride(0) == 112
         assert torch.equal(moved(x), got)
     assert net(x.half()).dtype == torch.float16
+    tied = torch.nn.Linear(60, 60).to(DEV)
+    both = quantize_linear(torch.nn.Sequential(tied, torch.nn.ReLU(), torch.nn.Sequential(tied)))
+    assert isinstance(both[0], Linear8bit) and both[2][0] is both[0]
+    assert isinstance(quantize_linear(tied), Linear8bit)
     conv = torch.nn.Conv2d(40, 24, 1).to(DEV)
     image = torch.randn(3, 40, 5, 7, device=DEV)
     y = Linear8bit(conv)(image)
