@@ -358,7 +358,7 @@ linear8_pair_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_cons
         const int quarter = wid & 3, half = wid >> 2;
         const uint32_t from = tmem + ((uint32_t)quarter << 21) + half * 128;
         const uint32_t taken_at = l8_map_shared(taken, 0);
-        int it = 0;
+        int it = 0, turn = 0;
         for (int tile = blockIdx.x >> 1; tile < tiles && ok; tile += pairs) {
             int m0, n0;
             place(tile, m0, n0);
@@ -431,9 +431,11 @@ linear8_pair_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_cons
 #pragma unroll
             for (int p = 0; p < 128 / C; ++p) {
                 const int c0 = n0 + p * C;
-                if (c0 >= a.outer) break;
-                uint8_t* const mine = staging + (2 * wid + (p & 1)) * L8P_STAGING;
-                if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");      // the part before the last has been read
+                if (c0 >= a.outer || rows <= 0) break;
+                // parts take turns from tile to tile, whatever each had of them: what was committed before the last one has been read
+                uint8_t* const mine = staging + (2 * wid + turn) * L8P_STAGING;
+                turn ^= 1;
+                if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
                 __syncwarp();
 #pragma unroll
                 for (int v = 0; v < C / V; ++v) {
@@ -449,7 +451,7 @@ linear8_pair_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_cons
                 if (a.whole_rows) {
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     __syncwarp();
-                    if (lane == 0 && rows > 0) {
+                    if (lane == 0) {
                         asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];" ::"l"(&y_map), "r"(smem_u32(mine)), "r"(c0), "r"(m0) : "memory");
                         asm volatile("cp.async.bulk.commit_group;" ::: "memory");
                     }

@@ -98,6 +98,17 @@ def test_product(m, k, n, dtype, bias):
     assert torch.equal(y, linear_8bit(x, w, b, dtype=dtype))      # always the same bits
 
 
+@pytest.mark.parametrize("m,k,n", [(2970, 126, 11684), (1500, 64, 20484), (5000, 250, 8012), (3000, 100, 9996)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_many_short_tiles(m, k, n, dtype):
+    """Several tiles a CTA, done faster than they are stored, the last ones of a row narrower than the others: nothing is stored from a buffer that the
+    next tile writes."""
+    from addernetcuda_b200.linear8 import linear_8bit
+    x, w, _ = _case(m, k, n, dtype, seed=m)
+    for _ in range(3):
+        _near(linear_8bit(x, w, dtype=dtype), x, w, None)
+
+
 def test_each_block_has_its_own_scale():
     """One code of 1 in each row: y is a product of two scales and a code, exactly."""
     from addernetcuda_b200.linear8 import Rows8, Weight8, linear_8bit
