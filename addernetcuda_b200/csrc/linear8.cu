@@ -13,6 +13,7 @@
 #include "kernels.h"
 #include "e4m3.cuh"
 #include "launch.cuh"
+#include "ring.h"
 #include "tma.cuh"
 
 namespace adder {
@@ -226,6 +227,11 @@ template <int CTAS> __device__ __forceinline__ void l8_load(uint32_t to, const C
 }
 // mbar_wait by a whole warp, which goes on or gives up as one.
 __device__ __forceinline__ bool l8_wait(uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)); }
+// Until the products have let go of every stage that a copy thread has used: their word goes to the shared memory of both CTAs of a pair, whenever
+// it is ready, so a CTA that left without it would leave a barrier on which an arrival is under way.
+template <int STAGES> __device__ __forceinline__ bool l8_released(uint64_t (&empty)[STAGES], int stage, int turn) {
+    return ring_drain<STAGES>(stage, turn, [&](int i, uint32_t parity) { return mbar_wait(&empty[i], parity); });
+}
 __device__ __forceinline__ void l8_prefetch_map(const CUtensorMap* map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }
 __device__ __forceinline__ void l8_cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
@@ -329,6 +335,7 @@ linear8_pair_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_cons
                         if (t >= 0) mbar_wait(&full[i], t & 1);
                     }
                 }
+                if (!l8_released(empty, stage, turn)) gave_up = 1;
             }
             __syncwarp();
         } else if (wid == 9) {      // ---- products
@@ -482,7 +489,7 @@ linear8_pair_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_cons
     }
     l8_before_sync();
     __syncthreads();
-    l8_cluster_sync();      // no CTA leaves while the other's products read its shared memory
+    l8_cluster_sync();      // no CTA leaves while the other's products read its shared memory, or before their word has come to its own
     if (threadIdx.x == 0 && gave_up) *error_flag = 1;
     if (wid == 9) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
 }
@@ -604,6 +611,7 @@ linear8_small_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_con
                     if (t >= 0) mbar_wait(&full[i], t & 1);
                 }
             }
+            if (!l8_released(empty, stage, turn)) gave_up = 1;
         }
         __syncwarp();
     } else if (wid == S::SUMS / 32 + 1) {      // ---- products

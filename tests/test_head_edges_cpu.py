@@ -1,0 +1,58 @@
+"""What the operators around a head do at their edges, as far as it needs no GPU."""
+import shutil
+import subprocess
+from pathlib import Path
+
+import pytest
+
+CSRC = Path(__file__).resolve().parent.parent / "addernetcuda_b200" / "csrc"
+
+RING = r"""
+#include "ring.h"
+#include <cstdio>
+#include <cstdlib>
+
+// Barriers of one arrival a phase, whose arrivals come some time after they were asked for, in order; a waiter may let `patience` of them come.
+template <int STAGES> int run(int uses, int delivered, int patience, bool& drained, bool& early) {
+    int over[STAGES] = {}, begun[STAGES] = {}, came = 0, stage = 0, turn = 0;
+    const auto come = [&] { if (came < uses) { ++over[came % STAGES]; ++came; return true; } return false; };
+    for (int use = 0; use < uses; ++use) {      // the producer: a stage's use begins when the one before is over
+        while (over[stage] < begun[stage]) come();
+        ++begun[stage];
+        if (++stage == STAGES) { stage = 0; ++turn; }
+    }
+    while (came < delivered) come();
+    drained = adder::ring_drain<STAGES>(stage, turn, [&](int i, unsigned parity) {
+        while ((unsigned)(over[i] & 1) == parity)      // the phase of that parity is not over
+            if (patience-- <= 0 || !come()) return false;
+        return true;
+    });
+    early = drained && came < uses;
+    return came;
+}
+template <int STAGES> void all() {
+    for (int uses = 0; uses <= 4 * STAGES + 1; ++uses)
+        for (int delivered = 0; delivered <= uses; ++delivered) {
+            bool drained, early;
+            const int came = run<STAGES>(uses, delivered, 1 << 20, drained, early);
+            if (!drained || early || came != uses) { std::printf("%d stages, %d uses, %d over: left with %d\n", STAGES, uses, delivered, came); std::exit(1); }
+            run<STAGES>(uses, uses, 0, drained, early);
+            if (!drained) { std::printf("%d stages, %d uses: waits for what never comes\n", STAGES, uses); std::exit(1); }
+            for (int patience = 0; patience < STAGES; ++patience) {
+                run<STAGES>(uses, delivered, patience, drained, early);
+                if (early) { std::printf("%d stages, %d uses, %d over: left early\n", STAGES, uses, delivered); std::exit(1); }
+            }
+        }
+}
+int main() { all<1>(); all<2>(); all<5>(); all<6>(); }
+"""
+
+
+@pytest.mark.skipif(shutil.which("g++") is None, reason="needs a C++ compiler")
+def test_a_ring_is_left_when_its_last_uses_are_over(tmp_path):
+    """The word that a stage is free goes to shared memory, whenever it is ready: a thread that has walked through the ring waits for the last word of
+    every stage, for no earlier one (whose parity may be the same) and for none that never comes."""
+    (tmp_path / "ring.cpp").write_text(RING)
+    subprocess.run(["g++", "-std=c++17", "-Wall", "-Werror", f"-I{CSRC}", str(tmp_path / "ring.cpp"), "-o", str(tmp_path / "ring")], check=True)
+    done = subprocess.run([str(tmp_path / "ring")], capture_output=True, text=True, timeout=60)
+    assert done.returncode == 0, done.stdout
