@@ -139,12 +139,12 @@ def rms_norm_8bit(x: torch.Tensor, weight: Optional[torch.Tensor] = None, eps: f
 
 class FusedRMSNorm(nn.RMSNorm):
     """nn.RMSNorm with `forward(x, residual=None, eight=False)`: with a residual it returns (norm of x + residual, x + residual), with
-    `eight` the norm in 8 bits (over one axis).  Same parameters and state-dict keys; an eps of None is that of x's type, as there.  CPU
-    tensors go through torch, and have no 8 bits."""
+    `eight` the norm in 8 bits (over one axis).  Same parameters and state-dict keys; an eps of None is float32's, in which 16-bit types are
+    computed, too, as there.  CPU tensors go through torch, and have no 8 bits."""
 
     def forward(self, x, residual=None, eight: bool = False):
         if x.is_cuda or eight:
-            eps = torch.finfo(x.dtype).eps if self.eps is None else self.eps
+            eps = torch.finfo(torch.float32).eps if self.eps is None else self.eps
             if not eight:
                 return rms_norm(x, self.normalized_shape, self.weight, eps, residual=residual)
             if len(self.normalized_shape) != 1 or x.shape[-1:] != self.normalized_shape:
