@@ -385,7 +385,8 @@ template <class T, int THREADS, int SECOND> __global__ void __launch_bounds__(TH
     const float gd = a.g_divergence != nullptr ? a.g_divergence[row] * a.inv_t : 0.f;
     const long long target = a.targets != nullptr && a.g_log_prob != nullptr ? a.targets[row] : a.ignore;
     const float gl = target == a.ignore ? 0.f : target < 0 || target >= a.classes ? NAN : a.g_log_prob[row];
-    // A row without classes of the teacher's has no part of the divergence; one with a NaN among them is NaN.
+    // A row without classes of the teacher's has no part of the divergence, nor has one whose divergence has no gradient (a row that is ignored), whatever
+    // the teacher says of it; one with a NaN among its shares is NaN.
     const float* mass = a.mass + row * a.k;
     const long long* at = a.indices + row * a.k;
     float some = 0.f;
@@ -395,7 +396,7 @@ template <class T, int THREADS, int SECOND> __global__ void __launch_bounds__(TH
     DsSlope<SECOND> slope;
     slope.m = m;
     slope.scale = a.scale;
-    const float soft = some == 0.f ? 0.f : some != some ? NAN : gd;
+    const float soft = some == 0.f || gd == 0.f ? 0.f : some != some ? NAN : gd;
     slope.soft = soft / s;
     slope.hard = -gl / s1;
     if (SECOND == ONE) slope.soft += slope.hard;
@@ -437,7 +438,7 @@ template <class T, int THREADS, int SECOND> __global__ void __launch_bounds__(TH
         if (i < begin || i >= end) continue;
         float g = i == target ? gl : 0.f;
         for (int l = 0; l < a.k; ++l)
-            if (at[l] == i) g -= soft * mass[l];
+            if (at[l] == i && soft != 0.f) g -= soft * mass[l];
         dx[i] = from_float<T>(slope.one(to_float(x[i])) + g);
     }
 }

@@ -331,7 +331,7 @@ ADDER_API int adder_b200_distillation_forward(const void* logits, int dtype, lon
                                               const long long* targets, long long ignore_index, float* divergence, float* log_prob,
                                               float* stats, float* mass, void* stream);
 /* grad_logits (contiguous, of the logits' type) <- the gradient of sum(grad_divergence * divergence + grad_log_prob * log_prob); gradients
- * that are NULL count as zeros.  Rows of nothing but -inf get zeros. */
+ * that are NULL count as zeros.  Rows of nothing but -inf get zeros; rows whose grad_divergence is 0 have nothing of the teacher's, NaN included. */
 ADDER_API int adder_b200_distillation_backward(const void* logits, int dtype, long long rows, long long classes, long long row_stride,
                                                const long long* indices, int k, float temperature, const long long* targets,
                                                long long ignore_index, const float* stats, const float* mass, const float* grad_divergence,

@@ -31,3 +31,34 @@ def test_the_norm_module_has_torchs_eps(dtype):
             assert bool(((got.double() - torchs).abs() <= 2 * allowed + 2 * U[dtype] * want.abs()).all())
         want = x.double() / (x.double().square().mean(-1, keepdim=True) + 2.0 ** -23).sqrt()
         assert (eight - want).norm() <= 2.0 ** -4 * want.norm()      # half a step of e4m3 each
+
+
+def _distill_inputs(rows, classes, k, dtype, seed):
+    torch.manual_seed(seed)
+    x = (2.5 * torch.randn(rows, classes, device=DEV)).to(dtype)
+    best, at = (x.float() + torch.randn(rows, classes, device=DEV)).topk(k, 1)
+    targets = torch.randint(0, classes, (rows,), device=DEV)
+    return x, (1.3 * best).to(dtype), at, targets
+
+
+@pytest.mark.parametrize("classes", [40, 3000, 40000])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_what_the_teacher_says_of_rows_that_do_not_count(classes, dtype):
+    """A row that is ignored, and one whose divergence is not asked for, has nothing of the teacher's in its gradient, whatever that is."""
+    from addernetcuda_b200.distill import DistillationLoss, distillation
+    x, z, at, targets = _distill_inputs(9, classes, 4, dtype, 1)
+    targets[:4] = -100
+    bad_z, bad_at = z.clone(), at.clone()
+    bad_at[0] = -100
+    bad_at[1, 2] = classes
+    bad_z[2, 1] = float("nan")
+    bad_z[3] = float("inf")
+    for loss_of in (DistillationLoss(2.0, 0.6), DistillationLoss(1.0, 0.5), DistillationLoss(3.0, 1.0)):
+        leaf = x.clone().requires_grad_()
+        clean, broken = (loss_of(leaf, targets, *t) for t in ((z, at), (bad_z, bad_at)))
+        assert torch.equal(clean, broken) and torch.isfinite(clean)
+        want, got = (torch.autograd.grad(t, leaf)[0] for t in (clean, broken))
+        assert torch.equal(got, want) and (got[:4] == 0).all() and got[4:].abs().sum() > 0
+    leaf = x.clone().requires_grad_()
+    want, got = (torch.autograd.grad(distillation(leaf, *t, 2.0, targets.clamp(min=0)).log_prob.sum(), leaf)[0] for t in ((z, at), (bad_z, bad_at)))
+    assert torch.equal(got, want) and torch.isfinite(got).all()
