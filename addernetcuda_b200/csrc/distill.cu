@@ -189,6 +189,7 @@ template <class T> struct DsTold {
             const bool in = i >= 0 && i < a.classes;
             named.at[j] = in ? (int)i : -1;
             named.z[j] = ds_value(a.teacher, a.teacher_type, row * a.k + j);
+            broken |= named.z[j] != named.z[j];      // at an empty place, too: log probabilities name no class in a row that has failed
             if (in) named.x[j] = to_float(x[i]);
         }
         x_target = target >= 0 && target < a.classes ? to_float(x[target]) : 0.f;

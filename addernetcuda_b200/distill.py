@@ -88,8 +88,9 @@ def distillation(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_ind
     Both are float32 and differentiable once with respect to the logits (a gradient of create_graph=True raises where it is
     differentiated); the teacher gets no gradient, and raises where it asks for one.  `teacher_logits` [..., k] are of any of the three types and
     need no common offset, so log probabilities will do.  An index of -1 is an empty place; a row without any has divergence 0.  A class
-    named twice has both shares.  A row with an index that is no class, or with a NaN or +inf, gives NaN; the divergence is +inf
-    where the teacher names a class whose logit is -inf."""
+    named twice has both shares.  A row with an index that is no class, or with a NaN or +inf, gives NaN, and so does a NaN of the teacher's
+    at an empty place: `token_log_probs` names no class in a row that has failed.  The divergence is +inf where the teacher names a class
+    whose logit is -inf.  A row whose divergence has a gradient of 0 takes nothing of the teacher's."""
     out = _native.distillation(logits, teacher_logits, teacher_indices, temperature, targets, ignore_index)
     if out is not None:
         return Distillation(*out)

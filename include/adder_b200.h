@@ -323,7 +323,8 @@ ADDER_API int adder_b200_linear_8bit(const unsigned char* x, const float* x_scal
 /* Distillation from a teacher's k <= 256 best classes of each row.  With t = softmax(teacher / temperature) over the classes indices[row][k]
  * (-1: none, which may stand anywhere; a class may stand twice) and p = softmax(logits / temperature) over all of the row:
  *   divergence[row]  sum of t (ln t - ln p): 0 where the teacher names no class or all its logits are -inf, +inf where p is 0 and t is not, NaN
- *                    where an index is no class or below -1, or a logit of the teacher's is NaN or +inf
+ *                    where an index is no class or below -1, a logit of the teacher's is NaN (at an empty place, too, as the best classes of a
+ *                    row that has failed are handed on), or one of a class is +inf
  *   log_prob[row]    log softmax(logits) at targets[row]: 0 where the target is ignore_index, NaN where it is no class; with targets alone
  * logits as those of adder_b200_log_probs_forward.  stats[row][3] and mass[row][k] (t) are kept for the backward call; both or neither. */
 ADDER_API int adder_b200_distillation_forward(const void* logits, int dtype, long long rows, long long classes, long long row_stride,

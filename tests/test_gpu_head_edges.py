@@ -62,3 +62,35 @@ def test_what_the_teacher_says_of_rows_that_do_not_count(classes, dtype):
     leaf = x.clone().requires_grad_()
     want, got = (torch.autograd.grad(distillation(leaf, *t, 2.0, targets.clamp(min=0)).log_prob.sum(), leaf)[0] for t in ((z, at), (bad_z, bad_at)))
     assert torch.equal(got, want) and torch.isfinite(got).all()
+
+
+@pytest.mark.parametrize("classes", [40, 3000, 40000])
+def test_a_teacher_that_fails_is_seen(classes):
+    """token_log_probs names no classes in a row with a NaN or an infinity: such a row's divergence is NaN, not that of a row without classes."""
+    from addernetcuda_b200.distill import distillation
+    from addernetcuda_b200.logprobs import token_log_probs
+    x, _, _, targets = _distill_inputs(6, classes, 4, torch.float32, 2)
+    teacher = x + torch.randn_like(x)
+    teacher[1, 3] = float("nan")
+    teacher[4, classes - 1] = float("inf")
+    best = token_log_probs(teacher, top_k=4)
+    leaf = x.clone().requires_grad_()
+    r = distillation(leaf, best.top_log_probs, best.top_indices, 2.0, targets)
+    assert r.divergence.isnan().tolist() == [False, True, False, False, True, False] and torch.isfinite(r.log_prob).all()
+    grad, = torch.autograd.grad(r.divergence.sum(), leaf)
+    assert grad[[1, 4]].isnan().all() and torch.isfinite(grad[[0, 2, 3, 5]]).all()
+
+
+@pytest.mark.parametrize("use_graph", [False, True])
+def test_a_step_with_a_teacher_that_fails(use_graph):
+    from addernetcuda_b200.train import TrainStep
+
+    class Teacher(torch.nn.Module):
+        def forward(self, images):
+            logits = images.flatten(1)[:, :30] * 3
+            return torch.where(torch.arange(16, device=DEV)[:, None] == 3, float("nan"), logits)
+
+    torch.manual_seed(3)
+    student = torch.nn.Sequential(torch.nn.Flatten(), torch.nn.Linear(48, 30)).to(DEV)
+    step = TrainStep(student, (16, 3, 4, 4), 30, teacher=Teacher(), use_graph=use_graph)
+    assert step.step(torch.randn(16, 3, 4, 4, device=DEV), torch.randint(0, 30, (16,), device=DEV)).isnan()
