@@ -117,8 +117,8 @@ def distillation(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_ind
 
 class DistillationLoss(nn.Module):
     """alpha * temperature^2 * divergence + (1 - alpha) * cross entropy, the mean over the targets that are not `ignore_index`:
-    forward(logits, targets, teacher_logits, teacher_indices).  `top_k` (at most 32) is how many classes `train.TrainStep` asks of its
-    teacher.  Computed and returned in float32."""
+    forward(logits, targets, teacher_logits, teacher_indices).  A term of weight 0 is left out.  `top_k` (at most 32) is how many classes
+    `train.TrainStep` asks of its teacher.  Computed and returned in float32."""
 
     def __init__(self, temperature: float = 1.0, alpha: float = 0.5, ignore_index: int = -100, top_k: int = 20):
         super().__init__()
@@ -130,8 +130,14 @@ class DistillationLoss(nn.Module):
         self.top_k = top_k
 
     def forward(self, logits, targets, teacher_logits, teacher_indices):
-        r = distillation(logits, teacher_logits, teacher_indices, self.temperature, targets, self.ignore_index)
+        labels = self.alpha < 1.0      # a term of weight 0 is left out: it may be infinite
+        r = distillation(logits, teacher_logits, teacher_indices, self.temperature, targets if labels else None, self.ignore_index)
+        if not labels:
+            _check_whole(targets, "targets", logits.shape[:-1], logits.device)
         counts = targets != self.ignore_index
-        divergence = torch.where(counts, r.divergence, 0.0)
-        loss = self.alpha * self.temperature ** 2 * divergence - (1.0 - self.alpha) * r.log_prob
+        loss = 0.0
+        if self.alpha > 0.0:
+            loss = self.alpha * self.temperature ** 2 * torch.where(counts, r.divergence, 0.0)
+        if labels:
+            loss = loss - (1.0 - self.alpha) * r.log_prob
         return loss.sum() / counts.sum()

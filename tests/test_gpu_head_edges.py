@@ -94,3 +94,38 @@ def test_a_step_with_a_teacher_that_fails(use_graph):
     student = torch.nn.Sequential(torch.nn.Flatten(), torch.nn.Linear(48, 30)).to(DEV)
     step = TrainStep(student, (16, 3, 4, 4), 30, teacher=Teacher(), use_graph=use_graph)
     assert step.step(torch.randn(16, 3, 4, 4, device=DEV), torch.randint(0, 30, (16,), device=DEV)).isnan()
+
+
+def test_a_term_of_weight_0_is_left_out():
+    """alpha = 0: an infinite divergence; alpha = 1: a label that the network rules out."""
+    from addernetcuda_b200.distill import DistillationLoss
+    x, z, at, targets = _distill_inputs(12, 64, 3, torch.float32, 4)
+    ruled_out = x.clone()
+    ruled_out[0, at[0, 0]] = float("-inf")
+    targets[0] = at[0, 1]
+    targets[-1] = -100
+    counts = targets != -100
+    leaf = ruled_out.requires_grad_()
+    loss = DistillationLoss(2.0, 0.0)(leaf, targets, z, at)
+    want = torch.nn.functional.cross_entropy(leaf.double(), targets)
+    assert abs(loss.double() - want) <= 1e-5 * want
+    got, ref = torch.autograd.grad(loss, leaf)[0], torch.autograd.grad(want, leaf)[0]
+    assert (got.double() - ref).norm() <= 1e-5 * ref.norm()
+
+    out = [c for c in range(64) if c not in at[1].tolist()][0]
+    ruled_out = x.clone()
+    ruled_out[1, out] = float("-inf")
+    targets[1] = out
+    leaf = ruled_out.requires_grad_()
+    loss = DistillationLoss(2.0, 1.0)(leaf, targets, z, at)
+    xd = leaf.double()
+    log_t = torch.log_softmax(z.double() / 2, 1)
+    each = (log_t.exp() * (log_t - torch.log_softmax(xd / 2, 1).gather(1, at))).sum(1)
+    want = 4 * (each * counts).sum() / counts.sum()
+    assert abs(loss.double() - want) <= 1e-5 * want
+    got, ref = torch.autograd.grad(loss, leaf)[0], torch.autograd.grad(want, leaf)[0]
+    assert (got.double() - ref).norm() <= 1e-5 * ref.norm()
+    for bad, kind in ((targets[:3], ValueError), (targets.float(), TypeError), (targets.cpu(), RuntimeError)):
+        for alpha in (0.0, 0.5, 1.0):
+            with pytest.raises(kind):
+                DistillationLoss(2.0, alpha)(x, bad, z, at)
