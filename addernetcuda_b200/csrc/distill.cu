@@ -473,6 +473,7 @@ template <class F> int with_second(float temperature, bool asked, F&& f) {
 
 int ds_check(long long rows, long long classes, long long row_stride, int dtype, int k, float temperature) {
     if (rows < 0 || classes <= 0 || k < 1 || (rows > 1 && row_stride < 0) || !(temperature > 0.f) || temperature == INFINITY) return ADDER_ERR_BAD_SHAPE;
+    if ((float)(1.4426950408889634 / temperature) == INFINITY) return ADDER_ERR_BAD_SHAPE;      // 0 times it, of the largest logit, would be NaN
     if (classes > 2147483647LL - 1024 || rows > 2147483647LL / 8 || k > DS_MAX_K || dtype < ADDER_TYPE_F32 || dtype > ADDER_TYPE_F16) return ADDER_ERR_UNSUPPORTED;
     return ADDER_OK;
 }

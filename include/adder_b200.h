@@ -326,6 +326,7 @@ ADDER_API int adder_b200_linear_8bit(const unsigned char* x, const float* x_scal
  *                    where an index is no class or below -1, a logit of the teacher's is NaN (at an empty place, too, as the best classes of a
  *                    row that has failed are handed on), or one of a class is +inf
  *   log_prob[row]    log softmax(logits) at targets[row]: 0 where the target is ignore_index, NaN where it is no class; with targets alone
+ * temperature is positive and finite, and so is 1.4427 / temperature in fp32 (it is above 4.3e-39).
  * logits as those of adder_b200_log_probs_forward.  stats[row][3] and mass[row][k] (t) are kept for the backward call; both or neither. */
 ADDER_API int adder_b200_distillation_forward(const void* logits, int dtype, long long rows, long long classes, long long row_stride,
                                               const void* teacher, int teacher_dtype, const long long* indices, int k, float temperature,

@@ -5,6 +5,8 @@ from pathlib import Path
 
 import pytest
 
+from tests.test_head_ops_cpu import P, SHAPE, _caller
+
 CSRC = Path(__file__).resolve().parent.parent / "addernetcuda_b200" / "csrc"
 
 RING = r"""
@@ -56,3 +58,13 @@ def test_a_ring_is_left_when_its_last_uses_are_over(tmp_path):
     subprocess.run(["g++", "-std=c++17", "-Wall", "-Werror", f"-I{CSRC}", str(tmp_path / "ring.cpp"), "-o", str(tmp_path / "ring")], check=True)
     done = subprocess.run([str(tmp_path / "ring")], capture_output=True, text=True, timeout=60)
     assert done.returncode == 0, done.stdout
+
+
+def test_temperatures_too_small_for_their_inverse():
+    """1 / T beyond fp32: 0 times infinity would be NaN.  The smallest that are taken have an inverse."""
+    fwd = _caller("adder_b200_distillation_forward", x=P, t=0, rows=2, v=10, xs=10, z=P, zt=0, at=P, k=3, tau=1.0, tg=None, ig=-100, d=P, lp=None, st=None, ma=None, s=None)
+    bwd = _caller("adder_b200_distillation_backward", x=P, t=0, rows=2, v=10, xs=10, at=P, k=3, tau=1.0, tg=None, ig=-100, st=P, ma=P, gd=P, gl=None, dx=P, s=None)
+    for tau in (1e-45, 1e-40, 4.2e-39):
+        assert fwd(tau=tau) == bwd(tau=tau) == SHAPE
+    for tau in (4.3e-39, 1e-37, 3e38):
+        assert fwd(tau=tau, rows=0) == bwd(tau=tau, rows=0) == 0
