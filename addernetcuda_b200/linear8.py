@@ -182,7 +182,9 @@ def linear_8bit(x: Union[torch.Tensor, Rows8], weight: Weight8, bias: Optional[t
 
 class Linear8bit(nn.Module):
     """A linear layer with its weight in 8 bits, for inference: `Linear8bit(linear)` of an nn.Linear on CUDA, or of a 1x1 nn.Conv2d (stride
-    1, no padding, one group), whose input and output then are [N, C, H, W].  The output has the input's type."""
+    1, no padding, one group), whose input and output then are [N, C, H, W].  The input of an nn.Linear's may be a `Rows8`, as
+    `rmsnorm.rms_norm_8bit` gives it.  The output has the type `dtype`, where it is None the input's, bfloat16 for a Rows8.  There is no
+    `weight`: the codes are `values` and `scales`."""
 
     def __init__(self, layer: nn.Module):
         super().__init__()
@@ -209,12 +211,18 @@ class Linear8bit(nn.Module):
         self._buffers["values"] = _padded(self._buffers["values"])
         return self
 
-    def forward(self, x):
+    def forward(self, x, dtype: Optional[torch.dtype] = None):
+        if isinstance(x, Rows8):
+            if self.convolution:
+                raise TypeError("a convolution's layer takes images [N, C, H, W], not rows in 8 bits")
+            dtype = torch.bfloat16 if dtype is None else dtype
+        elif dtype is None:
+            dtype = x.dtype
         if self.convolution:
             x = x.permute(0, 2, 3, 1)
-        bias = None if self.bias is None else self.bias.to(x.dtype)
+        bias = None if self.bias is None else self.bias.to(dtype)
         with torch.no_grad():
-            y = linear_8bit(x, Weight8(self.values, self.scales), bias)
+            y = linear_8bit(x, Weight8(self.values, self.scales), bias, dtype)
         return y.permute(0, 3, 1, 2) if self.convolution else y
 
     def extra_repr(self) -> str:

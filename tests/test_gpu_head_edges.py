@@ -129,3 +129,29 @@ def test_a_term_of_weight_0_is_left_out():
         for alpha in (0.0, 0.5, 1.0):
             with pytest.raises(kind):
                 DistillationLoss(2.0, alpha)(x, bad, z, at)
+
+
+def _rows8(m, k, dtype=torch.bfloat16):
+    from addernetcuda_b200.rmsnorm import rms_norm_8bit
+    with torch.no_grad():
+        return rms_norm_8bit(torch.randn(m, k, device=DEV).to(dtype))
+
+
+def test_a_layer_behind_a_norm_in_8_bits():
+    """Linear8bit takes codes, with and without a bias, as linear_8bit does; of several axes; no convolution does."""
+    from addernetcuda_b200.linear8 import Linear8bit, Rows8, Weight8, linear_8bit
+    torch.manual_seed(5)
+    x = _rows8(12, 300)
+    for bias in (False, True):
+        layer = torch.nn.Linear(300, 70, bias=bias).to(DEV)
+        eight = Linear8bit(layer)
+        y = eight(x)
+        b = layer.bias.detach().bfloat16() if bias else None
+        assert y.dtype == torch.bfloat16 and torch.equal(y, linear_8bit(x, Weight8(eight.values, eight.scales), b))
+        exact = x.dequantize(torch.float64) @ Weight8(eight.values, eight.scales).dequantize(torch.float64).t() + (b.double() if bias else 0.0)
+        assert (y.double() - exact).norm() <= 2.0 ** -8 * exact.norm()
+        three = Rows8(x.values.contiguous().view(3, 4, 300), x.scales.view(3, 4, 3))
+        assert torch.equal(eight(three), y.view(3, 4, 70))
+        assert torch.equal(eight(x, torch.float32), linear_8bit(x, Weight8(eight.values, eight.scales), layer.bias.detach() if bias else None, torch.float32))
+    with pytest.raises(TypeError):
+        Linear8bit(torch.nn.Conv2d(300, 8, 1).to(DEV))(x)
