@@ -199,7 +199,7 @@ class Linear8bit(nn.Module):
         values, scales = quantize_weight(weight)
         self.register_buffer("values", values)
         self.register_buffer("scales", scales)
-        self.register_buffer("bias", None if layer.bias is None else layer.bias.detach().float())
+        self.register_buffer("bias", None if layer.bias is None else layer.bias.detach().to(torch.float32, copy=True))
 
     def _apply(self, fn, recurse=True):
         # a module's .half(), .float() and the like are for parameters: what is held here keeps its types, and follows to a device alone

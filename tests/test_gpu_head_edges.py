@@ -155,3 +155,32 @@ def test_a_layer_behind_a_norm_in_8_bits():
         assert torch.equal(eight(x, torch.float32), linear_8bit(x, Weight8(eight.values, eight.scales), layer.bias.detach() if bias else None, torch.float32))
     with pytest.raises(TypeError):
         Linear8bit(torch.nn.Conv2d(300, 8, 1).to(DEV))(x)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_layers_bias(dtype):
+    """The layer against float64 of its codes, with a bias as large as the product; a layer of its own, whatever becomes of the one it was made of."""
+    from addernetcuda_b200.linear8 import Linear8bit, Weight8, quantize_rows
+    torch.manual_seed(6)
+    for make, x in ((lambda: torch.nn.Linear(200, 130), torch.randn(30, 200, device=DEV)), (lambda: torch.nn.Conv2d(200, 130, 1), torch.randn(2, 200, 3, 5, device=DEV))):
+        layer = make().to(DEV)
+        with torch.no_grad():
+            layer.bias.normal_()
+        x = x.to(dtype)
+        eight = Linear8bit(layer)
+        y = eight(x)
+        rows = x if x.dim() == 2 else x.permute(0, 2, 3, 1).reshape(-1, 200)
+        exact = quantize_rows(rows).dequantize(torch.float64) @ Weight8(eight.values, eight.scales).dequantize(torch.float64).t() + layer.bias.double().to(dtype).double()
+        got = y if x.dim() == 2 else y.permute(0, 2, 3, 1).reshape(-1, 130)
+        size = quantize_rows(rows).dequantize(torch.float64).abs() @ Weight8(eight.values, eight.scales).dequantize(torch.float64).abs().t() + layer.bias.double().abs()
+        # the output's rounding, 128 + 3 + blocks roundings of 2^-23 of the magnitudes, two of what dequantize rounds
+        assert bool(((got.double() - exact).abs() <= U[dtype] * exact.abs() * (1 + 2.0 ** -8) + 140 * 2.0 ** -23 * size).all())
+        with torch.no_grad():
+            layer.bias.zero_()
+            layer.weight.zero_()
+        assert torch.equal(eight(x), y)
+        state = {k: torch.zeros_like(v.float()).to(v.dtype) for k, v in eight.state_dict().items()}
+        with torch.no_grad():
+            layer.bias.fill_(1.0)
+        eight.load_state_dict(state)
+        assert (layer.bias == 1).all() and (eight(x) == 0).all()
