@@ -182,7 +182,7 @@ def linear_8bit(x: Union[torch.Tensor, Rows8], weight: Weight8, bias: Optional[t
 
 class Linear8bit(nn.Module):
     """A linear layer with its weight in 8 bits, for inference: `Linear8bit(linear)` of an nn.Linear on CUDA, or of a 1x1 nn.Conv2d (stride
-    1, no padding, one group), whose input and output then are [N, C, H, W].  The input of an nn.Linear's may be a `Rows8`, as
+    1, no padding, one group), whose input and output then are [N, C, H, W] or [C, H, W], in one order in memory.  The input of an nn.Linear's may be a `Rows8`, as
     `rmsnorm.rms_norm_8bit` gives it.  The output has the type `dtype`, where it is None the input's, bfloat16 for a Rows8.  There is no
     `weight`: the codes are `values` and `scales`."""
 
@@ -218,12 +218,19 @@ class Linear8bit(nn.Module):
             dtype = torch.bfloat16 if dtype is None else dtype
         elif dtype is None:
             dtype = x.dtype
+        channels_last = False
         if self.convolution:
-            x = x.permute(0, 2, 3, 1)
+            if x.dim() not in (3, 4):
+                raise ValueError(f"a convolution's layer takes images [N, C, H, W] or [C, H, W], got shape {tuple(x.shape)}")
+            channels_last = x.dim() == 4 and x.is_contiguous(memory_format=torch.channels_last)
+            x = x.movedim(-3, -1)
         bias = None if self.bias is None else self.bias.to(dtype)
         with torch.no_grad():
             y = linear_8bit(x, Weight8(self.values, self.scales), bias, dtype)
-        return y.permute(0, 3, 1, 2) if self.convolution else y
+        if not self.convolution:
+            return y
+        y = y.movedim(-1, -3)
+        return y if channels_last else y.contiguous()      # in the input's order, as nn.Conv2d gives it
 
     def extra_repr(self) -> str:
         return f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}"

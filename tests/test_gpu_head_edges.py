@@ -184,3 +184,21 @@ def test_a_layers_bias(dtype):
             layer.bias.fill_(1.0)
         eight.load_state_dict(state)
         assert (layer.bias == 1).all() and (eight(x) == 0).all()
+
+
+def test_a_convolutions_images():
+    """What nn.Conv2d takes and gives: an image without a batch, no images, outputs in the order of the input."""
+    from addernetcuda_b200.linear8 import Linear8bit
+    torch.manual_seed(7)
+    conv = torch.nn.Conv2d(40, 24, 1).to(DEV)
+    eight = Linear8bit(conv)
+    x = torch.randn(3, 40, 5, 7, device=DEV)
+    y = eight(x)
+    assert y.is_contiguous() and y.view(3, -1).shape == (3, 24 * 35)
+    assert torch.equal(eight(x[1]), eight(x[1:2])[0]) and eight(x[1]).is_contiguous()
+    last = eight(x.contiguous(memory_format=torch.channels_last))
+    assert torch.equal(last, y) and last.is_contiguous(memory_format=torch.channels_last)
+    assert eight(x[:0]).shape == conv(x[:0]).shape
+    for bad in (x[0, 0], x[None]):
+        with pytest.raises(ValueError):
+            eight(bad)
