@@ -87,25 +87,26 @@ def fold_batchnorm(model: nn.Module) -> nn.Module:
 def quantize_linear(model: nn.Module) -> nn.Module:
     """Replace, in place, every multiply-based linear layer of `model` (on CUDA) - nn.Linear, and 1x1 nn.Conv2d of stride 1 and one group without
     padding, as the `fc` of `addernetcuda_b200.resnet` - by a `linear8.Linear8bit` with its weight in 8 bits, and put the model in evaluation
-    mode.  Adder layers stay as they are: their |x - w| is no product.  Subclasses of the two stay, too.  A layer that stands in several places
-    is replaced by one; a model that is itself such a layer by what is returned."""
+    mode.  Adder layers stay as they are: their |x - w| is no product.  Subclasses of the two stay, too, and layers whose weight is computed by a
+    hook (pruning, weight norm) or read by their parent (those of nn.TransformerEncoderLayer).  Hooks of a replaced layer are not kept, nor is its
+    `weight`.  A layer that stands in several places is replaced by one; a model that is itself such a layer by what is returned.  Where a layer
+    cannot be put in 8 bits (another type, not on CUDA), this raises and nothing is replaced."""
+    def taken(layer) -> bool:
+        pointwise = type(layer) is nn.Conv2d and layer.kernel_size == (1, 1) and layer.stride == (1, 1) and layer.groups == 1 and \
+            layer.padding in ((0, 0), "valid")
+        return (type(layer) is nn.Linear or pointwise) and layer._parameters.get("weight") is not None
+
+    places = [(module, name, child) for module in model.modules() for name, child in module._modules.items()
+              if taken(child) and not (isinstance(module, nn.TransformerEncoderLayer) and name in ("linear1", "linear2"))]
+    for *_, layer in [*places, *([(model,)] if taken(model) else [])]:
+        Linear8bit.check(layer)
     model.eval()
     made = {}
-
-    def replacement(child: nn.Module):
-        pointwise = type(child) is nn.Conv2d and child.kernel_size == (1, 1) and child.stride == (1, 1) and child.groups == 1 and \
-            child.padding in ((0, 0), "valid")
-        if type(child) is not nn.Linear and not pointwise:
-            return None
-        if child not in made:
-            made[child] = Linear8bit(child).eval()
-        return made[child]
-
-    for module in list(model.modules()):
-        for name, child in list(module._modules.items()):
-            if child is not None and replacement(child) is not None:
-                setattr(module, name, replacement(child))
-    return replacement(model) or model
+    for module, name, layer in places:
+        if layer not in made:
+            made[layer] = Linear8bit(layer).eval()
+        setattr(module, name, made[layer])
+    return Linear8bit(model).eval() if taken(model) else model
 
 
 def accuracy(output: torch.Tensor, target: torch.Tensor, topk: Sequence[int] = (1,)):

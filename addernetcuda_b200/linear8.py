@@ -188,18 +188,26 @@ class Linear8bit(nn.Module):
 
     def __init__(self, layer: nn.Module):
         super().__init__()
+        self.check(layer)
         self.convolution = isinstance(layer, nn.Conv2d)
-        if self.convolution:
-            if layer.kernel_size != (1, 1) or layer.stride != (1, 1) or layer.padding not in ((0, 0), "valid") or layer.groups != 1:
-                raise ValueError("only convolutions of kernel size 1, stride 1 and one group without padding are linear layers")
-        elif not isinstance(layer, nn.Linear):
-            raise TypeError(f"layer must be an nn.Linear or an nn.Conv2d, got {type(layer).__name__}")
         weight = layer.weight.detach().flatten(1)
         self.out_features, self.in_features = weight.shape
         values, scales = quantize_weight(weight)
         self.register_buffer("values", values)
         self.register_buffer("scales", scales)
         self.register_buffer("bias", None if layer.bias is None else layer.bias.detach().to(torch.float32, copy=True))
+
+    @staticmethod
+    def check(layer: nn.Module) -> None:
+        """Raise for what cannot be put in 8 bits."""
+        if isinstance(layer, nn.Conv2d):
+            if layer.kernel_size != (1, 1) or layer.stride != (1, 1) or layer.padding not in ((0, 0), "valid") or layer.groups != 1:
+                raise ValueError("only convolutions of kernel size 1, stride 1 and one group without padding are linear layers")
+        elif not isinstance(layer, nn.Linear):
+            raise TypeError(f"layer must be an nn.Linear or an nn.Conv2d, got {type(layer).__name__}")
+        _check_input(layer.weight, "the layer's weight")
+        if layer.weight.shape[1] == 0:
+            raise ValueError(f"the layer's weight has shape {tuple(layer.weight.shape)}")
 
     def _apply(self, fn, recurse=True):
         # a module's .half(), .float() and the like are for parameters: what is held here keeps its types, and follows to a device alone

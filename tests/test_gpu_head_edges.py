@@ -202,3 +202,31 @@ def test_a_convolutions_images():
     for bad in (x[0, 0], x[None]):
         with pytest.raises(ValueError):
             eight(bad)
+
+
+def test_which_layers_are_put_in_8_bits():
+    """All or none, where one of them cannot be; none whose weight another module reads or computes."""
+    import copy
+    from torch.nn.utils import prune
+    from addernetcuda_b200.inference import quantize_linear
+    from addernetcuda_b200.linear8 import Linear8bit
+    torch.manual_seed(8)
+    for odd, kind in ((torch.nn.Linear(16, 16).to(DEV).double(), TypeError), (torch.nn.Linear(16, 16), RuntimeError)):
+        net = torch.nn.Sequential(torch.nn.Linear(16, 16).to(DEV), odd).train()
+        with pytest.raises(kind):
+            quantize_linear(net)
+        assert type(net[0]) is torch.nn.Linear and type(net[1]) is torch.nn.Linear and net.training
+    net = torch.nn.Sequential(torch.nn.Linear(32, 64), torch.nn.TransformerEncoder(torch.nn.TransformerEncoderLayer(64, 4, 128, batch_first=True), 2)).to(DEV)
+    x = torch.randn(2, 5, 32, device=DEV)
+    encoder = copy.deepcopy(net[1]).eval()
+    quantize_linear(net)
+    assert isinstance(net[0], Linear8bit)
+    for no_grad in (False, True):
+        with torch.set_grad_enabled(not no_grad):
+            assert torch.equal(net(x), encoder(net[0](x)))
+    pruned = torch.nn.Linear(16, 16).to(DEV)
+    prune.l1_unstructured(pruned, "weight", 0.5)
+    net = quantize_linear(torch.nn.Sequential(pruned, torch.nn.Linear(16, 16).to(DEV)))
+    assert net[0] is pruned and isinstance(net[1], Linear8bit)
+    prune.remove(pruned, "weight")
+    assert isinstance(quantize_linear(net)[0], Linear8bit)
