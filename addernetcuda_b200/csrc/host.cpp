@@ -1122,7 +1122,7 @@ PyObject* py_linear_8bit(PyObject*, PyObject* const* args, Py_ssize_t n) {
     }
     const int out_code = out_type == at::kFloat ? ADDER_TYPE_F32 : out_type == at::kBFloat16 ? ADDER_TYPE_BF16 : out_type == at::kHalf ? ADDER_TYPE_F16 : -1;
     int64_t outer, w_stride, rows, x_stride;
-    if (out_code < 0 || !codes_of(*wv, *ws, &outer, &w_stride) || wv->dim() != 2 || ws->size(0) != (outer + 127) / 128) Py_RETURN_NONE;
+    if (out_code < 0 || !codes_of(*wv, *ws, &outer, &w_stride) || wv->dim() != 2 || ws->size(0) != (outer + 127) / 128 || needs_node(*wv, *ws)) Py_RETURN_NONE;
     const int64_t inner = wv->size(1);
     const at::Tensor& first = x != nullptr ? *x : *xv;
     if (first.dim() < 1 || first.size(-1) != inner || first.device() != wv->device()) Py_RETURN_NONE;
@@ -1132,7 +1132,7 @@ PyObject* py_linear_8bit(PyObject*, PyObject* const* args, Py_ssize_t n) {
         type = type_code(*x);
         if (type < 0 || !unwrapped(*x) || x->numel() == 0 || !rows_of(*x, 1, inner, &x_stride) || needs_node(*x, *x)) Py_RETURN_NONE;
         rows = x->numel() / inner;
-    } else if (!codes_of(*xv, *xs, &rows, &x_stride) || xs->sizes().slice(0, lead.size()) != lead) {
+    } else if (!codes_of(*xv, *xs, &rows, &x_stride) || xs->sizes().slice(0, lead.size()) != lead || needs_node(*xv, *xs)) {
         Py_RETURN_NONE;
     }
     if (bias != nullptr && (!unwrapped(*bias) || !bias->is_contiguous() || bias->device() != wv->device() || bias->scalar_type() != out_type || bias->dim() != 1 ||

@@ -13,6 +13,7 @@ from typing import NamedTuple, Optional, Union
 
 import torch
 import torch.nn as nn
+from torch.autograd.forward_ad import unpack_dual
 
 from . import _lib, _native, adder_cuda
 from .layernorm import _check_input, _ptr, _rows, _whole
@@ -58,12 +59,22 @@ def _empty_rows(shape, dev):
     return Rows8(values, torch.empty((*shape[:-1], _blocks(shape[-1])), device=dev)), stride
 
 
+def _refuse_gradient(name: str, *tensors) -> None:
+    """Raise where a derivative of an operator that has none would be recorded, backward or forward."""
+    for t in tensors:
+        if t is None:
+            continue
+        if torch.is_grad_enabled() and t.requires_grad:
+            raise RuntimeError(f"{name} has no gradient: call it under torch.no_grad()")
+        if unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{name} has no gradient in forward mode either: give it the primal of a dual tensor")
+
+
 def _to_8bit(name: str, x: torch.Tensor, weight: bool):
     _check_input(x, "w" if weight else "x")
     if (x.dim() != 2 if weight else x.dim() < 1) or x.shape[-1] == 0:
         raise ValueError(f"{name} takes {'a matrix' if weight else 'rows'} of at least one column, got shape {tuple(x.shape)}")
-    if torch.is_grad_enabled() and x.requires_grad:
-        raise RuntimeError(f"{name} has no gradient: call it under torch.no_grad()")
+    _refuse_gradient(name, x)
     d = x.shape[-1]
     rows = x.numel() // d
     values, stride = _codes(x.shape[:-1], d, x.device)
@@ -163,11 +174,8 @@ def linear_8bit(x: Union[torch.Tensor, Rows8], weight: Weight8, bias: Optional[t
         _check_input(bias, "bias", dev)
         if bias.shape != (n,) or bias.dtype != dtype:
             raise ValueError(f"bias must have shape {(n,)} and type {dtype}, got {tuple(bias.shape)} {bias.dtype}")
-        if torch.is_grad_enabled() and bias.requires_grad:
-            raise RuntimeError("linear_8bit has no gradient: call it under torch.no_grad()")
+    _refuse_gradient("linear_8bit", *(x if isinstance(x, Rows8) else (x,)), *weight, bias)
     if not isinstance(x, Rows8):
-        if torch.is_grad_enabled() and x.requires_grad:
-            raise RuntimeError("linear_8bit has no gradient: call it under torch.no_grad()")
         x = quantize_rows(x)
     xv, xstride = _aligned(x.values)
     wv, wstride = _aligned(weight.values)

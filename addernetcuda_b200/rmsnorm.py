@@ -15,7 +15,7 @@ import torch.nn as nn
 
 from . import _lib, _native, adder_cuda
 from .layernorm import _check_input, _once, _ptr, _rows, _save, _saved, _sizes, _whole
-from .linear8 import Rows8, _empty_rows
+from .linear8 import Rows8, _empty_rows, _refuse_gradient
 
 
 class _RMSNorm(torch.autograd.Function):
@@ -120,8 +120,7 @@ def rms_norm_8bit(x: torch.Tensor, weight: Optional[torch.Tensor] = None, eps: f
     if out is not None:
         return Rows8(*out[:2]) if residual is None else (Rows8(*out[:2]), out[2])
     _check_call(x, tuple(x.shape[-1:]) if isinstance(x, torch.Tensor) else (), weight, eps, residual)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, residual, weight)):
-        raise RuntimeError("rms_norm_8bit has no gradient: call it under torch.no_grad()")
+    _refuse_gradient("rms_norm_8bit", x, residual, weight)
     rows, d = _sizes(x, x.shape[-1:])
     dev = x.device
     x2, xs = _rows(x, rows, d)

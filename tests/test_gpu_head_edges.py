@@ -230,3 +230,30 @@ def test_which_layers_are_put_in_8_bits():
     assert net[0] is pruned and isinstance(net[1], Linear8bit)
     prune.remove(pruned, "weight")
     assert isinstance(quantize_linear(net)[0], Linear8bit)
+
+
+def test_derivatives_are_refused():
+    """Operators without a gradient raise where one would be recorded, forward-mode tangents and trained scales among them."""
+    import torch.autograd.forward_ad as fwd
+    from addernetcuda_b200.linear8 import Rows8, Weight8, linear_8bit, quantize_rows, quantize_weight
+    from addernetcuda_b200.rmsnorm import rms_norm_8bit
+    x, t = torch.randn(4, 128, device=DEV), torch.randn(4, 128, device=DEV)
+    w = quantize_weight(torch.randn(64, 128, device=DEV))
+    rows = quantize_rows(x)
+    b = torch.zeros(64, device=DEV)
+    with fwd.dual_level():
+        dual = fwd.make_dual(x, t)
+        for call in (lambda: quantize_rows(dual), lambda: quantize_weight(dual), lambda: linear_8bit(dual, w), lambda: rms_norm_8bit(dual),
+                     lambda: rms_norm_8bit(x, residual=dual), lambda: rms_norm_8bit(x, fwd.make_dual(torch.ones(128, device=DEV), t[0])),
+                     lambda: linear_8bit(x, w, fwd.make_dual(b, torch.ones_like(b))),
+                     lambda: linear_8bit(Rows8(rows.values, fwd.make_dual(rows.scales, torch.ones_like(rows.scales))), w)):
+            for grad in (True, False):      # no_grad is for the backward mode alone
+                with torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match="no gradient"):
+                    call()
+        quantize_rows(fwd.unpack_dual(dual).primal)
+    for call in (lambda: linear_8bit(Rows8(rows.values, rows.scales.clone().requires_grad_()), w, dtype=torch.float32),
+                 lambda: linear_8bit(x, Weight8(w.values, w.scales.clone().requires_grad_()))):
+        with pytest.raises(RuntimeError, match="no gradient"):
+            call()
+        with torch.no_grad():
+            assert torch.equal(call(), linear_8bit(x, w))
