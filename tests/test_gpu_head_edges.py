@@ -257,3 +257,15 @@ def test_derivatives_are_refused():
             call()
         with torch.no_grad():
             assert torch.equal(call(), linear_8bit(x, w))
+
+
+@pytest.mark.parametrize("rows,classes,k", [(5, 10, 4), (64, 1000, 20), (7, 1001, 33), (1300, 3000, 5), (3, 32000, 32), (30, 50257, 8), (700, 10001, 256), (1, 128000, 100)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("tau", [2.0, 4.0])
+def test_temperatures_whose_second_exponential_is_a_power(rows, classes, k, dtype, tau):
+    from tests.test_gpu_distill import _call, _exact, _inputs, _near
+    x, z, at, targets, g, gl = _inputs(rows, classes, k, dtype, seed=rows + k)
+    r, grad = _call(x, z, at, tau, targets, g, gl)
+    want = _exact(x, z, at, tau, targets, g, gl)
+    for name, got in (("divergence", r.divergence), ("log_prob", r.log_prob), ("grad", grad)):
+        _near(got, want[name], name)
