@@ -5,15 +5,15 @@
 //     max(p_n(c) - q_n(c), 0) where n < L (p_n(c), without t_n, where the drafter gives no probabilities), or p_L(c) where n = L
 //   token = the first c with sum_{c' <= c} w(c') > u sum w  and  w(c) > 0
 //
-// The sums are held in 64 bits: differences of two fp32 values are exact there, and a border between two classes moves by some 1e-16 of the
-// whole, so the token does not depend on the order of a sum in practice (in 32 bits it would, for one draw in a hundred of 128000 classes).
+// The sums are held in 64 bits: differences of two values are exact there, and a border between two classes moves by some 1e-16 of the whole,
+// so the token does not depend on the order of a sum in practice (in 32 bits it would, for one draw in a hundred of 128000 classes).
 //
 // A sequence's row is split over a cluster of CTAs and their warps, a segment of consecutive classes a warp.  Every CTA finds n for itself,
 // sums its segments and leaves the sums with all CTAs of the cluster; then the CTA whose segment holds the border reads that again, a part a warp.
 //
 // What bounds it: of all rows only those of p_n and q_n are read, in lines that nothing has touched before, behind three loads that wait for one
 // another (the tokens, their probabilities, the row), and the segment's second reading waits for the sums.  One sequence of 32000 fp32 classes 6.4 us;
-// 64 of 128000 bf16 16.4 us, where the bytes alone take 5 (with 512 threads a CTA or 256, and with additions in fp32 instead of 64 bits, the same).
+// 64 of 128000 bf16 14.3 us, where the bytes alone take 5 (with 512 threads a CTA or 256, and with additions in fp32 instead of 64 bits, the same).
 #include "kernels.h"
 #include "elements.cuh"
 #include "launch.cuh"
@@ -50,18 +50,30 @@ __device__ __forceinline__ double dv_double(float w) {
     const uint32_t u = __float_as_uint(w);
     return __hiloint2double((int)((u >> 3) + 0x38000000u), (int)(u << 29));
 }
-// f - g, and what fp32 leaves out of it: nothing for two fp16 values of up to 1, and for bf16 where one is less than 2^16 times the other; beyond, the
-// difference is rounded, to 2^-25 of itself.  Differences of fp32 values are rounded more often, so what is left out counts (the operations
-// after d are exact as long as nothing overflows).
-template <class T> __device__ __forceinline__ float dv_difference(float f, float g, float& left) {
-    const float d = f - g;
-    left = 0.f;
-    if constexpr (sizeof(T) == 4) {
-        const float b = d - f;
-        const float e = (f - (d - b)) - (g + b);
-        if (d >= DV_LEAST && d < INFINITY) left = e;
-    }
+// f - g, and what fp32 leaves out of it.  The operations after d are exact as long as nothing overflows.
+__device__ __forceinline__ float dv_difference(float f, float g, float& left) {
+    const float d = f - g, b = d - f;
+    const float e = (f - (d - b)) - (g + b);
+    left = d >= DV_LEAST && d < INFINITY ? e : 0.f;
     return d;
+}
+// Differences of values in 16 bits, of which nothing is left out but where one is some 2^16 (bf16) or 2^13 (fp16) times the other: `far` stays 0 but
+// then.  For d > 0 and g >= 0 g + (d - f) is minus what is left out, exactly; where g is negative nothing is said.
+template <int VEC> __device__ __forceinline__ void dv_differences(const float (&f)[VEC], const float (&g)[VEC], float (&d)[VEC], uint32_t& far) {
+    if constexpr (VEC == 1) {
+        d[0] = f[0] - g[0];
+        far |= __float_as_uint(g[0] + (d[0] - f[0])) | (__float_as_uint(g[0]) & 0x80000000u);
+    } else {
+        const uint64_t minus = pack2(-1.f, -1.f);
+#pragma unroll
+        for (int j = 0; j < VEC; j += 2) {
+            const uint64_t f2 = pack2(f[j], f[j + 1]), g2 = pack2(g[j], g[j + 1]), d2 = fma2(g2, minus, f2);
+            float lo, hi;
+            unpack2(add2(g2, fma2(f2, minus, d2)), lo, hi);
+            unpack2(d2, d[j], d[j + 1]);
+            far |= __float_as_uint(lo) | __float_as_uint(hi) | ((__float_as_uint(g[j]) | __float_as_uint(g[j + 1])) & 0x80000000u);
+        }
+    }
 }
 // Inclusive sums over the lanes of a warp.
 __device__ __forceinline__ double dv_scan(double v, int lane) {
@@ -134,21 +146,46 @@ template <class T, int VEC> __global__ void __launch_bounds__(DV_THREADS) dv_ker
             float g[VEC];
             dv_load<T, VEC>(q_row + (size_t)v * VEC, g);
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) w[j] = dv_difference<T>(f[j], g[j], left[j]);
+            for (int j = 0; j < VEC; ++j) w[j] = dv_difference(f[j], g[j], left[j]);
         }
     };
-    // Sum of the weights of vectors from to to - 1, in every lane of a warp.
+    // Sum of the weights of vectors from to to - 1, in every lane of a warp.  In 16 bits what is left out of differences is asked for, and a lane that has
+    // any goes over its vectors again for it (64x6x128000 bf16 14.3 us; added up beside every difference 22, by a branch at
+    // each vector 20.5).
     const auto sum_of = [&](int from, int to, bool whole) {
         double sum[2] = {0.0, 0.0};
         float rest = 0.f;
+        if (sizeof(T) == 4 || q_row == nullptr || whole) {
 #pragma unroll 4
-        for (int v = from + lane; v < to; v += 32) {
-            float w[VEC], left[VEC];
-            weights(v, whole, w, left);
+            for (int v = from + lane; v < to; v += 32) {
+                float w[VEC], left[VEC];
+                weights(v, whole, w, left);
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                if (w[j] >= DV_LEAST) sum[j & 1] += dv_double(w[j]);
-                rest += left[j];
+                for (int j = 0; j < VEC; ++j) {
+                    if (w[j] >= DV_LEAST) sum[j & 1] += dv_double(w[j]);
+                    rest += left[j];
+                }
+            }
+        } else {
+            uint32_t far = 0;
+#pragma unroll 4
+            for (int v = from + lane; v < to; v += 32) {
+                float f[VEC], g[VEC], w[VEC];
+                dv_load<T, VEC>(p_row + (size_t)v * VEC, f);
+                dv_load<T, VEC>(q_row + (size_t)v * VEC, g);
+                dv_differences<VEC>(f, g, w, far);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j)
+                    if (w[j] >= DV_LEAST) sum[j & 1] += dv_double(w[j]);
+            }
+            if (far != 0) {
+#pragma unroll 1
+                for (int v = from + lane; v < to; v += 32) {
+                    float w[VEC], left[VEC];
+                    weights(v, false, w, left);
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) rest += left[j];
+                }
             }
         }
         double s = sum[0] + sum[1] + (double)rest;

@@ -269,3 +269,44 @@ def test_temperatures_whose_second_exponential_is_a_power(rows, classes, k, dtyp
     want = _exact(x, z, at, tau, targets, g, gl)
     for name, got in (("divergence", r.divergence), ("log_prob", r.log_prob), ("grad", grad)):
         _near(got, want[name], name)
+
+
+@pytest.mark.parametrize("classes", [3, 40000])
+@pytest.mark.parametrize("dtype,one,least", [(torch.float32, 1.0, 2.0 ** -30), (torch.bfloat16, 1.0, 2.0 ** -30), (torch.float16, 2.0, 2.0 ** -24)])
+def test_differences_of_far_probabilities(dtype, one, least, classes):
+    """Weights of one and of one - least, in either order, and a border between the two that lies by half of least beside the middle of their sum: it
+    shows whether least, which 32 bits cannot hold beside one, is part of the sum."""
+    from addernetcuda_b200.drafts import verify_drafts
+    p, q = torch.zeros(2, 2, classes, dtype=dtype, device=DEV), torch.zeros(2, 1, classes, dtype=dtype, device=DEV)
+    first, second = 0, classes - 2
+    p[:, 0, first] = p[:, 0, second] = one
+    q[0, 0, second] = least      # weights one, one - least: up to the first it is above the half
+    q[1, 0, first] = least       # weights one - least, one: it is below
+    q[:, 0, classes - 1] = 0.5   # the drafted class, which the target rules out
+    u = torch.tensor([[0.9, 0.5]], device=DEV).expand(2, 2).contiguous()
+    r = verify_drafts(p, q, torch.full((2, 1), classes - 1, device=DEV), u)
+    assert r.accepted.tolist() == [0, 0] and r.tokens[:, 0].tolist() == [first, second]
+
+
+@pytest.mark.parametrize("classes", [1001, 4096, 50000])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_weights_of_many_sizes(classes, dtype):
+    """Probabilities from 1 down to 2^-24, some of which are 0, some negative: as far apart as they come."""
+    from addernetcuda_b200.drafts import verify_drafts
+    torch.manual_seed(classes)
+    b = 60
+
+    def weights(*shape):
+        w = torch.exp2(-24 * torch.rand(*shape, device=DEV))
+        return torch.where(torch.rand(*shape, device=DEV) < 0.1, 0.0, w).to(dtype)
+
+    p, q = weights(b, 2, classes), weights(b, 1, classes)
+    q = torch.where(torch.rand(b, 1, classes, device=DEV) < 0.05, -q, q)
+    p[:, 0, 5], q[:, 0, 5] = 0, 1      # the drafted class
+    u = torch.rand(b, 2, device=DEV).clamp(min=0.1)
+    r = verify_drafts(p, q, torch.full((b, 1), 5, device=DEV), u)
+    w = (p[:, 0].double() - q[:, 0].double()).clamp(min=0)      # exact
+    reached = w.cumsum(1)
+    there = (reached > u[:, 1:].double() * reached[:, -1:]) & (w > 0)
+    want = torch.where(there, torch.arange(classes, device=DEV), classes).amin(1)
+    assert (r.accepted == 0).all() and torch.equal(r.tokens[:, 0], want)
