@@ -11,7 +11,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import _lib, _native, adder_cuda
-from .layernorm import _check_input, _ptr, _whole
+from .layernorm import _check_input, _ptr, _recorded, _whole
 
 
 class VerifiedDrafts(NamedTuple):
@@ -77,11 +77,17 @@ def verify_drafts(target_probs: torch.Tensor, draft_probs: Optional[torch.Tensor
     if lengths is not None:
         lengths = _check_whole(lengths, "lengths", (b,), dev)
     with torch.no_grad():
-        p, q, u = _planes(target_probs), _planes(draft_probs), _whole(uniforms)
-        result = VerifiedDrafts(torch.empty((b, places), dtype=torch.int64, device=dev), torch.empty(b, dtype=torch.int64, device=dev))
-        with torch.cuda.device(dev):
-            _lib.check(_lib.load().adder_b200_verify_drafts(
-                p.data_ptr(), _ptr(q), _lib.TYPE_CODES[p.dtype], tokens.data_ptr(), u.data_ptr(), _ptr(lengths), result.tokens.data_ptr(),
-                result.accepted.data_ptr(), b, places - 1, classes, p.stride(0), p.stride(1), q.stride(0) if q is not None else 0,
-                q.stride(1) if q is not None else 0, adder_cuda._stream(dev)), "adder_b200_verify_drafts")
-    return result
+        return VerifiedDrafts(*_recorded(_verify, target_probs, draft_probs, tokens, uniforms, lengths))
+
+
+def _verify(target_probs, draft_probs, tokens, uniforms, lengths):
+    (b, places, classes), dev = target_probs.shape, target_probs.device
+    p, q, u = _planes(target_probs), _planes(draft_probs), _whole(uniforms)
+    tokens, lengths = _whole(tokens), _whole(lengths)
+    out, accepted = torch.empty((b, places), dtype=torch.int64, device=dev), torch.empty(b, dtype=torch.int64, device=dev)
+    with torch.cuda.device(dev):
+        _lib.check(_lib.load().adder_b200_verify_drafts(
+            p.data_ptr(), _ptr(q), _lib.TYPE_CODES[p.dtype], tokens.data_ptr(), u.data_ptr(), _ptr(lengths), out.data_ptr(),
+            accepted.data_ptr(), b, places - 1, classes, p.stride(0), p.stride(1), q.stride(0) if q is not None else 0,
+            q.stride(1) if q is not None else 0, adder_cuda._stream(dev)), "adder_b200_verify_drafts")
+    return out, accepted

@@ -84,6 +84,23 @@ def _once(name: str, grad: Optional[torch.Tensor], *sources) -> Optional[torch.T
     return _Once.apply(name, grad, *sources)
 
 
+class _Recorded(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, call, *args):
+        state = torch._C._get_tracing_state()
+        torch._C._set_tracing_state(None)      # what `call` allocates and copies is no part of the trace
+        try:
+            return call(*args)
+        finally:
+            torch._C._set_tracing_state(state)
+
+
+def _recorded(call, *args):
+    """call(*args) of an operator without a gradient: in a torch.jit trace as one operation, where otherwise the allocation of its outputs would be
+    all that is recorded."""
+    return _Recorded.apply(call, *args) if torch.jit.is_tracing() else call(*args)
+
+
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, weight, bias, normalized_shape, eps, needs_grad):

@@ -16,7 +16,7 @@ import torch.nn as nn
 from torch.autograd.forward_ad import unpack_dual
 
 from . import _lib, _native, adder_cuda
-from .layernorm import _check_input, _ptr, _rows, _whole
+from .layernorm import _check_input, _ptr, _recorded, _rows, _whole
 
 BLOCK = 128
 
@@ -75,6 +75,10 @@ def _to_8bit(name: str, x: torch.Tensor, weight: bool):
     if (x.dim() != 2 if weight else x.dim() < 1) or x.shape[-1] == 0:
         raise ValueError(f"{name} takes {'a matrix' if weight else 'rows'} of at least one column, got shape {tuple(x.shape)}")
     _refuse_gradient(name, x)
+    return _recorded(_convert, name, x, weight)
+
+
+def _convert(name: str, x: torch.Tensor, weight: bool):
     d = x.shape[-1]
     rows = x.numel() // d
     values, stride = _codes(x.shape[:-1], d, x.device)
@@ -177,10 +181,15 @@ def linear_8bit(x: Union[torch.Tensor, Rows8], weight: Weight8, bias: Optional[t
     _refuse_gradient("linear_8bit", *(x if isinstance(x, Rows8) else (x,)), *weight, bias)
     if not isinstance(x, Rows8):
         x = quantize_rows(x)
-    xv, xstride = _aligned(x.values)
-    wv, wstride = _aligned(weight.values)
-    xs, ws, b = _whole(x.scales), _whole(weight.scales), _whole(bias)
-    y = torch.empty((*lead[:-1], n), dtype=dtype, device=dev)
+    return _recorded(_product, *x, *weight, bias, dtype)
+
+
+def _product(x, x_scales, weight, weight_scales, bias, dtype):
+    (n, k), dev = weight.shape, weight.device
+    xv, xstride = _aligned(x)
+    wv, wstride = _aligned(weight)
+    xs, ws, b = _whole(x_scales), _whole(weight_scales), _whole(bias)
+    y = torch.empty((*x.shape[:-1], n), dtype=dtype, device=dev)
     with torch.cuda.device(dev):
         _lib.check(_lib.load().adder_b200_linear_8bit(
             xv.data_ptr(), xs.data_ptr(), wv.data_ptr(), ws.data_ptr(), _ptr(b), y.data_ptr(), y.numel() // n if n else 0, k, n, xstride, wstride,

@@ -14,7 +14,7 @@ import torch
 import torch.nn as nn
 
 from . import _lib, _native, adder_cuda
-from .layernorm import _check_input, _once, _ptr, _rows, _save, _saved, _sizes, _whole
+from .layernorm import _check_input, _once, _ptr, _recorded, _rows, _save, _saved, _sizes, _whole
 from .linear8 import Rows8, _empty_rows, _refuse_gradient
 
 
@@ -121,6 +121,11 @@ def rms_norm_8bit(x: torch.Tensor, weight: Optional[torch.Tensor] = None, eps: f
         return Rows8(*out[:2]) if residual is None else (Rows8(*out[:2]), out[2])
     _check_call(x, tuple(x.shape[-1:]) if isinstance(x, torch.Tensor) else (), weight, eps, residual)
     _refuse_gradient("rms_norm_8bit", x, residual, weight)
+    out = _recorded(_norm_8bit, x, weight, float(eps), residual)
+    return Rows8(*out[:2]) if residual is None else (Rows8(*out[:2]), out[2])
+
+
+def _norm_8bit(x, weight, eps, residual):
     rows, d = _sizes(x, x.shape[-1:])
     dev = x.device
     x2, xs = _rows(x, rows, d)
@@ -131,9 +136,9 @@ def rms_norm_8bit(x: torch.Tensor, weight: Optional[torch.Tensor] = None, eps: f
     with torch.cuda.device(dev):
         _lib.check(_lib.load().adder_b200_rmsnorm_forward_8bit(
             x2.data_ptr(), _ptr(r2), _ptr(w), out.values.data_ptr(), out.scales.data_ptr(), _ptr(h), rows, d, xs, rs, stride,
-            _lib.TYPE_CODES[x.dtype], _lib.TYPE_CODES[(w if w is not None else x).dtype], float(eps), adder_cuda._stream(dev)),
+            _lib.TYPE_CODES[x.dtype], _lib.TYPE_CODES[(w if w is not None else x).dtype], eps, adder_cuda._stream(dev)),
             "adder_b200_rmsnorm_forward_8bit")
-    return out if residual is None else (out, h)
+    return tuple(out) if residual is None else (*out, h)
 
 
 class FusedRMSNorm(nn.RMSNorm):

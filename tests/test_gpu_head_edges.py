@@ -310,3 +310,37 @@ def test_weights_of_many_sizes(classes, dtype):
     there = (reached > u[:, 1:].double() * reached[:, -1:]) & (w > 0)
     want = torch.where(there, torch.arange(classes, device=DEV), classes).amin(1)
     assert (r.accepted == 0).all() and torch.equal(r.tokens[:, 0], want)
+
+
+def test_a_trace_records_the_operators():
+    """torch.jit.trace: the traced function follows new inputs, of other lengths too."""
+    from addernetcuda_b200.distill import distillation
+    from addernetcuda_b200.drafts import verify_drafts
+    from addernetcuda_b200.linear8 import Linear8bit, linear_8bit, quantize_rows, quantize_weight
+    from addernetcuda_b200.rmsnorm import rms_norm, rms_norm_8bit
+    torch.manual_seed(9)
+    layer, conv = (Linear8bit(m.to(DEV)) for m in (torch.nn.Linear(100, 70), torch.nn.Conv2d(100, 70, 1)))
+    w = quantize_weight(torch.randn(64, 100, device=DEV))
+    weight = torch.randn(100, device=DEV)
+
+    def rows(n):
+        return (torch.randn(n, 100, device=DEV),)
+
+    def drafts(n):
+        p, q = (torch.softmax(torch.randn(n, k, 4000, device=DEV), -1) for k in (3, 2))
+        return p, q, torch.randint(0, 4000, (n, 2), device=DEV), torch.rand(n, 3, device=DEV), torch.randint(0, 3, (n,), device=DEV)
+
+    def distilled(n):
+        return 2 * torch.randn(n, 100, device=DEV), torch.randn(n, 4, device=DEV), torch.randint(0, 100, (n, 4), device=DEV), torch.randint(0, 100, (n,), device=DEV)
+
+    for call, inputs in ((layer, rows), (conv, lambda n: (torch.randn(n, 100, 2, 3, device=DEV),)), (lambda x: rms_norm(x, 100, weight), rows),
+                         (lambda x: tuple(quantize_rows(x)), rows), (lambda x: tuple(quantize_weight(x)), rows), (lambda x: tuple(rms_norm_8bit(x, weight)), rows),
+                         (lambda x: linear_8bit(rms_norm_8bit(x, None, 1e-6, x)[0], w), rows), (lambda *a: tuple(verify_drafts(*a)), drafts),
+                         (lambda p, q, t, u, n: tuple(verify_drafts(p, None, t.int(), u)), drafts), (lambda x, z, at, t: tuple(distillation(x, z, at, 2.0, t)), distilled)):
+        with torch.no_grad():
+            traced = torch.jit.trace(call, inputs(3), check_trace=False)
+            for n in (3, 5):
+                new = inputs(n)
+                got, want = traced(*new), call(*new)
+                for g, e in zip(*((t,) if isinstance(t, torch.Tensor) else t for t in (got, want))):
+                    assert g.dtype == e.dtype and g.shape == e.shape and torch.equal(g.float(), e.float())
