@@ -16,18 +16,34 @@ import torch.nn as nn
 from . import _lib, _native, adder_cuda
 
 
+def _row_stride(shape, strides, d: int) -> Optional[int]:
+    """Elements from row to row of a tensor whose last axes make rows of d consecutive elements; None where it is no such tensor.  Asked of the
+    strides: a view that is refused while a torch.jit trace is made leaves an operation without a result in it, which ended the process."""
+    i, inner = len(shape), 1
+    while inner < d:
+        i -= 1
+        if shape[i] != 1 and strides[i] != inner:
+            return None
+        inner *= shape[i]
+    stride = want = None
+    for size, step in zip(reversed(shape[:i]), reversed(strides[:i])):
+        if size == 1:
+            continue
+        if stride is None:
+            stride = want = step
+        elif step != want:
+            return None
+        want *= size
+    return d if stride is None else stride
+
+
 def _rows(t: torch.Tensor, rows: int, d: int):
-    """(tensor, elements from row to row) of t as `rows` rows of d consecutive elements; a copy only where it is no such view."""
+    """(tensor, elements from row to row) of t as `rows` rows of d consecutive elements; a copy only where it has no such rows."""
     t = t.resolve_neg()
     if t.is_contiguous():
         return t, d
-    try:
-        v = t.view(rows, d)
-    except RuntimeError:
-        return t.contiguous(), d
-    if d > 1 and v.stride(1) != 1:
-        return t.contiguous(), d
-    return v, v.stride(0)
+    stride = _row_stride(t.shape, t.stride(), d)
+    return (t.contiguous(), d) if stride is None else (t, stride)
 
 
 def _whole(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:

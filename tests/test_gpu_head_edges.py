@@ -344,3 +344,29 @@ def test_a_trace_records_the_operators():
                 got, want = traced(*new), call(*new)
                 for g, e in zip(*((t,) if isinstance(t, torch.Tensor) else t for t in (got, want))):
                     assert g.dtype == e.dtype and g.shape == e.shape and torch.equal(g.float(), e.float())
+
+
+def test_a_trace_of_inputs_in_another_order():
+    """Rows that have to be copied, within the norms and the losses."""
+    from addernetcuda_b200.distill import distillation
+    from addernetcuda_b200.layernorm import FusedLayerNorm
+    from addernetcuda_b200.logprobs import token_log_probs
+    from addernetcuda_b200.rmsnorm import FusedRMSNorm
+    torch.manual_seed(10)
+
+    class Of(torch.nn.Module):
+        def __init__(self, call):
+            super().__init__()
+            self.call = call
+
+        def forward(self, x):
+            return self.call(x.movedim(-3, -1))
+
+    z, at = torch.randn(2, 4, 5, 3, device=DEV), torch.randint(0, 40, (2, 4, 5, 3), device=DEV)
+    for call in (FusedRMSNorm(40), FusedLayerNorm(40), lambda x: token_log_probs(x, at[..., 0]).log_prob, lambda x: distillation(x, z, at).divergence):
+        net = Of(call).to(DEV)
+        x, new = (torch.randn(2, 40, 4, 5, device=DEV) for _ in range(2))
+        for grad in (False, True):
+            with torch.set_grad_enabled(grad):
+                traced = torch.jit.trace(net, x, check_trace=False)
+                assert torch.equal(traced(new), net(new))

@@ -1,9 +1,12 @@
 """What the operators around a head do at their edges, as far as it needs no GPU."""
+import random
 import shutil
 import subprocess
+import sys
 from pathlib import Path
 
 import pytest
+import torch
 
 from tests.test_head_ops_cpu import P, SHAPE, _caller
 
@@ -68,3 +71,54 @@ def test_temperatures_too_small_for_their_inverse():
         assert fwd(tau=tau) == bwd(tau=tau) == SHAPE
     for tau in (4.3e-39, 1e-37, 3e38):
         assert fwd(tau=tau, rows=0) == bwd(tau=tau, rows=0) == 0
+
+
+def test_rows_of_views():
+    """Rows are found where a view of the same memory has them, and copied otherwise."""
+    from addernetcuda_b200.layernorm import _rows
+    rng = random.Random(0)
+    kept = 0
+    for _ in range(3000):
+        shape = [rng.choice([1, 2, 3, 5]) for _ in range(rng.randint(1, 4))]
+        t = torch.arange(20000).as_strided([s * rng.choice([1, 2]) for s in shape], torch.empty([2 * s for s in shape]).stride(), rng.choice([0, 1, 5]))
+        t = t[tuple(slice(rng.choice([0, 1]) if n > 1 else 0, n, rng.choice([1, 1, 2])) for n in t.shape)]
+        if rng.random() < 0.4:
+            t = t.permute(rng.sample(range(t.dim()), t.dim()))
+        if rng.random() < 0.2:
+            t = t[:1].expand(3, *t.shape[1:])
+        d = 1
+        for n in t.shape[t.dim() - rng.randint(1, t.dim()):]:
+            d *= n
+        rows = t.numel() // d
+        v, stride = _rows(t, rows, d)
+        got = torch.as_strided(v, (rows, d), (stride, 1), v.storage_offset())
+        assert torch.equal(got, t.reshape(rows, d))
+        try:
+            view = t.view(rows, d)
+            same = d == 1 or view.stride(1) == 1
+        except RuntimeError:
+            same = False
+        assert (v.data_ptr() == t.data_ptr()) == same
+        kept += same and not t.is_contiguous()
+    assert kept > 100
+
+
+TRACED = """
+import torch
+from addernetcuda_b200.layernorm import _rows
+class Copy(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x):
+        return torch.zeros_like(x, memory_format=torch.contiguous_format) if _rows(x, x.numel() // x.shape[-1], x.shape[-1])[1] else None
+class Net(torch.nn.Module):
+    def forward(self, x):
+        return Copy.apply(x.movedim(-3, -1))
+x = torch.randn(2, 3, 4, 5)
+assert torch.jit.trace(Net(), x, check_trace=False)(x).shape == (2, 4, 5, 3)
+"""
+
+
+def test_rows_that_are_copied_in_a_trace():
+    """In a process of its own, which a trace with a refused view in it ended."""
+    done = subprocess.run([sys.executable, "-c", TRACED], capture_output=True, text=True, timeout=300, cwd=CSRC.parent.parent)
+    assert done.returncode == 0, done.stderr[-2000:]
