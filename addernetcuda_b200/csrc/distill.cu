@@ -10,7 +10,9 @@
 //
 // What bounds it: memory (2048x128000 bf16: forward 89 us, 90 % of a copy's rate, with the label's probability at T = 2 or 4 96 us; backward 165 us,
 // 97 %), the exponential unit where two exponentials are taken (T = 3 with labels 149 us), and a row's beginning and end in shorter ones (2048x50257
-// with 64 classes of the teacher's 44 us, 71 %).  256x1000 fp32, a warp a row, waits for its loads: 6.8 us forward, 6.8 backward.
+// with 64 classes of the teacher's 44 us, 71 %).  256x1000 fp32, a warp a row, waits for its loads: 6.8 us forward, 6.8 backward.  Where the gradient's rows
+// lie otherwise on 16 bytes than the logits', the backward goes element by element: 2048x50257 in rows of 50304 275 us bf16 and 291 fp32, dense rows 88
+// and 142.
 #include "kernels.h"
 #include "launch.cuh"
 #include "logit_rows.cuh"

@@ -6,8 +6,8 @@
 // and added up in fp32.  y is rounded once.
 //
 // What bounds it.  Few tokens: the weight's bytes (8x4096x32000 24.7 us, 81 % of a copy's rate; 1x4096x4096 7.7 us, of which the weight takes 2.6: a
-// launch, the first copies and the join of a cluster).  Many tokens: products and sums in turn (8192x4096x16384 505 us, 2.17 PFLOP/s, 66 % of twice
-// the measured bf16 rate; alone, without the sums, 421): a block of 256 x 256 takes a pair 512 clocks of products, and its sums 650 of eight warps, of
+// launch, the first copies and the join of a cluster).  Many tokens: products and sums in turn (8192x4096x16384 among pauses 505 us, 2.17 PFLOP/s, 66 % of
+// twice the measured bf16 rate, and 421 without the sums; in passes one behind another, whose clocks fall, 595, 1.85 PFLOP/s, 56 %): a block of 256 x 256 takes a pair 512 clocks of products, and its sums 650 of eight warps, of
 // which 400 are their additions.  Between them a wave or two of tiles: 512x4096x4096 15.7 us, 1024x4096x4096 21.6, 4096x4096x4096 69.5.
 #include <algorithm>
 #include "kernels.h"

@@ -1,10 +1,11 @@
-// Tensor-memory-accelerator helpers: tiled bulk loads (cp.async.bulk.tensor) of boxes of an NCHW tensor
-// into shared memory, completion on an mbarrier, bounded waits.
+// Tensor-memory-accelerator helpers: tiled bulk loads (cp.async.bulk.tensor) of boxes of an NCHW tensor, or of
+// rows in 8 bits, into shared memory, completion on an mbarrier, bounded waits.
 //
-// Only the plain form is used: one CTA loads into its own shared memory from this GPU's own global memory.
-// Coordinates may be negative or run past the tensor: those elements arrive as zeros, which is how padding,
-// halos and ragged edges are produced without a single predicated instruction.  The innermost coordinate
-// of every load is a multiple of 4 floats (16 bytes), as the hardware requires.
+// A CTA loads into its own shared memory from this GPU's own global memory, never into several at once; those of a
+// pair count at one mbarrier.  Coordinates of a load may be negative or run past the tensor: those elements arrive as
+// zeros, which is how padding, halos and ragged edges are produced without a single predicated instruction.  Stores (rows
+// of a product) begin inside the tensor, and what lies outside is not written.  The innermost coordinate of every
+// copy is a multiple of 16 bytes, as the hardware requires.
 #pragma once
 #include <cuda.h>
 #include <cuda_runtime.h>

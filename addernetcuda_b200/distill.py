@@ -90,7 +90,9 @@ def distillation(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_ind
     need no common offset, so log probabilities will do.  An index of -1 is an empty place; a row without any has divergence 0.  A class
     named twice has both shares.  A row with an index that is no class, or with a NaN or +inf, gives NaN, and so does a NaN of the teacher's
     at an empty place: `token_log_probs` names no class in a row that has failed.  The divergence is +inf where the teacher names a class
-    whose logit is -inf.  A row whose divergence has a gradient of 0 takes nothing of the teacher's."""
+    whose logit is -inf.  A row whose divergence has a gradient of 0 takes nothing of the teacher's.  Logits may be a view such as
+    [..., :classes] of a padded buffer; views whose rows are not consecutive are copied.  The gradient of such a view takes two to three
+    times as long as that of dense rows, unless row stride and classes differ by a multiple of 16 bytes."""
     out = _native.distillation(logits, teacher_logits, teacher_indices, temperature, targets, ignore_index)
     if out is not None:
         return Distillation(*out)

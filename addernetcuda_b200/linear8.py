@@ -150,7 +150,8 @@ def linear_8bit(x: Union[torch.Tensor, Rows8], weight: Weight8, bias: Optional[t
 
     x is a `Rows8`, or a float32, bfloat16 or float16 tensor [..., columns], which goes through `quantize_rows`; `dtype` (float32, bfloat16
     or float16) is x's own type where it is None, bfloat16 for a Rows8.  `bias` [weight rows] has the type `dtype`.  Sums are fp32: each
-    128 columns' sum of code products is multiplied by its two scales and added up, and the result is rounded once.  Codes whose
+    128 columns' sum of code products is multiplied by its two scales (their product in fp32, which loses bits below 2^-126 and ends at 2^128)
+    and added up, and the result is rounded once.  Codes whose
     rows do not begin at multiples of 16 bytes are copied, at every call; those of this module's functions do.  No gradient."""
     if not isinstance(weight, Weight8):
         raise TypeError(f"weight must be a Weight8, got {type(weight).__name__}")
