@@ -19,6 +19,7 @@ import torch
 import torch.nn as nn
 
 from . import _lib, _native, adder_cuda
+from .layernorm import _recorded
 from .linear8 import Linear8bit
 from .logprobs import token_log_probs
 
@@ -55,15 +56,19 @@ class FoldedBatchNorm2d(nn.Module):
         z = _native.affine(y, self.scale, self.shift, residual, relu)
         if z is not None:
             return z
-        y = y.contiguous()
-        res = residual.contiguous() if residual is not None else None
-        n, c, h, w = y.shape
-        z = torch.empty_like(y)
-        with torch.cuda.device(y.device):
-            _lib.check(_lib.load().adder_b200_affine_forward(
-                y.data_ptr(), self.scale.data_ptr(), self.shift.data_ptr(), res.data_ptr() if res is not None else None,
-                z.data_ptr(), int(relu), n, c, h * w, adder_cuda._stream(y.device)), "adder_b200_affine_forward")
-        return z
+        return _recorded(_affine, y, self.scale, self.shift, residual, relu)
+
+
+def _affine(y, scale, shift, residual, relu):
+    y = y.contiguous()
+    res = residual.contiguous() if residual is not None else None
+    n, c, h, w = y.shape
+    z = torch.empty_like(y)
+    with torch.cuda.device(y.device):
+        _lib.check(_lib.load().adder_b200_affine_forward(
+            y.data_ptr(), scale.data_ptr(), shift.data_ptr(), res.data_ptr() if res is not None else None,
+            z.data_ptr(), int(relu), n, c, h * w, adder_cuda._stream(y.device)), "adder_b200_affine_forward")
+    return z
 
 
 def fold_batchnorm(model: nn.Module) -> nn.Module:

@@ -370,3 +370,21 @@ def test_a_trace_of_inputs_in_another_order():
             with torch.set_grad_enabled(grad):
                 traced = torch.jit.trace(net, x, check_trace=False)
                 assert torch.equal(traced(new), net(new))
+
+
+def test_a_trace_of_a_network_for_inference():
+    """Folded batch norms and a head in 8 bits: the traced network follows new images."""
+    from addernetcuda_b200 import resnet
+    from addernetcuda_b200.inference import fold_batchnorm, quantize_linear
+    torch.manual_seed(11)
+    net = resnet.resnet20().to(DEV)
+    images, new = (torch.randn(4, 3, 32, 32, device=DEV) for _ in range(2))
+    with torch.no_grad():
+        for m in net.modules():
+            if isinstance(m, torch.nn.BatchNorm2d):
+                m.momentum = 1.0
+        net.train()(images)
+        for prepare in (fold_batchnorm, quantize_linear):
+            prepare(net)
+            traced = torch.jit.trace(net, images, check_trace=False)
+            assert torch.equal(traced(new), net(new))
