@@ -200,9 +200,9 @@ def _product(x, x_scales, weight, weight_scales, bias, dtype):
 
 class Linear8bit(nn.Module):
     """A linear layer with its weight in 8 bits, for inference: `Linear8bit(linear)` of an nn.Linear on CUDA, or of a 1x1 nn.Conv2d (stride
-    1, no padding, one group), whose input and output then are [N, C, H, W] or [C, H, W], in one order in memory.  The input of an nn.Linear's may be a `Rows8`, as
-    `rmsnorm.rms_norm_8bit` gives it.  The output has the type `dtype`, where it is None the input's, bfloat16 for a Rows8.  There is no
-    `weight`: the codes are `values` and `scales`."""
+    1, no padding, one group), whose input and output then are [N, C, H, W] or [C, H, W], the output in the input's memory format.  The input of
+    an nn.Linear's may be a `Rows8`, as `rmsnorm.rms_norm_8bit` gives it.  The output has the type `dtype`, where it is None the input's,
+    bfloat16 for a Rows8, and carries no gradient, whatever the input asks for.  There is no `weight`: the codes are `values` and `scales`."""
 
     def __init__(self, layer: nn.Module):
         super().__init__()
